@@ -508,6 +508,85 @@ int lmc_layerwise_prefill_dma_copy(const lmc_dma_segment *copies, int64_t n, int
 int lmc_layerwise_prefill_dma_copy_diagnose(const lmc_dma_segment *copies, int64_t n,
                                             int32_t device_to_host, void *stream, double *copy_us);
 
+/* ------------------------------------------------------------------------
+ * Serving operators over the same paged caches (no reference counterpart).
+ * Every tensor is on one GPU; no tensor of the host is read in place.
+ * ------------------------------------------------------------------------ */
+
+/* Slot mapping, positions and block tables of a batch from its request
+ * lengths, in one launch.  query_lens and context_lens ([R] int32 or int64,
+ * both the same; negative lengths count as 0) are the new tokens of each
+ * request and those before them; block_table is [R, W] int32.  With start =
+ * the sum of the query_lens before request r, token t of [start, start +
+ * query_lens[r]) has position p = context_lens[r] + t - start and
+ *   slot_mapping[t] = block_table[r][p / block_size] * block_size + p % block_size,
+ * or -1 where the table has no page (a negative entry, or p past its row).
+ * slot_mapping and positions ([N] int64) get -1 and 0 behind the last token;
+ * tokens past N are left out.  query_start_loc ([R + 1] int32) and seq_lens
+ * ([R] int32, context + query) stop at 2^31 - 1.  positions, query_start_loc
+ * and seq_lens may be null.
+ * With free_blocks ([F] int32) the table is completed in place: entries
+ * ceil(context / block_size) .. ceil((context + query) / block_size) of each
+ * row, at most W, take blocks from free_blocks[free_cursor] on, request by
+ * request (-1 behind the list's end), and *next_cursor = free_cursor + the
+ * blocks asked for, also where the list ended before.  free_cursor and
+ * next_cursor are [1] int64, distinct, and may be null (a null cursor is 0).
+ * At most 16384 requests, W * block_size < 2^31. */
+int lmc_build_slot_mapping(const lmc_tensor *query_lens, const lmc_tensor *context_lens,
+                           const lmc_tensor *block_table, int64_t block_size,
+                           const lmc_tensor *slot_mapping, const lmc_tensor *positions,
+                           const lmc_tensor *query_start_loc, const lmc_tensor *seq_lens,
+                           const lmc_tensor *free_blocks, const lmc_tensor *free_cursor,
+                           const lmc_tensor *next_cursor, void *stream);
+
+/* Rotary positions: the pairs of dims [rotary_offset, rotary_offset + 2 *
+ * n_freq) of every head of query and key (halves when is_neox != 0, else
+ * interleaved) are turned by positions[t] * inv_freq[i] and multiplied by
+ * `scale`; inverse != 0 turns back by the same angle (the transpose, which is
+ * the gradient: `scale` multiplies there too).  query and key are
+ * [T, heads * head_size] or [T, heads, head_size] bf16, fp16 or fp32 (one
+ * dtype) with any token and head strides; either may be null.  query_out and
+ * key_out take the results (other dims are copied), null means in place.
+ * positions: [T] int64 or int32, any values; inv_freq: device array of n_freq
+ * doubles, radians per position.  Angles are formed in 64 bits. */
+int lmc_rotary_embedding(const lmc_tensor *positions, const lmc_tensor *query, const lmc_tensor *key,
+                         int64_t head_size, const double *inv_freq, int64_t n_freq, double scale,
+                         int32_t is_neox, int64_t rotary_offset, int32_t inverse,
+                         const lmc_tensor *query_out, const lmc_tensor *key_out, void *stream);
+
+/* lmc_rotary_embedding's forward rotation of query (to query_out, or in
+ * place; may be null) and key, with the rotated keys and the values written
+ * to the paged caches (MERGED_KV or SEPARATE_KV, any strides) at
+ * slot_mapping ([T] int64 or int32); key and value stay as they are.  Tokens
+ * whose slot lies outside the caches are not written.  Two tokens with one
+ * slot leave either's row. */
+int lmc_rotary_embedding_to_paged(const lmc_tensor *positions, const lmc_tensor *query, const lmc_tensor *key,
+                                  const lmc_tensor *value, const lmc_tensor *vllm_kv_caches, int32_t n_caches,
+                                  const lmc_tensor *slot_mapping, int64_t head_size, const double *inv_freq,
+                                  int64_t n_freq, double scale, int32_t is_neox, int64_t rotary_offset,
+                                  const lmc_tensor *query_out, int32_t kvcache_format, int32_t vllm_two_major,
+                                  void *stream);
+
+/* Attention of a batch whose requests share their first shared_len tokens.
+ * query and output: [T, heads, dim] bf16 or fp16; the caches MERGED_KV or
+ * SEPARATE_KV of that dtype, heads a multiple of theirs, dim 64, 96, 128, 192
+ * or 256.  Request r has tokens query_start_loc[r] .. query_start_loc[r + 1]
+ * ([R + 1] int32, from 0 and not decreasing) and seq_lens[r] ([R] int32) keys
+ * with them: its i-th of q tokens sees the keys 0 .. seq_lens[r] - q + i.
+ * Key j lies in block shared_blocks[j / block_size] for j < shared_len, else
+ * in block_table[r][j / block_size] ([R, W] int32); keys whose block lies
+ * outside the caches, or past the row's end, count as unseen, and unseen
+ * rows of the caches are never used, whatever they hold.  A token that sees
+ * no key gets zeros and an lse of -infinity; rows of output and lse behind
+ * query_start_loc[R] are left as they were.  lse ([T, heads] fp32, may be
+ * null): log of the sum of exp(scale * q . k). */
+int lmc_shared_prefix_attention(const lmc_tensor *query, const lmc_tensor *vllm_kv_caches, int32_t n_caches,
+                                const lmc_tensor *shared_blocks, int64_t shared_len,
+                                const lmc_tensor *block_table, const lmc_tensor *seq_lens,
+                                const lmc_tensor *query_start_loc, double scale, const lmc_tensor *output,
+                                const lmc_tensor *lse, int32_t kvcache_format, int32_t vllm_two_major,
+                                void *stream);
+
 /* Replaces get_gpu_pci_bus_id (pybind csrc/pybind.cpp:482): the PCI bus id
  * string of `device`, written NUL-terminated into buf[0..buf_len). */
 int lmc_get_gpu_pci_bus_id(int32_t device, char *buf, int32_t buf_len);

@@ -1,0 +1,432 @@
+// Rotary positions of queries and keys on MI355X (gfx950), forward and
+// inverse, with the option of writing the rotated keys and the values to
+// their paged caches.
+//
+//   (z1, z2) = (x1 c - x2 s, x2 c + x1 s),  (c, s) = scale * (cos, sin)(pos * inv_freq[i])
+//
+// for the pairs of dims [offset, offset + 2 n_freq) of each head (halves or
+// interleaved); the other dims pass through.  The inverse takes -s: the
+// transpose, which is the gradient of the rotation.
+//
+// No table: a table's row is as long as a key head and there are as many
+// rows as the longest context has positions, while the angle costs a few
+// 64-bit operations.  pos * inv_freq / 2 pi is formed in 64 bits and reduced
+// to an eighth of a turn there, so far positions lose nothing, and cos and
+// sin are polynomials of that rest in 32 bits (1.3e-7 relative).  A
+// workgroup computes the pairs of its tokens once and all heads read them
+// from LDS.  The key and value elements are widened to 32 bits, rotated, and
+// rounded once.
+//
+// HBM-bound: each element is read and written once.  A lane moves VP pairs
+// (two 16-byte accesses each way where the layout allows).
+#include "rope_math.h"
+#include "serving.h"
+
+#include <cmath>
+
+namespace lmc {
+
+namespace {
+
+// cos and sin of 2 pi r for |r| <= 1/8, least-maximum fits in r * r (own
+// fits: 5e-12 and 6e-11 before rounding).
+__device__ __forceinline__ void sincos_eighth(float r, float &s, float &c) {
+  const float u = r * r;
+  s = r * (6.28318531f + u * (-41.3417022f + u * (81.6052047f + u * (-76.6978700f + u * 41.4729485f))));
+  c = 1.0f + u * (-19.7392082f + u * (64.9393082f + u * (-85.4422989f + u * 59.2027969f)));
+}
+
+__device__ __forceinline__ void sincos_turn(int64_t pos, double inv_freq, float &s, float &c) {
+  constexpr double kInvTwoPi = 0.15915494309189533577;
+  const double t = static_cast<double>(pos) * (inv_freq * kInvTwoPi);
+  const double part = t - rint(t);                       // [-1/2, 1/2]
+  const double quarter = rint(part * 4.0);
+  const float r = static_cast<float>(part - quarter * 0.25);
+  float ps, pc;
+  sincos_eighth(r, ps, pc);
+  const int q = static_cast<int>(quarter) & 3;
+  s = (q & 1) ? pc : ps;
+  c = (q & 1) ? ps : pc;
+  if (q & 2) s = -s;
+  if (q == 1 || q == 2) c = -c;
+}
+
+// Rows of one tensor: heads of a token, and where they go.  Strides in elements.
+struct Rows {
+  const void *in;
+  void *out;
+  int64_t in_token, in_head, out_token, out_head;
+  uint32_t units;   // per token
+  uint32_t magic;   // ceil(2^32 / units per head): a division
+  uint32_t per_head;
+  int paged;        // out is a cache: rows at the token's slot
+};
+
+struct RotaryArgs {
+  const void *positions;
+  int pos_i32;
+  const double *inv_freq;
+  int half, offset;
+  float scale;
+  int inverse;
+  int64_t n_tokens;
+  int tokens_per_block;
+  uint32_t units;   // per token, all three
+  Rows q, k, v;
+  const int64_t *slots;
+  int slots_i32;
+  uint32_t block_size;
+  int64_t num_slots;
+  int64_t k_page, k_slot, v_page, v_slot;  // elements
+};
+
+constexpr int kThreads = 256;
+constexpr int kMaxTokens = 8;  // per workgroup
+
+template <typename KD, bool NEOX, int VP>
+__global__ void __launch_bounds__(kThreads) rotary_rows(RotaryArgs a) {
+  using S = typename KD::S;
+  using V = Pack<S, VP>;
+  extern __shared__ float cs[];  // cos [tokens][half], then sin
+  __shared__ int64_t row_k[kMaxTokens], row_v[kMaxTokens];
+  const int tid = threadIdx.x;
+  const int64_t t0 = static_cast<int64_t>(blockIdx.x) * a.tokens_per_block;
+  const int nt = static_cast<int>(min(static_cast<int64_t>(a.tokens_per_block), a.n_tokens - t0));
+  float *cosv = cs, *sinv = cs + a.tokens_per_block * a.half;
+  for (int i = tid; i < nt * a.half; i += kThreads) {
+    const int t = i / a.half, j = i - t * a.half;
+    const int64_t pos = a.pos_i32 ? static_cast<const int32_t *>(a.positions)[t0 + t]
+                                  : static_cast<const int64_t *>(a.positions)[t0 + t];
+    float s, c;
+    sincos_turn(pos, a.inv_freq[j], s, c);
+    cosv[i] = c * a.scale;
+    sinv[i] = (a.inverse ? -s : s) * a.scale;
+  }
+  if (a.slots && tid < nt) {
+    const int64_t slot = a.slots_i32 ? reinterpret_cast<const int32_t *>(a.slots)[t0 + tid] : a.slots[t0 + tid];
+    int64_t rk = -1, rv = -1;
+    if (slot >= 0 && slot < a.num_slots) {
+      const uint32_t x = static_cast<uint32_t>(slot), page = x / a.block_size, at = x - page * a.block_size;
+      rk = page * a.k_page + at * a.k_slot;
+      rv = page * a.v_page + at * a.v_slot;
+    }
+    row_k[tid] = rk;
+    row_v[tid] = rv;
+  }
+  __syncthreads();
+
+  const uint32_t total = nt * a.units;
+  const uint32_t chunk = (total + gridDim.y - 1) / gridDim.y;
+  const uint32_t end = min(total, (blockIdx.y + 1) * chunk);
+  uint32_t x = blockIdx.y * chunk + tid;
+  uint32_t t = x / a.units, w = x - t * a.units;
+  const uint32_t turned = a.half / VP;
+  for (; x < end; x += kThreads) {
+    const bool is_q = w < a.q.units, is_k = !is_q && w < a.q.units + a.k.units;
+    const Rows &rows = is_q ? a.q : is_k ? a.k : a.v;
+    const uint32_t y = w - (is_q ? 0 : is_k ? a.q.units : a.q.units + a.k.units);
+    const uint32_t h = rows.per_head == 1 ? y : __umulhi(y, rows.magic), u = y - h * rows.per_head;
+    const S *in = static_cast<const S *>(rows.in) + (t0 + t) * rows.in_token + h * rows.in_head;
+    const int64_t at = rows.paged ? (is_k ? row_k[t] : row_v[t]) : (t0 + t) * rows.out_token;
+    S *out = static_cast<S *>(rows.out) + at + h * rows.out_head;
+    if (at >= 0) {
+      if ((is_q || is_k) && u < turned) {
+        const int i0 = u * VP;
+        const int e1 = a.offset + (NEOX ? i0 : 2 * i0), e2 = NEOX ? e1 + a.half : e1 + VP;
+        const V p = *reinterpret_cast<const V *>(in + e1), r = *reinterpret_cast<const V *>(in + e2);
+        const float *c = cosv + t * a.half + i0, *s = sinv + t * a.half + i0;
+        V o1, o2;
+        if constexpr (NEOX) {
+#pragma unroll
+          for (int i = 0; i < VP; ++i) {
+            const float x1 = to_f32<KD>(p.v[i]), x2 = to_f32<KD>(r.v[i]);
+            o1.v[i] = from_f32<KD>(x1 * c[i] - x2 * s[i]);
+            o2.v[i] = from_f32<KD>(x2 * c[i] + x1 * s[i]);
+          }
+        } else {
+          S in2[2 * VP], out2[2 * VP];
+#pragma unroll
+          for (int i = 0; i < VP; ++i) {
+            in2[i] = p.v[i];
+            in2[VP + i] = r.v[i];
+          }
+#pragma unroll
+          for (int i = 0; i < VP; ++i) {
+            const float x1 = to_f32<KD>(in2[2 * i]), x2 = to_f32<KD>(in2[2 * i + 1]);
+            out2[2 * i] = from_f32<KD>(x1 * c[i] - x2 * s[i]);
+            out2[2 * i + 1] = from_f32<KD>(x2 * c[i] + x1 * s[i]);
+          }
+#pragma unroll
+          for (int i = 0; i < VP; ++i) {
+            o1.v[i] = out2[i];
+            o2.v[i] = out2[VP + i];
+          }
+        }
+        *reinterpret_cast<V *>(out + e1) = o1;
+        *reinterpret_cast<V *>(out + e2) = o2;
+      } else {
+        int e = ((is_q || is_k) ? u - turned : u) * VP;
+        if ((is_q || is_k) && e >= a.offset) e += 2 * a.half;
+        *reinterpret_cast<V *>(out + e) = *reinterpret_cast<const V *>(in + e);
+      }
+    }
+    w += kThreads;
+    while (w >= a.units) {
+      w -= a.units;
+      ++t;
+    }
+  }
+}
+
+template <typename KD, bool NEOX, int VP> void launch(const RotaryArgs &a, hipStream_t s) {
+  const int64_t blocks = (a.n_tokens + a.tokens_per_block - 1) / a.tokens_per_block;
+  // Few tokens: a unit a lane, spread over workgroups.
+  const int64_t per = (static_cast<int64_t>(a.tokens_per_block) * a.units + kThreads - 1) / kThreads;
+  const int64_t y = blocks >= 1024 ? 1 : std::min<int64_t>(per, 1024 / blocks);
+  const size_t shared = static_cast<size_t>(a.tokens_per_block) * a.half * 2 * sizeof(float);
+  hipLaunchKernelGGL((rotary_rows<KD, NEOX, VP>), dim3(static_cast<uint32_t>(blocks), static_cast<uint32_t>(y)),
+                     dim3(kThreads), shared, s, a);
+  hip_check(hipGetLastError(), "rotary_rows launch");
+}
+
+template <typename KD, bool NEOX> void launch_vp(const RotaryArgs &a, int vp, hipStream_t s) {
+  switch (vp) {
+  case 8:
+    if constexpr (sizeof(typename KD::S) == 2) launch<KD, NEOX, 8>(a, s);
+    break;
+  case 4: launch<KD, NEOX, 4>(a, s); break;
+  case 2: launch<KD, NEOX, 2>(a, s); break;
+  default: launch<KD, NEOX, 1>(a, s); break;
+  }
+}
+
+template <typename KD> void launch_style(const RotaryArgs &a, bool neox, int vp, hipStream_t s) {
+  neox ? launch_vp<KD, true>(a, vp, s) : launch_vp<KD, false>(a, vp, s);
+}
+
+// One tensor's token and head strides: [T, heads * D] or [T, heads, D].
+struct HeadView {
+  const lmc_tensor *t = nullptr;
+  int64_t token = 0, head = 0, heads = 0, dim = 0;
+};
+
+HeadView head_view(const lmc_tensor &t, const char *name, int64_t dim, int device, int32_t dtype) {
+  check_on(t, name, device, dtype);
+  HeadView v;
+  v.t = &t;
+  v.dim = dim;
+  check_value(t.ndim == 2 || t.ndim == 3, std::string(name) + " must be [tokens, heads * head_size] or [tokens, heads, head_size]");
+  for (int i = 0; i < t.ndim; ++i) check_value(t.strides[i] >= 0, std::string(name) + ": negative strides unsupported");
+  check_value(size(t, -1) <= 1 || stride(t, -1) == 1, std::string(name) + ": a head's dims must be adjacent");
+  v.token = t.strides[0];
+  if (t.ndim == 2) {
+    check_value(t.sizes[1] % dim == 0, std::string(name) + " width is not a multiple of head_size");
+    v.heads = t.sizes[1] / dim;
+    v.head = dim;
+  } else {
+    check_value(t.sizes[2] == dim, std::string(name) + " heads are not of head_size");
+    v.heads = t.sizes[1];
+    v.head = t.strides[1];
+  }
+  return v;
+}
+
+bool same_rows(const HeadView &a, const HeadView &b) {
+  return a.t->data == b.t->data && a.heads == b.heads && (a.t->sizes[0] <= 1 || a.token == b.token) &&
+         (a.heads <= 1 || a.head == b.head);
+}
+
+// Whether two tensors may share an element.  Column slices of one buffer
+// (the same token stride, each token's heads inside it) are told apart.
+bool may_share(const HeadView &a, const HeadView &b) {
+  if (!extents_meet(*a.t, *b.t)) return false;
+  const int64_t es = elem_size(*a.t);
+  const int64_t wa = ((a.heads - 1) * a.head + a.dim) * es, wb = ((b.heads - 1) * b.head + b.dim) * es;
+  const int64_t s = a.token * es;
+  if (a.token != b.token || wa > s || wb > s) return true;
+  const int64_t d = reinterpret_cast<intptr_t>(b.t->data) - reinterpret_cast<intptr_t>(a.t->data);
+  const int64_t m = ((d % s) + s) % s;
+  return !(m >= wa && m + wb <= s);
+}
+
+void rotary(const lmc_tensor *positions, const lmc_tensor *query, const lmc_tensor *key, const lmc_tensor *value,
+            const lmc_tensor *caches, int n_caches, int fmt, bool two_major, const lmc_tensor *slot_mapping,
+            int64_t head_size, const double *inv_freq, int64_t n_freq, double scale, bool neox, int64_t offset,
+            bool inverse, const lmc_tensor *query_out, const lmc_tensor *key_out, bool paged, hipStream_t stream) {
+  check_value(query || key, "neither query nor key is given");
+  const lmc_tensor &lead = deref(query ? query : key, query ? "query" : "key");
+  const int dev = lead.device;
+  check_value(dev >= 0, "query and key must be on a GPU");
+  if (lead.dtype != LMC_BF16 && lead.dtype != LMC_F16 && lead.dtype != LMC_F32)
+    fail(LMC_ERR_VALUE, "rotary positions take bfloat16, float16 or float32 queries and keys only");
+  check_value(head_size > 0 && head_size <= 8192, "head_size must be between 1 and 8192");
+  check_value(inv_freq != nullptr && n_freq > 0, "inv_freq is empty");
+  check_value(offset >= 0 && n_freq <= head_size / 2 && offset <= head_size - 2 * n_freq,
+              "the rotated dims [rotary_offset, rotary_offset + 2 * len(inv_freq)) do not lie in a head");
+  check_value(std::isfinite(scale), "scale must be finite");
+  const int64_t T = size(lead, 0), rot = 2 * n_freq, es = elem_size(lead);
+  const lmc_tensor &pos = deref(positions, "positions");
+  check_vector(pos, "positions", dev, LMC_I64, LMC_I32);
+  check_value(pos.sizes[0] == T, "positions must have one entry per token");
+
+  RotaryArgs a;
+  std::memset(&a, 0, sizeof(a));
+  int64_t grain = 16;  // bytes every address and length is a multiple of
+  auto need = [&](int64_t bytes) {
+    while (bytes % grain) grain /= 2;
+  };
+  HeadView views[5];
+  bool written[5];
+  int n_views = 0;
+  auto add = [&](Rows &rows, const lmc_tensor *in_t, const lmc_tensor *out_t, const char *name, const char *out_name,
+                 int64_t dim, bool turn) {
+    const HeadView in = head_view(deref(in_t, name), name, dim, dev, lead.dtype);
+    check_value(in.t->sizes[0] == T, std::string(name) + " has another number of tokens than the call's other tensors");
+    check_value(in.heads * dim <= INT32_MAX / 4, std::string(name) + " rows are too wide");
+    const int at = n_views++;
+    views[at] = in;
+    written[at] = false;
+    HeadView out = in;
+    bool moved = paged && rows.paged;
+    if (!moved && out_t) {
+      out = head_view(deref(out_t, out_name), out_name, dim, dev, lead.dtype);
+      check_value(out.t->sizes[0] == T && out.heads == in.heads, std::string(out_name) + " differs in shape from " + name);
+      moved = !same_rows(in, out);
+      if (moved) {
+        views[n_views] = out;
+        written[n_views++] = true;
+      }
+    }
+    if (!moved) written[at] = true;
+    if (!rows.paged)
+      check_value(rows_apart({T, out.heads, dim}, {out.token, out.head, 1}),
+                  std::string(moved ? out_name : name) + " has overlapping rows");
+    rows.in = in.t->data;
+    rows.in_token = in.token;
+    rows.in_head = in.head;
+    need(reinterpret_cast<uintptr_t>(in.t->data));
+    need(in.token * es);
+    need(in.head * es);
+    if (!rows.paged) {
+      rows.out = out.t->data;
+      rows.out_token = out.token;
+      rows.out_head = out.head;
+      need(reinterpret_cast<uintptr_t>(out.t->data));
+      need(out.token * es);
+      need(out.head * es);
+    }
+    need(dim * es);
+    rows.per_head = static_cast<uint32_t>(!turn ? dim : moved ? n_freq + dim - rot : n_freq);  // elements or pairs
+    rows.units = static_cast<uint32_t>(in.heads);                                              // heads, for now
+    return in;
+  };
+  a.k.paged = a.v.paged = paged;
+  if (query) add(a.q, query, query_out, "query", "query_out", head_size, true);
+  else check_value(!query_out, "query_out without query");
+  PagedKv kv;
+  if (paged) {
+    kv = paged_kv(caches, n_caches, fmt, two_major, "rotary_embedding_to_paged");
+    check_value(kv.device == dev && kv.dtype == lead.dtype, "the paged caches differ in device or dtype from the rows");
+    check_value(rows_apart({kv.pages, kv.block_size, kv.heads, kv.dim * es}, {kv.k_page, kv.k_token, kv.k_head, 1}) &&
+                    rows_apart({kv.pages, kv.block_size, kv.heads, kv.dim * es}, {kv.v_page, kv.v_token, kv.v_head, 1}),
+                "the paged caches have overlapping rows");
+    check_value(kv.dim == head_size, "the paged caches' heads are not of head_size");
+    const HeadView k = add(a.k, key, nullptr, "key", "", head_size, true);
+    const HeadView v = add(a.v, value, nullptr, "value", "", head_size, false);
+    check_value(k.heads == kv.heads && v.heads == kv.heads, "the paged caches have another number of heads than key and value");
+    for (int i = 0; i < n_views; ++i)
+      for (int c = 0; c < n_caches; ++c)
+        check_value(!extents_meet(*views[i].t, caches[c]), "the paged caches overlap the call's rows");
+    const lmc_tensor &sm = deref(slot_mapping, "slot_mapping");
+    check_vector(sm, "slot_mapping", dev, LMC_I64, LMC_I32);
+    check_value(sm.sizes[0] == T, "slot_mapping must have one entry per token");
+    a.slots = static_cast<const int64_t *>(sm.data);
+    a.slots_i32 = sm.dtype == LMC_I32;
+    a.block_size = static_cast<uint32_t>(kv.block_size);
+    a.num_slots = kv.pages * kv.block_size;
+    a.k.out = kv.k;
+    a.v.out = kv.v;
+    a.k.out_head = kv.k_head / es;
+    a.v.out_head = kv.v_head / es;
+    a.k_page = kv.k_page / es;
+    a.k_slot = kv.k_token / es;
+    a.v_page = kv.v_page / es;
+    a.v_slot = kv.v_token / es;
+    for (int64_t b : {static_cast<int64_t>(reinterpret_cast<uintptr_t>(kv.k)), static_cast<int64_t>(reinterpret_cast<uintptr_t>(kv.v)),
+                      kv.k_page, kv.k_token, kv.k_head, kv.v_page, kv.v_token, kv.v_head})
+      need(b);
+  } else {
+    if (key) add(a.k, key, key_out, "key", "key_out", head_size, true);
+    else check_value(!key_out, "key_out without key");
+  }
+  // What is written must not be read by another lane.
+  for (int i = 0; i < n_views; ++i)
+    for (int j = 0; j < i; ++j)
+      check_value(!(written[i] || written[j]) || !may_share(views[i], views[j]), "two of query, key, value and the outputs overlap");
+  if (T == 0) return;
+  need(n_freq * es);
+  need(offset * es);
+  const int vp = static_cast<int>(std::max<int64_t>(1, grain / es));
+  uint32_t units = 0;
+  for (Rows *r : {&a.q, &a.k, &a.v}) {
+    if (r->units == 0) continue;
+    r->per_head /= vp;
+    r->magic = static_cast<uint32_t>(((uint64_t(1) << 32) + r->per_head - 1) / r->per_head);
+    check_value(static_cast<uint64_t>(r->units) * r->per_head * r->per_head < (uint64_t(1) << 32), "rows are too wide");
+    r->units *= r->per_head;
+    units += r->units;
+  }
+  if (units == 0) return;
+  a.units = units;
+  a.positions = pos.data;
+  a.pos_i32 = pos.dtype == LMC_I32;
+  a.inv_freq = inv_freq;
+  a.half = static_cast<int>(n_freq);
+  a.offset = static_cast<int>(offset);
+  a.scale = static_cast<float>(scale);
+  a.inverse = inverse;
+  a.n_tokens = T;
+  check_value(T <= INT32_MAX, "too many tokens");
+  // Several tokens share a workgroup once there are workgroups enough, as
+  // long as their angles fit 16 KiB.
+  int tb = 1;
+  while (tb < kMaxTokens && T / (2 * tb) >= 1024 && tb * 2 * n_freq * 8 <= 16384) tb *= 2;
+  a.tokens_per_block = tb;
+  check_value(static_cast<int64_t>(tb) * units <= INT32_MAX, "rows are too wide");
+  DeviceGuard guard(dev);
+  switch (lead.dtype) {
+  case LMC_BF16: launch_style<BF16>(a, neox, vp, stream); break;
+  case LMC_F16: launch_style<F16>(a, neox, vp, stream); break;
+  default: launch_style<F32>(a, neox, vp, stream); break;
+  }
+}
+
+} // namespace
+
+} // namespace lmc
+
+using namespace lmc;
+
+extern "C" int lmc_rotary_embedding(const lmc_tensor *positions, const lmc_tensor *query, const lmc_tensor *key,
+                                    int64_t head_size, const double *inv_freq, int64_t n_freq, double scale,
+                                    int32_t is_neox, int64_t rotary_offset, int32_t inverse,
+                                    const lmc_tensor *query_out, const lmc_tensor *key_out, void *stream) {
+  return guarded([&] {
+    rotary(positions, query, key, nullptr, nullptr, 0, 0, false, nullptr, head_size, inv_freq, n_freq, scale,
+           is_neox != 0, rotary_offset, inverse != 0, query_out, key_out, false, static_cast<hipStream_t>(stream));
+  });
+}
+
+extern "C" int lmc_rotary_embedding_to_paged(const lmc_tensor *positions, const lmc_tensor *query,
+                                             const lmc_tensor *key, const lmc_tensor *value,
+                                             const lmc_tensor *vllm_kv_caches, int32_t n_caches,
+                                             const lmc_tensor *slot_mapping, int64_t head_size, const double *inv_freq,
+                                             int64_t n_freq, double scale, int32_t is_neox, int64_t rotary_offset,
+                                             const lmc_tensor *query_out, int32_t kvcache_format,
+                                             int32_t vllm_two_major, void *stream) {
+  return guarded([&] {
+    rotary(positions, query, key, value, vllm_kv_caches, n_caches, kvcache_format, vllm_two_major != 0, slot_mapping,
+           head_size, inv_freq, n_freq, scale, is_neox != 0, rotary_offset, false, query_out, nullptr, true,
+           static_cast<hipStream_t>(stream));
+  });
+}

@@ -1,0 +1,108 @@
+// Argument checks shared by the serving operators (slot maps, rotary
+// positions, shared-prefix attention): tensors of one GPU, and one layer's
+// paged K and V caches with every stride taken from the tensors.
+#pragma once
+
+#include "kv_geom.h"
+
+namespace lmc {
+
+// A device tensor of `device` with one of two dtypes.
+inline void check_on(const lmc_tensor &t, const char *name, int device, int32_t dtype, int32_t or_dtype = -1) {
+  if (t.device < 0 || t.device != device)
+    fail(LMC_ERR_VALUE, std::string(name) + " is not on the GPU of the call's other tensors");
+  if (t.dtype != dtype && t.dtype != or_dtype) fail(LMC_ERR_VALUE, std::string(name) + " has a dtype the call does not take");
+}
+
+// The same, 1-D with adjacent elements.
+inline void check_vector(const lmc_tensor &t, const char *name, int device, int32_t dtype, int32_t or_dtype = -1) {
+  check_on(t, name, device, dtype, or_dtype);
+  if (t.ndim != 1 || (t.sizes[0] > 1 && t.strides[0] != 1))
+    fail(LMC_ERR_VALUE, std::string(name) + " must be 1-D and contiguous");
+}
+
+// Whether the address ranges of two tensors meet.
+inline bool extents_meet(const lmc_tensor &a, const lmc_tensor &b) {
+  const int64_t na = extent_bytes(a), nb = extent_bytes(b);
+  const uintptr_t pa = reinterpret_cast<uintptr_t>(a.data), pb = reinterpret_cast<uintptr_t>(b.data);
+  return na > 0 && nb > 0 && pa < pb + nb && pb < pa + na;
+}
+
+// Whether no two elements of a strided layout are the same one: in order of
+// stride, each dim steps over all of the dims below it.
+inline bool rows_apart(std::vector<int64_t> sizes, std::vector<int64_t> strides) {
+  std::vector<std::pair<int64_t, int64_t>> dims;
+  for (size_t i = 0; i < sizes.size(); ++i) {
+    if (sizes[i] == 0) return true;
+    if (sizes[i] > 1) dims.emplace_back(strides[i], sizes[i]);
+  }
+  std::sort(dims.begin(), dims.end());
+  int64_t span = 1;
+  for (const auto &[stride, n] : dims) {
+    if (stride < span) return false;
+    span += stride * (n - 1);
+  }
+  return true;
+}
+
+// One layer's caches: row (page, offset, head) of K is at
+// k + page * k_page + offset * k_token + head * k_head (bytes).
+struct PagedKv {
+  uint8_t *k, *v;
+  int64_t k_page, k_token, k_head;
+  int64_t v_page, v_token, v_head;
+  int64_t pages;
+  int64_t block_size;
+  int64_t heads, dim;
+  int32_t dtype;
+  int device;
+};
+
+inline PagedKv paged_kv(const lmc_tensor *caches, int n, int fmt, bool two_major, const char *op) {
+  validate_vllm_caches(caches, n, fmt);
+  if (fmt != LMC_FMT_MERGED_KV && fmt != LMC_FMT_SEPARATE_KV)
+    fail(LMC_ERR_VALUE, std::string(op) + " takes MERGED_KV or SEPARATE_KV caches");
+  const lmc_tensor &k = deref(&caches[0], "vllm_kv_caches[0]");
+  PagedKv g;
+  g.dtype = k.dtype;
+  g.device = k.device;
+  check_value(k.device >= 0, std::string(op) + ": the paged caches are not on a GPU");
+  const int64_t es = elem_size(k);
+  g.k = static_cast<uint8_t *>(k.data);
+  if (fmt == LMC_FMT_MERGED_KV) {
+    // [2, pages, block, heads, dim] (two-major) or [pages, 2, block, heads, dim].
+    check_value(k.ndim == 5 && size(k, two_major ? 0 : 1) == 2, "a MERGED_KV cache is 5-D with K and V along its " +
+                                                                    std::string(two_major ? "first" : "second") + " dim");
+    g.pages = size(k, two_major ? 1 : 0);
+    g.k_page = g.v_page = stride(k, two_major ? 1 : 0) * es;
+    g.v = g.k + stride(k, two_major ? 0 : 1) * es;
+    g.v_token = stride(k, 2) * es;
+    g.v_head = stride(k, 3) * es;
+    check_value(size(k, 4) <= 1 || stride(k, 4) == 1, "a cache row's head dims must be adjacent");
+  } else {
+    const lmc_tensor &v = deref(&caches[1], "vllm_kv_caches[1]");
+    check_value(k.ndim == 4, "SEPARATE_KV caches are [pages, block, heads, dim]");
+    check_value(v.device == k.device && v.dtype == k.dtype, "K and V caches differ in device or dtype");
+    g.pages = size(k, 0);
+    g.k_page = stride(k, 0) * es;
+    g.v_page = stride(v, 0) * es;
+    g.v = static_cast<uint8_t *>(v.data);
+    g.v_token = stride(v, 1) * es;
+    g.v_head = stride(v, 2) * es;
+    check_value(size(v, 3) <= 1 || stride(v, 3) == 1, "a cache row's head dims must be adjacent");
+    check_value(size(k, 3) <= 1 || stride(k, 3) == 1, "a cache row's head dims must be adjacent");
+  }
+  g.block_size = size(k, -3);
+  g.heads = size(k, -2);
+  g.dim = size(k, -1);
+  g.k_token = stride(k, -3) * es;
+  g.k_head = stride(k, -2) * es;
+  for (int i = 0; i < k.ndim; ++i) check_value(k.strides[i] >= 0, "negative strides unsupported");
+  check_value(g.block_size > 0 && g.heads > 0 && g.dim > 0, "the paged caches hold no rows");
+  // Page numbers and slots are split in 32 bits.
+  check_value(g.pages <= INT32_MAX && g.block_size <= INT32_MAX && g.pages * g.block_size <= static_cast<int64_t>(UINT32_MAX),
+              "paged caches of more than 2^32 slots are not supported");
+  return g;
+}
+
+} // namespace lmc

@@ -41,6 +41,17 @@ using EncodeRowsFn = int (*)(const lmc_tensor *, int32_t, const lmc_tensor *, co
 using PackRowsFn = int (*)(const lmc_tensor *, const lmc_tensor *, const lmc_tensor *, void *);
 using DecodeFn = int (*)(const lmc_tensor *, const lmc_tensor *, const lmc_tensor *, const lmc_tensor *,
                          const lmc_tensor *, void *);
+using SlotMapFn = int (*)(const lmc_tensor *, const lmc_tensor *, const lmc_tensor *, int64_t, const lmc_tensor *,
+                          const lmc_tensor *, const lmc_tensor *, const lmc_tensor *, const lmc_tensor *,
+                          const lmc_tensor *, const lmc_tensor *, void *);
+using RotaryFn = int (*)(const lmc_tensor *, const lmc_tensor *, const lmc_tensor *, int64_t, const double *, int64_t,
+                         double, int32_t, int64_t, int32_t, const lmc_tensor *, const lmc_tensor *, void *);
+using RotaryPagedFn = int (*)(const lmc_tensor *, const lmc_tensor *, const lmc_tensor *, const lmc_tensor *,
+                              const lmc_tensor *, int32_t, const lmc_tensor *, int64_t, const double *, int64_t, double,
+                              int32_t, int64_t, const lmc_tensor *, int32_t, int32_t, void *);
+using PrefixAttnFn = int (*)(const lmc_tensor *, const lmc_tensor *, int32_t, const lmc_tensor *, int64_t,
+                             const lmc_tensor *, const lmc_tensor *, const lmc_tensor *, double, const lmc_tensor *,
+                             const lmc_tensor *, int32_t, int32_t, void *);
 using ErrFn = const char *(*)();
 
 struct Table {
@@ -56,6 +67,10 @@ struct Table {
   EncodeRowsFn encode_rows = nullptr;
   PackRowsFn pack_rows = nullptr;
   DecodeFn decode_chunk = nullptr;
+  SlotMapFn slot_map = nullptr;
+  RotaryFn rotary = nullptr;
+  RotaryPagedFn rotary_paged = nullptr;
+  PrefixAttnFn prefix_attn = nullptr;
   ErrFn last_error = nullptr;
 } g;
 
@@ -283,9 +298,97 @@ at::Tensor cachegen_decode_chunk(const at::Tensor &cdf, const at::Tensor &stream
   return out;
 }
 
+// ---------------------------------------------------------------------------
+// Serving operators
+// ---------------------------------------------------------------------------
+
+// A descriptor of a tensor that may be absent.
+struct Opt {
+  lmc_tensor d{};
+  bool there = false;
+  explicit Opt(const c10::optional<at::Tensor> &t) : there(t.has_value()) {
+    if (there) d = desc(*t);
+  }
+  const lmc_tensor *ptr() const { return there ? &d : nullptr; }
+};
+
+int gpu_of(const at::Tensor &t, const char *name) {
+  if (!t.is_cuda()) throw py::value_error(std::string(name) + " is not on a GPU");
+  return t.get_device();
+}
+
+void build_slot_mapping(const at::Tensor &query_lens, const at::Tensor &context_lens, const at::Tensor &block_table,
+                        int64_t block_size, const at::Tensor &slot_mapping, const c10::optional<at::Tensor> &positions,
+                        const c10::optional<at::Tensor> &query_start_loc, const c10::optional<at::Tensor> &seq_lens,
+                        const c10::optional<at::Tensor> &free_blocks, const c10::optional<at::Tensor> &free_cursor,
+                        const c10::optional<at::Tensor> &next_cursor) {
+  check_bound();
+  const int dev = gpu_of(slot_mapping, "slot_mapping");
+  const lmc_tensor q = desc(query_lens), c = desc(context_lens), b = desc(block_table), s = desc(slot_mapping);
+  const Opt p(positions), l(query_start_loc), n(seq_lens), f(free_blocks), u(free_cursor), v(next_cursor);
+  raise_for(g.slot_map(&q, &c, &b, block_size, &s, p.ptr(), l.ptr(), n.ptr(), f.ptr(), u.ptr(), v.ptr(), stream_of(dev)));
+}
+
+const double *frequencies(const at::Tensor &inv_freq, int dev) {
+  if (inv_freq.scalar_type() != at::kDouble || inv_freq.dim() != 1 || !inv_freq.is_contiguous())
+    throw py::value_error("inv_freq must be a contiguous 1-D float64 tensor");
+  if (!inv_freq.is_cuda() || inv_freq.get_device() != dev)
+    throw py::value_error("inv_freq is not on the GPU of the call's other tensors");
+  return inv_freq.data_ptr<double>();
+}
+
+void rotary_embedding(const at::Tensor &positions, const c10::optional<at::Tensor> &query,
+                      const c10::optional<at::Tensor> &key, int64_t head_size, const at::Tensor &inv_freq, bool is_neox,
+                      int64_t rotary_offset, double scale, bool inverse, const c10::optional<at::Tensor> &query_out,
+                      const c10::optional<at::Tensor> &key_out) {
+  check_bound();
+  if (!query && !key) throw py::value_error("neither query nor key is given");
+  const int dev = gpu_of(query ? *query : *key, query ? "query" : "key");
+  const double *f = frequencies(inv_freq, dev);
+  const lmc_tensor p = desc(positions);
+  const Opt q(query), k(key), qo(query_out), ko(key_out);
+  raise_for(g.rotary(&p, q.ptr(), k.ptr(), head_size, f, inv_freq.size(0), scale, is_neox, rotary_offset, inverse,
+                     qo.ptr(), ko.ptr(), stream_of(dev)));
+}
+
+void rotary_embedding_to_paged(const at::Tensor &positions, const c10::optional<at::Tensor> &query, const at::Tensor &key,
+                               const at::Tensor &value, const py::object &caches_obj, const at::Tensor &slot_mapping,
+                               int64_t head_size, const at::Tensor &inv_freq, bool is_neox, int64_t rotary_offset,
+                               double scale, const c10::optional<at::Tensor> &query_out, int64_t kvcache_format_raw,
+                               bool vllm_two_major) {
+  check_bound();
+  const int dev = gpu_of(key, "key");
+  const double *f = frequencies(inv_freq, dev);
+  const std::vector<at::Tensor> caches = normalize_kv_caches(caches_obj);
+  std::vector<lmc_tensor> cd;
+  for (const auto &c : caches) cd.push_back(desc(c));
+  const lmc_tensor p = desc(positions), k = desc(key), v = desc(value), s = desc(slot_mapping);
+  const Opt q(query), qo(query_out);
+  raise_for(g.rotary_paged(&p, q.ptr(), &k, &v, cd.data(), static_cast<int32_t>(cd.size()), &s, head_size, f,
+                           inv_freq.size(0), scale, is_neox, rotary_offset, qo.ptr(),
+                           static_cast<int32_t>(kvcache_format_raw), vllm_two_major, stream_of(dev)));
+}
+
+void shared_prefix_attention(const at::Tensor &query, const py::object &caches_obj, const at::Tensor &shared_blocks,
+                             int64_t shared_len, const at::Tensor &block_table, const at::Tensor &seq_lens,
+                             const at::Tensor &query_start_loc, double scale, const at::Tensor &output,
+                             const c10::optional<at::Tensor> &lse, int64_t kvcache_format_raw, bool vllm_two_major) {
+  check_bound();
+  const int dev = gpu_of(query, "query");
+  const std::vector<at::Tensor> caches = normalize_kv_caches(caches_obj);
+  std::vector<lmc_tensor> cd;
+  for (const auto &c : caches) cd.push_back(desc(c));
+  const lmc_tensor q = desc(query), b = desc(shared_blocks), t = desc(block_table), n = desc(seq_lens),
+                   l = desc(query_start_loc), o = desc(output);
+  const Opt e(lse);
+  raise_for(g.prefix_attn(&q, cd.data(), static_cast<int32_t>(cd.size()), &b, shared_len, &t, &n, &l, scale, &o, e.ptr(),
+                          static_cast<int32_t>(kvcache_format_raw), vllm_two_major, stream_of(dev)));
+}
+
 void bind(uintptr_t multi, uintptr_t single, uintptr_t load_flash, uintptr_t reshape_flash,
           uintptr_t rope, uintptr_t blend, uintptr_t cdf, uintptr_t encode, uintptr_t decode,
           uintptr_t encode_rows, uintptr_t pack_rows, uintptr_t decode_chunk,
+          uintptr_t slot_map, uintptr_t rotary, uintptr_t rotary_paged, uintptr_t prefix_attn,
           uintptr_t last_error) {
   g.multi = reinterpret_cast<MultiFn>(multi);
   g.single = reinterpret_cast<SingleFn>(single);
@@ -299,6 +402,10 @@ void bind(uintptr_t multi, uintptr_t single, uintptr_t load_flash, uintptr_t res
   g.encode_rows = reinterpret_cast<EncodeRowsFn>(encode_rows);
   g.pack_rows = reinterpret_cast<PackRowsFn>(pack_rows);
   g.decode_chunk = reinterpret_cast<DecodeFn>(decode_chunk);
+  g.slot_map = reinterpret_cast<SlotMapFn>(slot_map);
+  g.rotary = reinterpret_cast<RotaryFn>(rotary);
+  g.rotary_paged = reinterpret_cast<RotaryPagedFn>(rotary_paged);
+  g.prefix_attn = reinterpret_cast<PrefixAttnFn>(prefix_attn);
   g.last_error = reinterpret_cast<ErrFn>(last_error);
 }
 
@@ -322,6 +429,10 @@ PYBIND11_MODULE(_c_ops_ext, m) {
         });
   m.def("rotary_embedding_k_fused", &rotary_embedding_k_fused);
   m.def("blend_layer_to_paged", &blend_layer_to_paged);
+  m.def("build_slot_mapping", &build_slot_mapping);
+  m.def("rotary_embedding", &rotary_embedding);
+  m.def("rotary_embedding_to_paged", &rotary_embedding_to_paged);
+  m.def("shared_prefix_attention", &shared_prefix_attention);
   m.def("calculate_cdf", &calculate_cdf);
   m.def("cachegen_encode_chunk", &cachegen_encode_chunk);
   m.def("cachegen_decode_chunk", &cachegen_decode_chunk);

@@ -93,6 +93,14 @@ SIGNATURES = {
     "lmc_decode_fast_prefsum": [_T, _T, _T, _T, _vp],
     "lmc_cachegen_decode": [_T, _T, _T, _T, _T, _vp],
     "lmc_rotary_embedding_k_fused": [_T, _T, _T, _i64, _T, _i32, _vp],
+    "lmc_build_slot_mapping": [_T, _T, _T, _i64, _T, _T, _T, _T, _T, _T, _T, _vp],
+    "lmc_rotary_embedding": [_T, _T, _T, _i64, _vp, _i64, ctypes.c_double, _i32, _i64, _i32, _T, _T, _vp],
+    "lmc_rotary_embedding_to_paged": [
+        _T, _T, _T, _T, _T, _i32, _T, _i64, _vp, _i64, ctypes.c_double, _i32, _i64, _T, _i32, _i32, _vp,
+    ],
+    "lmc_shared_prefix_attention": [
+        _T, _T, _i32, _T, _i64, _T, _T, _T, ctypes.c_double, _T, _T, _i32, _i32, _vp,
+    ],
     "lmc_get_device_ptr": [_up, _sz, ctypes.POINTER(_up)],
     "lmc_register_mapping": [_up, _up, _sz, ctypes.POINTER(_up)],
     "lmc_unregister_ptr": [_up, ctypes.POINTER(_i32)],

@@ -50,6 +50,10 @@ try:
         _addr("lmc_cachegen_encode_rows"),
         _addr("lmc_cachegen_pack_rows"),
         _addr("lmc_cachegen_decode"),
+        _addr("lmc_build_slot_mapping"),
+        _addr("lmc_rotary_embedding"),
+        _addr("lmc_rotary_embedding_to_paged"),
+        _addr("lmc_shared_prefix_attention"),
         _addr("lmc_last_error"),
     )
 except ImportError:
@@ -574,6 +578,196 @@ def rotary_embedding_k_fused(oldPositions, newPositions, key, headSize, cosSinCa
     _run(
         _L.lmc_rotary_embedding_k_fused(
             _ref(a), _ref(b), _ref(k), int(headSize), _ref(c), int(bool(isNeox)), _stream(dev)
+        )
+    )
+
+
+# ---------------------------------------------------------------------------
+# Serving operators over the same paged caches (no reference counterpart)
+# ---------------------------------------------------------------------------
+
+
+def _opt(t):
+    return None if t is None else _ref(_desc(t))
+
+
+def _gpu_of(t: torch.Tensor, name: str) -> int:
+    if not t.is_cuda:
+        raise ValueError(f"{name} is not on a GPU")
+    return t.device.index
+
+
+def build_slot_mapping(
+    query_lens: torch.Tensor,
+    context_lens: torch.Tensor,
+    block_table: torch.Tensor,
+    block_size: int,
+    slot_mapping: torch.Tensor,
+    positions: Optional[torch.Tensor] = None,
+    query_start_loc: Optional[torch.Tensor] = None,
+    seq_lens: Optional[torch.Tensor] = None,
+    free_blocks: Optional[torch.Tensor] = None,
+    free_cursor: Optional[torch.Tensor] = None,
+    next_cursor: Optional[torch.Tensor] = None,
+) -> None:
+    """The slot mapping that the transfers take, from request lengths on the
+    GPU, in one launch.
+
+    query_lens and context_lens ([R] int32 or int64) are each request's new
+    tokens and those before them, block_table its pages ([R, W] int32, -1
+    where there is none).  Writes slot_mapping ([N] int64: the new tokens of
+    request 0, 1, ...; -1 without a page and behind the last token) and, where
+    given, positions ([N] int64, 0 behind the last token), query_start_loc
+    ([R + 1] int32) and seq_lens ([R] int32, context + query).
+
+    With free_blocks ([F] int32) the pages that the new tokens open are taken
+    from it, in order of requests, from entry free_cursor ([1] int64, 0 if
+    absent) on, and written to block_table; -1 behind its end.  next_cursor
+    ([1] int64, another tensor) gets free_cursor plus the pages asked for: a
+    value over F says that the list was too short.  At most 16384 requests."""
+    if _ext is not None:
+        _ext.build_slot_mapping(query_lens, context_lens, block_table, int(block_size), slot_mapping, positions,
+                                query_start_loc, seq_lens, free_blocks, free_cursor, next_cursor)
+        return
+    dev = _gpu_of(slot_mapping, "slot_mapping")
+    _run(
+        _L.lmc_build_slot_mapping(
+            _opt(query_lens), _opt(context_lens), _opt(block_table), int(block_size), _opt(slot_mapping),
+            _opt(positions), _opt(query_start_loc), _opt(seq_lens), _opt(free_blocks), _opt(free_cursor),
+            _opt(next_cursor), _stream(dev),
+        )
+    )
+
+
+def _frequencies(inv_freq: torch.Tensor, dev: int) -> int:
+    if inv_freq.dtype != torch.float64 or inv_freq.dim() != 1 or not inv_freq.is_contiguous():
+        raise ValueError("inv_freq must be a contiguous 1-D float64 tensor")
+    if not inv_freq.is_cuda or inv_freq.device.index != dev:
+        raise ValueError("inv_freq is not on the GPU of the call's other tensors")
+    return inv_freq.data_ptr()
+
+
+def rotary_embedding(
+    positions: torch.Tensor,
+    query: Optional[torch.Tensor],
+    key: Optional[torch.Tensor],
+    head_size: int,
+    inv_freq: torch.Tensor,
+    is_neox: bool = True,
+    rotary_offset: int = 0,
+    scale: float = 1.0,
+    inverse: bool = False,
+    query_out: Optional[torch.Tensor] = None,
+    key_out: Optional[torch.Tensor] = None,
+) -> None:
+    """Queries and keys turned to their positions, without a cos/sin table.
+
+    The pairs of dims [rotary_offset, rotary_offset + 2 * len(inv_freq)) of
+    each head (halves if is_neox, else interleaved) are turned by
+    positions[t] * inv_freq[i], formed in 64 bits, and multiplied by `scale`;
+    formats.rotary_inv_freq gives inv_freq and scale for the usual context
+    scalings.  query and key are [T, heads * head_size] or [T, heads,
+    head_size] (slices of a fused projection too), bfloat16, float16 or
+    float32; either may be None.  In place, or to query_out / key_out, which
+    get the other dims copied.  inverse turns back by the same angles (scale
+    multiplies there too): the transpose, so the gradient, and for scale 1 the
+    way from positioned keys to position-free ones.  positions ([T] int64 or
+    int32) may be negative: new - old positions re-rotate."""
+    if _ext is not None:
+        _ext.rotary_embedding(positions, query, key, int(head_size), inv_freq, bool(is_neox), int(rotary_offset),
+                              float(scale), bool(inverse), query_out, key_out)
+        return
+    if query is None and key is None:
+        raise ValueError("neither query nor key is given")
+    dev = _gpu_of(key, "key") if query is None else _gpu_of(query, "query")
+    f = _frequencies(inv_freq, dev)
+    _run(
+        _L.lmc_rotary_embedding(
+            _opt(positions), _opt(query), _opt(key), int(head_size), f, inv_freq.numel(), float(scale),
+            int(bool(is_neox)), int(rotary_offset), int(bool(inverse)), _opt(query_out), _opt(key_out), _stream(dev),
+        )
+    )
+
+
+def rotary_embedding_to_paged(
+    positions: torch.Tensor,
+    query: Optional[torch.Tensor],
+    key: torch.Tensor,
+    value: torch.Tensor,
+    vllm_kv_caches,
+    slot_mapping: torch.Tensor,
+    head_size: int,
+    inv_freq: torch.Tensor,
+    is_neox: bool = True,
+    rotary_offset: int = 0,
+    scale: float = 1.0,
+    query_out: Optional[torch.Tensor] = None,
+    kvcache_format_raw: int = 2,
+    vllm_two_major: bool = False,
+) -> None:
+    """rotary_embedding of query (in place or to query_out; may be None) and
+    key, the rotated keys and the values written to one layer's paged caches
+    (MERGED_KV or SEPARATE_KV) at slot_mapping in the same pass.  key and value
+    stay as they are; slots outside the caches, -1 among them, are skipped."""
+    if _ext is not None:
+        _ext.rotary_embedding_to_paged(positions, query, key, value, vllm_kv_caches, slot_mapping, int(head_size),
+                                       inv_freq, bool(is_neox), int(rotary_offset), float(scale), query_out,
+                                       int(kvcache_format_raw), bool(vllm_two_major))
+        return
+    dev = _gpu_of(key, "key")
+    f = _frequencies(inv_freq, dev)
+    caches = _normalize_kv_caches(vllm_kv_caches)
+    _run(
+        _L.lmc_rotary_embedding_to_paged(
+            _opt(positions), _opt(query), _opt(key), _opt(value), _cache_array(caches), len(caches),
+            _opt(slot_mapping), int(head_size), f, inv_freq.numel(), float(scale), int(bool(is_neox)),
+            int(rotary_offset), _opt(query_out), int(kvcache_format_raw), int(bool(vllm_two_major)), _stream(dev),
+        )
+    )
+
+
+def shared_prefix_attention(
+    query: torch.Tensor,
+    vllm_kv_caches,
+    shared_blocks: torch.Tensor,
+    shared_len: int,
+    block_table: torch.Tensor,
+    seq_lens: torch.Tensor,
+    query_start_loc: torch.Tensor,
+    scale: float,
+    output: torch.Tensor,
+    lse: Optional[torch.Tensor] = None,
+    kvcache_format_raw: int = 2,
+    vllm_two_major: bool = False,
+) -> None:
+    """Causal attention of a batch whose requests share their first
+    `shared_len` tokens, over one layer's paged caches: the shared keys are
+    read once for all rows, each request's own behind them.
+
+    query and output are [T, heads, dim], the caches MERGED_KV or SEPARATE_KV
+    with heads dividing the query's, bfloat16 or float16, dim 64, 96, 128, 192
+    or 256.  build_slot_mapping gives query_start_loc ([R + 1] int32) and
+    seq_lens ([R] int32, the new tokens included); a request's i-th of q new
+    tokens sees its first seq_lens[r] - q + i + 1 keys.  Key j is in block
+    shared_blocks[j // block_size] if j < shared_len, else in
+    block_table[r, j // block_size]; shared_len need not end a block.  Keys
+    whose block is outside the caches are unseen, and unseen rows are not
+    used, whatever they hold.  Tokens that see no key (or whose every score is
+    -infinity) get zeros and an lse of -infinity; rows behind the last request
+    are left as they were.  lse ([T, heads] float32): log of the sum of
+    exp(scale * q . k), to join with attention over further keys."""
+    if _ext is not None:
+        _ext.shared_prefix_attention(query, vllm_kv_caches, shared_blocks, int(shared_len), block_table, seq_lens,
+                                     query_start_loc, float(scale), output, lse, int(kvcache_format_raw),
+                                     bool(vllm_two_major))
+        return
+    dev = _gpu_of(query, "query")
+    caches = _normalize_kv_caches(vllm_kv_caches)
+    _run(
+        _L.lmc_shared_prefix_attention(
+            _opt(query), _cache_array(caches), len(caches), _opt(shared_blocks), int(shared_len), _opt(block_table),
+            _opt(seq_lens), _opt(query_start_loc), float(scale), _opt(output), _opt(lse), int(kvcache_format_raw),
+            int(bool(vllm_two_major)), _stream(dev),
         )
     )
 

@@ -30,6 +30,7 @@ upstream defines that format and is absent here.
 
 from __future__ import annotations
 
+import math
 import struct
 from dataclasses import dataclass
 from enum import Enum
@@ -50,6 +51,7 @@ __all__ = [
     "CacheGenChunk",
     "encode_chunk",
     "decode_chunk",
+    "rotary_inv_freq",
 ]
 
 
@@ -219,3 +221,100 @@ def decode_chunk(chunk: CacheGenChunk) -> torch.Tensor:
     if lengths.dtype != torch.int32 or not lengths.is_contiguous():
         lengths = lengths.to(torch.int32).contiguous()
     return c_ops.cachegen_decode_chunk(chunk.cdf, chunk.streams.to(dev), lengths, T)
+
+
+# ---------------------------------------------------------------------------
+# Rotary frequencies
+# ---------------------------------------------------------------------------
+
+
+def rotary_inv_freq(rotary_dim: int, base: float = 10000.0, scaling=None, seq_len: int = 0):
+    """(inv_freq, scale) for c_ops.rotary_embedding: float64 [rotary_dim / 2]
+    radians per position on the CPU, and the factor on cos and sin.
+
+    `scaling` is None or a dict as model configurations hold it, its
+    "rope_type" (or "type") one of
+      default   no scaling
+      linear    positions divided by "factor"
+      dynamic   a base that grows with seq_len past
+                "original_max_position_embeddings", by "factor"
+      yarn      high frequencies kept, low ones divided by "factor", a ramp
+                between "beta_fast" and "beta_slow" turns over the original
+                context; scale 0.1 ln(factor) + 1 unless "attention_factor",
+                or "mscale" and "mscale_all_dim", say otherwise
+      llama3    wavelengths over original / "low_freq_factor" divided by
+                "factor", those under original / "high_freq_factor" kept, a
+                blend between
+      longrope  frequencies divided by "long_factor"[i] where seq_len exceeds
+                the original context, else by "short_factor"[i]; scale
+                sqrt(1 + ln(factor) / ln(original)) unless "attention_factor"
+                says otherwise
+    """
+    if rotary_dim <= 0 or rotary_dim % 2:
+        raise ValueError("rotary_dim must be even and positive")
+    if not base > 0:
+        raise ValueError("base must be positive")
+    exponent = torch.arange(0, rotary_dim, 2, dtype=torch.float64) / rotary_dim
+    inv = float(base) ** -exponent
+    scaling = scaling or {}
+    kind = scaling.get("rope_type", scaling.get("type", "default"))
+    if kind == "default":
+        return inv, 1.0
+
+    def need(name):
+        if scaling.get(name) is None:
+            raise ValueError(f"{kind} scaling needs {name}")
+        return scaling[name]
+
+    if kind == "longrope":
+        original = float(need("original_max_position_embeddings"))
+        factors = torch.tensor(need("long_factor" if seq_len > original else "short_factor"), dtype=torch.float64)
+        if factors.numel() != rotary_dim // 2:
+            raise ValueError("longrope scaling needs one factor per frequency")
+        scale = scaling.get("attention_factor")
+        if scale is None:
+            factor = float(need("factor"))
+            scale = 1.0 if factor <= 1.0 else math.sqrt(1.0 + math.log(factor) / math.log(original))
+        return inv / factors, float(scale)
+
+    factor = float(need("factor"))
+    if factor <= 0:
+        raise ValueError("factor must be positive")
+    if kind == "linear":
+        return inv / factor, 1.0
+    original = float(need("original_max_position_embeddings"))
+    if kind == "dynamic":
+        if rotary_dim <= 2:
+            raise ValueError("dynamic scaling needs more than two rotary dims")
+        n = max(float(seq_len), original)
+        grown = base * (factor * n / original - (factor - 1.0)) ** (rotary_dim / (rotary_dim - 2.0))
+        return grown ** -exponent, 1.0
+    if kind == "llama3":
+        low, high = float(need("low_freq_factor")), float(need("high_freq_factor"))
+        if not high > low:
+            raise ValueError("high_freq_factor must be above low_freq_factor")
+        # Turns over the original context: under `low` scaled, over `high` kept.
+        keep = ((original * inv / (2.0 * math.pi) - low) / (high - low)).clamp(0.0, 1.0)
+        return inv * keep + inv / factor * (1.0 - keep), 1.0
+    if kind == "yarn":
+        fast, slow = float(scaling.get("beta_fast") or 32.0), float(scaling.get("beta_slow") or 1.0)
+
+        def dim_of(turns):
+            return rotary_dim * math.log(original / (turns * 2.0 * math.pi)) / (2.0 * math.log(base))
+
+        first, last = dim_of(fast), dim_of(slow)
+        if scaling.get("truncate", True):
+            first, last = math.floor(first), math.ceil(last)
+        first, last = max(first, 0), min(last, rotary_dim - 1)
+        span = last - first if last != first else 0.001
+        ramp = ((torch.arange(rotary_dim // 2, dtype=torch.float64) - first) / span).clamp(0.0, 1.0)
+
+        def grow(weight):
+            return 1.0 if factor <= 1.0 else 0.1 * weight * math.log(factor) + 1.0
+
+        scale = scaling.get("attention_factor")
+        if scale is None:
+            a, b = scaling.get("mscale"), scaling.get("mscale_all_dim")
+            scale = grow(float(a)) / grow(float(b)) if a and b else grow(1.0)
+        return inv / factor * ramp + inv * (1.0 - ramp), float(scale)
+    raise ValueError(f"unknown rotary scaling {kind!r}")
