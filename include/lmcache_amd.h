@@ -579,13 +579,18 @@ int lmc_rotary_embedding_to_paged(const lmc_tensor *positions, const lmc_tensor 
  * rows of the caches are never used, whatever they hold.  A token that sees
  * no key gets zeros and an lse of -infinity; rows of output and lse behind
  * query_start_loc[R] are left as they were.  lse ([T, heads] fp32, may be
- * null): log of the sum of exp(scale * q . k). */
+ * null): log of the sum of exp(scale * q . k).
+ * The call works in `workspace`, a 1-D uint8 tensor of the GPU on a 16-byte
+ * boundary: with workspace_bytes not null it only writes the size that this
+ * call needs there (0 for a call without rows), from the tensors' sizes
+ * alone.  Calls that may run at the same time take workspaces of their own.
+ * Rows of query, output and the caches start on 16-byte boundaries. */
 int lmc_shared_prefix_attention(const lmc_tensor *query, const lmc_tensor *vllm_kv_caches, int32_t n_caches,
                                 const lmc_tensor *shared_blocks, int64_t shared_len,
                                 const lmc_tensor *block_table, const lmc_tensor *seq_lens,
                                 const lmc_tensor *query_start_loc, double scale, const lmc_tensor *output,
-                                const lmc_tensor *lse, int32_t kvcache_format, int32_t vllm_two_major,
-                                void *stream);
+                                const lmc_tensor *lse, const lmc_tensor *workspace, int64_t *workspace_bytes,
+                                int32_t kvcache_format, int32_t vllm_two_major, void *stream);
 
 /* Replaces get_gpu_pci_bus_id (pybind csrc/pybind.cpp:482): the PCI bus id
  * string of `device`, written NUL-terminated into buf[0..buf_len). */

@@ -16,6 +16,13 @@ namespace lmc {
 
 namespace {
 
+typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
+typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
+typedef float f32x16 __attribute__((ext_vector_type(16)));
+typedef float f32x4 __attribute__((ext_vector_type(4)));
+typedef short s16x4 __attribute__((ext_vector_type(4)));
+typedef short s16x8 __attribute__((ext_vector_type(8)));
+
 struct AttnArgs {
   const void *q;
   int64_t q_token, q_head;  // elements
@@ -23,74 +30,594 @@ struct AttnArgs {
   int64_t o_token, o_head;
   float *lse;               // may be null
   int64_t lse_token, lse_head;
-  PagedKv kv;
+  const uint8_t *k, *v;
+  int64_t k_page, k_token, k_head, v_page, v_token, v_head;  // bytes
+  uint32_t pages, block_size, block_mul, block_shift;
   const int32_t *shared;
-  int64_t shared_len;
+  int shared_len;
   const int32_t *table;
   int64_t table_stride;
-  int64_t width;
+  uint32_t width, shared_width;
   const int32_t *seq_lens, *starts;
-  int n_requests;
-  int64_t n_tokens;
-  int heads, group;
-  float scale;
+  int n_requests, n_tokens;
+  int heads, kv_heads, group;
+  int max_keys;             // that a request can have
+  float scale2;             // scale * log2(e)
+  // Partial results: [parts][tokens * heads] rows of D sums, and (m, l).
+  float *part_o;
+  float2 *part_ml;
+  int prefix_parts, own_parts;
+  int prefix_tiles;         // row tiles of one KV head's rows
+  int prefix_chunk;         // keys of one prefix part
+  int prefix_groups, every; // groups of 8 workgroups, and how they are dealt
+  int own_tiles;            // row tiles of a request dealt to workgroups
+  int own_items;
 };
 
-// One wave per (token, query head): 64 keys a step, a lane a key for the
-// scores and a lane a dim for the sums.
-template <typename T> __global__ void __launch_bounds__(64) attend_rows(AttnArgs a) {
-  using S = typename T::S;
-  const int lane = threadIdx.x, h = blockIdx.y;
-  const int64_t t = blockIdx.x;
-  int r = 0;
-  while (r < a.n_requests && !(t >= a.starts[r] && t < a.starts[r + 1])) ++r;
-  if (r == a.n_requests) return;
-  const int64_t keys = static_cast<int64_t>(a.seq_lens[r]) - a.starts[r + 1] + t + 1;
-  const int D = static_cast<int>(a.kv.dim);
-  const S *q = static_cast<const S *>(a.q) + t * a.q_token + h * a.q_head;
-  const int64_t kh = h / a.group;
-  float m = -INFINITY, l = 0.f, o[4] = {0.f, 0.f, 0.f, 0.f};
-  auto page_of = [&](int64_t j) -> int64_t {
-    const int64_t b = j / a.kv.block_size;
-    if (j >= a.shared_len && b >= a.width) return -1;
-    const int64_t p = j < a.shared_len ? a.shared[b] : a.table[r * a.table_stride + b];
-    return p >= 0 && p < a.kv.pages ? p : -1;
-  };
-  for (int64_t j0 = 0; j0 < keys; j0 += 64) {
-    const int64_t j = j0 + lane;
-    const int64_t page = j < keys ? page_of(j) : -1, at = j % a.kv.block_size;
-    float s = -INFINITY;
-    if (page >= 0) {
-      const S *k = reinterpret_cast<const S *>(a.kv.k + page * a.kv.k_page + at * a.kv.k_token + kh * a.kv.k_head);
-      float x = 0.f;
-      for (int d = 0; d < D; ++d) x += to_f32<T>(q[d]) * to_f32<T>(k[d]);
-      s = x * a.scale;
-    }
-    float top = s;
-    for (int d = 1; d < 64; d <<= 1) top = fmaxf(top, __shfl_xor(top, d));
-    const float m2 = fmaxf(m, top);
-    const float base = m2 == -INFINITY ? 0.f : m2;
-    const float p = page >= 0 ? expf(s - base) : 0.f;
-    const float f = expf(m - base);
-    float sum = p;
-    for (int d = 1; d < 64; d <<= 1) sum += __shfl_xor(sum, d);
-    l = l * f + sum;
-    m = m2;
-    for (int c = 0; c < 4; ++c) o[c] *= f;
-    for (int i = 0; i < 64; ++i) {
-      const float pi = __shfl(p, i);
-      const int64_t pg = __shfl(page, i);
-      if (pg < 0) continue;
-      const int64_t ai = (j0 + i) % a.kv.block_size;
-      const S *v = reinterpret_cast<const S *>(a.kv.v + pg * a.kv.v_page + ai * a.kv.v_token + kh * a.kv.v_head);
-      for (int c = 0; c < 4; ++c)
-        if (lane + 64 * c < D) o[c] += pi * to_f32<T>(v[lane + 64 * c]);
+// Rows of zeros, read in the place of keys that nobody sees.
+__device__ const uint4 zero_row[32] = {};
+
+// MFMA operands of the two types: A rows are keys (or dims of V), B columns
+// are query rows.
+template <typename T> struct Mma;
+template <> struct Mma<BF16> {
+  using V8 = bf16x8;
+  static __device__ __forceinline__ f32x16 mul(V8 a, V8 b, f32x16 c) {
+    return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0);
+  }
+  static __device__ __forceinline__ __bf16 from(float x) { return static_cast<__bf16>(x); }
+  static constexpr uint32_t kInf = 0x7f80;
+};
+template <> struct Mma<F16> {
+  using V8 = f16x8;
+  static __device__ __forceinline__ f32x16 mul(V8 a, V8 b, f32x16 c) {
+    return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0);
+  }
+  static __device__ __forceinline__ _Float16 from(float x) { return static_cast<_Float16>(x); }
+  static constexpr uint32_t kInf = 0x7c00;
+};
+
+// The value of the lane 32 away beside the own one: (lower half's, upper half's).
+__device__ __forceinline__ float2 both_halves(float x) {
+  const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+  return make_float2(__uint_as_float(r[0]), __uint_as_float(r[1]));
+}
+
+// 16 bytes a lane from global memory to LDS at `lds` (uniform) + 16 * lane.
+// No register is written; fence_loads() waits.
+__device__ __forceinline__ void load_to_lds(const void *g, uint32_t lds) {
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off" ::"s"(__builtin_amdgcn_readfirstlane(lds)), "v"(g) : "memory");
+}
+__device__ __forceinline__ void fence_loads() { asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); }
+// LDS reads have their data: what they read may be written again.
+__device__ __forceinline__ void fence_reads() { asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory"); }
+
+typedef __attribute__((address_space(3))) uint8_t LdsByte;
+typedef __attribute__((address_space(3))) s16x4 LdsS4;
+typedef __attribute__((address_space(3))) s16x8 LdsS8;
+
+// Tiles of K and V keep their rows as they are; 16-byte piece c of row r
+// lies at piece c ^ swizzle(r), so that the 16 rows that one read of K
+// touches, and the 4 rows x 64 bytes of a transposed read of V, fall on
+// different banks.
+template <int D> __device__ __forceinline__ constexpr uint32_t k_swizzle(uint32_t r) {
+  return D % 128 == 0 ? r & 15 : D % 64 == 0 ? (r >> 1) & 7 : (r >> 2) & 3;
+}
+template <int D> __device__ __forceinline__ constexpr uint32_t v_swizzle(uint32_t r) {
+  return D % 128 == 0 ? (r & 3) << 2 : D % 64 == 0 ? ((r >> 1) & 1) << 2 : 0;
+}
+
+// One wave's 32 query rows: column n = lane & 31 of S^T and O^T.
+template <typename T, int D> struct Rows32 {
+  typename Mma<T>::V8 q[D / 16];
+  f32x16 o[D / 32];
+  float m, l;   // m in powers of two; l of this lane's keys
+  int limit;    // keys that the row sees; INT_MAX for a row that is none
+  int row;      // token * heads + head, or -1
+};
+
+template <int D> struct Geometry {
+  static constexpr int kPitch = 2 * D;           // bytes of a row
+  static constexpr int kPieces = D / 8;          // 16-byte pieces of a row
+  static constexpr int kLoads = 32 * D * 2 / 1024;  // wave loads of 32 rows
+};
+
+// Adds one tile of NB * 32 keys (in LDS at k, v) to the rows.  MASK: some
+// key of the tile is unseen (bit of `seen` clear, or past a row's limit).
+template <typename T, int D, int NB, bool MASK>
+__device__ __forceinline__ void add_tile(Rows32<T, D> &r, uint32_t k, uint32_t v, int j0, uint64_t seen, bool cut, float c) {
+  using M = Mma<T>;
+  using V8 = typename M::V8;
+  using G = Geometry<D>;
+  const int lane = threadIdx.x & 63, n = lane & 31, hb = lane >> 5;
+  f32x16 s[NB];
+#pragma unroll
+  for (int b = 0; b < NB; ++b)
+#pragma unroll
+    for (int i = 0; i < 16; ++i) s[b][i] = 0.f;
+  const uint32_t krow = k + n * G::kPitch, kx = k_swizzle<D>(n);
+#pragma unroll
+  for (int kc = 0; kc < D / 16; ++kc) {
+    const uint32_t at = krow + (((2 * kc + hb) ^ kx) << 4);
+#pragma unroll
+    for (int b = 0; b < NB; ++b) {
+      const s16x8 a = *reinterpret_cast<const LdsS8 *>(at + b * 32 * G::kPitch);
+      s[b] = M::mul(__builtin_bit_cast(V8, a), r.q[kc], s[b]);
     }
   }
-  S *out = static_cast<S *>(a.o) + t * a.o_token + h * a.o_head;
-  for (int c = 0; c < 4; ++c)
-    if (lane + 64 * c < D) out[lane + 64 * c] = from_f32<T>(l == 0.f ? 0.f : o[c] / l);
-  if (a.lse && lane == 0) a.lse[t * a.lse_token + h * a.lse_head] = m + logf(l);
+  if constexpr (MASK) {
+#pragma unroll
+    for (int b = 0; b < NB; ++b)
+#pragma unroll
+      for (int i = 0; i < 16; ++i) {
+        const int key = 32 * b + 8 * (i / 4) + 4 * hb + i % 4;
+        if (!((seen >> key) & 1) || j0 + key >= r.limit) s[b][i] = -INFINITY;
+      }
+  }
+  float top = s[0][0];
+#pragma unroll
+  for (int b = 0; b < NB; ++b)
+#pragma unroll
+    for (int i = 0; i < 16; ++i) top = fmaxf(top, s[b][i]);
+  const float2 tops = both_halves(top);
+  top = fmaxf(tops.x, tops.y) * c;
+  // The sums keep their reference point until a score passes it by 2^8: the
+  // weights stay below 256, where their relative rounding is the same.
+  if (__any(top > r.m + 8.f)) {
+    const float m = fmaxf(r.m, top);
+    const float f = m == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(r.m - m);
+    r.l *= f;
+#pragma unroll
+    for (int t = 0; t < D / 32; ++t)
+#pragma unroll
+      for (int i = 0; i < 16; ++i) r.o[t][i] *= f;
+    r.m = m;
+  }
+  const float base = r.m == -INFINITY ? 0.f : r.m;
+#pragma unroll
+  for (int b = 0; b < NB; ++b)
+#pragma unroll
+    for (int i = 0; i < 16; ++i) {
+      s[b][i] = __builtin_amdgcn_exp2f(s[b][i] * c - base);
+      r.l += s[b][i];
+    }
+  // O^T += V^T P^T.  The sum over keys may take them in any order: the order
+  // in which a lane holds its 8 of 16 weights, keys 4 hb + {0..3, 8..11}.
+  const int a = lane & 15;
+  const uint32_t vrow = 4 * hb + (a >> 2);
+  const uint32_t vx = v_swizzle<D>(vrow);
+  const uint32_t vcol = 2 * ((lane >> 4) & 1) + ((a & 3) >> 1);
+  const uint32_t vbase = v + vrow * G::kPitch + (a & 1) * 8;
+  bool odd = false;  // this tile's V holds an infinity or NaN that not every row sees
+  if constexpr (MASK) {
+    if (cut) {
+      bool bad = false;
+      for (int i = lane; i < NB * 32 * G::kPieces; i += 64) {
+        const s16x8 x = *reinterpret_cast<const LdsS8 *>(v + i * 16);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) bad |= (static_cast<uint32_t>(x[e]) & M::kInf) == M::kInf;
+      }
+      odd = __any(bad);
+    }
+  }
+#pragma unroll
+  for (int c2 = 0; c2 < 2 * NB; ++c2) {
+    V8 p;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) p[i] = M::from(s[c2 / 2][8 * (c2 & 1) + i]);
+#pragma unroll
+    for (int t = 0; t < D / 32; ++t) {
+      const uint32_t at = vbase + (((4 * t + vcol) ^ vx) << 4) + c2 * 16 * G::kPitch;
+      const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16(reinterpret_cast<LdsS4 *>(at));
+      const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16(reinterpret_cast<LdsS4 *>(at + 8 * G::kPitch));
+      s16x8 x = __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
+      if constexpr (MASK) {
+        if (odd) {
+#pragma unroll
+          for (int e = 0; e < 8; ++e)
+            if ((static_cast<uint32_t>(x[e]) & M::kInf) == M::kInf) x[e] = 0;
+        }
+      }
+      r.o[t] = M::mul(__builtin_bit_cast(V8, x), p, r.o[t]);
+    }
+  }
+  if constexpr (MASK) {
+    // What the product left out: infinities and NaN for the rows that see them.
+    if (odd) {
+      for (int key = 0; key < NB * 32; ++key) {
+        const bool see = ((seen >> key) & 1) && j0 + key < r.limit;
+#pragma unroll
+        for (int t = 0; t < D / 32; ++t)
+#pragma unroll
+          for (int i = 0; i < 16; ++i) {
+            const uint32_t d = 32 * t + 8 * (i / 4) + 4 * hb + i % 4;
+            const uint32_t at = v + key * G::kPitch + (((d >> 3) ^ v_swizzle<D>(key)) << 4) + (d & 7) * 2;
+            const uint16_t x = *reinterpret_cast<const __attribute__((address_space(3))) uint16_t *>(at);
+            if (see && (x & M::kInf) == M::kInf) r.o[t][i] += to_f32<T>(x);
+          }
+      }
+    }
+  }
+}
+
+// The keys [k0, k1) of one list of blocks, a tile at a time: where a wave's
+// lanes find the rows they load.
+template <int D, int KEYS> struct KeyTiles {
+  const AttnArgs &a;
+  const int32_t *list;
+  uint32_t n_list;
+  int k0, k1;
+  int64_t k_off, v_off;  // of the KV head
+  int page;              // of key `lane` of the next tile, loaded ahead
+
+  __device__ __forceinline__ int key(int j0) const { return j0 + ((threadIdx.x & 63) & (KEYS - 1)); }
+  __device__ __forceinline__ uint32_t block_of(int j) const {
+    return a.block_size == 1 ? j : __umulhi(j, a.block_mul) >> a.block_shift;
+  }
+  __device__ __forceinline__ void fetch(int j0) {
+    const int j = key(j0);
+    page = -1;
+    if (j < k1) {
+      const uint32_t b = block_of(j);
+      if (b < n_list) page = list[b];
+    }
+  }
+  // Row addresses of the fetched tile (a lane a key), and which keys exist.
+  __device__ __forceinline__ uint64_t rows(int j0, const uint8_t *&k, const uint8_t *&v) const {
+    const int j = key(j0);
+    const bool there = static_cast<uint32_t>(page) < a.pages;
+    const uint32_t at = j - block_of(j) * a.block_size;
+    const uint8_t *z = reinterpret_cast<const uint8_t *>(zero_row);
+    k = there ? a.k + k_off + page * a.k_page + at * a.k_token : z;
+    v = there ? a.v + v_off + page * a.v_page + at * a.v_token : z;
+    const uint64_t seen = __ballot(there);
+    return KEYS == 64 ? seen : seen & 0xffffffffu;
+  }
+};
+
+__device__ __forceinline__ const uint8_t *from_lane(const uint8_t *p, int lane) {
+  const uint64_t x = reinterpret_cast<uint64_t>(p);
+  const uint32_t lo = __builtin_amdgcn_ds_bpermute(lane * 4, static_cast<int>(x));
+  const uint32_t hi = __builtin_amdgcn_ds_bpermute(lane * 4, static_cast<int>(x >> 32));
+  return reinterpret_cast<const uint8_t *>((static_cast<uint64_t>(hi) << 32) | lo);
+}
+
+// This wave's share (loads w, w + step, ...) of a tile of `rows` key rows.
+template <int D, int ROWS, bool V>
+__device__ __forceinline__ void load_tile(const uint8_t *row, uint32_t lds, int w, int step) {
+  using G = Geometry<D>;
+  const int lane = threadIdx.x & 63;
+#pragma unroll
+  for (int i0 = 0; i0 < ROWS / 32 * G::kLoads; i0 += step) {
+    const int i = i0 + w;
+    const int x = i * 64 + lane, key = x / G::kPieces, at = x % G::kPieces;
+    const uint32_t piece = at ^ (V ? v_swizzle<D>(key) : k_swizzle<D>(key));
+    load_to_lds(from_lane(row, key) + piece * 16, lds + i * 1024);
+  }
+}
+
+// Whether a tile has to be masked row by row, and whether a row ends in it.
+template <typename T, int D> __device__ __forceinline__ bool ends_before(const Rows32<T, D> &r, int j1) {
+  return __any(r.limit < j1);
+}
+
+template <typename T, int D, int NB>
+__device__ __forceinline__ void add_any_tile(Rows32<T, D> &r, uint32_t k, uint32_t v, int j0, int k1, uint64_t seen, float c) {
+  constexpr uint64_t kAll = NB == 2 ? ~uint64_t(0) : 0xffffffffu;
+  const bool cut = ends_before<T, D>(r, min(j0 + 32 * NB, k1));
+  if (cut || seen != kAll) add_tile<T, D, NB, true>(r, k, v, j0, seen, cut, c);
+  else add_tile<T, D, NB, false>(r, k, v, j0, seen, false, c);
+}
+
+// Query rows to registers: row n of `m` (head-local row numbers).
+template <typename T, int D> __device__ __forceinline__ void load_rows(const AttnArgs &a, Rows32<T, D> &r, int t, int head, int limit) {
+  using S = typename T::S;
+  const int hb = (threadIdx.x & 63) >> 5;
+  const bool there = t >= 0;
+  r.row = there ? t * a.heads + head : -1;
+  r.limit = there && limit > 0 ? limit : INT32_MAX;
+  const S *q = static_cast<const S *>(a.q) + (there ? t * a.q_token + head * a.q_head : 0);
+#pragma unroll
+  for (int kc = 0; kc < D / 16; ++kc) {
+    s16x8 x = {0, 0, 0, 0, 0, 0, 0, 0};
+    if (there) x = *reinterpret_cast<const s16x8 *>(q + kc * 16 + hb * 8);
+    r.q[kc] = __builtin_bit_cast(typename Mma<T>::V8, x);
+  }
+#pragma unroll
+  for (int i = 0; i < D / 32; ++i)
+#pragma unroll
+    for (int e = 0; e < 16; ++e) r.o[i][e] = 0.f;
+  r.m = -INFINITY;
+  r.l = 0.f;
+}
+
+template <int D> struct Lds {
+  static constexpr int kNarrow = 4 * 2 * 32 * D * 2;       // a tile of 32 keys a wave
+  static constexpr int kWide = 2 * 2 * 64 * D * 2;         // two tiles of 64 keys
+  static constexpr int kSums = 4 * D * 33 * 4 + 4 * 32 * 8;  // O^T of four waves, and (m, l)
+  static constexpr int kBytes = kNarrow > kSums ? (kNarrow > kWide ? kNarrow : kWide) : (kSums > kWide ? kSums : kWide);
+};
+
+// The four waves' sums to their part.  MERGE: the waves hold the same 32
+// rows over different keys.  A row whose limit is 0 or less gets nothing.
+template <typename T, int D, bool MERGE>
+__device__ __forceinline__ void store_part(const AttnArgs &a, const Rows32<T, D> &r, bool dead, int part, uint8_t *lds) {
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, n = lane & 31, hb = lane >> 5;
+  float *sums = reinterpret_cast<float *>(lds);
+  float2 *ml = reinterpret_cast<float2 *>(lds + 4 * D * 33 * 4);
+  const float2 ls = both_halves(r.l);
+  __syncthreads();
+  float *own = sums + wave * D * 33;
+#pragma unroll
+  for (int t = 0; t < D / 32; ++t)
+#pragma unroll
+    for (int i = 0; i < 16; ++i) own[(32 * t + 8 * (i / 4) + 4 * hb + i % 4) * 33 + n] = r.o[t][i];
+  if (hb == 0) ml[wave * 32 + n] = dead ? make_float2(-INFINITY, 0.f) : make_float2(r.m, ls.x + ls.y);
+  __syncthreads();
+  const int64_t rows = static_cast<int64_t>(a.n_tokens) * a.heads;
+  constexpr int kQuads = D / 4;
+  if constexpr (MERGE) {
+    for (int x = threadIdx.x; x < 32 * kQuads; x += 256) {
+      const int i = x / kQuads, d = x % kQuads * 4;
+      const int row = __builtin_amdgcn_ds_bpermute(i * 4, r.row);
+      if (row < 0) continue;
+      float2 w[4];
+      float top = -INFINITY;
+#pragma unroll
+      for (int g = 0; g < 4; ++g) {
+        w[g] = ml[g * 32 + i];
+        top = fmaxf(top, w[g].x);
+      }
+      const float base = top == -INFINITY ? 0.f : top;
+      float l = 0.f;
+      f32x4 o = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int g = 0; g < 4; ++g) {
+        if (w[g].y == 0.f) continue;
+        const float f = __builtin_amdgcn_exp2f(w[g].x - base);
+        l += f * w[g].y;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) o[e] += f * sums[(g * D + d + e) * 33 + i];
+      }
+      if (d == 0) a.part_ml[part * rows + row] = make_float2(top, l);
+      if (l != 0.f) *reinterpret_cast<f32x4 *>(a.part_o + (part * rows + row) * D + d) = o;
+    }
+  } else {
+    for (int x = lane; x < 32 * kQuads; x += 64) {
+      const int i = x / kQuads, d = x % kQuads * 4;
+      const int row = __builtin_amdgcn_ds_bpermute(i * 4, r.row);
+      if (row < 0) continue;
+      const float2 w = ml[wave * 32 + i];
+      f32x4 o;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) o[e] = own[(d + e) * 33 + i];
+      if (d == 0) a.part_ml[part * rows + row] = w;
+      if (w.y != 0.f) *reinterpret_cast<f32x4 *>(a.part_o + (part * rows + row) * D + d) = o;
+    }
+  }
+}
+
+// Four waves, the same 32 rows, a quarter of the tiles each in LDS of its
+// own: few rows, bound by the bytes of K and V.
+template <typename T, int D>
+__device__ __forceinline__ void attend_narrow(const AttnArgs &a, Rows32<T, D> &r, KeyTiles<D, 32> &tiles, uint32_t lds) {
+  const int wave = threadIdx.x >> 6;
+  const uint32_t k = lds + wave * (2 * 32 * D * 2), v = k + 32 * D * 2;
+  int j0 = tiles.k0 + 32 * wave;
+  if (j0 >= tiles.k1) return;
+  const uint8_t *kr, *vr;
+  tiles.fetch(j0);
+  uint64_t seen = tiles.rows(j0, kr, vr);
+  load_tile<D, 32, false>(kr, k, 0, 1);
+  load_tile<D, 32, true>(vr, v, 0, 1);
+  tiles.fetch(j0 + 128);
+  for (; j0 < tiles.k1; j0 += 128) {
+    fence_loads();
+    add_any_tile<T, D, 1>(r, k, v, j0, tiles.k1, seen, a.scale2);
+    if (j0 + 128 < tiles.k1) {
+      seen = tiles.rows(j0 + 128, kr, vr);
+      fence_reads();
+      load_tile<D, 32, false>(kr, k, 0, 1);
+      load_tile<D, 32, true>(vr, v, 0, 1);
+      tiles.fetch(j0 + 256);
+    }
+  }
+}
+
+// Four waves of 32 rows each over tiles of 64 keys that they share: many
+// rows, bound by the matrix cores.
+template <typename T, int D>
+__device__ __forceinline__ void attend_wide(const AttnArgs &a, Rows32<T, D> &r, KeyTiles<D, 64> &tiles, uint32_t lds) {
+  const int wave = threadIdx.x >> 6;
+  constexpr uint32_t kTile = 64 * D * 2;
+  int j0 = tiles.k0;
+  const uint8_t *kr, *vr;
+  tiles.fetch(j0);
+  uint64_t seen = tiles.rows(j0, kr, vr);
+  load_tile<D, 64, false>(kr, lds, wave, 4);
+  load_tile<D, 64, true>(vr, lds + kTile, wave, 4);
+  tiles.fetch(j0 + 64);
+  for (int stage = 0; j0 < tiles.k1; j0 += 64, stage ^= 1) {
+    fence_loads();
+    __syncthreads();
+    const uint64_t now = seen;
+    if (j0 + 64 < tiles.k1) {
+      const uint32_t to = lds + (stage ^ 1) * 2 * kTile;
+      seen = tiles.rows(j0 + 64, kr, vr);
+      load_tile<D, 64, false>(kr, to, wave, 4);
+      load_tile<D, 64, true>(vr, to + kTile, wave, 4);
+      tiles.fetch(j0 + 128);
+    }
+    const uint32_t at = lds + stage * 2 * kTile;
+    add_any_tile<T, D, 2>(r, at, at + kTile, j0, tiles.k1, now, a.scale2);
+  }
+}
+
+// The request of token t, or -1: the number of requests that start at or
+// before it, less one.
+__device__ __forceinline__ int request_of(const AttnArgs &a, int t) {
+  const int R = a.n_requests;
+  int r = min(t, R - 1);  // one token a request, the usual case
+  if (!(a.starts[r] <= t && t < a.starts[r + 1])) {
+    int lo = 0, hi = R;   // the first of 0 .. R whose start lies behind t
+    while (lo < hi) {
+      const int mid = (lo + hi) >> 1;
+      if (a.starts[mid] > t) hi = mid;
+      else lo = mid + 1;
+    }
+    r = lo - 1;
+    if (r < 0 || r >= R || a.starts[R] <= t) return -1;
+  }
+  return r;
+}
+
+// Keys that token t of request r sees; there are none behind the table's row.
+__device__ __forceinline__ int limit_of(const AttnArgs &a, int r, int t) {
+  const int64_t n = static_cast<int64_t>(a.seq_lens[r]) - a.starts[r + 1] + t + 1;
+  return static_cast<int>(max(static_cast<int64_t>(0), min(n, static_cast<int64_t>(a.max_keys))));
+}
+
+// Groups of 8 consecutive workgroups (one an XCD) take prefix work, every
+// `every`-th of them, or the requests' own keys.  The row tiles of one (KV
+// head, prefix part) go to one XCD, whose L2 then holds that part.
+template <typename T, int D, bool WIDE> __global__ void __launch_bounds__(256, D > 128 ? 1 : 2) attend(AttnArgs a) {
+  extern __shared__ uint8_t lds[];
+  const uint32_t at = static_cast<uint32_t>(reinterpret_cast<uintptr_t>((__attribute__((address_space(3))) uint8_t *)lds));
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, n = lane & 31;
+  const int group = blockIdx.x / 8, xcd = blockIdx.x % 8;
+  const int before = min(a.prefix_groups, (group + a.every - 1) / a.every);  // prefix groups before this one
+  Rows32<T, D> r;
+  if (group % a.every == 0 && group / a.every < a.prefix_groups) {
+    const int k = group / a.every;
+    const int pair = k / a.prefix_tiles * 8 + xcd, tile = k % a.prefix_tiles;
+    if (pair >= a.kv_heads * a.prefix_parts) return;
+    const int h = pair % a.kv_heads, part = pair / a.kv_heads;
+    const int x = tile * (WIDE ? 128 : 32) + (WIDE ? wave * 32 : 0) + n;
+    int t = x < a.n_tokens * a.group ? x / a.group : -1, limit = 0;
+    if (t >= 0) {
+      const int q = request_of(a, t);
+      if (q < 0) t = -1;
+      else limit = limit_of(a, q, t);
+    }
+    load_rows<T, D>(a, r, t, h * a.group + (t < 0 ? 0 : x % a.group), limit);
+    KeyTiles<D, WIDE ? 64 : 32> tiles{a, a.shared, a.shared_width, part * a.prefix_chunk,
+                                      min(a.shared_len, (part + 1) * a.prefix_chunk), h * a.k_head, h * a.v_head, -1};
+    if constexpr (WIDE) attend_wide<T, D>(a, r, tiles, at);
+    else attend_narrow<T, D>(a, r, tiles, at);
+    store_part<T, D, !WIDE>(a, r, limit <= 0, part, lds);
+    return;
+  }
+  // A request's own keys.
+  const int item = (group - before) * 8 + xcd;
+  if (item >= a.own_items) return;
+  const int h = item % a.kv_heads, y = item / a.kv_heads;
+  const int part = y % a.own_parts, z = y / a.own_parts;
+  const int first = z % a.own_tiles, q = z / a.own_tiles;
+  const int t0 = max(0, a.starts[q]), t1 = min(a.n_tokens, a.starts[q + 1]);
+  const int n_rows = max(0, t1 - t0) * a.group;
+  const int end = t1 > t0 ? limit_of(a, q, t1 - 1) : 0;
+  // The part's keys, whole rounds of the four waves' tiles.
+  const int own = max(0, end - a.shared_len);
+  const int chunk = ((own + a.own_parts - 1) / a.own_parts + 127) / 128 * 128;
+  const int k0 = a.shared_len + min(own, part * chunk), k1 = a.shared_len + min(own, (part + 1) * chunk);
+  for (int m = first * 32; m < n_rows; m += a.own_tiles * 32) {
+    const int x = m + n;
+    const int t = x < n_rows ? t0 + x / a.group : -1;
+    const int limit = t >= 0 ? limit_of(a, q, t) : 0;
+    load_rows<T, D>(a, r, t, h * a.group + (t < 0 ? 0 : x % a.group), limit);
+    KeyTiles<D, 32> tiles{a, a.table + q * a.table_stride, a.width, k0, k1, h * a.k_head, h * a.v_head, -1};
+    attend_narrow<T, D>(a, r, tiles, at);
+    store_part<T, D, true>(a, r, limit <= 0, a.prefix_parts + part, lds);
+    __syncthreads();
+  }
+}
+
+// Joins a row's parts.
+template <typename T, int D> __global__ void __launch_bounds__(256) join_parts(AttnArgs a) {
+  constexpr int kQuads = D / 4, kRows = 256 / kQuads;
+  using S = typename T::S;
+  const int64_t rows = static_cast<int64_t>(a.n_tokens) * a.heads;
+  const int64_t row = static_cast<int64_t>(blockIdx.x) * kRows + threadIdx.x / kQuads;
+  if (threadIdx.x / kQuads >= kRows || row >= rows) return;
+  const int t = static_cast<int>(row / a.heads), h = static_cast<int>(row % a.heads), d = threadIdx.x % kQuads * 4;
+  if (t < a.starts[0] || t >= a.starts[a.n_requests]) return;
+  const int parts = a.prefix_parts + a.own_parts;
+  float top = -INFINITY;
+  for (int p = 0; p < parts; ++p) top = fmaxf(top, a.part_ml[p * rows + row].x);
+  const float base = top == -INFINITY ? 0.f : top;
+  float l = 0.f;
+  f32x4 o = {0.f, 0.f, 0.f, 0.f};
+  for (int p = 0; p < parts; ++p) {
+    const float2 w = a.part_ml[p * rows + row];
+    if (w.y == 0.f) continue;
+    const float f = __builtin_amdgcn_exp2f(w.x - base);
+    l += f * w.y;
+    const f32x4 x = *reinterpret_cast<const f32x4 *>(a.part_o + (p * rows + row) * D + d);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) o[e] += f * x[e];
+  }
+  const float inv = l == 0.f ? 0.f : 1.f / l;
+  Pack<S, 4> y;
+#pragma unroll
+  for (int e = 0; e < 4; ++e) y.v[e] = from_f32<T>(o[e] * inv);
+  *reinterpret_cast<Pack<S, 4> *>(static_cast<S *>(a.o) + t * a.o_token + h * a.o_head + d) = y;
+  if (a.lse && d == 0) a.lse[t * a.lse_token + h * a.lse_head] = l == 0.f ? -INFINITY : (base + log2f(l)) * 0.69314718056f;
+}
+
+template <typename T, int D> void launch(const AttnArgs &a, bool wide, uint32_t groups, hipStream_t s) {
+  const void *fn = wide ? reinterpret_cast<const void *>(attend<T, D, true>) : reinterpret_cast<const void *>(attend<T, D, false>);
+  hip_check(hipFuncSetAttribute(fn, hipFuncAttributeMaxDynamicSharedMemorySize, Lds<D>::kBytes), "attend shared memory");
+  if (wide) hipLaunchKernelGGL((attend<T, D, true>), dim3(groups * 8), dim3(256), Lds<D>::kBytes, s, a);
+  else hipLaunchKernelGGL((attend<T, D, false>), dim3(groups * 8), dim3(256), Lds<D>::kBytes, s, a);
+  hip_check(hipGetLastError(), "attend launch");
+  constexpr int kRows = 256 / (D / 4);
+  const int64_t rows = static_cast<int64_t>(a.n_tokens) * a.heads;
+  hipLaunchKernelGGL((join_parts<T, D>), dim3(static_cast<uint32_t>((rows + kRows - 1) / kRows)), dim3(256), 0, s, a);
+  hip_check(hipGetLastError(), "join_parts launch");
+}
+
+template <typename T> void launch_dim(const AttnArgs &a, int64_t dim, bool wide, uint32_t groups, hipStream_t s) {
+  switch (dim) {
+  case 64: launch<T, 64>(a, wide, groups, s); break;
+  case 96: launch<T, 96>(a, wide, groups, s); break;
+  case 128: launch<T, 128>(a, wide, groups, s); break;
+  case 192: launch<T, 192>(a, wide, groups, s); break;
+  default: launch<T, 256>(a, wide, groups, s); break;
+  }
+}
+
+// Key numbers and what is added to them stay far from 2^31.
+constexpr int64_t kMaxKeys = int64_t(1) << 30;
+
+// How a call's work is cut, from its sizes alone (the lengths are on the GPU).
+struct Plan {
+  bool wide;
+  int prefix_tiles, prefix_parts, prefix_chunk;
+  int own_tiles, own_parts;
+};
+
+Plan make_plan(int64_t T, int64_t R, int64_t kv_heads, int64_t group, int64_t shared_len, int64_t table_keys) {
+  Plan p;
+  const int64_t rows = T * group;  // of a KV head
+  p.wide = rows > 64;
+  const int64_t m = p.wide ? 128 : 32, tile = p.wide ? 64 : 128;
+  p.prefix_tiles = static_cast<int>((rows + m - 1) / m);
+  // Workgroups for two of a CU, parts of at least one round of tiles each.
+  const int64_t items = p.prefix_tiles * kv_heads;
+  const int64_t most = std::max<int64_t>(1, (shared_len + 2 * tile - 1) / (2 * tile));
+  p.prefix_parts = shared_len == 0 ? 0 : static_cast<int>(std::min<int64_t>(most, std::max<int64_t>(1, 512 / items)));
+  p.prefix_chunk = 0;
+  if (p.prefix_parts) {
+    p.prefix_chunk = static_cast<int>(((shared_len + p.prefix_parts - 1) / p.prefix_parts + tile - 1) / tile * tile);
+    p.prefix_parts = static_cast<int>((shared_len + p.prefix_chunk - 1) / p.prefix_chunk);
+  }
+  const int64_t per = (T + R - 1) / R * group;  // rows of a request, about
+  p.own_tiles = static_cast<int>(std::max<int64_t>(1, (per + 31) / 32));
+  const int64_t own = std::max<int64_t>(0, table_keys - shared_len);
+  const int64_t own_items = R * kv_heads * p.own_tiles;
+  const int64_t own_most = std::max<int64_t>(1, (own + 255) / 256);
+  p.own_parts = static_cast<int>(std::min<int64_t>(own_most, std::max<int64_t>(1, 512 / own_items)));
+  return p;
 }
 
 } // namespace
@@ -103,8 +630,8 @@ extern "C" int lmc_shared_prefix_attention(const lmc_tensor *query, const lmc_te
                                            const lmc_tensor *shared_blocks, int64_t shared_len,
                                            const lmc_tensor *block_table, const lmc_tensor *seq_lens,
                                            const lmc_tensor *query_start_loc, double scale, const lmc_tensor *output,
-                                           const lmc_tensor *lse, int32_t kvcache_format, int32_t vllm_two_major,
-                                           void *stream) {
+                                           const lmc_tensor *lse, const lmc_tensor *workspace, int64_t *workspace_bytes,
+                                           int32_t kvcache_format, int32_t vllm_two_major, void *stream) {
   return guarded([&] {
     const lmc_tensor &q = deref(query, "query");
     const lmc_tensor &o = deref(output, "output");
@@ -136,7 +663,8 @@ extern "C" int lmc_shared_prefix_attention(const lmc_tensor *query, const lmc_te
     check_value(qs.sizes[0] == R + 1, "query_start_loc must have one entry per request and one more");
     check_value(bt.ndim == 2 && bt.sizes[0] == R, "block_table must be [requests, pages]");
     check_value(bt.sizes[1] <= 1 || bt.strides[1] == 1, "block_table rows must be contiguous");
-    check_value(shared_len >= 0 && shared_len <= INT32_MAX, "shared_len must be between 0 and 2^31 - 1");
+    check_value(shared_len >= 0 && shared_len <= kMaxKeys, "shared_len must be between 0 and 2^30");
+    check_value(bt.sizes[1] * kv.block_size <= kMaxKeys, "a block_table row spans more than 2^30 keys");
     check_value((shared_len + kv.block_size - 1) / kv.block_size <= sb.sizes[0], "shared_blocks has too few blocks for shared_len");
     check_value(scale > 0 && std::isfinite(scale), "scale must be positive and finite");
     AttnArgs a;
@@ -149,31 +677,87 @@ extern "C" int lmc_shared_prefix_attention(const lmc_tensor *query, const lmc_te
       a.lse_token = e.strides[0];
       a.lse_head = e.strides[1];
     }
+    auto on_16 = [](int64_t x) { return x % 16 == 0; };
+    check_value(on_16(reinterpret_cast<intptr_t>(kv.k)) && on_16(reinterpret_cast<intptr_t>(kv.v)) && on_16(kv.k_page) &&
+                    on_16(kv.k_token) && on_16(kv.k_head) && on_16(kv.v_page) && on_16(kv.v_token) && on_16(kv.v_head),
+                "the paged caches' rows must start on 16-byte boundaries");
+    check_value(on_16(reinterpret_cast<intptr_t>(q.data)) && on_16(q.strides[0] * 2) && on_16(q.strides[1] * 2) &&
+                    on_16(reinterpret_cast<intptr_t>(o.data)) && on_16(o.strides[0] * 2) && on_16(o.strides[1] * 2),
+                "rows of query and output must start on 16-byte boundaries");
+    check_value(rows_apart({T, Hq, kv.dim}, {o.strides[0], o.strides[1], 1}), "output has overlapping rows");
+    check_value(T * Hq <= INT32_MAX / 128 && R <= INT32_MAX / 4096, "too many rows");
+    const int64_t group = kv.heads ? Hq / kv.heads : 0;
+    if (workspace_bytes) *workspace_bytes = 0;
     if (T == 0 || Hq == 0 || R == 0) return;
+    const int64_t keys = bt.sizes[1] * kv.block_size;
+    const Plan p = make_plan(T, R, kv.heads, group, shared_len, keys);
+    const int64_t parts = p.prefix_parts + p.own_parts, rows = T * Hq;
+    const int64_t bytes = parts * rows * (kv.dim * 4 + 8);
+    if (workspace_bytes) {
+      *workspace_bytes = bytes;
+      return;
+    }
+    const lmc_tensor &ws = deref(workspace, "workspace");
+    check_on(ws, "workspace", dev, LMC_U8);
+    check_value(ws.ndim == 1 && (ws.sizes[0] <= 1 || ws.strides[0] == 1) && ws.sizes[0] >= bytes &&
+                    on_16(reinterpret_cast<intptr_t>(ws.data)),
+                "workspace must be 1-D, contiguous, on a 16-byte boundary and of at least " + std::to_string(bytes) + " bytes");
     a.q = q.data;
     a.q_token = q.strides[0];
     a.q_head = q.strides[1];
     a.o = o.data;
     a.o_token = o.strides[0];
     a.o_head = o.strides[1];
-    a.kv = kv;
+    a.k = kv.k;
+    a.v = kv.v;
+    a.k_page = kv.k_page;
+    a.k_token = kv.k_token;
+    a.k_head = kv.k_head;
+    a.v_page = kv.v_page;
+    a.v_token = kv.v_token;
+    a.v_head = kv.v_head;
+    a.pages = static_cast<uint32_t>(kv.pages);
+    // j / block_size = umulhi(j, mul) >> shift for j < 2^31 (block_size > 1).
+    a.block_size = static_cast<uint32_t>(kv.block_size);
+    if (kv.block_size > 1) {
+      uint32_t log = 1;
+      while ((int64_t(1) << log) < kv.block_size) ++log;
+      a.block_mul = static_cast<uint32_t>((uint64_t(1) << (31 + log)) / kv.block_size + 1);
+      a.block_shift = log - 1;
+    }
     a.shared = static_cast<const int32_t *>(sb.data);
-    a.shared_len = shared_len;
+    a.shared_len = static_cast<int>(shared_len);
+    a.shared_width = static_cast<uint32_t>(sb.sizes[0]);
     a.table = static_cast<const int32_t *>(bt.data);
     a.table_stride = bt.strides[0];
-    a.width = bt.sizes[1];
+    a.width = static_cast<uint32_t>(bt.sizes[1]);
     a.seq_lens = static_cast<const int32_t *>(sl.data);
     a.starts = static_cast<const int32_t *>(qs.data);
     a.n_requests = static_cast<int>(R);
-    a.n_tokens = T;
+    a.n_tokens = static_cast<int>(T);
     a.heads = static_cast<int>(Hq);
-    a.group = static_cast<int>(Hq / kv.heads);
-    a.scale = static_cast<float>(scale);
+    a.kv_heads = static_cast<int>(kv.heads);
+    a.group = static_cast<int>(group);
+    a.max_keys = static_cast<int>(std::max(shared_len, keys));
+    a.scale2 = static_cast<float>(scale * 1.4426950408889634);
+    a.part_o = static_cast<float *>(ws.data);
+    a.part_ml = reinterpret_cast<float2 *>(a.part_o + parts * rows * kv.dim);
+    a.prefix_parts = p.prefix_parts;
+    a.own_parts = p.own_parts;
+    a.prefix_tiles = p.prefix_tiles;
+    a.prefix_chunk = p.prefix_chunk;
+    a.own_tiles = p.own_tiles;
+    const int64_t own_items = R * kv.heads * p.own_tiles * p.own_parts;
+    check_value(own_items <= INT32_MAX / 2, "too many rows");
+    a.own_items = static_cast<int>(own_items);
+    const int64_t own_groups = (own_items + 7) / 8;
+    const int64_t prefix_groups = (kv.heads * p.prefix_parts + 7) / 8 * p.prefix_tiles;
+    a.prefix_groups = static_cast<int>(prefix_groups);
+    a.every = prefix_groups ? static_cast<int>((own_groups + prefix_groups) / prefix_groups) : 1;
     DeviceGuard guard(dev);
-    const dim3 grid(static_cast<uint32_t>(T), static_cast<uint32_t>(Hq));
     const hipStream_t s = static_cast<hipStream_t>(stream);
-    if (kv.dtype == LMC_BF16) hipLaunchKernelGGL(attend_rows<BF16>, grid, dim3(64), 0, s, a);
-    else hipLaunchKernelGGL(attend_rows<F16>, grid, dim3(64), 0, s, a);
-    hip_check(hipGetLastError(), "attend_rows launch");
+    const uint32_t groups = static_cast<uint32_t>(own_groups + prefix_groups);
+    if (kv.dtype == LMC_BF16) launch_dim<BF16>(a, kv.dim, p.wide, groups, s);
+    else launch_dim<F16>(a, kv.dim, p.wide, groups, s);
   });
 }

@@ -51,7 +51,7 @@ using RotaryPagedFn = int (*)(const lmc_tensor *, const lmc_tensor *, const lmc_
                               int32_t, int64_t, const lmc_tensor *, int32_t, int32_t, void *);
 using PrefixAttnFn = int (*)(const lmc_tensor *, const lmc_tensor *, int32_t, const lmc_tensor *, int64_t,
                              const lmc_tensor *, const lmc_tensor *, const lmc_tensor *, double, const lmc_tensor *,
-                             const lmc_tensor *, int32_t, int32_t, void *);
+                             const lmc_tensor *, const lmc_tensor *, int64_t *, int32_t, int32_t, void *);
 using ErrFn = const char *(*)();
 
 struct Table {
@@ -381,8 +381,17 @@ void shared_prefix_attention(const at::Tensor &query, const py::object &caches_o
   const lmc_tensor q = desc(query), b = desc(shared_blocks), t = desc(block_table), n = desc(seq_lens),
                    l = desc(query_start_loc), o = desc(output);
   const Opt e(lse);
-  raise_for(g.prefix_attn(&q, cd.data(), static_cast<int32_t>(cd.size()), &b, shared_len, &t, &n, &l, scale, &o, e.ptr(),
-                          static_cast<int32_t>(kvcache_format_raw), vllm_two_major, stream_of(dev)));
+  auto call = [&](const lmc_tensor *w, int64_t *bytes) {
+    raise_for(g.prefix_attn(&q, cd.data(), static_cast<int32_t>(cd.size()), &b, shared_len, &t, &n, &l, scale, &o,
+                            e.ptr(), w, bytes, static_cast<int32_t>(kvcache_format_raw), vllm_two_major, stream_of(dev)));
+  };
+  int64_t bytes = 0;
+  call(nullptr, &bytes);
+  if (bytes == 0) return;
+  // Scratch of this call: the allocator hands it out again in stream order.
+  const at::Tensor space = at::empty({bytes}, query.options().dtype(at::kByte));
+  const lmc_tensor w = desc(space);
+  call(&w, nullptr);
 }
 
 void bind(uintptr_t multi, uintptr_t single, uintptr_t load_flash, uintptr_t reshape_flash,

@@ -99,7 +99,7 @@ SIGNATURES = {
         _T, _T, _T, _T, _T, _i32, _T, _i64, _vp, _i64, ctypes.c_double, _i32, _i64, _T, _i32, _i32, _vp,
     ],
     "lmc_shared_prefix_attention": [
-        _T, _T, _i32, _T, _i64, _T, _T, _T, ctypes.c_double, _T, _T, _i32, _i32, _vp,
+        _T, _T, _i32, _T, _i64, _T, _T, _T, ctypes.c_double, _T, _T, _T, ctypes.POINTER(_i64), _i32, _i32, _vp,
     ],
     "lmc_get_device_ptr": [_up, _sz, ctypes.POINTER(_up)],
     "lmc_register_mapping": [_up, _up, _sz, ctypes.POINTER(_up)],

@@ -763,13 +763,20 @@ def shared_prefix_attention(
         return
     dev = _gpu_of(query, "query")
     caches = _normalize_kv_caches(vllm_kv_caches)
-    _run(
-        _L.lmc_shared_prefix_attention(
-            _opt(query), _cache_array(caches), len(caches), _opt(shared_blocks), int(shared_len), _opt(block_table),
-            _opt(seq_lens), _opt(query_start_loc), float(scale), _opt(output), _opt(lse), int(kvcache_format_raw),
-            int(bool(vllm_two_major)), _stream(dev),
+
+    def call(workspace, size):
+        _run(
+            _L.lmc_shared_prefix_attention(
+                _opt(query), _cache_array(caches), len(caches), _opt(shared_blocks), int(shared_len),
+                _opt(block_table), _opt(seq_lens), _opt(query_start_loc), float(scale), _opt(output), _opt(lse),
+                _opt(workspace), size, int(kvcache_format_raw), int(bool(vllm_two_major)), _stream(dev),
+            )
         )
-    )
+
+    size = ctypes.c_int64(0)
+    call(None, ctypes.byref(size))
+    if size.value:
+        call(torch.empty(size.value, dtype=torch.uint8, device=query.device), None)
 
 
 # ---------------------------------------------------------------------------

@@ -171,6 +171,18 @@ def test_table_shorter_than_the_request(ops):
     _check(ops, c)
 
 
+def test_lengths_far_past_the_table(ops):
+    """A request said to be 2^31 - 1 long ends where its table's row ends."""
+    c = _case(16, [1, 2, 1], [96, 80, 64], 40, 16, 4, 2, 64)
+    c["seq"][0] = 2**31 - 1
+    c["seq"][1] = -(2**31)
+    caches, kw = _device_caches(c)
+    out, lse = c["out"].to(DEV), c["lse"].to(DEV)
+    _call(ops, c, caches, kw, c["q"].to(DEV), out, lse)
+    torch.cuda.synchronize()
+    _hold(c, out, lse, _want(dict(c, seq=torch.tensor([96, 0, 64]))))
+
+
 def test_unseen_infinities_among_several_tokens(ops):
     """A later token's key and value hold NaN and infinity: earlier tokens of
     the request do not see them, the later one does."""

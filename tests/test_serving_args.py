@@ -187,11 +187,11 @@ def test_rotary_to_paged_refusals(over, text):
 
 def _attention(**over):
     a = dict(q=_t(BF16, 5, 8, 64), caches=_caches(), shared=_t(I32, 3), P=40, table=_t(I32, 4, 9), seq=_t(I32, 4),
-             starts=_t(I32, 5), scale=0.125, o=_t(BF16, 5, 8, 64), lse=_t(F32, 5, 8), fmt=2, two=0)
+             starts=_t(I32, 5), scale=0.125, o=_t(BF16, 5, 8, 64), lse=_t(F32, 5, 8), ws=_t(_lib.U8, 1 << 20), fmt=2, two=0)
     a.update(over)
     return L.lmc_shared_prefix_attention(_ptr(a["q"]), a["caches"], len(a["caches"]), _ptr(a["shared"]), a["P"],
                                          _ptr(a["table"]), _ptr(a["seq"]), _ptr(a["starts"]), a["scale"], _ptr(a["o"]),
-                                         _ptr(a["lse"]), a["fmt"], a["two"], None)
+                                         _ptr(a["lse"]), _ptr(a["ws"]), None, a["fmt"], a["two"], None)
 
 
 @pytest.mark.parametrize("over,text", [
@@ -209,8 +209,10 @@ def _attention(**over):
     ({"shared": _t(I64, 3)}, "shared_blocks has a dtype"),
     ({"shared": _t(I32, 2)}, "too few blocks"),
     ({"P": -1}, "shared_len must be"),
+    ({"P": 2**30 + 1}, "shared_len must be"),
     ({"table": _t(I32, 3, 9)}, "block_table must be"),
     ({"table": _t(I32, 4, 9, strides=[18, 2])}, "rows must be contiguous"),
+    ({"table": _t(I32, 4, 2**26 + 1)}, "more than 2^30 keys"),
     ({"seq": _t(I64, 4)}, "seq_lens has a dtype"),
     ({"starts": _t(I32, 4)}, "query_start_loc must have"),
     ({"scale": 0.0}, "scale must be positive"),
@@ -218,6 +220,13 @@ def _attention(**over):
     ({"scale": math.nan}, "scale must be positive"),
     ({"lse": _t(F32, 5, 7)}, "lse must be"),
     ({"lse": _t(BF16, 5, 8)}, "lse has a dtype"),
+    ({"ws": None}, "workspace is null"),
+    ({"ws": _t(_lib.U8, 5000)}, "workspace must be"),
+    ({"ws": _t(_lib.U8, 1 << 20, data=(1 << 35) + 8)}, "workspace must be"),
+    ({"q": _t(BF16, 5, 8, 64, strides=[516, 64, 1])}, "rows of query and output must start"),
+    ({"o": _t(BF16, 5, 8, 64, strides=[64, 64, 1])}, "output has overlapping rows"),
+    ({"o": _t(BF16, 5, 8, 64, data=(1 << 35) + 2)}, "rows of query and output must start"),
+    ({"caches": _one(_t(BF16, 6, 2, 16, 2, 64, data=(1 << 35) + 8)), "fmt": 1}, "the paged caches' rows must start"),
 ])
 def test_prefix_attention_refusals(over, text):
     _refuses(_attention(**over), text)
