@@ -11,6 +11,7 @@
 #include "serving.h"
 
 #include <cmath>
+#include <type_traits>
 
 namespace lmc {
 
@@ -49,7 +50,7 @@ struct AttnArgs {
   int prefix_parts, own_parts;
   int prefix_tiles;         // row tiles of one KV head's rows
   int prefix_chunk;         // keys of one prefix part
-  int prefix_groups, every; // groups of 8 workgroups, and how they are dealt
+  int prefix_groups;        // groups of 8 workgroups, the first of the launch
   int own_tiles;            // row tiles of a request dealt to workgroups
   int own_items;
 };
@@ -122,10 +123,62 @@ template <int D> struct Geometry {
   static constexpr int kLoads = 32 * D * 2 / 1024;  // wave loads of 32 rows
 };
 
-// Adds one tile of NB * 32 keys (in LDS at k, v) to the rows.  MASK: some
-// key of the tile is unseen (bit of `seen` clear, or past a row's limit).
-template <typename T, int D, int NB, bool MASK>
-__device__ __forceinline__ void add_tile(Rows32<T, D> &r, uint32_t k, uint32_t v, int j0, uint64_t seen, bool cut, float c) {
+// Whether a tile of V holds an infinity or a NaN.
+template <typename T, int D, int KEYS>
+__device__ __forceinline__ bool has_odd(uint32_t v) {
+  bool bad = false;
+  for (int i = threadIdx.x & 63; i < KEYS * D / 8; i += 64) {
+    const s16x8 x = *reinterpret_cast<const LdsS8 *>(v + i * 16);
+#pragma unroll
+    for (int e = 0; e < 8; ++e) bad |= (static_cast<uint32_t>(x[e]) & Mma<T>::kInf) == Mma<T>::kInf;
+  }
+  return __any(bad);
+}
+
+// Takes the infinities and NaN out of a tile of V that holds keys which some
+// rows see and others do not: a weight of zero would make NaN of them.  The
+// rows that see such a key get its infinities and NaN added here.  SHARED:
+// the four waves work on one tile, and all of them come here.
+template <typename T, int D, int KEYS, bool SHARED>
+__device__ __forceinline__ void take_odd_out(Rows32<T, D> &r, uint32_t v, int j0, uint64_t seen) {
+  using M = Mma<T>;
+  constexpr int kPitch = Geometry<D>::kPitch;
+  const int lane = threadIdx.x & 63, hb = lane >> 5;
+#pragma unroll 1
+  for (int key = 0; key < KEYS; ++key) {
+    const bool see = ((seen >> key) & 1) && j0 + key < r.limit;
+    const uint32_t row = v + key * kPitch + 8 * hb, x = v_swizzle<D>(key) << 4;
+#pragma unroll
+    for (int t = 0; t < D / 32; ++t)
+#pragma unroll
+      for (int q = 0; q < 4; ++q) {
+        const s16x4 y = *reinterpret_cast<const LdsS4 *>(row + ((64 * t + 16 * q) ^ x));
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+          if (see && (static_cast<uint32_t>(y[e]) & M::kInf) == M::kInf)
+            r.o[t][4 * q + e] += to_f32<T>(static_cast<uint16_t>(y[e]));
+        asm volatile("" ::: "memory");  // (few registers here)
+      }
+  }
+  if constexpr (SHARED) __syncthreads();
+#pragma unroll 1
+  for (int i = lane; i < KEYS * D / 8; i += 64) {
+    s16x8 x = *reinterpret_cast<const LdsS8 *>(v + i * 16);
+#pragma unroll
+    for (int e = 0; e < 8; ++e)
+      if ((static_cast<uint32_t>(x[e]) & M::kInf) == M::kInf) x[e] = 0;
+    *reinterpret_cast<LdsS8 *>(v + i * 16) = x;
+  }
+  if constexpr (SHARED) __syncthreads();
+  else fence_reads();
+}
+
+// Adds one tile of NB * 32 keys (in LDS at k, v) to the rows.  masked: some
+// key of the tile is unseen (its bit of `seen` is clear, or it lies past a
+// row's limit); cut: some row of the workgroup ends inside the tile.
+template <typename T, int D, int NB>
+__device__ __forceinline__ void add_tile(Rows32<T, D> &r, uint32_t k, uint32_t v, int j0, uint64_t seen, bool masked, bool cut,
+                                         float c) {
   using M = Mma<T>;
   using V8 = typename M::V8;
   using G = Geometry<D>;
@@ -145,14 +198,18 @@ __device__ __forceinline__ void add_tile(Rows32<T, D> &r, uint32_t k, uint32_t v
       s[b] = M::mul(__builtin_bit_cast(V8, a), r.q[kc], s[b]);
     }
   }
-  if constexpr (MASK) {
+  if (masked) {
+    // Bit 32 b + 8 (i / 4) + i % 4: whether the row sees key 4 hb further.
+    uint64_t bits = seen >> (4 * hb);
+    const int left = r.limit - j0 - 4 * hb;
+    if (left < 64) bits &= left > 0 ? (uint64_t(1) << left) - 1 : 0;
 #pragma unroll
-    for (int b = 0; b < NB; ++b)
+    for (int b = 0; b < NB; ++b) {
+      const uint32_t half = static_cast<uint32_t>(bits >> (32 * b));
 #pragma unroll
-      for (int i = 0; i < 16; ++i) {
-        const int key = 32 * b + 8 * (i / 4) + 4 * hb + i % 4;
-        if (!((seen >> key) & 1) || j0 + key >= r.limit) s[b][i] = -INFINITY;
-      }
+      for (int i = 0; i < 16; ++i)
+        if (!(half & (1u << (8 * (i / 4) + i % 4)))) s[b][i] = -INFINITY;
+    }
   }
   float top = s[0][0];
 #pragma unroll
@@ -181,6 +238,7 @@ __device__ __forceinline__ void add_tile(Rows32<T, D> &r, uint32_t k, uint32_t v
       s[b][i] = __builtin_amdgcn_exp2f(s[b][i] * c - base);
       r.l += s[b][i];
     }
+  if (cut && has_odd<T, D, NB * 32>(v)) take_odd_out<T, D, NB * 32, NB == 2>(r, v, j0, seen);
   // O^T += V^T P^T.  The sum over keys may take them in any order: the order
   // in which a lane holds its 8 of 16 weights, keys 4 hb + {0..3, 8..11}.
   const int a = lane & 15;
@@ -188,18 +246,6 @@ __device__ __forceinline__ void add_tile(Rows32<T, D> &r, uint32_t k, uint32_t v
   const uint32_t vx = v_swizzle<D>(vrow);
   const uint32_t vcol = 2 * ((lane >> 4) & 1) + ((a & 3) >> 1);
   const uint32_t vbase = v + vrow * G::kPitch + (a & 1) * 8;
-  bool odd = false;  // this tile's V holds an infinity or NaN that not every row sees
-  if constexpr (MASK) {
-    if (cut) {
-      bool bad = false;
-      for (int i = lane; i < NB * 32 * G::kPieces; i += 64) {
-        const s16x8 x = *reinterpret_cast<const LdsS8 *>(v + i * 16);
-#pragma unroll
-        for (int e = 0; e < 8; ++e) bad |= (static_cast<uint32_t>(x[e]) & M::kInf) == M::kInf;
-      }
-      odd = __any(bad);
-    }
-  }
 #pragma unroll
   for (int c2 = 0; c2 < 2 * NB; ++c2) {
     V8 p;
@@ -210,32 +256,8 @@ __device__ __forceinline__ void add_tile(Rows32<T, D> &r, uint32_t k, uint32_t v
       const uint32_t at = vbase + (((4 * t + vcol) ^ vx) << 4) + c2 * 16 * G::kPitch;
       const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16(reinterpret_cast<LdsS4 *>(at));
       const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16(reinterpret_cast<LdsS4 *>(at + 8 * G::kPitch));
-      s16x8 x = __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
-      if constexpr (MASK) {
-        if (odd) {
-#pragma unroll
-          for (int e = 0; e < 8; ++e)
-            if ((static_cast<uint32_t>(x[e]) & M::kInf) == M::kInf) x[e] = 0;
-        }
-      }
+      const s16x8 x = __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
       r.o[t] = M::mul(__builtin_bit_cast(V8, x), p, r.o[t]);
-    }
-  }
-  if constexpr (MASK) {
-    // What the product left out: infinities and NaN for the rows that see them.
-    if (odd) {
-      for (int key = 0; key < NB * 32; ++key) {
-        const bool see = ((seen >> key) & 1) && j0 + key < r.limit;
-#pragma unroll
-        for (int t = 0; t < D / 32; ++t)
-#pragma unroll
-          for (int i = 0; i < 16; ++i) {
-            const uint32_t d = 32 * t + 8 * (i / 4) + 4 * hb + i % 4;
-            const uint32_t at = v + key * G::kPitch + (((d >> 3) ^ v_swizzle<D>(key)) << 4) + (d & 7) * 2;
-            const uint16_t x = *reinterpret_cast<const __attribute__((address_space(3))) uint16_t *>(at);
-            if (see && (x & M::kInf) == M::kInf) r.o[t][i] += to_f32<T>(x);
-          }
-      }
     }
   }
 }
@@ -296,19 +318,6 @@ __device__ __forceinline__ void load_tile(const uint8_t *row, uint32_t lds, int 
   }
 }
 
-// Whether a tile has to be masked row by row, and whether a row ends in it.
-template <typename T, int D> __device__ __forceinline__ bool ends_before(const Rows32<T, D> &r, int j1) {
-  return __any(r.limit < j1);
-}
-
-template <typename T, int D, int NB>
-__device__ __forceinline__ void add_any_tile(Rows32<T, D> &r, uint32_t k, uint32_t v, int j0, int k1, uint64_t seen, float c) {
-  constexpr uint64_t kAll = NB == 2 ? ~uint64_t(0) : 0xffffffffu;
-  const bool cut = ends_before<T, D>(r, min(j0 + 32 * NB, k1));
-  if (cut || seen != kAll) add_tile<T, D, NB, true>(r, k, v, j0, seen, cut, c);
-  else add_tile<T, D, NB, false>(r, k, v, j0, seen, false, c);
-}
-
 // Query rows to registers: row n of `m` (head-local row numbers).
 template <typename T, int D> __device__ __forceinline__ void load_rows(const AttnArgs &a, Rows32<T, D> &r, int t, int head, int limit) {
   using S = typename T::S;
@@ -342,7 +351,7 @@ template <int D> struct Lds {
 // rows over different keys.  A row whose limit is 0 or less gets nothing.
 template <typename T, int D, bool MERGE>
 __device__ __forceinline__ void store_part(const AttnArgs &a, const Rows32<T, D> &r, bool dead, int part, uint8_t *lds) {
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, n = lane & 31, hb = lane >> 5;
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), n = lane & 31, hb = lane >> 5;
   float *sums = reinterpret_cast<float *>(lds);
   float2 *ml = reinterpret_cast<float2 *>(lds + 4 * D * 33 * 4);
   const float2 ls = both_halves(r.l);
@@ -400,8 +409,8 @@ __device__ __forceinline__ void store_part(const AttnArgs &a, const Rows32<T, D>
 // Four waves, the same 32 rows, a quarter of the tiles each in LDS of its
 // own: few rows, bound by the bytes of K and V.
 template <typename T, int D>
-__device__ __forceinline__ void attend_narrow(const AttnArgs &a, Rows32<T, D> &r, KeyTiles<D, 32> &tiles, uint32_t lds) {
-  const int wave = threadIdx.x >> 6;
+__device__ __forceinline__ void attend_narrow(const AttnArgs &a, Rows32<T, D> &r, KeyTiles<D, 32> &tiles, int least, uint32_t lds) {
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const uint32_t k = lds + wave * (2 * 32 * D * 2), v = k + 32 * D * 2;
   int j0 = tiles.k0 + 32 * wave;
   if (j0 >= tiles.k1) return;
@@ -413,7 +422,8 @@ __device__ __forceinline__ void attend_narrow(const AttnArgs &a, Rows32<T, D> &r
   tiles.fetch(j0 + 128);
   for (; j0 < tiles.k1; j0 += 128) {
     fence_loads();
-    add_any_tile<T, D, 1>(r, k, v, j0, tiles.k1, seen, a.scale2);
+    const bool cut = least < min(j0 + 32, tiles.k1);
+    add_tile<T, D, 1>(r, k, v, j0, seen, cut || seen != 0xffffffffu, cut, a.scale2);
     if (j0 + 128 < tiles.k1) {
       seen = tiles.rows(j0 + 128, kr, vr);
       fence_reads();
@@ -427,8 +437,8 @@ __device__ __forceinline__ void attend_narrow(const AttnArgs &a, Rows32<T, D> &r
 // Four waves of 32 rows each over tiles of 64 keys that they share: many
 // rows, bound by the matrix cores.
 template <typename T, int D>
-__device__ __forceinline__ void attend_wide(const AttnArgs &a, Rows32<T, D> &r, KeyTiles<D, 64> &tiles, uint32_t lds) {
-  const int wave = threadIdx.x >> 6;
+__device__ __forceinline__ void attend_wide(const AttnArgs &a, Rows32<T, D> &r, KeyTiles<D, 64> &tiles, int least, uint32_t lds) {
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   constexpr uint32_t kTile = 64 * D * 2;
   int j0 = tiles.k0;
   const uint8_t *kr, *vr;
@@ -449,7 +459,8 @@ __device__ __forceinline__ void attend_wide(const AttnArgs &a, Rows32<T, D> &r, 
       tiles.fetch(j0 + 128);
     }
     const uint32_t at = lds + stage * 2 * kTile;
-    add_any_tile<T, D, 2>(r, at, at + kTile, j0, tiles.k1, now, a.scale2);
+    const bool cut = least < min(j0 + 64, tiles.k1);
+    add_tile<T, D, 2>(r, at, at + kTile, j0, now, cut || now != ~uint64_t(0), cut, a.scale2);
   }
 }
 
@@ -477,19 +488,34 @@ __device__ __forceinline__ int limit_of(const AttnArgs &a, int r, int t) {
   return static_cast<int>(max(static_cast<int64_t>(0), min(n, static_cast<int64_t>(a.max_keys))));
 }
 
-// Groups of 8 consecutive workgroups (one an XCD) take prefix work, every
-// `every`-th of them, or the requests' own keys.  The row tiles of one (KV
-// head, prefix part) go to one XCD, whose L2 then holds that part.
+// The least limit of a wave's rows, or (ALL) of the four waves'.
+template <bool ALL> __device__ __forceinline__ int least_limit(int limit, uint8_t *lds) {
+#pragma unroll
+  for (int d = 1; d < 32; d <<= 1) limit = min(limit, __shfl_xor(limit, d));
+  if constexpr (ALL) {
+    int *w = reinterpret_cast<int *>(lds);
+    if ((threadIdx.x & 63) == 0) w[threadIdx.x >> 6] = limit;
+    __syncthreads();
+    limit = min(min(w[0], w[1]), min(w[2], w[3]));
+    __syncthreads();
+  }
+  return __builtin_amdgcn_readfirstlane(limit);
+}
+
+// The first workgroups take the prefix, the others the requests' own keys:
+// the long ones start first, one on every other CU or so, and both kinds run
+// beside each other (dealing them in turn instead put all prefix work on half
+// of the CUs, since the dispatcher goes round the shader engines).  Of 8
+// consecutive workgroups each runs on an XCD of its own; the row tiles of one
+// (KV head, prefix part) go to one XCD, whose L2 then holds that part.
 template <typename T, int D, bool WIDE> __global__ void __launch_bounds__(256, D > 128 ? 1 : 2) attend(AttnArgs a) {
   extern __shared__ uint8_t lds[];
   const uint32_t at = static_cast<uint32_t>(reinterpret_cast<uintptr_t>((__attribute__((address_space(3))) uint8_t *)lds));
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, n = lane & 31;
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), n = lane & 31;
   const int group = blockIdx.x / 8, xcd = blockIdx.x % 8;
-  const int before = min(a.prefix_groups, (group + a.every - 1) / a.every);  // prefix groups before this one
   Rows32<T, D> r;
-  if (group % a.every == 0 && group / a.every < a.prefix_groups) {
-    const int k = group / a.every;
-    const int pair = k / a.prefix_tiles * 8 + xcd, tile = k % a.prefix_tiles;
+  if (group < a.prefix_groups) {
+    const int pair = group / a.prefix_tiles * 8 + xcd, tile = group % a.prefix_tiles;
     if (pair >= a.kv_heads * a.prefix_parts) return;
     const int h = pair % a.kv_heads, part = pair / a.kv_heads;
     const int x = tile * (WIDE ? 128 : 32) + (WIDE ? wave * 32 : 0) + n;
@@ -502,13 +528,14 @@ template <typename T, int D, bool WIDE> __global__ void __launch_bounds__(256, D
     load_rows<T, D>(a, r, t, h * a.group + (t < 0 ? 0 : x % a.group), limit);
     KeyTiles<D, WIDE ? 64 : 32> tiles{a, a.shared, a.shared_width, part * a.prefix_chunk,
                                       min(a.shared_len, (part + 1) * a.prefix_chunk), h * a.k_head, h * a.v_head, -1};
-    if constexpr (WIDE) attend_wide<T, D>(a, r, tiles, at);
-    else attend_narrow<T, D>(a, r, tiles, at);
+    const int least = least_limit<WIDE>(r.limit, lds);
+    if constexpr (WIDE) attend_wide<T, D>(a, r, tiles, least, at);
+    else attend_narrow<T, D>(a, r, tiles, least, at);
     store_part<T, D, !WIDE>(a, r, limit <= 0, part, lds);
     return;
   }
   // A request's own keys.
-  const int item = (group - before) * 8 + xcd;
+  const int item = (group - a.prefix_groups) * 8 + xcd;
   if (item >= a.own_items) return;
   const int h = item % a.kv_heads, y = item / a.kv_heads;
   const int part = y % a.own_parts, z = y / a.own_parts;
@@ -526,33 +553,63 @@ template <typename T, int D, bool WIDE> __global__ void __launch_bounds__(256, D
     const int limit = t >= 0 ? limit_of(a, q, t) : 0;
     load_rows<T, D>(a, r, t, h * a.group + (t < 0 ? 0 : x % a.group), limit);
     KeyTiles<D, 32> tiles{a, a.table + q * a.table_stride, a.width, k0, k1, h * a.k_head, h * a.v_head, -1};
-    attend_narrow<T, D>(a, r, tiles, at);
+    attend_narrow<T, D>(a, r, tiles, least_limit<false>(r.limit, lds), at);
     store_part<T, D, true>(a, r, limit <= 0, a.prefix_parts + part, lds);
     __syncthreads();
   }
 }
 
-// Joins a row's parts.
+// Joins the parts of a row: four waves take a quarter of them each, D / 4
+// lanes a row.
 template <typename T, int D> __global__ void __launch_bounds__(256) join_parts(AttnArgs a) {
-  constexpr int kQuads = D / 4, kRows = 256 / kQuads;
+  constexpr int kQuads = D / 4, kRows = 64 / kQuads;
   using S = typename T::S;
+  __shared__ f32x4 sums[4][64];
+  __shared__ float2 weights[4][kRows];
   const int64_t rows = static_cast<int64_t>(a.n_tokens) * a.heads;
-  const int64_t row = static_cast<int64_t>(blockIdx.x) * kRows + threadIdx.x / kQuads;
-  if (threadIdx.x / kQuads >= kRows || row >= rows) return;
-  const int t = static_cast<int>(row / a.heads), h = static_cast<int>(row % a.heads), d = threadIdx.x % kQuads * 4;
-  if (t < a.starts[0] || t >= a.starts[a.n_requests]) return;
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int i = lane / kQuads, d = lane % kQuads * 4;
+  const int64_t row = static_cast<int64_t>(blockIdx.x) * kRows + i;
+  const bool there = i < kRows && row < rows;
+  const int t = there ? static_cast<int>(row / a.heads) : -1, h = static_cast<int>(row % a.heads);
+  const bool live = t >= a.starts[0] && t < a.starts[a.n_requests];
   const int parts = a.prefix_parts + a.own_parts;
-  float top = -INFINITY;
-  for (int p = 0; p < parts; ++p) top = fmaxf(top, a.part_ml[p * rows + row].x);
-  const float base = top == -INFINITY ? 0.f : top;
-  float l = 0.f;
+  float m = -INFINITY, l = 0.f;
   f32x4 o = {0.f, 0.f, 0.f, 0.f};
-  for (int p = 0; p < parts; ++p) {
-    const float2 w = a.part_ml[p * rows + row];
-    if (w.y == 0.f) continue;
-    const float f = __builtin_amdgcn_exp2f(w.x - base);
-    l += f * w.y;
-    const f32x4 x = *reinterpret_cast<const f32x4 *>(a.part_o + (p * rows + row) * D + d);
+  if (live) {
+#pragma unroll 4
+    for (int p = wave; p < parts; p += 4) {
+      const float2 w = a.part_ml[p * rows + row];
+      if (w.y == 0.f) continue;
+      const f32x4 x = *reinterpret_cast<const f32x4 *>(a.part_o + (p * rows + row) * D + d);
+      const float top = fmaxf(m, w.x), base = top == -INFINITY ? 0.f : top;
+      const float f = __builtin_amdgcn_exp2f(m - base), g = __builtin_amdgcn_exp2f(w.x - base);
+      l = l * f + w.y * g;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) o[e] = o[e] * f + x[e] * g;
+      m = top;
+    }
+    sums[wave][lane] = o;
+    if (d == 0) weights[wave][i] = make_float2(m, l);
+  }
+  __syncthreads();
+  if (wave != 0 || !live) return;
+  float2 w[4];
+  float top = -INFINITY;
+#pragma unroll
+  for (int g = 0; g < 4; ++g) {
+    w[g] = weights[g][i];
+    top = fmaxf(top, w[g].x);
+  }
+  const float base = top == -INFINITY ? 0.f : top;
+  l = 0.f;
+  o = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+  for (int g = 0; g < 4; ++g) {
+    if (w[g].y == 0.f) continue;
+    const float f = __builtin_amdgcn_exp2f(w[g].x - base);
+    const f32x4 x = sums[g][lane];
+    l += f * w[g].y;
 #pragma unroll
     for (int e = 0; e < 4; ++e) o[e] += f * x[e];
   }
@@ -570,7 +627,7 @@ template <typename T, int D> void launch(const AttnArgs &a, bool wide, uint32_t 
   if (wide) hipLaunchKernelGGL((attend<T, D, true>), dim3(groups * 8), dim3(256), Lds<D>::kBytes, s, a);
   else hipLaunchKernelGGL((attend<T, D, false>), dim3(groups * 8), dim3(256), Lds<D>::kBytes, s, a);
   hip_check(hipGetLastError(), "attend launch");
-  constexpr int kRows = 256 / (D / 4);
+  constexpr int kRows = 64 / (D / 4);
   const int64_t rows = static_cast<int64_t>(a.n_tokens) * a.heads;
   hipLaunchKernelGGL((join_parts<T, D>), dim3(static_cast<uint32_t>((rows + kRows - 1) / kRows)), dim3(256), 0, s, a);
   hip_check(hipGetLastError(), "join_parts launch");
@@ -602,19 +659,27 @@ Plan make_plan(int64_t T, int64_t R, int64_t kv_heads, int64_t group, int64_t sh
   p.wide = rows > 64;
   const int64_t m = p.wide ? 128 : 32, tile = p.wide ? 64 : 128;
   p.prefix_tiles = static_cast<int>((rows + m - 1) / m);
-  // Workgroups for two of a CU, parts of at least one round of tiles each.
-  const int64_t items = p.prefix_tiles * kv_heads;
-  const int64_t most = std::max<int64_t>(1, (shared_len + 2 * tile - 1) / (2 * tile));
-  p.prefix_parts = shared_len == 0 ? 0 : static_cast<int>(std::min<int64_t>(most, std::max<int64_t>(1, 512 / items)));
+  const int64_t per = (T + R - 1) / R * group;  // rows of a request, about
+  p.own_tiles = static_cast<int>(std::max<int64_t>(1, (per + 31) / 32));
+  const int64_t own = std::max<int64_t>(0, table_keys - shared_len);
+  const int64_t items = p.prefix_tiles * kv_heads, own_items = R * kv_heads * p.own_tiles;
+  // Two workgroups fit a CU.  The prefix gets its share of those 512 places,
+  // at a key of its own in half of the time of a request's own key (which
+  // comes from memory, while all row tiles read the prefix; requests have
+  // half of their tables' keys on the average), so that both end together:
+  // 256 requests, 32 heads over 16384 keys, 1024 own: 178 us; with twice the
+  // share 195, with three times 215.  A part has four wide tiles or one round
+  // of narrow ones at least: it costs a row of 32-bit sums to write and read.
+  const double prefix_cost = static_cast<double>(items) * shared_len;
+  const double own_cost = static_cast<double>(own_items) * own * 1.0;
+  const int64_t places = static_cast<int64_t>(512 * prefix_cost / (prefix_cost + own_cost + 1));
+  const int64_t most = std::max<int64_t>(1, shared_len / (p.wide ? 4 * tile : tile));
+  p.prefix_parts = shared_len == 0 ? 0 : static_cast<int>(std::min<int64_t>(most, std::max<int64_t>(1, (places + items / 2) / items)));
   p.prefix_chunk = 0;
   if (p.prefix_parts) {
     p.prefix_chunk = static_cast<int>(((shared_len + p.prefix_parts - 1) / p.prefix_parts + tile - 1) / tile * tile);
     p.prefix_parts = static_cast<int>((shared_len + p.prefix_chunk - 1) / p.prefix_chunk);
   }
-  const int64_t per = (T + R - 1) / R * group;  // rows of a request, about
-  p.own_tiles = static_cast<int>(std::max<int64_t>(1, (per + 31) / 32));
-  const int64_t own = std::max<int64_t>(0, table_keys - shared_len);
-  const int64_t own_items = R * kv_heads * p.own_tiles;
   const int64_t own_most = std::max<int64_t>(1, (own + 255) / 256);
   p.own_parts = static_cast<int>(std::min<int64_t>(own_most, std::max<int64_t>(1, 512 / own_items)));
   return p;
@@ -753,7 +818,6 @@ extern "C" int lmc_shared_prefix_attention(const lmc_tensor *query, const lmc_te
     const int64_t own_groups = (own_items + 7) / 8;
     const int64_t prefix_groups = (kv.heads * p.prefix_parts + 7) / 8 * p.prefix_tiles;
     a.prefix_groups = static_cast<int>(prefix_groups);
-    a.every = prefix_groups ? static_cast<int>((own_groups + prefix_groups) / prefix_groups) : 1;
     DeviceGuard guard(dev);
     const hipStream_t s = static_cast<hipStream_t>(stream);
     const uint32_t groups = static_cast<uint32_t>(own_groups + prefix_groups);
