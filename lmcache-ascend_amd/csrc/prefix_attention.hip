@@ -24,6 +24,11 @@ typedef float f32x4 __attribute__((ext_vector_type(4)));
 typedef short s16x4 __attribute__((ext_vector_type(4)));
 typedef short s16x8 __attribute__((ext_vector_type(8)));
 
+// Keys of a part of a request's own ones where requests are many: 256 requests
+// over 16384 shared and up to 1024 own keys take 165 us with 384, 170 with 256
+// (more starts and ends), 179 with 128.
+constexpr int kOwnChunk = 384;
+
 struct AttnArgs {
   const void *q;
   int64_t q_token, q_head;  // elements
@@ -51,7 +56,8 @@ struct AttnArgs {
   int prefix_tiles;         // row tiles of one KV head's rows
   int prefix_chunk;         // keys of one prefix part
   int prefix_groups;        // groups of 8 workgroups, the first of the launch
-  int own_tiles;            // row tiles of a request dealt to workgroups
+  int own_tiles;            // row tiles of a request dealt to waves
+  int own_want;             // parts of a request's own keys that fill the chip
   int own_items;
 };
 
@@ -84,14 +90,26 @@ __device__ __forceinline__ float2 both_halves(float x) {
   return make_float2(__uint_as_float(r[0]), __uint_as_float(r[1]));
 }
 
-// 16 bytes a lane from global memory to LDS at `lds` (uniform) + 16 * lane.
-// No register is written; fence_loads() waits.
-__device__ __forceinline__ void load_to_lds(const void *g, uint32_t lds) {
-  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off" ::"s"(__builtin_amdgcn_readfirstlane(lds)), "v"(g) : "memory");
+// 16 bytes a lane from global memory to LDS at `lds` (uniform) + 16 * lane:
+// from base (uniform) + off, or from an address of the lane's.  No register
+// is written; wait_loads<N>() waits until at most N loads are under way.
+__device__ __forceinline__ uint64_t uniform(const void *p) {
+  const uint64_t x = reinterpret_cast<uint64_t>(p);
+  const uint32_t lo = __builtin_amdgcn_readfirstlane(static_cast<uint32_t>(x));
+  const uint32_t hi = __builtin_amdgcn_readfirstlane(static_cast<uint32_t>(x >> 32));
+  return (static_cast<uint64_t>(hi) << 32) | lo;
 }
-__device__ __forceinline__ void fence_loads() { asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); }
+__device__ __forceinline__ void load_to_lds(const uint8_t *base, uint32_t off, uint32_t lds) {
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(__builtin_amdgcn_readfirstlane(lds)), "v"(off),
+               "s"(uniform(base))
+               : "memory");
+}
+__device__ __forceinline__ void load_to_lds(const uint8_t *at, uint32_t lds) {
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off" ::"s"(__builtin_amdgcn_readfirstlane(lds)), "v"(at) : "memory");
+}
+template <int N> __device__ __forceinline__ void wait_loads() { asm volatile("s_waitcnt vmcnt(%0)" ::"n"(N) : "memory"); }
 // LDS reads have their data: what they read may be written again.
-__device__ __forceinline__ void fence_reads() { asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory"); }
+__device__ __forceinline__ void wait_reads() { asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory"); }
 
 typedef __attribute__((address_space(3))) uint8_t LdsByte;
 typedef __attribute__((address_space(3))) s16x4 LdsS4;
@@ -120,7 +138,6 @@ template <typename T, int D> struct Rows32 {
 template <int D> struct Geometry {
   static constexpr int kPitch = 2 * D;           // bytes of a row
   static constexpr int kPieces = D / 8;          // 16-byte pieces of a row
-  static constexpr int kLoads = 32 * D * 2 / 1024;  // wave loads of 32 rows
 };
 
 // Whether a tile of V holds an infinity or a NaN.
@@ -170,56 +187,65 @@ __device__ __forceinline__ void take_odd_out(Rows32<T, D> &r, uint32_t v, int j0
     *reinterpret_cast<LdsS8 *>(v + i * 16) = x;
   }
   if constexpr (SHARED) __syncthreads();
-  else fence_reads();
+  else wait_reads();
 }
 
-// Adds one tile of NB * 32 keys (in LDS at k, v) to the rows.  masked: some
-// key of the tile is unseen (its bit of `seen` is clear, or it lies past a
-// row's limit); cut: some row of the workgroup ends inside the tile.
+// The steps of a tile of NB * 32 keys, in LDS at k and v.
+
+// S^T = K Q^T: lane (n, hb) gets the scores of row n with the keys 32 b + 8 i
+// + 4 hb + j of s[b][4 i + j].
 template <typename T, int D, int NB>
-__device__ __forceinline__ void add_tile(Rows32<T, D> &r, uint32_t k, uint32_t v, int j0, uint64_t seen, bool masked, bool cut,
-                                         float c) {
+__device__ __forceinline__ void scores(const Rows32<T, D> &r, uint32_t k, f32x16 (&s)[NB]) {
   using M = Mma<T>;
-  using V8 = typename M::V8;
-  using G = Geometry<D>;
+  constexpr int kPitch = Geometry<D>::kPitch;
   const int lane = threadIdx.x & 63, n = lane & 31, hb = lane >> 5;
-  f32x16 s[NB];
+  const uint32_t krow = k + n * kPitch, kx = k_swizzle<D>(n);
 #pragma unroll
   for (int b = 0; b < NB; ++b)
 #pragma unroll
     for (int i = 0; i < 16; ++i) s[b][i] = 0.f;
-  const uint32_t krow = k + n * G::kPitch, kx = k_swizzle<D>(n);
 #pragma unroll
   for (int kc = 0; kc < D / 16; ++kc) {
     const uint32_t at = krow + (((2 * kc + hb) ^ kx) << 4);
 #pragma unroll
     for (int b = 0; b < NB; ++b) {
-      const s16x8 a = *reinterpret_cast<const LdsS8 *>(at + b * 32 * G::kPitch);
-      s[b] = M::mul(__builtin_bit_cast(V8, a), r.q[kc], s[b]);
+      const s16x8 a = *reinterpret_cast<const LdsS8 *>(at + b * 32 * kPitch);
+      s[b] = M::mul(__builtin_bit_cast(typename M::V8, a), r.q[kc], s[b]);
     }
   }
-  if (masked) {
-    // Bit 32 b + 8 (i / 4) + i % 4: whether the row sees key 4 hb further.
-    uint64_t bits = seen >> (4 * hb);
-    const int left = r.limit - j0 - 4 * hb;
-    if (left < 64) bits &= left > 0 ? (uint64_t(1) << left) - 1 : 0;
+}
+
+// Takes out the keys that the row does not see: those whose bit of `seen` is
+// clear and those past its limit.
+template <int NB> __device__ __forceinline__ void hide(f32x16 (&s)[NB], int limit, int j0, uint64_t seen) {
+  const int hb = (threadIdx.x & 63) >> 5;
+  // Bit 32 b + 8 i + j: key 4 hb further.
+  uint64_t bits = seen >> (4 * hb);
+  const int left = limit - j0 - 4 * hb;
+  if (left < 64) bits &= left > 0 ? (uint64_t(1) << left) - 1 : 0;
 #pragma unroll
-    for (int b = 0; b < NB; ++b) {
-      const uint32_t half = static_cast<uint32_t>(bits >> (32 * b));
+  for (int b = 0; b < NB; ++b) {
+    const uint32_t half = static_cast<uint32_t>(bits >> (32 * b));
 #pragma unroll
-      for (int i = 0; i < 16; ++i)
-        if (!(half & (1u << (8 * (i / 4) + i % 4)))) s[b][i] = -INFINITY;
-    }
+    for (int i = 0; i < 16; ++i)
+      if (!(half & (1u << (8 * (i / 4) + i % 4)))) s[b][i] = -INFINITY;
   }
+}
+
+// The largest score of the row in the tile, in powers of two.
+template <int NB> __device__ __forceinline__ float largest(const f32x16 (&s)[NB], float c) {
   float top = s[0][0];
 #pragma unroll
   for (int b = 0; b < NB; ++b)
 #pragma unroll
     for (int i = 0; i < 16; ++i) top = fmaxf(top, s[b][i]);
   const float2 tops = both_halves(top);
-  top = fmaxf(tops.x, tops.y) * c;
-  // The sums keep their reference point until a score passes it by 2^8: the
-  // weights stay below 256, where their relative rounding is the same.
+  return fmaxf(tops.x, tops.y) * c;
+}
+
+// The sums keep their reference point until a score passes it by 2^8: the
+// weights stay below 256, where their relative rounding is the same.
+template <typename T, int D> __device__ __forceinline__ void refer_to(Rows32<T, D> &r, float top) {
   if (__any(top > r.m + 8.f)) {
     const float m = fmaxf(r.m, top);
     const float f = m == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(r.m - m);
@@ -230,91 +256,153 @@ __device__ __forceinline__ void add_tile(Rows32<T, D> &r, uint32_t k, uint32_t v
       for (int i = 0; i < 16; ++i) r.o[t][i] *= f;
     r.m = m;
   }
+}
+
+// Weights, rounded to the type once for the product with V (l sums them
+// before the rounding).
+template <typename T, int D, int NB>
+__device__ __forceinline__ void weigh(Rows32<T, D> &r, const f32x16 (&s)[NB], typename Mma<T>::V8 (&p)[2 * NB], float c) {
   const float base = r.m == -INFINITY ? 0.f : r.m;
 #pragma unroll
   for (int b = 0; b < NB; ++b)
 #pragma unroll
     for (int i = 0; i < 16; ++i) {
-      s[b][i] = __builtin_amdgcn_exp2f(s[b][i] * c - base);
-      r.l += s[b][i];
+      const float w = __builtin_amdgcn_exp2f(s[b][i] * c - base);
+      r.l += w;
+      p[2 * b + i / 8][i % 8] = Mma<T>::from(w);
     }
-  if (cut && has_odd<T, D, NB * 32>(v)) take_odd_out<T, D, NB * 32, NB == 2>(r, v, j0, seen);
-  // O^T += V^T P^T.  The sum over keys may take them in any order: the order
-  // in which a lane holds its 8 of 16 weights, keys 4 hb + {0..3, 8..11}.
-  const int a = lane & 15;
+}
+
+// O^T += V^T P^T.  The sum over keys may take them in any order: the order in
+// which a lane holds its 8 of 16 weights, keys 4 hb + {0..3, 8..11}.
+template <typename T, int D, int NB>
+__device__ __forceinline__ void add_values(Rows32<T, D> &r, uint32_t v, const typename Mma<T>::V8 (&p)[2 * NB]) {
+  using M = Mma<T>;
+  constexpr int kPitch = Geometry<D>::kPitch;
+  const int lane = threadIdx.x & 63, hb = lane >> 5, a = lane & 15;
   const uint32_t vrow = 4 * hb + (a >> 2);
   const uint32_t vx = v_swizzle<D>(vrow);
   const uint32_t vcol = 2 * ((lane >> 4) & 1) + ((a & 3) >> 1);
-  const uint32_t vbase = v + vrow * G::kPitch + (a & 1) * 8;
+  const uint32_t vbase = v + vrow * kPitch + (a & 1) * 8;
 #pragma unroll
-  for (int c2 = 0; c2 < 2 * NB; ++c2) {
-    V8 p;
-#pragma unroll
-    for (int i = 0; i < 8; ++i) p[i] = M::from(s[c2 / 2][8 * (c2 & 1) + i]);
+  for (int c2 = 0; c2 < 2 * NB; ++c2)
 #pragma unroll
     for (int t = 0; t < D / 32; ++t) {
-      const uint32_t at = vbase + (((4 * t + vcol) ^ vx) << 4) + c2 * 16 * G::kPitch;
+      const uint32_t at = vbase + (((4 * t + vcol) ^ vx) << 4) + c2 * 16 * kPitch;
       const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16(reinterpret_cast<LdsS4 *>(at));
-      const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16(reinterpret_cast<LdsS4 *>(at + 8 * G::kPitch));
+      const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16(reinterpret_cast<LdsS4 *>(at + 8 * kPitch));
       const s16x8 x = __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
-      r.o[t] = M::mul(__builtin_bit_cast(V8, x), p, r.o[t]);
+      r.o[t] = M::mul(__builtin_bit_cast(typename M::V8, x), p[c2], r.o[t]);
     }
-  }
 }
 
-// The keys [k0, k1) of one list of blocks, a tile at a time: where a wave's
-// lanes find the rows they load.
-template <int D, int KEYS> struct KeyTiles {
+// Where a group of 16 keys lies: if it is whole, there and in one block of
+// the caches, at k + i * k_token and v + i * v_token.
+struct Place {
+  const uint8_t *k, *v;
+  bool whole;
+};
+
+// The keys [k0, k1) of one list of blocks for one KV head, in groups of 16:
+// 32 keys every `stride` from `first` (a multiple of 16).  A lane looks up a
+// group, so 64 of them at a time; each is then a few reads of a lane.
+struct Keys {
   const AttnArgs &a;
   const int32_t *list;
   uint32_t n_list;
-  int k0, k1;
-  int64_t k_off, v_off;  // of the KV head
-  int page;              // of key `lane` of the next tile, loaded ahead
+  int k0, k1, first, stride;
+  int64_t k_off, v_off;  // of the head
+  bool holes;            // blocks may lie outside the caches: ask for each key
+  int base = 0;          // group of lane 0
+  uint64_t groups = 0;   // which lanes' groups are whole
+  uint64_t k = 0, v = 0;
 
-  __device__ __forceinline__ int key(int j0) const { return j0 + ((threadIdx.x & 63) & (KEYS - 1)); }
-  __device__ __forceinline__ uint32_t block_of(int j) const {
+  __device__ __forceinline__ uint32_t block_of(uint32_t j) const {
     return a.block_size == 1 ? j : __umulhi(j, a.block_mul) >> a.block_shift;
   }
-  __device__ __forceinline__ void fetch(int j0) {
-    const int j = key(j0);
-    page = -1;
-    if (j < k1) {
-      const uint32_t b = block_of(j);
-      if (b < n_list) page = list[b];
-    }
+  // The block of a lane's key, -1 without one.
+  __device__ __forceinline__ int page(int j) const {
+    if (j < k0 || j >= k1) return -1;
+    const uint32_t b = block_of(j);
+    const int p = b < n_list ? list[b] : -1;
+    return static_cast<uint32_t>(p) < a.pages ? p : -1;
   }
-  // Row addresses of the fetched tile (a lane a key), and which keys exist.
-  __device__ __forceinline__ uint64_t rows(int j0, const uint8_t *&k, const uint8_t *&v) const {
-    const int j = key(j0);
-    const bool there = static_cast<uint32_t>(page) < a.pages;
-    const uint32_t at = j - block_of(j) * a.block_size;
-    const uint8_t *z = reinterpret_cast<const uint8_t *>(zero_row);
-    k = there ? a.k + k_off + page * a.k_page + at * a.k_token : z;
-    v = there ? a.v + v_off + page * a.v_page + at * a.v_token : z;
-    const uint64_t seen = __ballot(there);
-    return KEYS == 64 ? seen : seen & 0xffffffffu;
+  __device__ __forceinline__ int key(int g) const { return first + g / 2 * stride + g % 2 * 16; }
+  __device__ __forceinline__ void look_up(int g) {
+    base = g;
+    const int j = key(g + (threadIdx.x & 63));
+    const int p = page(max(j, k0));
+    const int at = j - static_cast<int>(block_of(j) * a.block_size);
+    groups = __ballot(p >= 0 && j >= k0 && j + 16 <= k1 && a.block_size % 16 == 0);
+    if (__any(p < 0 && j + 16 > k0 && j < k1)) holes = true;
+    k = reinterpret_cast<uint64_t>(a.k + k_off) + p * a.k_page + at * a.k_token;
+    v = reinterpret_cast<uint64_t>(a.v + v_off) + p * a.v_page + at * a.v_token;
+  }
+  static __device__ __forceinline__ const uint8_t *lane_of(uint64_t x, int lane) {
+    const uint32_t lo = __builtin_amdgcn_readlane(static_cast<uint32_t>(x), lane);
+    const uint32_t hi = __builtin_amdgcn_readlane(static_cast<uint32_t>(x >> 32), lane);
+    return reinterpret_cast<const uint8_t *>((static_cast<uint64_t>(hi) << 32) | lo);
+  }
+  __device__ __forceinline__ Place place(int g) {
+    if (g - base >= 64) look_up(g & ~63);
+    const int l = g - base;
+    return {lane_of(k, l), lane_of(v, l), ((groups >> l) & 1) != 0};
+  }
+  // Whether all of the N keys from j0 are there; which of them are.
+  template <int N> __device__ __forceinline__ bool all(int j0) const { return j0 >= k0 && j0 + N <= k1 && !holes; }
+  template <int N> __device__ __forceinline__ uint64_t seen(int j0) const {
+    uint64_t bits = N == 64 ? ~uint64_t(0) : (uint64_t(1) << N % 64) - 1;
+    if (j0 < k0) bits &= k0 - j0 < 64 ? ~uint64_t(0) << (k0 - j0) : 0;
+    if (j0 + 64 > k1) bits &= k1 > j0 ? ~uint64_t(0) >> (j0 + 64 - k1) : 0;
+    if (holes) bits &= __ballot(page(j0 + (threadIdx.x & (N - 1))) >= 0);
+    return bits;
   }
 };
 
-__device__ __forceinline__ const uint8_t *from_lane(const uint8_t *p, int lane) {
-  const uint64_t x = reinterpret_cast<uint64_t>(p);
-  const uint32_t lo = __builtin_amdgcn_ds_bpermute(lane * 4, static_cast<int>(x));
-  const uint32_t hi = __builtin_amdgcn_ds_bpermute(lane * 4, static_cast<int>(x >> 32));
-  return reinterpret_cast<const uint8_t *>((static_cast<uint64_t>(hi) << 32) | lo);
+// Load i of the D / 32 loads of a group of 16 rows: this lane's row and
+// piece of it, as an offset from the group's first row.
+template <int D, bool V> __device__ __forceinline__ uint32_t row_offset(int i, int64_t token) {
+  constexpr int kPieces = Geometry<D>::kPieces;
+  const int x = i * 64 + (threadIdx.x & 63), row = x / kPieces;
+  return static_cast<uint32_t>(row * token) + ((x % kPieces) ^ (V ? v_swizzle<D>(row) : k_swizzle<D>(row))) * 16;
 }
 
-// This wave's share (loads w, w + step, ...) of a tile of `rows` key rows.
-template <int D, int ROWS, bool V>
-__device__ __forceinline__ void load_tile(const uint8_t *row, uint32_t lds, int w, int step) {
-  using G = Geometry<D>;
-  const int lane = threadIdx.x & 63;
+// The D / 32 loads of the group of 16 rows from `key`, row by row: where it
+// is not whole.  Rows of zeros stand for the keys that are not there.
+template <int D, bool V> __device__ __forceinline__ void load_single_rows(const Keys &s, int key, uint32_t lds) {
+  constexpr int kPieces = Geometry<D>::kPieces;
+  const AttnArgs &a = s.a;
+#pragma unroll 1
+  for (int i = 0; i < D / 32; ++i) {
+    const int x = i * 64 + (threadIdx.x & 63), row = x / kPieces, j = key + row;
+    const uint32_t piece = ((x % kPieces) ^ (V ? v_swizzle<D>(row) : k_swizzle<D>(row))) * 16;
+    const int p = s.page(j);
+    const int at = j - static_cast<int>(s.block_of(j) * a.block_size);
+    const uint8_t *from = reinterpret_cast<const uint8_t *>(zero_row);
+    if (p >= 0) from = V ? a.v + s.v_off + p * a.v_page + at * a.v_token : a.k + s.k_off + p * a.k_page + at * a.k_token;
+    load_to_lds(from + piece, lds + i * 1024);
+  }
+}
+
+// A group's K or V to LDS, off[i] as row_offset gives it.
+template <int D, bool V>
+__device__ __forceinline__ void load_group(const Keys &s, const Place &at, int key, const uint32_t (&off)[D / 32], uint32_t lds) {
+  if (at.whole) {
 #pragma unroll
-  for (int i0 = 0; i0 < ROWS / 32 * G::kLoads; i0 += step) {
-    const int i = i0 + w;
-    const int x = i * 64 + lane, key = x / G::kPieces, at = x % G::kPieces;
-    const uint32_t piece = at ^ (V ? v_swizzle<D>(key) : k_swizzle<D>(key));
-    load_to_lds(from_lane(row, key) + piece * 16, lds + i * 1024);
+    for (int i = 0; i < D / 32; ++i) load_to_lds(V ? at.v : at.k, off[i], lds + i * 1024);
+  } else {
+    load_single_rows<D, V>(s, key, lds);
+  }
+}
+
+// The query rows are there: waited for here and not in the loops, where the
+// wait would be for all loads under way.
+template <typename T, int D> __device__ __forceinline__ void wait_rows(Rows32<T, D> &r) {
+#pragma unroll
+  for (int kc = 0; kc < D / 16; ++kc) {
+    s16x8 x = __builtin_bit_cast(s16x8, r.q[kc]);
+    asm volatile("" : "+v"(x));
+    r.q[kc] = __builtin_bit_cast(typename Mma<T>::V8, x);
   }
 }
 
@@ -341,8 +429,8 @@ template <typename T, int D> __device__ __forceinline__ void load_rows(const Att
 }
 
 template <int D> struct Lds {
-  static constexpr int kNarrow = 4 * 2 * 32 * D * 2;       // a tile of 32 keys a wave
-  static constexpr int kWide = 2 * 2 * 64 * D * 2;         // two tiles of 64 keys
+  static constexpr int kNarrow = 4 * 2 * 32 * D * 2;       // a block of 32 keys a wave
+  static constexpr int kWide = 2 * 2 * 64 * D * 2;         // two blocks of 64 keys
   static constexpr int kSums = 4 * D * 33 * 4 + 4 * 32 * 8;  // O^T of four waves, and (m, l)
   static constexpr int kBytes = kNarrow > kSums ? (kNarrow > kWide ? kNarrow : kWide) : (kSums > kWide ? kSums : kWide);
 };
@@ -406,61 +494,222 @@ __device__ __forceinline__ void store_part(const AttnArgs &a, const Rows32<T, D>
   }
 }
 
-// Four waves, the same 32 rows, a quarter of the tiles each in LDS of its
-// own: few rows, bound by the bytes of K and V.
+// One wave's sums to their part, straight from the registers.
 template <typename T, int D>
-__device__ __forceinline__ void attend_narrow(const AttnArgs &a, Rows32<T, D> &r, KeyTiles<D, 32> &tiles, int least, uint32_t lds) {
-  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const uint32_t k = lds + wave * (2 * 32 * D * 2), v = k + 32 * D * 2;
-  int j0 = tiles.k0 + 32 * wave;
-  if (j0 >= tiles.k1) return;
-  const uint8_t *kr, *vr;
-  tiles.fetch(j0);
-  uint64_t seen = tiles.rows(j0, kr, vr);
-  load_tile<D, 32, false>(kr, k, 0, 1);
-  load_tile<D, 32, true>(vr, v, 0, 1);
-  tiles.fetch(j0 + 128);
-  for (; j0 < tiles.k1; j0 += 128) {
-    fence_loads();
-    const bool cut = least < min(j0 + 32, tiles.k1);
-    add_tile<T, D, 1>(r, k, v, j0, seen, cut || seen != 0xffffffffu, cut, a.scale2);
-    if (j0 + 128 < tiles.k1) {
-      seen = tiles.rows(j0 + 128, kr, vr);
-      fence_reads();
-      load_tile<D, 32, false>(kr, k, 0, 1);
-      load_tile<D, 32, true>(vr, v, 0, 1);
-      tiles.fetch(j0 + 256);
+__device__ __forceinline__ void store_rows(const AttnArgs &a, const Rows32<T, D> &r, bool dead, int part) {
+  const int hb = (threadIdx.x & 63) >> 5;
+  const float2 ls = both_halves(r.l);
+  if (r.row < 0) return;
+  const int64_t at = part * (static_cast<int64_t>(a.n_tokens) * a.heads) + r.row;
+  const float l = dead ? 0.f : ls.x + ls.y;
+  if (hb == 0) a.part_ml[at] = make_float2(dead ? -INFINITY : r.m, l);
+  if (l == 0.f) return;
+#pragma unroll
+  for (int t = 0; t < D / 32; ++t)
+#pragma unroll
+    for (int b = 0; b < 4; ++b) {
+      f32x4 o;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) o[e] = r.o[t][4 * b + e];
+      *reinterpret_cast<f32x4 *>(a.part_o + at * D + 32 * t + 8 * b + 4 * hb) = o;
     }
+}
+
+// One wave's 32 rows over the blocks of `keys`, in LDS of its own: few rows,
+// bound by the bytes of K and V.  The next block's K is loaded once this
+// one's has been read, while V is used, and its V after that, so some load is
+// always under way.
+template <typename T, int D>
+__device__ __forceinline__ void attend_narrow(const AttnArgs &a, Rows32<T, D> &r, Keys &keys, int least, uint32_t k) {
+  constexpr int kPer = D / 32;  // loads of a group
+  const uint32_t v = k + 32 * D * 2;
+  int j0 = keys.first;
+  if (j0 >= keys.k1) return;
+  uint32_t k_off[kPer], v_off[kPer];
+#pragma unroll
+  for (int i = 0; i < kPer; ++i) {
+    k_off[i] = row_offset<D, false>(i, a.k_token);
+    v_off[i] = row_offset<D, true>(i, a.v_token);
+  }
+  Place lo, hi;
+  auto load_k = [&](int j) {
+    load_group<D, false>(keys, lo, j, k_off, k);
+    load_group<D, false>(keys, hi, j + 16, k_off, k + kPer * 1024);
+  };
+  auto load_v = [&](int j) {
+    load_group<D, true>(keys, lo, j, v_off, v);
+    load_group<D, true>(keys, hi, j + 16, v_off, v + kPer * 1024);
+  };
+  keys.look_up(0);
+  lo = keys.place(0);
+  hi = keys.place(1);
+  load_k(j0);
+  load_v(j0);
+  wait_rows<T, D>(r);
+  for (int b = 0; j0 < keys.k1; j0 += keys.stride, ++b) {
+    const int next = j0 + keys.stride;
+    const bool more = next < keys.k1;
+    const bool cut = least < min(j0 + 32, keys.k1);
+    f32x16 s[1];
+    typename Mma<T>::V8 p[2];
+    wait_loads<2 * kPer>();
+    scores<T, D, 1>(r, k, s);
+    wait_reads();
+    if (more) {
+      lo = keys.place(2 * b + 2);
+      hi = keys.place(2 * b + 3);
+      load_k(next);
+    }
+    uint64_t seen = 0;
+    if (cut || !keys.template all<32>(j0)) {
+      seen = keys.template seen<32>(j0);
+      hide<1>(s, r.limit, j0, seen);
+    }
+    refer_to<T, D>(r, largest<1>(s, a.scale2));
+    weigh<T, D, 1>(r, s, p, a.scale2);
+    if (more) wait_loads<2 * kPer>();
+    else wait_loads<0>();
+    if (cut && has_odd<T, D, 32>(v)) take_odd_out<T, D, 32, false>(r, v, j0, seen);
+    add_values<T, D, 1>(r, v, p);
+    wait_reads();
+    if (more) load_v(next);
   }
 }
 
-// Four waves of 32 rows each over tiles of 64 keys that they share: many
-// rows, bound by the matrix cores.
+// Four waves of 32 rows each over blocks of 64 keys that they share: many
+// rows, bound by the matrix cores.  The scores of the next block are computed
+// beside the weights of this one, and their maximum beside the product with
+// V: a wave has a SIMD to itself, or shares it with one that waits for
+// memory, and has to keep matrix and vector units busy.  K and V have two
+// buffers each, K a block ahead.  Each wave loads a group of 16 keys.
 template <typename T, int D>
-__device__ __forceinline__ void attend_wide(const AttnArgs &a, Rows32<T, D> &r, KeyTiles<D, 64> &tiles, int least, uint32_t lds) {
+__device__ __forceinline__ void attend_wide(const AttnArgs &a, Rows32<T, D> &r, Keys &keys, int least, uint32_t lds) {
+  using M = Mma<T>;
+  using V8 = typename M::V8;
+  constexpr int kPer = D / 32, kSteps = D / 8, kPitch = Geometry<D>::kPitch;
+  constexpr uint32_t kBlock = 64 * kPitch, kGroup = 16 * kPitch;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  constexpr uint32_t kTile = 64 * D * 2;
-  int j0 = tiles.k0;
-  const uint8_t *kr, *vr;
-  tiles.fetch(j0);
-  uint64_t seen = tiles.rows(j0, kr, vr);
-  load_tile<D, 64, false>(kr, lds, wave, 4);
-  load_tile<D, 64, true>(vr, lds + kTile, wave, 4);
-  tiles.fetch(j0 + 64);
-  for (int stage = 0; j0 < tiles.k1; j0 += 64, stage ^= 1) {
-    fence_loads();
+  const float c = a.scale2;
+  const int k0 = keys.k0, k1 = keys.k1, n = (k1 - k0 + 63) / 64;
+  uint32_t k_off[kPer], v_off[kPer];
+#pragma unroll
+  for (int i = 0; i < kPer; ++i) {
+    k_off[i] = row_offset<D, false>(i, a.k_token);
+    v_off[i] = row_offset<D, true>(i, a.v_token);
+  }
+  const uint32_t own = lds + wave * kGroup;
+  keys.look_up(0);
+  Place now = keys.place(wave), last;  // of the block whose K, and the one whose V is loaded
+  load_group<D, false>(keys, now, k0 + 16 * wave, k_off, own);
+  load_group<D, true>(keys, now, k0 + 16 * wave, v_off, own + 2 * kBlock);
+  if (n > 1) {
+    now = keys.place(4 + wave);
+    load_group<D, false>(keys, now, k0 + 64 + 16 * wave, k_off, own + kBlock);
+  }
+  wait_rows<T, D>(r);
+  wait_loads<0>();
+  __syncthreads();
+  f32x16 s[2];
+  scores<T, D, 2>(r, lds, s);
+  uint64_t seen = 0;
+  bool cut = least < min(k0 + 64, k1);
+  if (cut || !keys.template all<64>(k0)) {
+    seen = keys.template seen<64>(k0);
+    hide<2>(s, r.limit, k0, seen);
+  }
+  float top = largest<2>(s, c);
+  const int lane = threadIdx.x & 63, row = lane & 31, hb = lane >> 5, al = lane & 15;
+  const uint32_t vrow = 4 * hb + (al >> 2), vcol = 2 * ((lane >> 4) & 1) + ((al & 3) >> 1);
+  // A lane's first row and 16-byte piece of K and V.
+  uint32_t krow = row * kPitch, kpiece = hb ^ k_swizzle<D>(row);
+  uint32_t vlane = vrow * kPitch + (al & 1) * 8, vpiece = vcol ^ v_swizzle<D>(vrow);
+#pragma unroll 1
+  for (int j = 0; j < n; ++j) {
+    // K of the next block and V of this one are there, and every wave has
+    // read K of this one and V of the last one.
+    wait_loads<0>();
     __syncthreads();
-    const uint64_t now = seen;
-    if (j0 + 64 < tiles.k1) {
-      const uint32_t to = lds + (stage ^ 1) * 2 * kTile;
-      seen = tiles.rows(j0 + 64, kr, vr);
-      load_tile<D, 64, false>(kr, to, wave, 4);
-      load_tile<D, 64, true>(vr, to + kTile, wave, 4);
-      tiles.fetch(j0 + 128);
+    const int j0 = k0 + 64 * j;
+    const uint32_t odd = (j & 1) * kBlock;
+    if (j + 1 < n) {
+      last = now;
+      if (j + 2 < n) {
+        now = keys.place(4 * (j + 2) + wave);
+        load_group<D, false>(keys, now, j0 + 128 + 16 * wave, k_off, own + odd);
+      }
+      load_group<D, true>(keys, last, j0 + 64 + 16 * wave, v_off, own + 2 * kBlock + (kBlock - odd));
     }
-    const uint32_t at = lds + stage * 2 * kTile;
-    const bool cut = least < min(j0 + 64, tiles.k1);
-    add_tile<T, D, 2>(r, at, at + kTile, j0, now, cut || now != ~uint64_t(0), cut, a.scale2);
+    const uint32_t k = lds + (kBlock - odd), v = lds + 2 * kBlock + odd;
+    // (addresses are computed in each block and not kept in registers)
+    asm volatile("" : "+v"(krow), "+v"(kpiece), "+v"(vlane), "+v"(vpiece));
+    refer_to<T, D>(r, top);
+    const float base = r.m == -INFINITY ? 0.f : r.m;
+    auto read_k = [&](int x) {
+      return *reinterpret_cast<const LdsS8 *>(k + krow + (((2 * (x / 2)) ^ kpiece) << 4) + x % 2 * 32 * kPitch);
+    };
+    auto read_v = [&](int c2, int t) {
+      const uint32_t at = v + vlane + (((4 * t) ^ vpiece) << 4) + c2 * 16 * kPitch;
+      const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16(reinterpret_cast<LdsS4 *>(at));
+      const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16(reinterpret_cast<LdsS4 *>(at + 8 * kPitch));
+      return static_cast<s16x8>(__builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
+    };
+    V8 p[4];
+    auto weigh_one = [&](int i) {
+      const float w = __builtin_amdgcn_exp2f(s[i / 16][i % 16] * c - base);
+      r.l += w;
+      p[i / 8][i % 8] = M::from(w);
+    };
+    s16x8 kf[8];
+#pragma unroll
+    for (int x = 0; x < 8; ++x) kf[x] = read_k(x);
+#pragma unroll
+    for (int i = 0; i < 16; ++i) weigh_one(i);
+    __builtin_amdgcn_sched_barrier(0);
+    f32x16 next[2];
+#pragma unroll
+    for (int b = 0; b < 2; ++b)
+#pragma unroll
+      for (int i = 0; i < 16; ++i) next[b][i] = 0.f;
+#pragma unroll
+    for (int x = 0; x < kSteps; ++x) {
+      next[x % 2] = M::mul(__builtin_bit_cast(V8, kf[x % 8]), r.q[x / 2], next[x % 2]);
+      if (x + 8 < kSteps) kf[x % 8] = read_k(x + 8);
+      // Between the products: the other half of the weights.
+#pragma unroll
+      for (int i = 16 + x * 16 / kSteps; i < 16 + (x + 1) * 16 / kSteps; ++i) weigh_one(i);
+      __builtin_amdgcn_sched_barrier(0);
+    }
+    // (the weights are computed here, not where they are used)
+#pragma unroll
+    for (int x = 0; x < 4; ++x) {
+      s16x8 y = __builtin_bit_cast(s16x8, p[x]);
+      asm volatile("" : "+v"(y));
+      p[x] = __builtin_bit_cast(V8, y);
+    }
+    if (cut && has_odd<T, D, 64>(v)) take_odd_out<T, D, 64, true>(r, v, j0, seen);
+    s16x8 vf[2][kPer];
+#pragma unroll
+    for (int t = 0; t < kPer; ++t) vf[0][t] = read_v(0, t);
+    s[0] = next[0];
+    s[1] = next[1];
+    cut = least < min(j0 + 128, k1);
+    if (cut || !keys.template all<64>(j0 + 64)) {
+      seen = keys.template seen<64>(j0 + 64);
+      hide<2>(s, r.limit, j0 + 64, seen);
+    }
+    top = s[0][0];
+#pragma unroll
+    for (int x = 0; x < kSteps; ++x) {
+      const int t = x % kPer, c2 = x / kPer;
+      r.o[t] = M::mul(__builtin_bit_cast(V8, vf[c2 % 2][t]), p[c2], r.o[t]);
+      if (c2 < 3) vf[(c2 + 1) % 2][t] = read_v(c2 + 1, t);
+      // Between the products: the next block's maximum.
+#pragma unroll
+      for (int i = x * 32 / kSteps; i < (x + 1) * 32 / kSteps; ++i) top = fmaxf(top, s[i / 16][i % 16]);
+      __builtin_amdgcn_sched_barrier(0);
+    }
+    const float2 tops = both_halves(top);
+    top = fmaxf(tops.x, tops.y) * c;
   }
 }
 
@@ -502,6 +751,15 @@ template <bool ALL> __device__ __forceinline__ int least_limit(int limit, uint8_
   return __builtin_amdgcn_readfirstlane(limit);
 }
 
+// Keys of one part of a request with `own` keys of its own: parts enough to
+// fill the chip, of one tile at least and 8 where requests are many (a part's
+// start and end cost about two tiles' time), and no more than there are.
+__device__ __forceinline__ int own_chunk(const AttnArgs &a, int own) {
+  own = max(own, 1);
+  const int most = (own + a.own_parts - 1) / a.own_parts, fill = min(kOwnChunk, (own + a.own_want - 1) / a.own_want);
+  return (max(most, fill) + 31) / 32 * 32;
+}
+
 // The first workgroups take the prefix, the others the requests' own keys:
 // the long ones start first, one on every other CU or so, and both kinds run
 // beside each other (dealing them in turn instead put all prefix work on half
@@ -526,36 +784,39 @@ template <typename T, int D, bool WIDE> __global__ void __launch_bounds__(256, D
       else limit = limit_of(a, q, t);
     }
     load_rows<T, D>(a, r, t, h * a.group + (t < 0 ? 0 : x % a.group), limit);
-    KeyTiles<D, WIDE ? 64 : 32> tiles{a, a.shared, a.shared_width, part * a.prefix_chunk,
-                                      min(a.shared_len, (part + 1) * a.prefix_chunk), h * a.k_head, h * a.v_head, -1};
+    const int k0 = part * a.prefix_chunk, k1 = min(a.shared_len, k0 + a.prefix_chunk);
+    Keys keys{a, a.shared, a.shared_width, k0, k1, k0 + (WIDE ? 0 : 32 * wave), WIDE ? 32 : 128, h * a.k_head, h * a.v_head,
+              a.block_size % 16 != 0};
     const int least = least_limit<WIDE>(r.limit, lds);
-    if constexpr (WIDE) attend_wide<T, D>(a, r, tiles, least, at);
-    else attend_narrow<T, D>(a, r, tiles, least, at);
+    if constexpr (WIDE) attend_wide<T, D>(a, r, keys, least, at);
+    else attend_narrow<T, D>(a, r, keys, least, at + wave * (2 * 32 * D * 2));
     store_part<T, D, !WIDE>(a, r, limit <= 0, part, lds);
     return;
   }
-  // A request's own keys.
-  const int item = (group - a.prefix_groups) * 8 + xcd;
+  // A request's own keys: a wave an item, on its own.  The KV heads of a
+  // request are neighbours, so that a workgroup reads whole rows of tokens.
+  const int item = ((blockIdx.x - a.prefix_groups * 8) * 4 + wave);
   if (item >= a.own_items) return;
+  // (the parts that only long requests have come last: in turn they would
+  // fall on some XCDs alone)
   const int h = item % a.kv_heads, y = item / a.kv_heads;
-  const int part = y % a.own_parts, z = y / a.own_parts;
-  const int first = z % a.own_tiles, q = z / a.own_tiles;
+  const int first = y % a.own_tiles, z = y / a.own_tiles;
+  const int q = z % a.n_requests, part = z / a.n_requests;
   const int t0 = max(0, a.starts[q]), t1 = min(a.n_tokens, a.starts[q + 1]);
   const int n_rows = max(0, t1 - t0) * a.group;
   const int end = t1 > t0 ? limit_of(a, q, t1 - 1) : 0;
-  // The part's keys, whole rounds of the four waves' tiles.
-  const int own = max(0, end - a.shared_len);
-  const int chunk = ((own + a.own_parts - 1) / a.own_parts + 127) / 128 * 128;
-  const int k0 = a.shared_len + min(own, part * chunk), k1 = a.shared_len + min(own, (part + 1) * chunk);
+  // Parts from a multiple of 32 keys: only the first one begins inside a group.
+  const int from = a.shared_len & ~31, chunk = own_chunk(a, end - from);
+  const int k0 = from + min(part * chunk, max(0, end - from));
   for (int m = first * 32; m < n_rows; m += a.own_tiles * 32) {
     const int x = m + n;
     const int t = x < n_rows ? t0 + x / a.group : -1;
     const int limit = t >= 0 ? limit_of(a, q, t) : 0;
     load_rows<T, D>(a, r, t, h * a.group + (t < 0 ? 0 : x % a.group), limit);
-    KeyTiles<D, 32> tiles{a, a.table + q * a.table_stride, a.width, k0, k1, h * a.k_head, h * a.v_head, -1};
-    attend_narrow<T, D>(a, r, tiles, least_limit<false>(r.limit, lds), at);
-    store_part<T, D, true>(a, r, limit <= 0, a.prefix_parts + part, lds);
-    __syncthreads();
+    Keys keys{a, a.table + q * a.table_stride, a.width, max(a.shared_len, k0), min(end, k0 + chunk), k0, 32, h * a.k_head,
+              h * a.v_head, a.block_size % 16 != 0};
+    attend_narrow<T, D>(a, r, keys, least_limit<false>(r.limit, lds), at + wave * (2 * 32 * D * 2));
+    store_rows<T, D>(a, r, limit <= 0, a.prefix_parts + part);
   }
 }
 
@@ -577,17 +838,27 @@ template <typename T, int D> __global__ void __launch_bounds__(256) join_parts(A
   float m = -INFINITY, l = 0.f;
   f32x4 o = {0.f, 0.f, 0.f, 0.f};
   if (live) {
-#pragma unroll 4
-    for (int p = wave; p < parts; p += 4) {
-      const float2 w = a.part_ml[p * rows + row];
-      if (w.y == 0.f) continue;
-      const f32x4 x = *reinterpret_cast<const f32x4 *>(a.part_o + (p * rows + row) * D + d);
-      const float top = fmaxf(m, w.x), base = top == -INFINITY ? 0.f : top;
-      const float f = __builtin_amdgcn_exp2f(m - base), g = __builtin_amdgcn_exp2f(w.x - base);
-      l = l * f + w.y * g;
+    for (int p0 = wave; p0 < parts; p0 += 16) {
+      float2 w[4];
+      f32x4 x[4];
 #pragma unroll
-      for (int e = 0; e < 4; ++e) o[e] = o[e] * f + x[e] * g;
-      m = top;
+      for (int k = 0; k < 4; ++k) {
+        const int p = p0 + 4 * k;
+        w[k] = p < parts ? a.part_ml[p * rows + row] : make_float2(-INFINITY, 0.f);
+      }
+#pragma unroll
+      for (int k = 0; k < 4; ++k)
+        if (w[k].y != 0.f) x[k] = *reinterpret_cast<const f32x4 *>(a.part_o + ((p0 + 4 * k) * rows + row) * D + d);
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        if (w[k].y == 0.f) continue;
+        const float top = fmaxf(m, w[k].x), base = top == -INFINITY ? 0.f : top;
+        const float f = __builtin_amdgcn_exp2f(m - base), g = __builtin_amdgcn_exp2f(w[k].x - base);
+        l = l * f + w[k].y * g;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) o[e] = o[e] * f + x[k][e] * g;
+        m = top;
+      }
     }
     sums[wave][lane] = o;
     if (d == 0) weights[wave][i] = make_float2(m, l);
@@ -650,7 +921,7 @@ constexpr int64_t kMaxKeys = int64_t(1) << 30;
 struct Plan {
   bool wide;
   int prefix_tiles, prefix_parts, prefix_chunk;
-  int own_tiles, own_parts;
+  int own_tiles, own_parts, own_want;
 };
 
 Plan make_plan(int64_t T, int64_t R, int64_t kv_heads, int64_t group, int64_t shared_len, int64_t table_keys) {
@@ -663,16 +934,17 @@ Plan make_plan(int64_t T, int64_t R, int64_t kv_heads, int64_t group, int64_t sh
   p.own_tiles = static_cast<int>(std::max<int64_t>(1, (per + 31) / 32));
   const int64_t own = std::max<int64_t>(0, table_keys - shared_len);
   const int64_t items = p.prefix_tiles * kv_heads, own_items = R * kv_heads * p.own_tiles;
-  // Two workgroups fit a CU.  The prefix gets its share of those 512 places,
-  // at a key of its own in half of the time of a request's own key (which
-  // comes from memory, while all row tiles read the prefix; requests have
-  // half of their tables' keys on the average), so that both end together:
-  // 256 requests, 32 heads over 16384 keys, 1024 own: 178 us; with twice the
-  // share 195, with three times 215.  A part has four wide tiles or one round
-  // of narrow ones at least: it costs a row of 32-bit sums to write and read.
+  // Two workgroups fit a CU.  The prefix gets 3/2 of its share of those 512
+  // places, at a key of its own in half of the time of a request's own key
+  // (which comes from memory, while all row tiles read the prefix; requests
+  // are taken to have half of their tables' keys, 512 at most), so that both
+  // end together: 256 requests, 32 heads over 16384 keys, 1024 own: 169 us,
+  // with two thirds of that 180, with five thirds 194.  A part has four wide
+  // blocks or one round of narrow ones at least: it costs a row of 32-bit
+  // sums to write and read.
   const double prefix_cost = static_cast<double>(items) * shared_len;
-  const double own_cost = static_cast<double>(own_items) * own * 1.0;
-  const int64_t places = static_cast<int64_t>(512 * prefix_cost / (prefix_cost + own_cost + 1));
+  const double own_cost = static_cast<double>(own_items) * std::min<int64_t>(own, 1024);
+  const int64_t places = static_cast<int64_t>(std::min(512.0, 768 * prefix_cost / (prefix_cost + own_cost + 1)));
   const int64_t most = std::max<int64_t>(1, shared_len / (p.wide ? 4 * tile : tile));
   p.prefix_parts = shared_len == 0 ? 0 : static_cast<int>(std::min<int64_t>(most, std::max<int64_t>(1, (places + items / 2) / items)));
   p.prefix_chunk = 0;
@@ -680,8 +952,13 @@ Plan make_plan(int64_t T, int64_t R, int64_t kv_heads, int64_t group, int64_t sh
     p.prefix_chunk = static_cast<int>(((shared_len + p.prefix_parts - 1) / p.prefix_parts + tile - 1) / tile * tile);
     p.prefix_parts = static_cast<int>((shared_len + p.prefix_chunk - 1) / p.prefix_chunk);
   }
-  const int64_t own_most = std::max<int64_t>(1, (own + 255) / 256);
-  p.own_parts = static_cast<int>(std::min<int64_t>(own_most, std::max<int64_t>(1, 512 / own_items)));
+  // Own keys: parts enough to fill the chip and of kOwnChunk keys at most, up
+  // to 8, or to 64 where that makes 4096 waves; a request takes those that its
+  // length calls for (own_chunk).
+  p.own_want = static_cast<int>(std::max<int64_t>(1, (2048 + own_items - 1) / own_items));
+  const int64_t own_most = std::min<int64_t>(std::max<int64_t>(8, std::min<int64_t>(64, 4096 / own_items)),
+                                             std::max<int64_t>(p.own_want, (own + 31 + kOwnChunk - 1) / kOwnChunk));
+  p.own_parts = static_cast<int>(std::max<int64_t>(1, std::min<int64_t>(own_most, (own + 62) / 32)));
   return p;
 }
 
@@ -812,10 +1089,11 @@ extern "C" int lmc_shared_prefix_attention(const lmc_tensor *query, const lmc_te
     a.prefix_tiles = p.prefix_tiles;
     a.prefix_chunk = p.prefix_chunk;
     a.own_tiles = p.own_tiles;
+    a.own_want = p.own_want;
     const int64_t own_items = R * kv.heads * p.own_tiles * p.own_parts;
     check_value(own_items <= INT32_MAX / 2, "too many rows");
     a.own_items = static_cast<int>(own_items);
-    const int64_t own_groups = (own_items + 7) / 8;
+    const int64_t own_groups = (own_items + 31) / 32;
     const int64_t prefix_groups = (kv.heads * p.prefix_parts + 7) / 8 * p.prefix_tiles;
     a.prefix_groups = static_cast<int>(prefix_groups);
     DeviceGuard guard(dev);

@@ -171,6 +171,17 @@ def test_table_shorter_than_the_request(ops):
     _check(ops, c)
 
 
+@pytest.mark.parametrize("R", [1, 40])
+def test_tables_much_wider_than_the_requests(ops, R):
+    """Tables as wide as the longest context: most parts of the own keys are
+    empty, and what lies in the tables behind a request is not read."""
+    c = _case(17, [1] * R, [290 + 5 * r for r in range(R)], 270, 16, 8, 2, 64)
+    wide = torch.full((R, 4000), 2**30, dtype=torch.int32)
+    wide[:, : c["table"].shape[1]] = c["table"]
+    c["table"] = wide
+    _check(ops, c)
+
+
 def test_lengths_far_past_the_table(ops):
     """A request said to be 2^31 - 1 long ends where its table's row ends."""
     c = _case(16, [1, 2, 1], [96, 80, 64], 40, 16, 4, 2, 64)
