@@ -328,13 +328,20 @@ struct Keys {
     return static_cast<uint32_t>(p) < a.pages ? p : -1;
   }
   __device__ __forceinline__ int key(int g) const { return first + g / 2 * stride + g % 2 * 16; }
-  __device__ __forceinline__ void look_up(int g) {
+  // The entry of the list for this lane's group of the 64 from g, and what
+  // follows from it (apart, so that other loads can be under way between).
+  __device__ __forceinline__ int entry(int g) const {
+    const uint32_t b = block_of(min(max(key(g + (threadIdx.x & 63)), k0), k1));
+    return n_list ? list[min(b, n_list - 1)] : -1;
+  }
+  __device__ __forceinline__ void look_up(int g, int entry) {
     base = g;
     const int j = key(g + (threadIdx.x & 63));
-    const int p = page(max(j, k0));
+    const bool in = j + 16 > k0 && j < k1;
+    const int p = in && block_of(max(j, k0)) < n_list && static_cast<uint32_t>(entry) < a.pages ? entry : -1;
     const int at = j - static_cast<int>(block_of(j) * a.block_size);
     groups = __ballot(p >= 0 && j >= k0 && j + 16 <= k1 && a.block_size % 16 == 0);
-    if (__any(p < 0 && j + 16 > k0 && j < k1)) holes = true;
+    if (__any(in && p < 0)) holes = true;
     k = reinterpret_cast<uint64_t>(a.k + k_off) + p * a.k_page + at * a.k_token;
     v = reinterpret_cast<uint64_t>(a.v + v_off) + p * a.v_page + at * a.v_token;
   }
@@ -344,7 +351,7 @@ struct Keys {
     return reinterpret_cast<const uint8_t *>((static_cast<uint64_t>(hi) << 32) | lo);
   }
   __device__ __forceinline__ Place place(int g) {
-    if (g - base >= 64) look_up(g & ~63);
+    if (g - base >= 64) look_up(g & ~63, entry(g & ~63));
     const int l = g - base;
     return {lane_of(k, l), lane_of(v, l), ((groups >> l) & 1) != 0};
   }
@@ -520,7 +527,7 @@ __device__ __forceinline__ void store_rows(const AttnArgs &a, const Rows32<T, D>
 // one's has been read, while V is used, and its V after that, so some load is
 // always under way.
 template <typename T, int D>
-__device__ __forceinline__ void attend_narrow(const AttnArgs &a, Rows32<T, D> &r, Keys &keys, int least, uint32_t k) {
+__device__ __forceinline__ void attend_narrow(const AttnArgs &a, Rows32<T, D> &r, Keys &keys, int entry, int least, uint32_t k) {
   constexpr int kPer = D / 32;  // loads of a group
   const uint32_t v = k + 32 * D * 2;
   int j0 = keys.first;
@@ -540,7 +547,7 @@ __device__ __forceinline__ void attend_narrow(const AttnArgs &a, Rows32<T, D> &r
     load_group<D, true>(keys, lo, j, v_off, v);
     load_group<D, true>(keys, hi, j + 16, v_off, v + kPer * 1024);
   };
-  keys.look_up(0);
+  keys.look_up(0, entry);
   lo = keys.place(0);
   hi = keys.place(1);
   load_k(j0);
@@ -583,7 +590,7 @@ __device__ __forceinline__ void attend_narrow(const AttnArgs &a, Rows32<T, D> &r
 // memory, and has to keep matrix and vector units busy.  K and V have two
 // buffers each, K a block ahead.  Each wave loads a group of 16 keys.
 template <typename T, int D>
-__device__ __forceinline__ void attend_wide(const AttnArgs &a, Rows32<T, D> &r, Keys &keys, int least, uint32_t lds) {
+__device__ __forceinline__ void attend_wide(const AttnArgs &a, Rows32<T, D> &r, Keys &keys, int entry, int least, uint32_t lds) {
   using M = Mma<T>;
   using V8 = typename M::V8;
   constexpr int kPer = D / 32, kSteps = D / 8, kPitch = Geometry<D>::kPitch;
@@ -598,7 +605,7 @@ __device__ __forceinline__ void attend_wide(const AttnArgs &a, Rows32<T, D> &r, 
     v_off[i] = row_offset<D, true>(i, a.v_token);
   }
   const uint32_t own = lds + wave * kGroup;
-  keys.look_up(0);
+  keys.look_up(0, entry);
   Place now = keys.place(wave), last;  // of the block whose K, and the one whose V is loaded
   load_group<D, false>(keys, now, k0 + 16 * wave, k_off, own);
   load_group<D, true>(keys, now, k0 + 16 * wave, v_off, own + 2 * kBlock);
@@ -713,29 +720,44 @@ __device__ __forceinline__ void attend_wide(const AttnArgs &a, Rows32<T, D> &r, 
   }
 }
 
-// The request of token t, or -1: the number of requests that start at or
-// before it, less one.
-__device__ __forceinline__ int request_of(const AttnArgs &a, int t) {
-  const int R = a.n_requests;
-  int r = min(t, R - 1);  // one token a request, the usual case
-  if (!(a.starts[r] <= t && t < a.starts[r + 1])) {
-    int lo = 0, hi = R;   // the first of 0 .. R whose start lies behind t
+// Keys that token t sees of a request of `seq` keys whose tokens end at
+// `stop`; there are none behind the table's row.
+__device__ __forceinline__ int limit_of(const AttnArgs &a, int seq, int stop, int t) {
+  const int64_t n = static_cast<int64_t>(seq) - stop + t + 1;
+  return static_cast<int>(max(static_cast<int64_t>(0), min(n, static_cast<int64_t>(a.max_keys))));
+}
+
+// The request of a token: tried first as one token a request (a load of all
+// that is needed then, before the answer is known), else by bisection.
+struct Request {
+  int r, start, stop, seq, end;
+
+  __device__ __forceinline__ Request(const AttnArgs &a, int t) {
+    r = min(max(t, 0), a.n_requests - 1);
+    start = a.starts[r];
+    stop = a.starts[r + 1];
+    seq = a.seq_lens[r];
+    end = a.starts[a.n_requests];
+  }
+  // False if token t is none of a request's.
+  __device__ __forceinline__ bool find(const AttnArgs &a, int t) {
+    if (start <= t && t < stop) return true;
+    if (t >= end) return false;
+    int lo = 0, hi = a.n_requests;  // the first of 0 .. R whose start lies behind t
     while (lo < hi) {
       const int mid = (lo + hi) >> 1;
       if (a.starts[mid] > t) hi = mid;
       else lo = mid + 1;
     }
+    if (lo == 0) return false;
     r = lo - 1;
-    if (r < 0 || r >= R || a.starts[R] <= t) return -1;
+    stop = a.starts[lo];
+    seq = a.seq_lens[r];
+    return true;
   }
-  return r;
-}
+};
 
-// Keys that token t of request r sees; there are none behind the table's row.
-__device__ __forceinline__ int limit_of(const AttnArgs &a, int r, int t) {
-  const int64_t n = static_cast<int64_t>(a.seq_lens[r]) - a.starts[r + 1] + t + 1;
-  return static_cast<int>(max(static_cast<int64_t>(0), min(n, static_cast<int64_t>(a.max_keys))));
-}
+typedef const __attribute__((address_space(4))) int32_t *ScalarInts;
 
 // The least limit of a wave's rows, or (ALL) of the four waves'.
 template <bool ALL> __device__ __forceinline__ int least_limit(int limit, uint8_t *lds) {
@@ -778,18 +800,19 @@ template <typename T, int D, bool WIDE> __global__ void __launch_bounds__(256, D
     const int h = pair % a.kv_heads, part = pair / a.kv_heads;
     const int x = tile * (WIDE ? 128 : 32) + (WIDE ? wave * 32 : 0) + n;
     int t = x < a.n_tokens * a.group ? x / a.group : -1, limit = 0;
-    if (t >= 0) {
-      const int q = request_of(a, t);
-      if (q < 0) t = -1;
-      else limit = limit_of(a, q, t);
-    }
-    load_rows<T, D>(a, r, t, h * a.group + (t < 0 ? 0 : x % a.group), limit);
     const int k0 = part * a.prefix_chunk, k1 = min(a.shared_len, k0 + a.prefix_chunk);
     Keys keys{a, a.shared, a.shared_width, k0, k1, k0 + (WIDE ? 0 : 32 * wave), WIDE ? 32 : 128, h * a.k_head, h * a.v_head,
               a.block_size % 16 != 0};
+    const int entry = keys.entry(0);
+    Request q(a, t);
+    if (t >= 0) {
+      if (q.find(a, t)) limit = limit_of(a, q.seq, q.stop, t);
+      else t = -1;
+    }
+    load_rows<T, D>(a, r, t, h * a.group + (t < 0 ? 0 : x % a.group), limit);
     const int least = least_limit<WIDE>(r.limit, lds);
-    if constexpr (WIDE) attend_wide<T, D>(a, r, keys, least, at);
-    else attend_narrow<T, D>(a, r, keys, least, at + wave * (2 * 32 * D * 2));
+    if constexpr (WIDE) attend_wide<T, D>(a, r, keys, entry, least, at);
+    else attend_narrow<T, D>(a, r, keys, entry, least, at + wave * (2 * 32 * D * 2));
     store_part<T, D, !WIDE>(a, r, limit <= 0, part, lds);
     return;
   }
@@ -802,20 +825,30 @@ template <typename T, int D, bool WIDE> __global__ void __launch_bounds__(256, D
   const int h = item % a.kv_heads, y = item / a.kv_heads;
   const int first = y % a.own_tiles, z = y / a.own_tiles;
   const int q = z % a.n_requests, part = z / a.n_requests;
-  const int t0 = max(0, a.starts[q]), t1 = min(a.n_tokens, a.starts[q + 1]);
+  const ScalarInts starts = (ScalarInts)(a.starts + q), seq_lens = (ScalarInts)(a.seq_lens + q);
+  const int start = starts[0], stop = starts[1], seq = seq_lens[0];
+  const int t0 = max(0, start), t1 = min(a.n_tokens, stop);
   const int n_rows = max(0, t1 - t0) * a.group;
-  const int end = t1 > t0 ? limit_of(a, q, t1 - 1) : 0;
+  const int end = t1 > t0 ? limit_of(a, seq, stop, t1 - 1) : 0;
   // Parts from a multiple of 32 keys: only the first one begins inside a group.
   const int from = a.shared_len & ~31, chunk = own_chunk(a, end - from);
   const int k0 = from + min(part * chunk, max(0, end - from));
   for (int m = first * 32; m < n_rows; m += a.own_tiles * 32) {
     const int x = m + n;
     const int t = x < n_rows ? t0 + x / a.group : -1;
-    const int limit = t >= 0 ? limit_of(a, q, t) : 0;
-    load_rows<T, D>(a, r, t, h * a.group + (t < 0 ? 0 : x % a.group), limit);
+    const int limit = t >= 0 ? limit_of(a, seq, stop, t) : 0;
+    const int head = h * a.group + (t < 0 ? 0 : x % a.group);
     Keys keys{a, a.table + q * a.table_stride, a.width, max(a.shared_len, k0), min(end, k0 + chunk), k0, 32, h * a.k_head,
               h * a.v_head, a.block_size % 16 != 0};
-    attend_narrow<T, D>(a, r, keys, least_limit<false>(r.limit, lds), at + wave * (2 * 32 * D * 2));
+    if (keys.k0 >= keys.k1) {  // an empty part
+      if (t >= 0 && lane < 32)
+        a.part_ml[(a.prefix_parts + part) * (static_cast<int64_t>(a.n_tokens) * a.heads) + t * a.heads + head] =
+            make_float2(-INFINITY, 0.f);
+      continue;
+    }
+    const int entry = keys.entry(0);
+    load_rows<T, D>(a, r, t, head, limit);
+    attend_narrow<T, D>(a, r, keys, entry, least_limit<false>(r.limit, lds), at + wave * (2 * 32 * D * 2));
     store_rows<T, D>(a, r, limit <= 0, a.prefix_parts + part);
   }
 }
@@ -833,22 +866,23 @@ template <typename T, int D> __global__ void __launch_bounds__(256) join_parts(A
   const int64_t row = static_cast<int64_t>(blockIdx.x) * kRows + i;
   const bool there = i < kRows && row < rows;
   const int t = there ? static_cast<int>(row / a.heads) : -1, h = static_cast<int>(row % a.heads);
-  const bool live = t >= a.starts[0] && t < a.starts[a.n_requests];
   const int parts = a.prefix_parts + a.own_parts;
+  auto weight = [&](int p) { return there && p < parts ? a.part_ml[p * rows + row] : make_float2(-INFINITY, 0.f); };
+  float2 w[4];
+#pragma unroll
+  for (int k = 0; k < 4; ++k) w[k] = weight(wave + 4 * k);
+  const bool live = t >= a.starts[0] && t < a.starts[a.n_requests];
   float m = -INFINITY, l = 0.f;
   f32x4 o = {0.f, 0.f, 0.f, 0.f};
   if (live) {
     for (int p0 = wave; p0 < parts; p0 += 16) {
-      float2 w[4];
       f32x4 x[4];
-#pragma unroll
-      for (int k = 0; k < 4; ++k) {
-        const int p = p0 + 4 * k;
-        w[k] = p < parts ? a.part_ml[p * rows + row] : make_float2(-INFINITY, 0.f);
-      }
 #pragma unroll
       for (int k = 0; k < 4; ++k)
         if (w[k].y != 0.f) x[k] = *reinterpret_cast<const f32x4 *>(a.part_o + ((p0 + 4 * k) * rows + row) * D + d);
+      float2 next[4];
+#pragma unroll
+      for (int k = 0; k < 4; ++k) next[k] = weight(p0 + 16 + 4 * k);
 #pragma unroll
       for (int k = 0; k < 4; ++k) {
         if (w[k].y == 0.f) continue;
@@ -859,13 +893,14 @@ template <typename T, int D> __global__ void __launch_bounds__(256) join_parts(A
         for (int e = 0; e < 4; ++e) o[e] = o[e] * f + x[k][e] * g;
         m = top;
       }
+#pragma unroll
+      for (int k = 0; k < 4; ++k) w[k] = next[k];
     }
     sums[wave][lane] = o;
     if (d == 0) weights[wave][i] = make_float2(m, l);
   }
   __syncthreads();
   if (wave != 0 || !live) return;
-  float2 w[4];
   float top = -INFINITY;
 #pragma unroll
   for (int g = 0; g < 4; ++g) {
@@ -945,7 +980,7 @@ Plan make_plan(int64_t T, int64_t R, int64_t kv_heads, int64_t group, int64_t sh
   const double prefix_cost = static_cast<double>(items) * shared_len;
   const double own_cost = static_cast<double>(own_items) * std::min<int64_t>(own, 1024);
   const int64_t places = static_cast<int64_t>(std::min(512.0, 768 * prefix_cost / (prefix_cost + own_cost + 1)));
-  const int64_t most = std::max<int64_t>(1, shared_len / (p.wide ? 4 * tile : tile));
+  const int64_t most = p.wide ? std::max<int64_t>(1, shared_len / (4 * tile)) : (shared_len + tile - 1) / tile;
   p.prefix_parts = shared_len == 0 ? 0 : static_cast<int>(std::min<int64_t>(most, std::max<int64_t>(1, (places + items / 2) / items)));
   p.prefix_chunk = 0;
   if (p.prefix_parts) {
