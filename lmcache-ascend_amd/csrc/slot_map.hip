@@ -18,6 +18,10 @@
 // and last token, so long prompts search once a wave.  A page that this call
 // takes from the free list is read from the list, not from the table, which
 // another workgroup is writing.
+//
+// A decode step's few tokens are latency: launch, lengths, pages, store.
+// Requests of a few new tokens need no search, and their pages are loaded
+// beside the sums.
 #include "serving.h"
 
 namespace lmc {
@@ -43,6 +47,7 @@ struct SlotMapArgs {
   int64_t n_free;
   const int64_t *cursor;       // null: 0
   int64_t *next_cursor;        // may be null
+  int token_blocks;            // workgroups of the tokens; those behind them complete the table
 };
 
 constexpr uint32_t kTop = 0x7fffffffu;
@@ -72,38 +77,72 @@ __device__ __forceinline__ int find(const uint32_t *sums, int lo, int hi, uint32
   return lo;
 }
 
+// Adds of the lanes below, in the wave's registers.
+__device__ __forceinline__ uint32_t sums_to(uint32_t x) {
+#define LMC_STEP(ctrl, rows) x = add_sat(x, __builtin_amdgcn_update_dpp(0, x, ctrl, rows, 0xf, false))
+  LMC_STEP(0x111, 0xf);  // 1, 2, 4 and 8 lanes down within 16
+  LMC_STEP(0x112, 0xf);
+  LMC_STEP(0x114, 0xf);
+  LMC_STEP(0x118, 0xf);
+  LMC_STEP(0x142, 0xa);  // the 16 lanes before, and the 32 before
+  LMC_STEP(0x143, 0xc);
+#undef LMC_STEP
+  return x;
+}
+
+// Requests of at most this many new tokens are written by the thread that
+// summed them up: no search, and the page is loaded beside the sums.
+constexpr uint32_t kShort = 8;
+constexpr int kUnroll = 4;  // tokens of a lane that are under way together
+
 __global__ void __launch_bounds__(1024) slot_map(SlotMapArgs a) {
   extern __shared__ uint32_t lds[];
   const int R = a.n_requests, nt = blockDim.x, tid = threadIdx.x;
   const int lane = tid & 63, wave = tid >> 6;
   const bool grow = a.grow != 0;
   uint32_t *sq = lds, *sb = lds + R + 1;  // sums before each request; sb only with a free list
-  __shared__ uint32_t part[2][kWaves];
-  uint32_t carry_q = 0, carry_b = 0;
+  __shared__ uint32_t part[3][kWaves];
+  uint32_t carry_q = 0, carry_b = 0, any_long = 0;
+  const int64_t cursor = grow && a.cursor ? *a.cursor : 0;
+  const int64_t cap = static_cast<int64_t>(a.width) * a.block_size;  // < 2^31
+  auto free_at = [&](int64_t i) {
+    i += cursor;
+    return i >= 0 && i < a.n_free ? a.free_blocks[i] : -1;
+  };
+  auto write = [&](int64_t t, int64_t pos, uint32_t at, int32_t page) {
+    a.slots[t] = page >= 0 ? static_cast<int64_t>(page) * a.block_size + at : -1;
+    if (a.positions) a.positions[t] = pos;
+  };
   for (int r0 = 0; r0 < R; r0 += nt) {
     const int r = r0 + tid;
-    uint32_t q = 0, b = 0;
+    const bool mine = r < R && (r0 / nt) % a.token_blocks == static_cast<int>(blockIdx.x);
+    uint32_t q = 0, b = 0, have = a.width;
+    int64_t c = 0;
+    int32_t page = -1;
     if (r < R) {
-      const int64_t ql = len_at(a.query_lens, a.lens_i64, r), cl = len_at(a.context_lens, a.lens_i64, r);
+      const int64_t ql = len_at(a.query_lens, a.lens_i64, r);
+      c = len_at(a.context_lens, a.lens_i64, r);
       q = static_cast<uint32_t>(ql < kTop ? ql : kTop);
-      const int64_t end = cl > INT64_MAX - ql ? INT64_MAX : cl + ql;
-      if (grow) b = pages_for(end, a) - pages_for(cl, a);
+      const int64_t end = c > INT64_MAX - ql ? INT64_MAX : c + ql;
+      if (grow) {
+        have = pages_for(c, a);
+        b = pages_for(end, a) - have;
+      }
+      if (mine && q && q <= kShort && c < cap) {
+        const uint32_t j = static_cast<uint32_t>(c) / a.block_size;
+        if (j < have) page = a.table[r * a.table_stride + j];
+      }
       if (blockIdx.x == 0 && a.seq_lens) a.seq_lens[r] = static_cast<int32_t>(end < kTop ? end : kTop);
     }
-    uint32_t iq = q, ib = b;  // inclusive sums of the wave
-    for (int d = 1; d < 64; d <<= 1) {
-      const uint32_t uq = __shfl_up(iq, d), ub = __shfl_up(ib, d);
-      if (lane >= d) {
-        iq = add_sat(iq, uq);
-        ib = add_sat(ib, ub);
-      }
-    }
+    const uint32_t iq = sums_to(q), ib = grow ? sums_to(b) : 0;
     // (not iq - q: the sum may have stopped at its top)
     uint32_t eq = __shfl_up(iq, 1), eb = __shfl_up(ib, 1);
     if (lane == 0) eq = eb = 0;
+    const bool longer = __any(q > kShort);
     if (lane == 63) {
       part[0][wave] = iq;
       part[1][wave] = ib;
+      part[2][wave] = longer;
     }
     __syncthreads();
     uint32_t bq = carry_q, bb = carry_b;
@@ -114,12 +153,28 @@ __global__ void __launch_bounds__(1024) slot_map(SlotMapArgs a) {
       }
       carry_q = add_sat(carry_q, part[0][w]);
       carry_b = add_sat(carry_b, part[1][w]);
+      any_long |= part[2][w];
     }
+    const uint32_t start = add_sat(bq, eq), before_b = add_sat(bb, eb);
     if (r < R) {
-      const uint32_t before_q = add_sat(bq, eq), before_b = add_sat(bb, eb);
-      sq[r] = before_q;
+      sq[r] = start;
       if (grow) sb[r] = before_b;
-      if (blockIdx.x == 0 && a.starts) a.starts[r] = static_cast<int32_t>(before_q);
+      if (blockIdx.x == 0 && a.starts) a.starts[r] = static_cast<int32_t>(start);
+    }
+    if (mine && q <= kShort) {
+      for (uint32_t i = 0; i < q && start + i < a.n_tokens; ++i) {
+        const int64_t pos = c + i;
+        uint32_t at = 0;
+        if (pos >= 0 && pos < cap) {
+          const uint32_t p = static_cast<uint32_t>(pos), j = p / a.block_size;
+          at = p - j * a.block_size;
+          if (j >= have) page = free_at(static_cast<int64_t>(before_b) + (j - have));
+          else if (i && at == 0) page = a.table[r * a.table_stride + j];
+        } else {
+          page = -1;
+        }
+        write(start + i, pos, at, page);
+      }
     }
     __syncthreads();
   }
@@ -128,45 +183,67 @@ __global__ void __launch_bounds__(1024) slot_map(SlotMapArgs a) {
     if (grow) sb[R] = carry_b;
     if (blockIdx.x == 0) {
       if (a.starts) a.starts[R] = static_cast<int32_t>(carry_q);
-      if (grow && a.next_cursor) *a.next_cursor = (a.cursor ? *a.cursor : 0) + carry_b;
+      if (grow && a.next_cursor) *a.next_cursor = cursor + carry_b;
     }
   }
   __syncthreads();
-  const int64_t cursor = grow && a.cursor ? *a.cursor : 0;
-  auto free_at = [&](int64_t i) {
-    i += cursor;
-    return i >= 0 && i < a.n_free ? a.free_blocks[i] : -1;
-  };
-  const int64_t step = static_cast<int64_t>(gridDim.x) * nt;
-  const int64_t first = static_cast<int64_t>(blockIdx.x) * nt + tid;
-
-  for (int64_t t = first; t < a.n_tokens; t += step) {
-    int64_t pos = 0, slot = -1;
-    if (t < carry_q) {
-      // The wave's tokens t - lane .. t + 63 - lane lie between two requests.
-      const uint32_t x = static_cast<uint32_t>(t), x0 = x - lane;
-      const uint32_t x1 = static_cast<uint32_t>(min(static_cast<int64_t>(x0) + 63, static_cast<int64_t>(carry_q) - 1));
-      const int lo = find(sq, 0, R - 1, __builtin_amdgcn_readfirstlane(x0));
-      const int hi = find(sq, lo, R - 1, __builtin_amdgcn_readfirstlane(x1));
-      const int r = find(sq, lo, hi, x);
-      const int64_t c = len_at(a.context_lens, a.lens_i64, r);
-      pos = c + (x - sq[r]);
-      if (pos < static_cast<int64_t>(a.width) * a.block_size) {
-        const uint32_t p = static_cast<uint32_t>(pos), j = p / a.block_size;
-        const uint32_t have = grow ? pages_for(c, a) : a.width;
-        const int32_t page = j < have ? a.table[r * a.table_stride + j] : free_at(static_cast<int64_t>(sb[r]) + (j - have));
-        if (page >= 0) slot = static_cast<int64_t>(page) * a.block_size + (p - j * a.block_size);
-      }
-    }
-    a.slots[t] = slot;
-    if (a.positions) a.positions[t] = pos;
-  }
-  if (grow) {
-    for (int64_t u = first; u < carry_b; u += step) {
+  // New table entries, in workgroups of their own.
+  if (static_cast<int>(blockIdx.x) >= a.token_blocks) {
+    const int64_t step = static_cast<int64_t>(gridDim.x - a.token_blocks) * nt;
+    for (int64_t u = static_cast<int64_t>(blockIdx.x - a.token_blocks) * nt + tid; u < carry_b; u += step) {
+      const int32_t page = free_at(u);
       const int r = find(sb, 0, R - 1, static_cast<uint32_t>(u));
       const uint32_t j = pages_for(len_at(a.context_lens, a.lens_i64, r), a) + static_cast<uint32_t>(u - sb[r]);
-      a.table[r * a.table_stride + j] = free_at(u);
+      a.table[r * a.table_stride + j] = page;
     }
+    return;
+  }
+  const int64_t step = static_cast<int64_t>(a.token_blocks) * nt;
+
+  // Tokens of the longer requests, kUnroll times 64 of them a wave, and the
+  // entries behind the last token.
+  const int64_t total = carry_q;
+  int64_t t0 = (static_cast<int64_t>(blockIdx.x) * nt + wave * 64) * kUnroll;
+  if (!any_long) t0 += total / (step * kUnroll) * (step * kUnroll);
+  for (; t0 < a.n_tokens; t0 += step * kUnroll) {
+    int lo = 0, hi = 0;
+    if (t0 < total && any_long) {
+      lo = find(sq, 0, R - 1, static_cast<uint32_t>(t0));
+      hi = find(sq, lo, R - 1, static_cast<uint32_t>(min(t0 + 64 * kUnroll, total) - 1));
+    }
+    int64_t pos[kUnroll];
+    int r[kUnroll];
+    int32_t page[kUnroll];
+    uint32_t at[kUnroll];
+    bool todo[kUnroll];
+#pragma unroll
+    for (int u = 0; u < kUnroll; ++u) {
+      const int64_t t = t0 + 64 * u + lane;
+      todo[u] = t < a.n_tokens && (t >= total || any_long);
+      r[u] = -1;
+      pos[u] = 0;
+      if (todo[u] && t < total) {
+        r[u] = find(sq, lo, hi, static_cast<uint32_t>(t));
+        todo[u] = sq[r[u] + 1] - sq[r[u]] > kShort;
+        if (todo[u]) pos[u] = len_at(a.context_lens, a.lens_i64, r[u]);
+      }
+    }
+#pragma unroll
+    for (int u = 0; u < kUnroll; ++u) {
+      page[u] = -1;
+      at[u] = 0;
+      if (!todo[u] || r[u] < 0) continue;
+      const uint32_t have = grow ? pages_for(pos[u], a) : a.width;
+      pos[u] += static_cast<uint32_t>(t0 + 64 * u + lane) - sq[r[u]];
+      if (pos[u] >= 0 && pos[u] < cap) {
+        const uint32_t p = static_cast<uint32_t>(pos[u]), j = p / a.block_size;
+        at[u] = p - j * a.block_size;
+        page[u] = j < have ? a.table[r[u] * a.table_stride + j] : free_at(static_cast<int64_t>(sb[r[u]]) + (j - have));
+      }
+    }
+#pragma unroll
+    for (int u = 0; u < kUnroll; ++u)
+      if (todo[u]) write(t0 + 64 * u + lane, pos[u], at[u], page[u]);
   }
 }
 
@@ -202,7 +279,7 @@ extern "C" int lmc_build_slot_mapping(const lmc_tensor *query_lens, const lmc_te
     check_value(block_size > 0 && block_size < (int64_t(1) << 31), "block_size must be positive");
     check_value(bt.sizes[1] == 0 || block_size <= INT32_MAX / bt.sizes[1], "a block_table row spans 2^31 positions or more");
     check_value(R * bt.sizes[1] <= INT32_MAX, "block_table has 2^31 entries or more");
-    check_value(N <= INT32_MAX, "slot_mapping has 2^31 entries or more");
+    check_value(N <= INT32_MAX - 65536, "slot_mapping has too many entries");
     SlotMapArgs a;
     std::memset(&a, 0, sizeof(a));
     a.query_lens = ql.data;
@@ -263,14 +340,17 @@ extern "C" int lmc_build_slot_mapping(const lmc_tensor *query_lens, const lmc_te
     if (R == 0 && N == 0 && !a.starts && !a.next_cursor) return;
     DeviceGuard guard(dev);
     const int nt = R > 256 ? 1024 : 256;
-    const int64_t entries = std::max(N, a.grow ? R * bt.sizes[1] / 16 : int64_t(0));
-    const int64_t blocks = std::min<int64_t>(std::max<int64_t>(1, (entries + 4 * nt - 1) / (4 * nt)), 1024);
+    const int64_t blocks = std::min<int64_t>(std::max<int64_t>(1, (N + kUnroll * nt - 1) / (kUnroll * nt)), 1024);
+    a.token_blocks = static_cast<int>(blocks);
+    // About a new page a request and a block of new tokens.
+    const int64_t pages = std::min(R * bt.sizes[1], R + N / block_size);
+    const int64_t table_blocks = a.grow ? std::min<int64_t>(std::max<int64_t>(1, (pages + nt - 1) / nt), 256) : 0;
     const size_t shared = (a.grow ? 2 : 1) * (R + 1) * sizeof(uint32_t);
     if (shared > 48 * 1024)
       hip_check(hipFuncSetAttribute(reinterpret_cast<const void *>(slot_map), hipFuncAttributeMaxDynamicSharedMemorySize,
                                     static_cast<int>(shared)),
                 "slot_map shared memory");
-    hipLaunchKernelGGL(slot_map, dim3(static_cast<uint32_t>(blocks)), dim3(nt), shared, static_cast<hipStream_t>(stream), a);
+    hipLaunchKernelGGL(slot_map, dim3(static_cast<uint32_t>(blocks + table_blocks)), dim3(nt), shared, static_cast<hipStream_t>(stream), a);
     hip_check(hipGetLastError(), "slot_map launch");
   });
 }

@@ -106,6 +106,27 @@ def test_lengths_whose_sum_passes_32_bits(ops):
     _run(ops, [3, 2**40, 7], [0, 2**62, 5], table, 8, 100, lens=torch.int64)
 
 
+def test_short_and_long_requests_in_one_batch(ops):
+    """Requests of 7, 8 and 9 new tokens, of none and of thousands, next to
+    each other and behind the first 256."""
+    for seed, R in ((1, 40), (2, 700)):
+        rng = np.random.default_rng(seed)
+        query = rng.choice([0, 1, 7, 8, 9, 10, 65, 2000 if R < 100 else 300], R).tolist()
+        context = rng.integers(0, 200, R)
+        width = (200 + 2001) // 16 + 1
+        table = rng.permutation(R * width).reshape(R, width)
+        _run(ops, query, context.tolist(), table, 16, sum(query) + 11)
+        for r in range(R):
+            table[r, -(-context[r] // 16):] = -1
+        _run(ops, query, context.tolist(), table, 16, sum(query) + 11, rng.permutation(R * width).tolist(), 5)
+
+
+def test_contexts_at_the_top_of_64_bits(ops):
+    table = np.arange(6).reshape(2, 3)
+    for q in (3, 40):
+        _run(ops, [q, 2], [2**63 - 1 - q, 4], table, 8, q + 5, lens=torch.int64)
+
+
 def test_slots_past_32_bits(ops):
     table = np.array([[2**31 - 1, 2**30]], np.int64)
     _run(ops, [20], [0], table, 16, 20)
