@@ -18,7 +18,8 @@
 // rounded once.
 //
 // HBM-bound: each element is read and written once.  A lane moves VP pairs
-// (two 16-byte accesses each way where the layout allows).
+// (two 16-byte accesses each way where the layout allows); 16384 tokens of 32
+// query and 8 KV heads of 128 bf16 dims to their pages take 73 us, 5.4 TB/s.
 #include "rope_math.h"
 #include "serving.h"
 
@@ -81,12 +82,88 @@ struct RotaryArgs {
 };
 
 constexpr int kThreads = 256;
-constexpr int kMaxTokens = 8;  // per workgroup
+constexpr int kMaxTokens = 2;  // per workgroup
+
+// Rounded to the type once (by the conversion instructions).
+template <typename KD> __device__ __forceinline__ typename KD::S rounded(float x);
+template <> __device__ __forceinline__ uint16_t rounded<BF16>(float x) { return __builtin_bit_cast(uint16_t, static_cast<__bf16>(x)); }
+template <> __device__ __forceinline__ uint16_t rounded<F16>(float x) { return __builtin_bit_cast(uint16_t, static_cast<_Float16>(x)); }
+template <> __device__ __forceinline__ float rounded<F32>(float x) { return x; }
+
+// VP pairs: a and b are their first and second halves, or 2 VP elements of
+// interleaved pairs in order.
+template <typename KD, bool NEOX, int VP>
+__device__ __forceinline__ void turn(typename VecOf<VP * sizeof(typename KD::S)>::T &a,
+                                     typename VecOf<VP * sizeof(typename KD::S)>::T &b, const float *c, const float *s) {
+  using S = typename KD::S;
+  using V = typename VecOf<VP * sizeof(S)>::T;
+  using P = Pack<S, VP>;
+  S in[2 * VP], out[2 * VP];
+  P u = __builtin_bit_cast(P, a), v = __builtin_bit_cast(P, b);
+#pragma unroll
+  for (int i = 0; i < VP; ++i) {
+    in[i] = u.v[i];
+    in[VP + i] = v.v[i];
+  }
+#pragma unroll
+  for (int i = 0; i < VP; ++i) {
+    const int i1 = NEOX ? i : 2 * i, i2 = NEOX ? VP + i : 2 * i + 1;
+    const float x1 = to_f32<KD>(in[i1]), x2 = to_f32<KD>(in[i2]);
+    out[i1] = rounded<KD>(x1 * c[i] - x2 * s[i]);
+    out[i2] = rounded<KD>(x2 * c[i] + x1 * s[i]);
+  }
+#pragma unroll
+  for (int i = 0; i < VP; ++i) {
+    u.v[i] = out[i];
+    v.v[i] = out[VP + i];
+  }
+  a = __builtin_bit_cast(V, u);
+  b = __builtin_bit_cast(V, v);
+}
+
+// The units of one tensor's rows of this workgroup's tokens: TURN rotates the
+// first of each head and copies the others, else all are copied.
+template <typename KD, bool NEOX, int VP, bool TURN>
+__device__ __forceinline__ void rows_of(const RotaryArgs &a, const Rows &rows, int64_t t0, int nt, const float *cosv,
+                                        const float *sinv, const int64_t *paged_row) {
+  using S = typename KD::S;
+  using V = typename VecOf<VP * sizeof(S)>::T;
+  // Streaming stores: 8192 tokens of 40 heads take 29 us with them, 38
+  // without; few tokens the same either way.
+  auto store = [&](S *to, V v) { __builtin_nontemporal_store(v, reinterpret_cast<V *>(to)); };
+  const uint32_t total = nt * rows.units, step = kThreads * gridDim.y, turned = TURN ? a.half / VP : 0;
+  uint32_t x = blockIdx.y * kThreads + threadIdx.x;
+  if (x >= total) return;
+  uint32_t t = x / rows.units, w = x - t * rows.units;
+  for (; x < total; x += step) {
+    const uint32_t h = rows.per_head == 1 ? w : __umulhi(w, rows.magic), u = w - h * rows.per_head;
+    const int64_t at = rows.paged ? paged_row[t] : (t0 + t) * rows.out_token;
+    const S *in = static_cast<const S *>(rows.in) + (t0 + t) * rows.in_token + h * rows.in_head;
+    if (at >= 0) {
+      S *out = static_cast<S *>(rows.out) + at + h * rows.out_head;
+      if (u < turned) {
+        const uint32_t i0 = u * VP;
+        const uint32_t e1 = a.offset + (NEOX ? i0 : 2 * i0), e2 = e1 + (NEOX ? a.half : VP);
+        V p = *reinterpret_cast<const V *>(in + e1), q = *reinterpret_cast<const V *>(in + e2);
+        turn<KD, NEOX, VP>(p, q, cosv + t * a.half + i0, sinv + t * a.half + i0);
+        store(out + e1, p);
+        store(out + e2, q);
+      } else {
+        uint32_t e = (u - turned) * VP;
+        if (TURN && e >= static_cast<uint32_t>(a.offset)) e += 2 * a.half;
+        store(out + e, *reinterpret_cast<const V *>(in + e));
+      }
+    }
+    w += step;
+    while (w >= rows.units) {
+      w -= rows.units;
+      ++t;
+    }
+  }
+}
 
 template <typename KD, bool NEOX, int VP>
 __global__ void __launch_bounds__(kThreads) rotary_rows(RotaryArgs a) {
-  using S = typename KD::S;
-  using V = Pack<S, VP>;
   extern __shared__ float cs[];  // cos [tokens][half], then sin
   __shared__ int64_t row_k[kMaxTokens], row_v[kMaxTokens];
   const int tid = threadIdx.x;
@@ -114,68 +191,9 @@ __global__ void __launch_bounds__(kThreads) rotary_rows(RotaryArgs a) {
     row_v[tid] = rv;
   }
   __syncthreads();
-
-  const uint32_t total = nt * a.units;
-  const uint32_t chunk = (total + gridDim.y - 1) / gridDim.y;
-  const uint32_t end = min(total, (blockIdx.y + 1) * chunk);
-  uint32_t x = blockIdx.y * chunk + tid;
-  uint32_t t = x / a.units, w = x - t * a.units;
-  const uint32_t turned = a.half / VP;
-  for (; x < end; x += kThreads) {
-    const bool is_q = w < a.q.units, is_k = !is_q && w < a.q.units + a.k.units;
-    const Rows &rows = is_q ? a.q : is_k ? a.k : a.v;
-    const uint32_t y = w - (is_q ? 0 : is_k ? a.q.units : a.q.units + a.k.units);
-    const uint32_t h = rows.per_head == 1 ? y : __umulhi(y, rows.magic), u = y - h * rows.per_head;
-    const S *in = static_cast<const S *>(rows.in) + (t0 + t) * rows.in_token + h * rows.in_head;
-    const int64_t at = rows.paged ? (is_k ? row_k[t] : row_v[t]) : (t0 + t) * rows.out_token;
-    S *out = static_cast<S *>(rows.out) + at + h * rows.out_head;
-    if (at >= 0) {
-      if ((is_q || is_k) && u < turned) {
-        const int i0 = u * VP;
-        const int e1 = a.offset + (NEOX ? i0 : 2 * i0), e2 = NEOX ? e1 + a.half : e1 + VP;
-        const V p = *reinterpret_cast<const V *>(in + e1), r = *reinterpret_cast<const V *>(in + e2);
-        const float *c = cosv + t * a.half + i0, *s = sinv + t * a.half + i0;
-        V o1, o2;
-        if constexpr (NEOX) {
-#pragma unroll
-          for (int i = 0; i < VP; ++i) {
-            const float x1 = to_f32<KD>(p.v[i]), x2 = to_f32<KD>(r.v[i]);
-            o1.v[i] = from_f32<KD>(x1 * c[i] - x2 * s[i]);
-            o2.v[i] = from_f32<KD>(x2 * c[i] + x1 * s[i]);
-          }
-        } else {
-          S in2[2 * VP], out2[2 * VP];
-#pragma unroll
-          for (int i = 0; i < VP; ++i) {
-            in2[i] = p.v[i];
-            in2[VP + i] = r.v[i];
-          }
-#pragma unroll
-          for (int i = 0; i < VP; ++i) {
-            const float x1 = to_f32<KD>(in2[2 * i]), x2 = to_f32<KD>(in2[2 * i + 1]);
-            out2[2 * i] = from_f32<KD>(x1 * c[i] - x2 * s[i]);
-            out2[2 * i + 1] = from_f32<KD>(x2 * c[i] + x1 * s[i]);
-          }
-#pragma unroll
-          for (int i = 0; i < VP; ++i) {
-            o1.v[i] = out2[i];
-            o2.v[i] = out2[VP + i];
-          }
-        }
-        *reinterpret_cast<V *>(out + e1) = o1;
-        *reinterpret_cast<V *>(out + e2) = o2;
-      } else {
-        int e = ((is_q || is_k) ? u - turned : u) * VP;
-        if ((is_q || is_k) && e >= a.offset) e += 2 * a.half;
-        *reinterpret_cast<V *>(out + e) = *reinterpret_cast<const V *>(in + e);
-      }
-    }
-    w += kThreads;
-    while (w >= a.units) {
-      w -= a.units;
-      ++t;
-    }
-  }
+  if (a.q.units) rows_of<KD, NEOX, VP, true>(a, a.q, t0, nt, cosv, sinv, nullptr);
+  if (a.k.units) rows_of<KD, NEOX, VP, true>(a, a.k, t0, nt, cosv, sinv, row_k);
+  if (a.v.units) rows_of<KD, NEOX, VP, false>(a, a.v, t0, nt, nullptr, nullptr, row_v);
 }
 
 template <typename KD, bool NEOX, int VP> void launch(const RotaryArgs &a, hipStream_t s) {
@@ -387,10 +405,10 @@ void rotary(const lmc_tensor *positions, const lmc_tensor *query, const lmc_tens
   a.inverse = inverse;
   a.n_tokens = T;
   check_value(T <= INT32_MAX, "too many tokens");
-  // Several tokens share a workgroup once there are workgroups enough, as
-  // long as their angles fit 16 KiB.
-  int tb = 1;
-  while (tb < kMaxTokens && T / (2 * tb) >= 1024 && tb * 2 * n_freq * 8 <= 16384) tb *= 2;
+  // Two tokens share a workgroup once there are workgroups enough (their
+  // angles then fill its lanes): 16384 tokens of 32 + 8 + 8 heads to their
+  // pages take 73 us with two, 74 with one, 79 with four and 93 with eight.
+  const int tb = T >= 2048 ? kMaxTokens : 1;
   a.tokens_per_block = tb;
   check_value(static_cast<int64_t>(tb) * units <= INT32_MAX, "rows are too wide");
   DeviceGuard guard(dev);
