@@ -929,7 +929,8 @@ template <typename T, int D> __global__ void __launch_bounds__(256) join_parts(A
 
 template <typename T, int D> void launch(const AttnArgs &a, bool wide, uint32_t groups, hipStream_t s) {
   const void *fn = wide ? reinterpret_cast<const void *>(attend<T, D, true>) : reinterpret_cast<const void *>(attend<T, D, false>);
-  hip_check(hipFuncSetAttribute(fn, hipFuncAttributeMaxDynamicSharedMemorySize, Lds<D>::kBytes), "attend shared memory");
+  if (Lds<D>::kBytes > 64 * 1024)
+    hip_check(hipFuncSetAttribute(fn, hipFuncAttributeMaxDynamicSharedMemorySize, Lds<D>::kBytes), "attend shared memory");
   if (wide) hipLaunchKernelGGL((attend<T, D, true>), dim3(groups * 8), dim3(256), Lds<D>::kBytes, s, a);
   else hipLaunchKernelGGL((attend<T, D, false>), dim3(groups * 8), dim3(256), Lds<D>::kBytes, s, a);
   hip_check(hipGetLastError(), "attend launch");
@@ -1026,43 +1027,43 @@ extern "C" int lmc_shared_prefix_attention(const lmc_tensor *query, const lmc_te
     check_on(bt, "block_table", dev, LMC_I32);
     check_vector(sl, "seq_lens", dev, LMC_I32);
     check_vector(qs, "query_start_loc", dev, LMC_I32);
-    check_value(kv.dim == 64 || kv.dim == 96 || kv.dim == 128 || kv.dim == 192 || kv.dim == 256,
+    expect(kv.dim == 64 || kv.dim == 96 || kv.dim == 128 || kv.dim == 192 || kv.dim == 256,
                 "shared_prefix_attention takes heads of 64, 96, 128, 192 or 256 dims");
-    check_value(q.ndim == 3 && o.ndim == 3, "query and output must be [tokens, heads, dim]");
+    expect(q.ndim == 3 && o.ndim == 3, "query and output must be [tokens, heads, dim]");
     const int64_t T = q.sizes[0], R = sl.sizes[0], Hq = q.sizes[1];
     for (int i = 0; i < 3; ++i) {
-      check_value(q.sizes[i] == o.sizes[i], "query and output differ in shape");
-      check_value(q.strides[i] >= 0 && o.strides[i] >= 0, "negative strides unsupported");
+      expect(q.sizes[i] == o.sizes[i], "query and output differ in shape");
+      expect(q.strides[i] >= 0 && o.strides[i] >= 0, "negative strides unsupported");
     }
-    check_value(q.sizes[2] == kv.dim, "query heads are not of the caches' dim");
-    check_value(q.strides[2] == 1 && o.strides[2] == 1, "a head's dims must be adjacent");
-    check_value(Hq % kv.heads == 0, "query heads are not a multiple of the caches' heads");
-    check_value(qs.sizes[0] == R + 1, "query_start_loc must have one entry per request and one more");
-    check_value(bt.ndim == 2 && bt.sizes[0] == R, "block_table must be [requests, pages]");
-    check_value(bt.sizes[1] <= 1 || bt.strides[1] == 1, "block_table rows must be contiguous");
-    check_value(shared_len >= 0 && shared_len <= kMaxKeys, "shared_len must be between 0 and 2^30");
-    check_value(bt.sizes[1] * kv.block_size <= kMaxKeys, "a block_table row spans more than 2^30 keys");
-    check_value((shared_len + kv.block_size - 1) / kv.block_size <= sb.sizes[0], "shared_blocks has too few blocks for shared_len");
-    check_value(scale > 0 && std::isfinite(scale), "scale must be positive and finite");
+    expect(q.sizes[2] == kv.dim, "query heads are not of the caches' dim");
+    expect(q.strides[2] == 1 && o.strides[2] == 1, "a head's dims must be adjacent");
+    expect(Hq % kv.heads == 0, "query heads are not a multiple of the caches' heads");
+    expect(qs.sizes[0] == R + 1, "query_start_loc must have one entry per request and one more");
+    expect(bt.ndim == 2 && bt.sizes[0] == R, "block_table must be [requests, pages]");
+    expect(bt.sizes[1] <= 1 || bt.strides[1] == 1, "block_table rows must be contiguous");
+    expect(shared_len >= 0 && shared_len <= kMaxKeys, "shared_len must be between 0 and 2^30");
+    expect(bt.sizes[1] * kv.block_size <= kMaxKeys, "a block_table row spans more than 2^30 keys");
+    expect((shared_len + kv.block_size - 1) / kv.block_size <= sb.sizes[0], "shared_blocks has too few blocks for shared_len");
+    expect(scale > 0 && std::isfinite(scale), "scale must be positive and finite");
     AttnArgs a;
     std::memset(&a, 0, sizeof(a));
     if (lse) {
       const lmc_tensor &e = deref(lse, "lse");
       check_on(e, "lse", dev, LMC_F32);
-      check_value(e.ndim == 2 && e.sizes[0] == T && e.sizes[1] == Hq, "lse must be [tokens, heads]");
+      expect(e.ndim == 2 && e.sizes[0] == T && e.sizes[1] == Hq, "lse must be [tokens, heads]");
       a.lse = static_cast<float *>(e.data);
       a.lse_token = e.strides[0];
       a.lse_head = e.strides[1];
     }
     auto on_16 = [](int64_t x) { return x % 16 == 0; };
-    check_value(on_16(reinterpret_cast<intptr_t>(kv.k)) && on_16(reinterpret_cast<intptr_t>(kv.v)) && on_16(kv.k_page) &&
+    expect(on_16(reinterpret_cast<intptr_t>(kv.k)) && on_16(reinterpret_cast<intptr_t>(kv.v)) && on_16(kv.k_page) &&
                     on_16(kv.k_token) && on_16(kv.k_head) && on_16(kv.v_page) && on_16(kv.v_token) && on_16(kv.v_head),
                 "the paged caches' rows must start on 16-byte boundaries");
-    check_value(on_16(reinterpret_cast<intptr_t>(q.data)) && on_16(q.strides[0] * 2) && on_16(q.strides[1] * 2) &&
+    expect(on_16(reinterpret_cast<intptr_t>(q.data)) && on_16(q.strides[0] * 2) && on_16(q.strides[1] * 2) &&
                     on_16(reinterpret_cast<intptr_t>(o.data)) && on_16(o.strides[0] * 2) && on_16(o.strides[1] * 2),
                 "rows of query and output must start on 16-byte boundaries");
-    check_value(rows_apart({T, Hq, kv.dim}, {o.strides[0], o.strides[1], 1}), "output has overlapping rows");
-    check_value(T * Hq <= INT32_MAX / 128 && R <= INT32_MAX / 4096, "too many rows");
+    expect(rows_apart({T, Hq, kv.dim}, {o.strides[0], o.strides[1], 1}), "output has overlapping rows");
+    expect(T * Hq <= INT32_MAX / 128 && R <= INT32_MAX / 4096, "too many rows");
     const int64_t group = kv.heads ? Hq / kv.heads : 0;
     if (workspace_bytes) *workspace_bytes = 0;
     if (T == 0 || Hq == 0 || R == 0) return;
@@ -1076,9 +1077,9 @@ extern "C" int lmc_shared_prefix_attention(const lmc_tensor *query, const lmc_te
     }
     const lmc_tensor &ws = deref(workspace, "workspace");
     check_on(ws, "workspace", dev, LMC_U8);
-    check_value(ws.ndim == 1 && (ws.sizes[0] <= 1 || ws.strides[0] == 1) && ws.sizes[0] >= bytes &&
+    expect(ws.ndim == 1 && (ws.sizes[0] <= 1 || ws.strides[0] == 1) && ws.sizes[0] >= bytes &&
                     on_16(reinterpret_cast<intptr_t>(ws.data)),
-                "workspace must be 1-D, contiguous, on a 16-byte boundary and of at least " + std::to_string(bytes) + " bytes");
+                "workspace must be 1-D, contiguous, on a 16-byte boundary and of at least ", (bytes), " bytes");
     a.q = q.data;
     a.q_token = q.strides[0];
     a.q_head = q.strides[1];
@@ -1126,7 +1127,7 @@ extern "C" int lmc_shared_prefix_attention(const lmc_tensor *query, const lmc_te
     a.own_tiles = p.own_tiles;
     a.own_want = p.own_want;
     const int64_t own_items = R * kv.heads * p.own_tiles * p.own_parts;
-    check_value(own_items <= INT32_MAX / 2, "too many rows");
+    expect(own_items <= INT32_MAX / 2, "too many rows");
     a.own_items = static_cast<int>(own_items);
     const int64_t own_groups = (own_items + 31) / 32;
     const int64_t prefix_groups = (kv.heads * p.prefix_parts + 7) / 8 * p.prefix_tiles;

@@ -61,6 +61,7 @@ struct Rows {
   uint32_t magic;   // ceil(2^32 / units per head): a division
   uint32_t per_head;
   int paged;        // out is a cache: rows at the token's slot
+  uint32_t first_block, blocks;  // workgroups (y) that take these rows
 };
 
 struct RotaryArgs {
@@ -123,16 +124,17 @@ __device__ __forceinline__ void turn(typename VecOf<VP * sizeof(typename KD::S)>
 
 // The units of one tensor's rows of this workgroup's tokens: TURN rotates the
 // first of each head and copies the others, else all are copied.
-template <typename KD, bool NEOX, int VP, bool TURN>
+template <typename KD, bool NEOX, int VP, bool STREAM, bool TURN>
 __device__ __forceinline__ void rows_of(const RotaryArgs &a, const Rows &rows, int64_t t0, int nt, const float *cosv,
                                         const float *sinv, const int64_t *paged_row) {
   using S = typename KD::S;
   using V = typename VecOf<VP * sizeof(S)>::T;
-  // Streaming stores: 8192 tokens of 40 heads take 29 us with them, 38
-  // without; few tokens the same either way.
-  auto store = [&](S *to, V v) { __builtin_nontemporal_store(v, reinterpret_cast<V *>(to)); };
-  const uint32_t total = nt * rows.units, step = kThreads * gridDim.y, turned = TURN ? a.half / VP : 0;
-  uint32_t x = blockIdx.y * kThreads + threadIdx.x;
+  auto store = [&](S *to, V v) {
+    if constexpr (STREAM) __builtin_nontemporal_store(v, reinterpret_cast<V *>(to));
+    else *reinterpret_cast<V *>(to) = v;
+  };
+  const uint32_t total = nt * rows.units, step = kThreads * rows.blocks, turned = TURN ? a.half / VP : 0;
+  uint32_t x = (blockIdx.y - rows.first_block) * kThreads + threadIdx.x;
   if (x >= total) return;
   uint32_t t = x / rows.units, w = x - t * rows.units;
   for (; x < total; x += step) {
@@ -162,7 +164,7 @@ __device__ __forceinline__ void rows_of(const RotaryArgs &a, const Rows &rows, i
   }
 }
 
-template <typename KD, bool NEOX, int VP>
+template <typename KD, bool NEOX, int VP, bool STREAM>
 __global__ void __launch_bounds__(kThreads) rotary_rows(RotaryArgs a) {
   extern __shared__ float cs[];  // cos [tokens][half], then sin
   __shared__ int64_t row_k[kMaxTokens], row_v[kMaxTokens];
@@ -191,19 +193,31 @@ __global__ void __launch_bounds__(kThreads) rotary_rows(RotaryArgs a) {
     row_v[tid] = rv;
   }
   __syncthreads();
-  if (a.q.units) rows_of<KD, NEOX, VP, true>(a, a.q, t0, nt, cosv, sinv, nullptr);
-  if (a.k.units) rows_of<KD, NEOX, VP, true>(a, a.k, t0, nt, cosv, sinv, row_k);
-  if (a.v.units) rows_of<KD, NEOX, VP, false>(a, a.v, t0, nt, nullptr, nullptr, row_v);
+  // One tensor, or all of them where a workgroup has the tokens to itself.
+  auto mine = [&](const Rows &rows) { return blockIdx.y - rows.first_block < rows.blocks; };
+  if (mine(a.q)) rows_of<KD, NEOX, VP, STREAM, true>(a, a.q, t0, nt, cosv, sinv, nullptr);
+  if (mine(a.k)) rows_of<KD, NEOX, VP, STREAM, true>(a, a.k, t0, nt, cosv, sinv, row_k);
+  if (mine(a.v)) rows_of<KD, NEOX, VP, STREAM, false>(a, a.v, t0, nt, nullptr, nullptr, row_v);
 }
 
-template <typename KD, bool NEOX, int VP> void launch(const RotaryArgs &a, hipStream_t s) {
+template <typename KD, bool NEOX, int VP> void launch(RotaryArgs a, hipStream_t s) {
   const int64_t blocks = (a.n_tokens + a.tokens_per_block - 1) / a.tokens_per_block;
-  // Few tokens: a unit a lane, spread over workgroups.
-  const int64_t per = (static_cast<int64_t>(a.tokens_per_block) * a.units + kThreads - 1) / kThreads;
-  const int64_t y = blocks >= 1024 ? 1 : std::min<int64_t>(per, 1024 / blocks);
+  // Few tokens: a unit a lane, spread over workgroups, and the tensors apart
+  // (a decode step is latency).  Many: all of a token's rows in one.
+  uint32_t y = 0;
+  for (Rows *r : {&a.q, &a.k, &a.v}) {
+    const int64_t units = static_cast<int64_t>(a.tokens_per_block) * r->units;
+    r->first_block = blocks >= 1024 ? 0 : y;
+    r->blocks = static_cast<uint32_t>(blocks >= 1024 ? units > 0 : std::min<int64_t>((units + kThreads - 1) / kThreads, 1024 / blocks));
+    y = std::max(y, r->first_block + r->blocks);
+  }
   const size_t shared = static_cast<size_t>(a.tokens_per_block) * a.half * 2 * sizeof(float);
-  hipLaunchKernelGGL((rotary_rows<KD, NEOX, VP>), dim3(static_cast<uint32_t>(blocks), static_cast<uint32_t>(y)),
-                     dim3(kThreads), shared, s, a);
+  // Streaming stores past 8 MiB: 8192 tokens of 40 heads take 28 us with them
+  // and 38 without, a decode step's 48 tokens to their pages 4.6 and 3.4.
+  const bool stream = a.n_tokens * a.units * VP * static_cast<int64_t>(sizeof(typename KD::S)) >= (int64_t(8) << 20);
+  const dim3 grid(static_cast<uint32_t>(blocks), static_cast<uint32_t>(y));
+  if (stream) hipLaunchKernelGGL((rotary_rows<KD, NEOX, VP, true>), grid, dim3(kThreads), shared, s, a);
+  else hipLaunchKernelGGL((rotary_rows<KD, NEOX, VP, false>), grid, dim3(kThreads), shared, s, a);
   hip_check(hipGetLastError(), "rotary_rows launch");
 }
 
@@ -233,16 +247,16 @@ HeadView head_view(const lmc_tensor &t, const char *name, int64_t dim, int devic
   HeadView v;
   v.t = &t;
   v.dim = dim;
-  check_value(t.ndim == 2 || t.ndim == 3, std::string(name) + " must be [tokens, heads * head_size] or [tokens, heads, head_size]");
-  for (int i = 0; i < t.ndim; ++i) check_value(t.strides[i] >= 0, std::string(name) + ": negative strides unsupported");
-  check_value(size(t, -1) <= 1 || stride(t, -1) == 1, std::string(name) + ": a head's dims must be adjacent");
+  expect(t.ndim == 2 || t.ndim == 3, name, " must be [tokens, heads * head_size] or [tokens, heads, head_size]");
+  for (int i = 0; i < t.ndim; ++i) expect(t.strides[i] >= 0, name, ": negative strides unsupported");
+  expect(size(t, -1) <= 1 || stride(t, -1) == 1, name, ": a head's dims must be adjacent");
   v.token = t.strides[0];
   if (t.ndim == 2) {
-    check_value(t.sizes[1] % dim == 0, std::string(name) + " width is not a multiple of head_size");
+    expect(t.sizes[1] % dim == 0, name, " width is not a multiple of head_size");
     v.heads = t.sizes[1] / dim;
     v.head = dim;
   } else {
-    check_value(t.sizes[2] == dim, std::string(name) + " heads are not of head_size");
+    expect(t.sizes[2] == dim, name, " heads are not of head_size");
     v.heads = t.sizes[1];
     v.head = t.strides[1];
   }
@@ -271,21 +285,21 @@ void rotary(const lmc_tensor *positions, const lmc_tensor *query, const lmc_tens
             const lmc_tensor *caches, int n_caches, int fmt, bool two_major, const lmc_tensor *slot_mapping,
             int64_t head_size, const double *inv_freq, int64_t n_freq, double scale, bool neox, int64_t offset,
             bool inverse, const lmc_tensor *query_out, const lmc_tensor *key_out, bool paged, hipStream_t stream) {
-  check_value(query || key, "neither query nor key is given");
+  expect(query || key, "neither query nor key is given");
   const lmc_tensor &lead = deref(query ? query : key, query ? "query" : "key");
   const int dev = lead.device;
-  check_value(dev >= 0, "query and key must be on a GPU");
+  expect(dev >= 0, "query and key must be on a GPU");
   if (lead.dtype != LMC_BF16 && lead.dtype != LMC_F16 && lead.dtype != LMC_F32)
     fail(LMC_ERR_VALUE, "rotary positions take bfloat16, float16 or float32 queries and keys only");
-  check_value(head_size > 0 && head_size <= 8192, "head_size must be between 1 and 8192");
-  check_value(inv_freq != nullptr && n_freq > 0, "inv_freq is empty");
-  check_value(offset >= 0 && n_freq <= head_size / 2 && offset <= head_size - 2 * n_freq,
+  expect(head_size > 0 && head_size <= 8192, "head_size must be between 1 and 8192");
+  expect(inv_freq != nullptr && n_freq > 0, "inv_freq is empty");
+  expect(offset >= 0 && n_freq <= head_size / 2 && offset <= head_size - 2 * n_freq,
               "the rotated dims [rotary_offset, rotary_offset + 2 * len(inv_freq)) do not lie in a head");
-  check_value(std::isfinite(scale), "scale must be finite");
+  expect(std::isfinite(scale), "scale must be finite");
   const int64_t T = size(lead, 0), rot = 2 * n_freq, es = elem_size(lead);
   const lmc_tensor &pos = deref(positions, "positions");
   check_vector(pos, "positions", dev, LMC_I64, LMC_I32);
-  check_value(pos.sizes[0] == T, "positions must have one entry per token");
+  expect(pos.sizes[0] == T, "positions must have one entry per token");
 
   RotaryArgs a;
   std::memset(&a, 0, sizeof(a));
@@ -299,8 +313,8 @@ void rotary(const lmc_tensor *positions, const lmc_tensor *query, const lmc_tens
   auto add = [&](Rows &rows, const lmc_tensor *in_t, const lmc_tensor *out_t, const char *name, const char *out_name,
                  int64_t dim, bool turn) {
     const HeadView in = head_view(deref(in_t, name), name, dim, dev, lead.dtype);
-    check_value(in.t->sizes[0] == T, std::string(name) + " has another number of tokens than the call's other tensors");
-    check_value(in.heads * dim <= INT32_MAX / 4, std::string(name) + " rows are too wide");
+    expect(in.t->sizes[0] == T, name, " has another number of tokens than the call's other tensors");
+    expect(in.heads * dim <= INT32_MAX / 4, name, " rows are too wide");
     const int at = n_views++;
     views[at] = in;
     written[at] = false;
@@ -308,7 +322,7 @@ void rotary(const lmc_tensor *positions, const lmc_tensor *query, const lmc_tens
     bool moved = paged && rows.paged;
     if (!moved && out_t) {
       out = head_view(deref(out_t, out_name), out_name, dim, dev, lead.dtype);
-      check_value(out.t->sizes[0] == T && out.heads == in.heads, std::string(out_name) + " differs in shape from " + name);
+      expect(out.t->sizes[0] == T && out.heads == in.heads, out_name, " differs in shape from ", name);
       moved = !same_rows(in, out);
       if (moved) {
         views[n_views] = out;
@@ -317,8 +331,8 @@ void rotary(const lmc_tensor *positions, const lmc_tensor *query, const lmc_tens
     }
     if (!moved) written[at] = true;
     if (!rows.paged)
-      check_value(rows_apart({T, out.heads, dim}, {out.token, out.head, 1}),
-                  std::string(moved ? out_name : name) + " has overlapping rows");
+      expect(rows_apart({T, out.heads, dim}, {out.token, out.head, 1}),
+                  (moved ? out_name : name), " has overlapping rows");
     rows.in = in.t->data;
     rows.in_token = in.token;
     rows.in_head = in.head;
@@ -340,24 +354,24 @@ void rotary(const lmc_tensor *positions, const lmc_tensor *query, const lmc_tens
   };
   a.k.paged = a.v.paged = paged;
   if (query) add(a.q, query, query_out, "query", "query_out", head_size, true);
-  else check_value(!query_out, "query_out without query");
+  else expect(!query_out, "query_out without query");
   PagedKv kv;
   if (paged) {
     kv = paged_kv(caches, n_caches, fmt, two_major, "rotary_embedding_to_paged");
-    check_value(kv.device == dev && kv.dtype == lead.dtype, "the paged caches differ in device or dtype from the rows");
-    check_value(rows_apart({kv.pages, kv.block_size, kv.heads, kv.dim * es}, {kv.k_page, kv.k_token, kv.k_head, 1}) &&
+    expect(kv.device == dev && kv.dtype == lead.dtype, "the paged caches differ in device or dtype from the rows");
+    expect(rows_apart({kv.pages, kv.block_size, kv.heads, kv.dim * es}, {kv.k_page, kv.k_token, kv.k_head, 1}) &&
                     rows_apart({kv.pages, kv.block_size, kv.heads, kv.dim * es}, {kv.v_page, kv.v_token, kv.v_head, 1}),
                 "the paged caches have overlapping rows");
-    check_value(kv.dim == head_size, "the paged caches' heads are not of head_size");
+    expect(kv.dim == head_size, "the paged caches' heads are not of head_size");
     const HeadView k = add(a.k, key, nullptr, "key", "", head_size, true);
     const HeadView v = add(a.v, value, nullptr, "value", "", head_size, false);
-    check_value(k.heads == kv.heads && v.heads == kv.heads, "the paged caches have another number of heads than key and value");
+    expect(k.heads == kv.heads && v.heads == kv.heads, "the paged caches have another number of heads than key and value");
     for (int i = 0; i < n_views; ++i)
       for (int c = 0; c < n_caches; ++c)
-        check_value(!extents_meet(*views[i].t, caches[c]), "the paged caches overlap the call's rows");
+        expect(!extents_meet(*views[i].t, caches[c]), "the paged caches overlap the call's rows");
     const lmc_tensor &sm = deref(slot_mapping, "slot_mapping");
     check_vector(sm, "slot_mapping", dev, LMC_I64, LMC_I32);
-    check_value(sm.sizes[0] == T, "slot_mapping must have one entry per token");
+    expect(sm.sizes[0] == T, "slot_mapping must have one entry per token");
     a.slots = static_cast<const int64_t *>(sm.data);
     a.slots_i32 = sm.dtype == LMC_I32;
     a.block_size = static_cast<uint32_t>(kv.block_size);
@@ -375,12 +389,12 @@ void rotary(const lmc_tensor *positions, const lmc_tensor *query, const lmc_tens
       need(b);
   } else {
     if (key) add(a.k, key, key_out, "key", "key_out", head_size, true);
-    else check_value(!key_out, "key_out without key");
+    else expect(!key_out, "key_out without key");
   }
   // What is written must not be read by another lane.
   for (int i = 0; i < n_views; ++i)
     for (int j = 0; j < i; ++j)
-      check_value(!(written[i] || written[j]) || !may_share(views[i], views[j]), "two of query, key, value and the outputs overlap");
+      expect(!(written[i] || written[j]) || !may_share(views[i], views[j]), "two of query, key, value and the outputs overlap");
   if (T == 0) return;
   need(n_freq * es);
   need(offset * es);
@@ -390,7 +404,7 @@ void rotary(const lmc_tensor *positions, const lmc_tensor *query, const lmc_tens
     if (r->units == 0) continue;
     r->per_head /= vp;
     r->magic = static_cast<uint32_t>(((uint64_t(1) << 32) + r->per_head - 1) / r->per_head);
-    check_value(static_cast<uint64_t>(r->units) * r->per_head * r->per_head < (uint64_t(1) << 32), "rows are too wide");
+    expect(static_cast<uint64_t>(r->units) * r->per_head * r->per_head < (uint64_t(1) << 32), "rows are too wide");
     r->units *= r->per_head;
     units += r->units;
   }
@@ -404,13 +418,13 @@ void rotary(const lmc_tensor *positions, const lmc_tensor *query, const lmc_tens
   a.scale = static_cast<float>(scale);
   a.inverse = inverse;
   a.n_tokens = T;
-  check_value(T <= INT32_MAX, "too many tokens");
+  expect(T <= INT32_MAX, "too many tokens");
   // Two tokens share a workgroup once there are workgroups enough (their
   // angles then fill its lanes): 16384 tokens of 32 + 8 + 8 heads to their
   // pages take 73 us with two, 74 with one, 79 with four and 93 with eight.
   const int tb = T >= 2048 ? kMaxTokens : 1;
   a.tokens_per_block = tb;
-  check_value(static_cast<int64_t>(tb) * units <= INT32_MAX, "rows are too wide");
+  expect(static_cast<int64_t>(tb) * units <= INT32_MAX, "rows are too wide");
   DeviceGuard guard(dev);
   switch (lead.dtype) {
   case LMC_BF16: launch_style<BF16>(a, neox, vp, stream); break;

@@ -5,7 +5,18 @@
 
 #include "kv_geom.h"
 
+#include <initializer_list>
+#include <sstream>
+
 namespace lmc {
+
+// A failed check is LMC_ERR_VALUE; its message is put together only then.
+template <typename... Parts> inline void expect(bool ok, const Parts &...parts) {
+  if (__builtin_expect(ok, 1)) return;
+  std::ostringstream text;
+  (text << ... << parts);
+  fail(LMC_ERR_VALUE, text.str());
+}
 
 // A device tensor of `device` with one of two dtypes.
 inline void check_on(const lmc_tensor &t, const char *name, int device, int32_t dtype, int32_t or_dtype = -1) {
@@ -30,17 +41,20 @@ inline bool extents_meet(const lmc_tensor &a, const lmc_tensor &b) {
 
 // Whether no two elements of a strided layout are the same one: in order of
 // stride, each dim steps over all of the dims below it.
-inline bool rows_apart(std::vector<int64_t> sizes, std::vector<int64_t> strides) {
-  std::vector<std::pair<int64_t, int64_t>> dims;
-  for (size_t i = 0; i < sizes.size(); ++i) {
-    if (sizes[i] == 0) return true;
-    if (sizes[i] > 1) dims.emplace_back(strides[i], sizes[i]);
+inline bool rows_apart(std::initializer_list<int64_t> sizes, std::initializer_list<int64_t> strides) {
+  std::pair<int64_t, int64_t> dims[LMC_MAX_DIMS];
+  int n = 0;
+  const int64_t *stride = strides.begin();
+  for (const int64_t size : sizes) {
+    if (size == 0) return true;
+    if (size > 1) dims[n++] = {*stride, size};
+    ++stride;
   }
-  std::sort(dims.begin(), dims.end());
+  std::sort(dims, dims + n);
   int64_t span = 1;
-  for (const auto &[stride, n] : dims) {
-    if (stride < span) return false;
-    span += stride * (n - 1);
+  for (int i = 0; i < n; ++i) {
+    if (dims[i].first < span) return false;
+    span += dims[i].first * (dims[i].second - 1);
   }
   return true;
 }
@@ -66,41 +80,41 @@ inline PagedKv paged_kv(const lmc_tensor *caches, int n, int fmt, bool two_major
   PagedKv g;
   g.dtype = k.dtype;
   g.device = k.device;
-  check_value(k.device >= 0, std::string(op) + ": the paged caches are not on a GPU");
+  expect(k.device >= 0, op, ": the paged caches are not on a GPU");
   const int64_t es = elem_size(k);
   g.k = static_cast<uint8_t *>(k.data);
   if (fmt == LMC_FMT_MERGED_KV) {
     // [2, pages, block, heads, dim] (two-major) or [pages, 2, block, heads, dim].
-    check_value(k.ndim == 5 && size(k, two_major ? 0 : 1) == 2, "a MERGED_KV cache is 5-D with K and V along its " +
-                                                                    std::string(two_major ? "first" : "second") + " dim");
+    expect(k.ndim == 5 && size(k, two_major ? 0 : 1) == 2, "a MERGED_KV cache is 5-D with K and V along its ",
+           two_major ? "first" : "second", " dim");
     g.pages = size(k, two_major ? 1 : 0);
     g.k_page = g.v_page = stride(k, two_major ? 1 : 0) * es;
     g.v = g.k + stride(k, two_major ? 0 : 1) * es;
     g.v_token = stride(k, 2) * es;
     g.v_head = stride(k, 3) * es;
-    check_value(size(k, 4) <= 1 || stride(k, 4) == 1, "a cache row's head dims must be adjacent");
+    expect(size(k, 4) <= 1 || stride(k, 4) == 1, "a cache row's head dims must be adjacent");
   } else {
     const lmc_tensor &v = deref(&caches[1], "vllm_kv_caches[1]");
-    check_value(k.ndim == 4, "SEPARATE_KV caches are [pages, block, heads, dim]");
-    check_value(v.device == k.device && v.dtype == k.dtype, "K and V caches differ in device or dtype");
+    expect(k.ndim == 4, "SEPARATE_KV caches are [pages, block, heads, dim]");
+    expect(v.device == k.device && v.dtype == k.dtype, "K and V caches differ in device or dtype");
     g.pages = size(k, 0);
     g.k_page = stride(k, 0) * es;
     g.v_page = stride(v, 0) * es;
     g.v = static_cast<uint8_t *>(v.data);
     g.v_token = stride(v, 1) * es;
     g.v_head = stride(v, 2) * es;
-    check_value(size(v, 3) <= 1 || stride(v, 3) == 1, "a cache row's head dims must be adjacent");
-    check_value(size(k, 3) <= 1 || stride(k, 3) == 1, "a cache row's head dims must be adjacent");
+    expect(size(v, 3) <= 1 || stride(v, 3) == 1, "a cache row's head dims must be adjacent");
+    expect(size(k, 3) <= 1 || stride(k, 3) == 1, "a cache row's head dims must be adjacent");
   }
   g.block_size = size(k, -3);
   g.heads = size(k, -2);
   g.dim = size(k, -1);
   g.k_token = stride(k, -3) * es;
   g.k_head = stride(k, -2) * es;
-  for (int i = 0; i < k.ndim; ++i) check_value(k.strides[i] >= 0, "negative strides unsupported");
-  check_value(g.block_size > 0 && g.heads > 0 && g.dim > 0, "the paged caches hold no rows");
+  for (int i = 0; i < k.ndim; ++i) expect(k.strides[i] >= 0, "negative strides unsupported");
+  expect(g.block_size > 0 && g.heads > 0 && g.dim > 0, "the paged caches hold no rows");
   // Page numbers and slots are split in 32 bits.
-  check_value(g.pages <= INT32_MAX && g.block_size <= INT32_MAX && g.pages * g.block_size <= static_cast<int64_t>(UINT32_MAX),
+  expect(g.pages <= INT32_MAX && g.block_size <= INT32_MAX && g.pages * g.block_size <= static_cast<int64_t>(UINT32_MAX),
               "paged caches of more than 2^32 slots are not supported");
   return g;
 }

@@ -265,21 +265,21 @@ extern "C" int lmc_build_slot_mapping(const lmc_tensor *query_lens, const lmc_te
     const lmc_tensor &bt = deref(block_table, "block_table");
     const lmc_tensor &sm = deref(slot_mapping, "slot_mapping");
     const int dev = sm.device;
-    check_value(dev >= 0, "slot_mapping is not on a GPU");
+    expect(dev >= 0, "slot_mapping is not on a GPU");
     check_vector(sm, "slot_mapping", dev, LMC_I64);
     check_vector(ql, "query_lens", dev, LMC_I32, LMC_I64);
     check_vector(cl, "context_lens", dev, ql.dtype);
     check_on(bt, "block_table", dev, LMC_I32);
     const int64_t R = ql.sizes[0], N = sm.sizes[0];
-    check_value(cl.sizes[0] == R, "query_lens and context_lens differ in length");
-    check_value(bt.ndim == 2 && bt.sizes[0] == R, "block_table must be [requests, pages]");
-    check_value(bt.sizes[1] <= 1 || bt.strides[1] == 1, "block_table rows must be contiguous");
-    check_value(R <= 1 || bt.strides[0] >= bt.sizes[1], "block_table rows overlap");
-    check_value(R <= kMaxRequests, "a call takes at most " + std::to_string(kMaxRequests) + " requests");
-    check_value(block_size > 0 && block_size < (int64_t(1) << 31), "block_size must be positive");
-    check_value(bt.sizes[1] == 0 || block_size <= INT32_MAX / bt.sizes[1], "a block_table row spans 2^31 positions or more");
-    check_value(R * bt.sizes[1] <= INT32_MAX, "block_table has 2^31 entries or more");
-    check_value(N <= INT32_MAX - 65536, "slot_mapping has too many entries");
+    expect(cl.sizes[0] == R, "query_lens and context_lens differ in length");
+    expect(bt.ndim == 2 && bt.sizes[0] == R, "block_table must be [requests, pages]");
+    expect(bt.sizes[1] <= 1 || bt.strides[1] == 1, "block_table rows must be contiguous");
+    expect(R <= 1 || bt.strides[0] >= bt.sizes[1], "block_table rows overlap");
+    expect(R <= kMaxRequests, "a call takes at most ", kMaxRequests, " requests");
+    expect(block_size > 0 && block_size < (int64_t(1) << 31), "block_size must be positive");
+    expect(bt.sizes[1] == 0 || block_size <= INT32_MAX / bt.sizes[1], "a block_table row spans 2^31 positions or more");
+    expect(R * bt.sizes[1] <= INT32_MAX, "block_table has 2^31 entries or more");
+    expect(N <= INT32_MAX - 65536, "slot_mapping has too many entries");
     SlotMapArgs a;
     std::memset(&a, 0, sizeof(a));
     a.query_lens = ql.data;
@@ -295,48 +295,48 @@ extern "C" int lmc_build_slot_mapping(const lmc_tensor *query_lens, const lmc_te
     if (positions) {
       const lmc_tensor &p = deref(positions, "positions");
       check_vector(p, "positions", dev, LMC_I64);
-      check_value(p.sizes[0] == N, "positions and slot_mapping differ in length");
+      expect(p.sizes[0] == N, "positions and slot_mapping differ in length");
       a.positions = static_cast<int64_t *>(p.data);
     }
     if (query_start_loc) {
       const lmc_tensor &q = deref(query_start_loc, "query_start_loc");
       check_vector(q, "query_start_loc", dev, LMC_I32);
-      check_value(q.sizes[0] == R + 1, "query_start_loc must have one entry per request and one more");
+      expect(q.sizes[0] == R + 1, "query_start_loc must have one entry per request and one more");
       a.starts = static_cast<int32_t *>(q.data);
     }
     if (seq_lens) {
       const lmc_tensor &q = deref(seq_lens, "seq_lens");
       check_vector(q, "seq_lens", dev, LMC_I32);
-      check_value(q.sizes[0] == R, "seq_lens must have one entry per request");
+      expect(q.sizes[0] == R, "seq_lens must have one entry per request");
       a.seq_lens = static_cast<int32_t *>(q.data);
     }
     if (free_blocks) {
       const lmc_tensor &f = deref(free_blocks, "free_blocks");
       check_vector(f, "free_blocks", dev, LMC_I32);
-      check_value(!extents_meet(f, bt), "free_blocks overlaps block_table");
+      expect(!extents_meet(f, bt), "free_blocks overlaps block_table");
       a.grow = 1;
       a.free_blocks = static_cast<const int32_t *>(f.data);
       a.n_free = f.sizes[0];
     } else {
-      check_value(!free_cursor && !next_cursor, "free_cursor and next_cursor go with free_blocks");
+      expect(!free_cursor && !next_cursor, "free_cursor and next_cursor go with free_blocks");
     }
     if (free_cursor) {
       const lmc_tensor &c = deref(free_cursor, "free_cursor");
       check_vector(c, "free_cursor", dev, LMC_I64);
-      check_value(c.sizes[0] == 1, "free_cursor must have one entry");
+      expect(c.sizes[0] == 1, "free_cursor must have one entry");
       a.cursor = static_cast<const int64_t *>(c.data);
     }
     if (next_cursor) {
       const lmc_tensor &c = deref(next_cursor, "next_cursor");
       check_vector(c, "next_cursor", dev, LMC_I64);
-      check_value(c.sizes[0] == 1, "next_cursor must have one entry");
-      check_value(!free_cursor || !extents_meet(c, deref(free_cursor, "free_cursor")),
+      expect(c.sizes[0] == 1, "next_cursor must have one entry");
+      expect(!free_cursor || !extents_meet(c, deref(free_cursor, "free_cursor")),
                   "next_cursor is free_cursor: workgroups read the one while the other is written");
       a.next_cursor = static_cast<int64_t *>(c.data);
     }
     // Every workgroup reads the lengths while the first ones write.
     for (const lmc_tensor *out : {slot_mapping, positions, query_start_loc, seq_lens, next_cursor, block_table})
-      check_value(!out || (!extents_meet(*out, ql) && !extents_meet(*out, cl)), "an output overlaps the lengths it is computed from");
+      expect(!out || (!extents_meet(*out, ql) && !extents_meet(*out, cl)), "an output overlaps the lengths it is computed from");
     if (R == 0 && N == 0 && !a.starts && !a.next_cursor) return;
     DeviceGuard guard(dev);
     const int nt = R > 256 ? 1024 : 256;
