@@ -11,6 +11,7 @@
 #include "serving.h"
 
 #include <cmath>
+#include <limits>
 #include <type_traits>
 
 namespace lmc {
@@ -1044,13 +1045,16 @@ extern "C" int lmc_shared_prefix_attention(const lmc_tensor *query, const lmc_te
     expect(shared_len >= 0 && shared_len <= kMaxKeys, "shared_len must be between 0 and 2^30");
     expect(bt.sizes[1] * kv.block_size <= kMaxKeys, "a block_table row spans more than 2^30 keys");
     expect((shared_len + kv.block_size - 1) / kv.block_size <= sb.sizes[0], "shared_blocks has too few blocks for shared_len");
-    expect(scale > 0 && std::isfinite(scale), "scale must be positive and finite");
+    // (a scale of zero in 32 bits would make NaN of the keys that are not seen)
+    const float scale2 = static_cast<float>(scale * 1.4426950408889634);
+    expect(scale2 >= std::numeric_limits<float>::min() && std::isfinite(scale2), "scale must be positive and finite in 32 bits");
     AttnArgs a;
     std::memset(&a, 0, sizeof(a));
     if (lse) {
       const lmc_tensor &e = deref(lse, "lse");
       check_on(e, "lse", dev, LMC_F32);
       expect(e.ndim == 2 && e.sizes[0] == T && e.sizes[1] == Hq, "lse must be [tokens, heads]");
+      expect(rows_apart({T, Hq}, {e.strides[0], e.strides[1]}), "lse has overlapping rows");
       a.lse = static_cast<float *>(e.data);
       a.lse_token = e.strides[0];
       a.lse_head = e.strides[1];
@@ -1063,6 +1067,9 @@ extern "C" int lmc_shared_prefix_attention(const lmc_tensor *query, const lmc_te
                     on_16(reinterpret_cast<intptr_t>(o.data)) && on_16(o.strides[0] * 2) && on_16(o.strides[1] * 2),
                 "rows of query and output must start on 16-byte boundaries");
     expect(rows_apart({T, Hq, kv.dim}, {o.strides[0], o.strides[1], 1}), "output has overlapping rows");
+    // A lane's offset from the first of 16 rows has 32 bits.
+    expect(kv.block_size == 1 || std::max(kv.k_token, kv.v_token) < (int64_t(1) << 27),
+                "rows of the paged caches are 2^27 bytes or more apart");
     expect(T * Hq <= INT32_MAX / 128 && R <= INT32_MAX / 4096, "too many rows");
     const int64_t group = kv.heads ? Hq / kv.heads : 0;
     if (workspace_bytes) *workspace_bytes = 0;
@@ -1080,6 +1087,17 @@ extern "C" int lmc_shared_prefix_attention(const lmc_tensor *query, const lmc_te
     expect(ws.ndim == 1 && (ws.sizes[0] <= 1 || ws.strides[0] == 1) && ws.sizes[0] >= bytes &&
                     on_16(reinterpret_cast<intptr_t>(ws.data)),
                 "workspace must be 1-D, contiguous, on a 16-byte boundary and of at least ", (bytes), " bytes");
+    // The parts are joined in a launch of its own: output and lse may lie over query.
+    expect(!lse || !may_share(o, *lse), "output and lse overlap");
+    for (const lmc_tensor *out : {output, lse, workspace}) {
+      if (!out) continue;
+      expect(!extents_meet(*out, qs) && !extents_meet(*out, sl) && !extents_meet(*out, bt) && !extents_meet(*out, sb),
+                  "output, lse or workspace overlap the tables or the lengths");
+      for (int i = 0; i < n_caches; ++i)
+        expect(!extents_meet(*out, vllm_kv_caches[i]), "output, lse or workspace overlap the paged caches");
+    }
+    expect(!extents_meet(ws, q) && !extents_meet(ws, o) && !(lse && extents_meet(ws, *lse)),
+                "workspace overlaps query, output or lse");
     a.q = q.data;
     a.q_token = q.strides[0];
     a.q_head = q.strides[1];
@@ -1117,7 +1135,7 @@ extern "C" int lmc_shared_prefix_attention(const lmc_tensor *query, const lmc_te
     a.kv_heads = static_cast<int>(kv.heads);
     a.group = static_cast<int>(group);
     a.max_keys = static_cast<int>(std::max(shared_len, keys));
-    a.scale2 = static_cast<float>(scale * 1.4426950408889634);
+    a.scale2 = scale2;
     a.part_o = static_cast<float *>(ws.data);
     a.part_ml = reinterpret_cast<float2 *>(a.part_o + parts * rows * kv.dim);
     a.prefix_parts = p.prefix_parts;

@@ -268,19 +268,6 @@ bool same_rows(const HeadView &a, const HeadView &b) {
          (a.heads <= 1 || a.head == b.head);
 }
 
-// Whether two tensors may share an element.  Column slices of one buffer
-// (the same token stride, each token's heads inside it) are told apart.
-bool may_share(const HeadView &a, const HeadView &b) {
-  if (!extents_meet(*a.t, *b.t)) return false;
-  const int64_t es = elem_size(*a.t);
-  const int64_t wa = ((a.heads - 1) * a.head + a.dim) * es, wb = ((b.heads - 1) * b.head + b.dim) * es;
-  const int64_t s = a.token * es;
-  if (a.token != b.token || wa > s || wb > s) return true;
-  const int64_t d = reinterpret_cast<intptr_t>(b.t->data) - reinterpret_cast<intptr_t>(a.t->data);
-  const int64_t m = ((d % s) + s) % s;
-  return !(m >= wa && m + wb <= s);
-}
-
 void rotary(const lmc_tensor *positions, const lmc_tensor *query, const lmc_tensor *key, const lmc_tensor *value,
             const lmc_tensor *caches, int n_caches, int fmt, bool two_major, const lmc_tensor *slot_mapping,
             int64_t head_size, const double *inv_freq, int64_t n_freq, double scale, bool neox, int64_t offset,
@@ -295,7 +282,7 @@ void rotary(const lmc_tensor *positions, const lmc_tensor *query, const lmc_tens
   expect(inv_freq != nullptr && n_freq > 0, "inv_freq is empty");
   expect(offset >= 0 && n_freq <= head_size / 2 && offset <= head_size - 2 * n_freq,
               "the rotated dims [rotary_offset, rotary_offset + 2 * len(inv_freq)) do not lie in a head");
-  expect(std::isfinite(scale), "scale must be finite");
+  expect(std::isfinite(static_cast<float>(scale)), "scale must be finite in 32 bits");
   const int64_t T = size(lead, 0), rot = 2 * n_freq, es = elem_size(lead);
   const lmc_tensor &pos = deref(positions, "positions");
   check_vector(pos, "positions", dev, LMC_I64, LMC_I32);
@@ -394,7 +381,19 @@ void rotary(const lmc_tensor *positions, const lmc_tensor *query, const lmc_tens
   // What is written must not be read by another lane.
   for (int i = 0; i < n_views; ++i)
     for (int j = 0; j < i; ++j)
-      expect(!(written[i] || written[j]) || !may_share(views[i], views[j]), "two of query, key, value and the outputs overlap");
+      expect(!(written[i] || written[j]) || !may_share(*views[i].t, *views[j].t), "two of query, key, value and the outputs overlap");
+  // Nor may a workgroup write what others take their angles and slots from.
+  lmc_tensor freq = pos;  // n_freq doubles: as wide as I64
+  freq.data = const_cast<double *>(inv_freq);
+  freq.dtype = LMC_I64;
+  freq.sizes[0] = n_freq;
+  freq.strides[0] = 1;
+  for (const lmc_tensor *in : {positions, paged ? slot_mapping : positions, static_cast<const lmc_tensor *>(&freq)}) {
+    for (int i = 0; i < n_views; ++i)
+      expect(!written[i] || !extents_meet(*views[i].t, *in), "positions, slot_mapping or inv_freq overlap what the call writes");
+    for (int c = 0; c < n_caches; ++c)
+      expect(!extents_meet(caches[c], *in), "positions, slot_mapping or inv_freq overlap the paged caches");
+  }
   if (T == 0) return;
   need(n_freq * es);
   need(offset * es);

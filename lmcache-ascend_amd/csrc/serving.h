@@ -39,6 +39,20 @@ inline bool extents_meet(const lmc_tensor &a, const lmc_tensor &b) {
   return na > 0 && nb > 0 && pa < pb + nb && pb < pa + na;
 }
 
+// Whether two tensors may share an element.  Column slices of one buffer (the
+// same stride of the first dim, each row's elements inside it) are told apart.
+inline bool may_share(const lmc_tensor &a, const lmc_tensor &b) {
+  if (!extents_meet(a, b)) return false;
+  if (a.ndim == 0 || b.ndim == 0) return true;
+  const int64_t s = a.strides[0] * elem_size(a);
+  const int64_t wa = extent_bytes(a) - (a.sizes[0] - 1) * s;
+  const int64_t wb = extent_bytes(b) - (b.sizes[0] - 1) * b.strides[0] * elem_size(b);
+  if (b.strides[0] * elem_size(b) != s || wa > s || wb > s) return true;
+  const int64_t d = reinterpret_cast<intptr_t>(b.data) - reinterpret_cast<intptr_t>(a.data);
+  const int64_t m = ((d % s) + s) % s;
+  return !(m >= wa && m + wb <= s);
+}
+
 // Whether no two elements of a strided layout are the same one: in order of
 // stride, each dim steps over all of the dims below it.
 inline bool rows_apart(std::initializer_list<int64_t> sizes, std::initializer_list<int64_t> strides) {
@@ -105,6 +119,7 @@ inline PagedKv paged_kv(const lmc_tensor *caches, int n, int fmt, bool two_major
     g.v_head = stride(v, 2) * es;
     expect(size(v, 3) <= 1 || stride(v, 3) == 1, "a cache row's head dims must be adjacent");
     expect(size(k, 3) <= 1 || stride(k, 3) == 1, "a cache row's head dims must be adjacent");
+    for (int i = 0; i < v.ndim; ++i) expect(v.strides[i] >= 0, "negative strides unsupported");
   }
   g.block_size = size(k, -3);
   g.heads = size(k, -2);

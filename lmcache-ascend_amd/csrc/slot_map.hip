@@ -337,6 +337,15 @@ extern "C" int lmc_build_slot_mapping(const lmc_tensor *query_lens, const lmc_te
     // Every workgroup reads the lengths while the first ones write.
     for (const lmc_tensor *out : {slot_mapping, positions, query_start_loc, seq_lens, next_cursor, block_table})
       expect(!out || (!extents_meet(*out, ql) && !extents_meet(*out, cl)), "an output overlaps the lengths it is computed from");
+    const lmc_tensor *grown = free_blocks ? block_table : nullptr;
+    const lmc_tensor *outs[] = {slot_mapping, positions, query_start_loc, seq_lens, next_cursor, grown};
+    for (const lmc_tensor *out : outs) {
+      if (!out) continue;
+      for (const lmc_tensor *in : {block_table, free_blocks, free_cursor})
+        expect(!in || in == out || !extents_meet(*out, *in), "an output overlaps the table or the free list");
+      for (const lmc_tensor *other : outs)
+        expect(!other || other == out || !extents_meet(*out, *other), "two outputs overlap");
+    }
     if (R == 0 && N == 0 && !a.starts && !a.next_cursor) return;
     DeviceGuard guard(dev);
     const int nt = R > 256 ? 1024 : 256;

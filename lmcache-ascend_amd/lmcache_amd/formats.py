@@ -274,6 +274,8 @@ def rotary_inv_freq(rotary_dim: int, base: float = 10000.0, scaling=None, seq_le
         scale = scaling.get("attention_factor")
         if scale is None:
             factor = float(need("factor"))
+            if not original > 1:
+                raise ValueError("original_max_position_embeddings must be above 1")
             scale = 1.0 if factor <= 1.0 else math.sqrt(1.0 + math.log(factor) / math.log(original))
         return inv / factors, float(scale)
 
@@ -283,6 +285,8 @@ def rotary_inv_freq(rotary_dim: int, base: float = 10000.0, scaling=None, seq_le
     if kind == "linear":
         return inv / factor, 1.0
     original = float(need("original_max_position_embeddings"))
+    if not original > 0:
+        raise ValueError("original_max_position_embeddings must be positive")
     if kind == "dynamic":
         if rotary_dim <= 2:
             raise ValueError("dynamic scaling needs more than two rotary dims")
@@ -297,6 +301,8 @@ def rotary_inv_freq(rotary_dim: int, base: float = 10000.0, scaling=None, seq_le
         keep = ((original * inv / (2.0 * math.pi) - low) / (high - low)).clamp(0.0, 1.0)
         return inv * keep + inv / factor * (1.0 - keep), 1.0
     if kind == "yarn":
+        if not base > 1:
+            raise ValueError("yarn scaling needs a base above 1")
         fast, slow = float(scaling.get("beta_fast") or 32.0), float(scaling.get("beta_slow") or 1.0)
 
         def dim_of(turns):

@@ -232,6 +232,53 @@ def test_prefix_attention_refusals(over, text):
     _refuses(_attention(**over), text)
 
 
+_O = _t(BF16, 5, 8, 64)
+_SEQ, _STARTS, _TABLE, _POOL = _t(I32, 4), _t(I32, 5), _t(I32, 4, 9), _t(I32, 9)
+_PAGES = _caches()
+_FLAT = _t(I64, 20)
+_WIDE = 1 << 27
+
+
+def _negative():
+    arr = _caches()
+    arr[1].strides[0] = -arr[1].strides[0]
+    return arr
+
+
+@pytest.mark.parametrize("call,over,text", [
+    # what one workgroup reads while another writes it, and outputs over outputs
+    (_slots, {"slots": _FLAT, "positions": _t(I64, 20, data=_FLAT.data + 8)}, "two outputs overlap"),
+    (_slots, {"starts": _STARTS, "seq": _t(I32, 4, data=_STARTS.data)}, "two outputs overlap"),
+    (_slots, {"table": _TABLE, "starts": _t(I32, 5, data=_TABLE.data + 16)}, "overlaps the table"),
+    (_slots, {"free": _POOL, "seq": _t(I32, 4, data=_POOL.data)}, "overlaps the table or the free list"),
+    (_slots, {"free": _POOL, "cursor": _CURSOR, "positions": _t(I64, 20, data=_CURSOR.data - 8)}, "free list"),
+    (_slots, {"free": _POOL, "following": _t(I64, 1, data=_FLAT.data + 24), "slots": _FLAT}, "two outputs overlap"),
+    (_rotary, {"pos": _FLAT, "q": _t(BF16, 20, 256, data=_FLAT.data), "k": None}, "overlap what the call writes"),
+    (_rotary, {"q": _t(BF16, 5, 256, data=1 << 35), "k": None}, "overlap what the call writes"),
+    (_rotary, {"q": _t(BF16, 5, 256), "k": None, "qo": _t(BF16, 5, 256, data=(1 << 35) + 16)}, "overlap what the call writes"),
+    (_rotary, {"scale": 1e300}, "scale must be finite"),
+    (_paged, {"slots": _t(I64, 5, data=_PAGES[0].data), "caches": _PAGES}, "overlap the paged caches"),
+    (_paged, {"caches": _negative()}, "negative strides"),
+    (_attention, {"caches": _negative()}, "negative strides"),
+    (_attention, {"scale": 1e-60}, "scale must be positive"),
+    (_attention, {"scale": 1e60}, "scale must be positive"),
+    (_attention, {"lse": _t(F32, 5, 8, strides=[4, 1])}, "lse has overlapping rows"),
+    (_attention, {"lse": _t(F32, 5, 8, strides=[0, 1])}, "lse has overlapping rows"),
+    (_attention, {"o": _O, "lse": _t(F32, 5, 8, data=_O.data + 64)}, "output and lse overlap"),
+    (_attention, {"o": _O, "ws": _t(_lib.U8, 1 << 20, data=_O.data)}, "workspace overlaps"),
+    (_attention, {"q": _O, "ws": _t(_lib.U8, 1 << 20, data=_O.data)}, "workspace overlaps"),
+    (_attention, {"lse": _t(F32, 5, 8, data=_SEQ.data), "seq": _SEQ}, "overlap the tables or the lengths"),
+    (_attention, {"o": _t(BF16, 5, 8, 64, data=_STARTS.data), "starts": _STARTS}, "overlap the tables or the lengths"),
+    (_attention, {"o": _t(BF16, 5, 8, 64, data=_PAGES[1].data), "caches": _PAGES}, "overlap the paged caches"),
+    (_attention, {"ws": _t(_lib.U8, 1 << 20, data=_PAGES[0].data), "caches": _PAGES}, "overlap the paged caches"),
+    # 15 rows of a group of 16 lie within 32 bits of its first
+    (_attention, {"caches": _one(_t(BF16, 1, 2, 16, 2, 64, strides=[32 * _WIDE, 16 * _WIDE, _WIDE // 2, 64, 1])), "fmt": 1},
+     "2^27 bytes or more apart"),
+])
+def test_overlaps_strides_and_scales_are_refused(call, over, text):
+    _refuses(call(**over), text)
+
+
 def test_python_refuses_cpu_tensors():
     x = torch.zeros((2, 64))
     f = torch.ones(32, dtype=torch.float64)
@@ -313,6 +360,9 @@ def test_inv_freq_longrope():
     (7,), (0,), (8, 0.0), (8, 1e4, {"rope_type": "linear"}), (8, 1e4, {"rope_type": "linear", "factor": 0}),
     (8, 1e4, {"rope_type": "nothing", "factor": 2, "original_max_position_embeddings": 5}),
     (8, 1e4, {"rope_type": "yarn", "factor": 2}),
+    (8, 1.0, {"rope_type": "yarn", "factor": 2, "original_max_position_embeddings": 5}),
+    (8, 1e4, {"rope_type": "yarn", "factor": 2, "original_max_position_embeddings": 0}),
+    (4, 1e4, {"rope_type": "longrope", "factor": 2, "original_max_position_embeddings": 1, "short_factor": [1.0, 1.0]}),
     (8, 1e4, {"rope_type": "longrope", "factor": 2, "original_max_position_embeddings": 5, "short_factor": [1.0]}),
 ])
 def test_inv_freq_refusals(args):
