@@ -342,3 +342,89 @@ def test_no_tokens(ops):
                                 1.0, out)
     torch.cuda.synchronize()
     assert torch.equal(out.cpu(), c["out"])
+
+
+@pytest.mark.parametrize("dim", [64, 128, 256])
+def test_unseen_infinity_in_a_prefix_of_many_rows(ops, dim):
+    """Tiles of 128 rows: one request ends before a key whose value holds
+    infinities, the others see it."""
+    P, R, short, key = 300, 80, 5, 150
+    seq = [P + 1 + r % 7 for r in range(R)]
+    seq[short] = 100
+    c = _case(dim, [1] * R, seq, P, 16, 4, 2, dim)
+    page, at = int(c["shared"][key // 16]), key % 16
+    c["v"][page, at, :, ::3] = float("inf")
+    caches, kw = _device_caches(c)
+    out = c["out"].to(DEV)
+    _call(ops, c, caches, kw, c["q"].to(DEV), out, None)
+    torch.cuda.synchronize()
+    got = out.double().cpu().numpy()
+    others = [r for r in range(R) if r != short]
+    assert np.isposinf(got[others][:, :, ::3]).all() and np.isfinite(got[others][:, :, 1::3]).all()
+    c["v"] = torch.nan_to_num(c["v"], nan=0.0, posinf=0.0)
+    c["k"] = torch.nan_to_num(c["k"], nan=0.0)
+    want = _want(c)
+    assert (np.abs(got[short] - want[0][short]) <= want[2][short]).all()
+    assert (np.abs(got - want[0]) <= want[2])[:, :, 1::3].all()
+
+
+@pytest.mark.parametrize("P", [0, 100])
+def test_prompts_in_chunks(ops, P):
+    """Hundreds of tokens a request: several tiles of 32 rows each over the
+    request's own keys."""
+    q_lens = [130, 0, 257, 1]
+    _check(ops, _case(21 + P, q_lens, [P + n + 9 for n in q_lens], P, 16, 6, 2, 64, pad=3))
+
+
+@pytest.mark.parametrize("R", [3, 50])
+def test_output_over_the_query(ops, R):
+    c = _case(22, [1] * R, [90 + i for i in range(R)], 70, 16, 8, 2, 64)
+    caches, kw = _device_caches(c)
+    q, lse = c["q"].to(DEV), c["lse"].to(DEV)
+    _call(ops, c, caches, kw, q, q, lse)
+    torch.cuda.synchronize()
+    _hold(c, q, lse)
+
+
+def test_output_and_lse_as_columns_of_one_buffer(ops):
+    c = _case(23, [1, 2, 1], [90, 85, 77], 70, 16, 8, 2, 64)
+    caches, kw = _device_caches(c)
+    T, H, D = c["q"].shape
+    rows = torch.zeros((T, H * (D * 2 + 4) + 16), dtype=torch.uint8, device=DEV)
+    out = rows.view(torch.bfloat16)[:, : H * D].view(T, H, D)
+    lse = rows.view(torch.float32)[:, H * D // 2: H * D // 2 + H]
+    _call(ops, c, caches, kw, c["q"].to(DEV), out, lse)
+    torch.cuda.synchronize()
+    _hold(c, out, lse)
+    assert (rows[:, H * (D * 2 + 4):] == 0).all()
+
+
+def test_two_streams_at_once(ops):
+    """Each call works in scratch of its own."""
+    cases = [_case(s, [1] * 40, [420 + 3 * i for i in range(40)], 400, 16, 8, 2, 64) for s in (24, 25)]
+    held = [(c, _device_caches(c), c["q"].to(DEV), c["out"].to(DEV), c["lse"].to(DEV), torch.cuda.Stream()) for c in cases]
+    torch.cuda.synchronize()
+    for _ in range(3):
+        for c, (caches, kw), q, out, lse, stream in held:
+            with torch.cuda.stream(stream):
+                _call(ops, c, caches, kw, q, out, lse)
+    torch.cuda.synchronize()
+    for c, _, _, out, lse, _ in held:
+        _hold(c, out, lse)
+
+
+def test_one_block_several_times(ops):
+    """Requests that own one block together, and one that has it twice."""
+    c = _case(26, [1, 1, 2], [112, 112, 112], 64, 16, 4, 2, 128)
+    c["table"][1] = c["table"][0]
+    c["table"][2, 5] = c["table"][2, 4]
+    _check(ops, c)
+
+
+def test_one_request_with_one_key(ops):
+    """Its value, whatever the query, and an lse of the score."""
+    for P in (0, 1):
+        c = _case(27, [1], [1], P, 16, 2, 1, 64)
+        out = _check(ops, c)
+        page = int(c["shared"][0]) if P else int(c["table"][0, 0])
+        assert torch.equal(out[0].cpu(), c["v"][page, 0].expand(2, 64))

@@ -253,3 +253,21 @@ def test_infinities_and_nans_stay_in_their_pairs(ops):
         differ[t, e] = False
     assert not differ.any()
     assert torch.isnan(b[1, 3]) and torch.isnan(b[1, 35])
+
+
+def test_two_tokens_with_one_slot(ops):
+    """Either's row, whole: K and V are each one token's."""
+    T, H, dim, block = 600, 2, 64, 16
+    inv, pos = _inv(32).to(DEV), torch.zeros(T, dtype=torch.int64, device=DEV)
+    rows = torch.arange(T, device=DEV, dtype=torch.float32)[:, None].expand(T, H * dim).contiguous()
+    caches = tuple(torch.full((2, block, H, dim), -1.0, device=DEV) for _ in range(2))
+    slots = torch.full((T,), 5, dtype=torch.int64, device=DEV)
+    slots[::2] = 21
+    ops.rotary_embedding_to_paged(pos, None, rows, rows.clone(), caches, slots, dim, inv)
+    torch.cuda.synchronize()
+    for c in caches:
+        flat = c.view(2 * block, H * dim).cpu()
+        for slot, odd in ((5, 1), (21, 0)):
+            assert set(flat[slot].long().tolist()) <= set(range(odd, T, 2))
+        flat[[5, 21]] = -1.0
+        assert (flat == -1.0).all()
