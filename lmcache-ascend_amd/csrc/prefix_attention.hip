@@ -7,6 +7,31 @@
 // over the keys j of token t's request up to the token's own position.  Keys
 // before shared_len lie in the blocks of one list for the whole batch, the
 // others in the request's row of the block table.
+//
+// One pass over the keys with the running maximum and sum of each row; the
+// key range is cut into parts, whose sums (32 bits, with their maximum) a
+// second launch joins:
+//
+//   * The prefix: rows of all requests together, a KV head's heads beside each
+//     other, against one part of the shared keys.  With more than 64 rows a
+//     KV head, tiles of 128 rows and blocks of 64 keys (attend_wide), bound by
+//     the matrix cores and their operands from LDS; else 32 rows and a block
+//     of 32 keys a wave (attend_narrow).
+//   * Each request's own keys: a wave a part (attend_narrow), bound by the
+//     bytes of K and V: 4 to 16 rows stand in tiles of 32, which costs less
+//     than the loads do.
+//
+// S^T = K Q^T and O^T = V^T P^T on 32 x 32 x 16 matrix instructions: a lane
+// holds one row's weights for half of a block's keys, in the order in which
+// the second product takes them, so that maximum, sum and weights stay in
+// registers; K and V go from memory to LDS without registers between, and V
+// is read from there transposed.
+//
+// 256 requests, 32 heads over 8 KV heads of 128 bf16 dims, 16384 shared and 1
+// to 1024 own keys: 158 us (71 GFLOP, 607 MB), of which 11 the join; the
+// prefix alone takes 95 us (750 TFLOP/s), the own keys alone 115 (4.7 TB/s).
+// 64 requests over 4096 shared and the same own keys: 49 us.  4 requests over
+// 1000 shared and 1 to 200 own keys: 12 us, the latency of two launches.
 #include "rope_math.h"
 #include "serving.h"
 
@@ -26,8 +51,10 @@ typedef short s16x4 __attribute__((ext_vector_type(4)));
 typedef short s16x8 __attribute__((ext_vector_type(8)));
 
 // Keys of a part of a request's own ones where requests are many: 256 requests
-// over 16384 shared and up to 1024 own keys take 165 us with 384, 170 with 256
-// (more starts and ends), 179 with 128.
+// over 16384 shared and up to 1024 own keys take 163 us with 384, 170 with 256
+// (more starts and ends), 179 with 128.  An equal share of all own keys for
+// every wave, over the requests' borders, took as long (160 against 163) and
+// cost small batches 2 of 12 us.
 constexpr int kOwnChunk = 384;
 
 struct AttnArgs {
@@ -975,8 +1002,8 @@ Plan make_plan(int64_t T, int64_t R, int64_t kv_heads, int64_t group, int64_t sh
   // places, at a key of its own in half of the time of a request's own key
   // (which comes from memory, while all row tiles read the prefix; requests
   // are taken to have half of their tables' keys, 512 at most), so that both
-  // end together: 256 requests, 32 heads over 16384 keys, 1024 own: 169 us,
-  // with two thirds of that 180, with five thirds 194.  A part has four wide
+  // end together: 256 requests, 32 heads over 16384 keys, up to 1024 own: 163
+  // us, with two thirds of that 180, with five thirds 194.  A part has four wide
   // blocks or one round of narrow ones at least: it costs a row of 32-bit
   // sums to write and read.
   const double prefix_cost = static_cast<double>(items) * shared_len;

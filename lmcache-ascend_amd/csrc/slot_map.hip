@@ -21,7 +21,8 @@
 //
 // A decode step's few tokens are latency: launch, lengths, pages, store.
 // Requests of a few new tokens need no search, and their pages are loaded
-// beside the sums.
+// beside the sums.  64 requests of one token with a free list: 4.5 us (3.7 in
+// a graph); 256 requests of up to 4096 tokens: 7.8 us.
 #include "serving.h"
 
 namespace lmc {
