@@ -28,9 +28,9 @@
 // is read from there transposed.
 //
 // 256 requests, 32 heads over 8 KV heads of 128 bf16 dims, 16384 shared and 1
-// to 1024 own keys: 158 us (71 GFLOP, 607 MB), of which 11 the join; the
-// prefix alone takes 95 us (750 TFLOP/s), the own keys alone 115 (4.7 TB/s).
-// 64 requests over 4096 shared and the same own keys: 49 us.  4 requests over
+// to 1024 own keys: 153 us (71 GFLOP, 607 MB), of which 11 the join; the
+// prefix alone takes 95 us (750 TFLOP/s), the own keys alone 106 (5.1 TB/s).
+// 64 requests over 4096 shared and the same own keys: 42 us.  4 requests over
 // 1000 shared and 1 to 200 own keys: 12 us, the latency of two launches.
 #include "rope_math.h"
 #include "serving.h"
@@ -51,9 +51,10 @@ typedef short s16x4 __attribute__((ext_vector_type(4)));
 typedef short s16x8 __attribute__((ext_vector_type(8)));
 
 // Keys of a part of a request's own ones where requests are many: 256 requests
-// over 16384 shared and up to 1024 own keys take 163 us with 384, 170 with 256
-// (more starts and ends), 179 with 128.  An equal share of all own keys for
-// every wave, over the requests' borders, took as long (160 against 163) and
+// over 16384 shared and up to 1024 own keys take 151 us with 384, 156 with 256
+// (more starts and ends) and 149 with 512, which takes 116 over 1024 shared keys
+// against 112.  An equal share of all own keys for every wave, over the
+// requests' borders, took as long (124 against 120 for the own keys alone) and
 // cost small batches 2 of 12 us.
 constexpr int kOwnChunk = 384;
 
@@ -127,10 +128,18 @@ __device__ __forceinline__ uint64_t uniform(const void *p) {
   const uint32_t hi = __builtin_amdgcn_readfirstlane(static_cast<uint32_t>(x >> 32));
   return (static_cast<uint64_t>(hi) << 32) | lo;
 }
-__device__ __forceinline__ void load_to_lds(const uint8_t *base, uint32_t off, uint32_t lds) {
-  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(__builtin_amdgcn_readfirstlane(lds)), "v"(off),
-               "s"(uniform(base))
-               : "memory");
+// ONCE: nothing else reads these keys (a request's own), so they need not
+// stay in the caches: own keys alone, 256 requests of 1 to 1024, take 106 us so
+// and 120 without; the shared keys, which all row tiles read, take 4% longer.
+template <bool ONCE> __device__ __forceinline__ void load_to_lds(const uint8_t *base, uint32_t off, uint32_t lds) {
+  if constexpr (ONCE)
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2 nt" ::"s"(__builtin_amdgcn_readfirstlane(lds)),
+                 "v"(off), "s"(uniform(base))
+                 : "memory");
+  else
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(__builtin_amdgcn_readfirstlane(lds)), "v"(off),
+                 "s"(uniform(base))
+                 : "memory");
 }
 __device__ __forceinline__ void load_to_lds(const uint8_t *at, uint32_t lds) {
   asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off" ::"s"(__builtin_amdgcn_readfirstlane(lds)), "v"(at) : "memory");
@@ -420,11 +429,11 @@ template <int D, bool V> __device__ __forceinline__ void load_single_rows(const 
 }
 
 // A group's K or V to LDS, off[i] as row_offset gives it.
-template <int D, bool V>
+template <int D, bool V, bool ONCE>
 __device__ __forceinline__ void load_group(const Keys &s, const Place &at, int key, const uint32_t (&off)[D / 32], uint32_t lds) {
   if (at.whole) {
 #pragma unroll
-    for (int i = 0; i < D / 32; ++i) load_to_lds(V ? at.v : at.k, off[i], lds + i * 1024);
+    for (int i = 0; i < D / 32; ++i) load_to_lds<ONCE>(V ? at.v : at.k, off[i], lds + i * 1024);
   } else {
     load_single_rows<D, V>(s, key, lds);
   }
@@ -554,7 +563,7 @@ __device__ __forceinline__ void store_rows(const AttnArgs &a, const Rows32<T, D>
 // bound by the bytes of K and V.  The next block's K is loaded once this
 // one's has been read, while V is used, and its V after that, so some load is
 // always under way.
-template <typename T, int D>
+template <typename T, int D, bool ONCE>
 __device__ __forceinline__ void attend_narrow(const AttnArgs &a, Rows32<T, D> &r, Keys &keys, int entry, int least, uint32_t k) {
   constexpr int kPer = D / 32;  // loads of a group
   const uint32_t v = k + 32 * D * 2;
@@ -568,12 +577,12 @@ __device__ __forceinline__ void attend_narrow(const AttnArgs &a, Rows32<T, D> &r
   }
   Place lo, hi;
   auto load_k = [&](int j) {
-    load_group<D, false>(keys, lo, j, k_off, k);
-    load_group<D, false>(keys, hi, j + 16, k_off, k + kPer * 1024);
+    load_group<D, false, ONCE>(keys, lo, j, k_off, k);
+    load_group<D, false, ONCE>(keys, hi, j + 16, k_off, k + kPer * 1024);
   };
   auto load_v = [&](int j) {
-    load_group<D, true>(keys, lo, j, v_off, v);
-    load_group<D, true>(keys, hi, j + 16, v_off, v + kPer * 1024);
+    load_group<D, true, ONCE>(keys, lo, j, v_off, v);
+    load_group<D, true, ONCE>(keys, hi, j + 16, v_off, v + kPer * 1024);
   };
   keys.look_up(0, entry);
   lo = keys.place(0);
@@ -635,11 +644,11 @@ __device__ __forceinline__ void attend_wide(const AttnArgs &a, Rows32<T, D> &r, 
   const uint32_t own = lds + wave * kGroup;
   keys.look_up(0, entry);
   Place now = keys.place(wave), last;  // of the block whose K, and the one whose V is loaded
-  load_group<D, false>(keys, now, k0 + 16 * wave, k_off, own);
-  load_group<D, true>(keys, now, k0 + 16 * wave, v_off, own + 2 * kBlock);
+  load_group<D, false, false>(keys, now, k0 + 16 * wave, k_off, own);
+  load_group<D, true, false>(keys, now, k0 + 16 * wave, v_off, own + 2 * kBlock);
   if (n > 1) {
     now = keys.place(4 + wave);
-    load_group<D, false>(keys, now, k0 + 64 + 16 * wave, k_off, own + kBlock);
+    load_group<D, false, false>(keys, now, k0 + 64 + 16 * wave, k_off, own + kBlock);
   }
   wait_rows<T, D>(r);
   wait_loads<0>();
@@ -670,9 +679,9 @@ __device__ __forceinline__ void attend_wide(const AttnArgs &a, Rows32<T, D> &r, 
       last = now;
       if (j + 2 < n) {
         now = keys.place(4 * (j + 2) + wave);
-        load_group<D, false>(keys, now, j0 + 128 + 16 * wave, k_off, own + odd);
+        load_group<D, false, false>(keys, now, j0 + 128 + 16 * wave, k_off, own + odd);
       }
-      load_group<D, true>(keys, last, j0 + 64 + 16 * wave, v_off, own + 2 * kBlock + (kBlock - odd));
+      load_group<D, true, false>(keys, last, j0 + 64 + 16 * wave, v_off, own + 2 * kBlock + (kBlock - odd));
     }
     const uint32_t k = lds + (kBlock - odd), v = lds + 2 * kBlock + odd;
     // (addresses are computed in each block and not kept in registers)
@@ -840,7 +849,7 @@ template <typename T, int D, bool WIDE> __global__ void __launch_bounds__(256, D
     load_rows<T, D>(a, r, t, h * a.group + (t < 0 ? 0 : x % a.group), limit);
     const int least = least_limit<WIDE>(r.limit, lds);
     if constexpr (WIDE) attend_wide<T, D>(a, r, keys, entry, least, at);
-    else attend_narrow<T, D>(a, r, keys, entry, least, at + wave * (2 * 32 * D * 2));
+    else attend_narrow<T, D, false>(a, r, keys, entry, least, at + wave * (2 * 32 * D * 2));
     store_part<T, D, !WIDE>(a, r, limit <= 0, part, lds);
     return;
   }
@@ -876,7 +885,7 @@ template <typename T, int D, bool WIDE> __global__ void __launch_bounds__(256, D
     }
     const int entry = keys.entry(0);
     load_rows<T, D>(a, r, t, head, limit);
-    attend_narrow<T, D>(a, r, keys, entry, least_limit<false>(r.limit, lds), at + wave * (2 * 32 * D * 2));
+    attend_narrow<T, D, true>(a, r, keys, entry, least_limit<false>(r.limit, lds), at + wave * (2 * 32 * D * 2));
     store_rows<T, D>(a, r, limit <= 0, a.prefix_parts + part);
   }
 }
@@ -1002,15 +1011,18 @@ Plan make_plan(int64_t T, int64_t R, int64_t kv_heads, int64_t group, int64_t sh
   // places, at a key of its own in half of the time of a request's own key
   // (which comes from memory, while all row tiles read the prefix; requests
   // are taken to have half of their tables' keys, 512 at most), so that both
-  // end together: 256 requests, 32 heads over 16384 keys, up to 1024 own: 163
-  // us, with two thirds of that 180, with five thirds 194.  A part has four wide
+  // end together: 256 requests, 32 heads over 16384 keys, up to 1024 own: 151
+  // to 155 us, with 7/4 of its share 160.  A part has four wide
   // blocks or one round of narrow ones at least: it costs a row of 32-bit
-  // sums to write and read.
+  // sums to write and read.  Under three parts are rounded up, since one
+  // part's time is then the call's: 256 requests over 4096 and 8192 shared
+  // keys take 118 and 126 us with 2 and 3, 134 and 135 with 1 and 2; above,
+  // the nearest is better (12000 keys: 138 us with 3, 142 with 4).
   const double prefix_cost = static_cast<double>(items) * shared_len;
   const double own_cost = static_cast<double>(own_items) * std::min<int64_t>(own, 1024);
   const int64_t places = static_cast<int64_t>(std::min(512.0, 768 * prefix_cost / (prefix_cost + own_cost + 1)));
   const int64_t most = p.wide ? std::max<int64_t>(1, shared_len / (4 * tile)) : (shared_len + tile - 1) / tile;
-  p.prefix_parts = shared_len == 0 ? 0 : static_cast<int>(std::min<int64_t>(most, std::max<int64_t>(1, (places + items / 2) / items)));
+  p.prefix_parts = shared_len == 0 ? 0 : static_cast<int>(std::min<int64_t>(most, std::max<int64_t>(1, (places + (places < 3 * items ? items - 1 : items / 2)) / items)));
   p.prefix_chunk = 0;
   if (p.prefix_parts) {
     p.prefix_chunk = static_cast<int>(((shared_len + p.prefix_parts - 1) / p.prefix_parts + tile - 1) / tile * tile);
