@@ -531,7 +531,8 @@ int lmc_layerwise_prefill_dma_copy_diagnose(const lmc_dma_segment *copies, int64
  * request (-1 behind the list's end), and *next_cursor = free_cursor + the
  * blocks asked for, also where the list ended before.  free_cursor and
  * next_cursor are [1] int64, distinct, and may be null (a null cursor is 0).
- * At most 16384 requests, W * block_size < 2^31. */
+ * At most 16384 requests, W * block_size < 2^31.  Outputs overlap neither each
+ * other nor what the call reads. */
 int lmc_build_slot_mapping(const lmc_tensor *query_lens, const lmc_tensor *context_lens,
                            const lmc_tensor *block_table, int64_t block_size,
                            const lmc_tensor *slot_mapping, const lmc_tensor *positions,
@@ -584,7 +585,11 @@ int lmc_rotary_embedding_to_paged(const lmc_tensor *positions, const lmc_tensor 
  * boundary: with workspace_bytes not null it only writes the size that this
  * call needs there (0 for a call without rows), from the tensors' sizes
  * alone.  Calls that may run at the same time take workspaces of their own.
- * Rows of query, output and the caches start on 16-byte boundaries. */
+ * Rows of query, output and the caches start on 16-byte boundaries, the
+ * caches' rows less than 2^27 bytes apart.  output and lse may lie over query,
+ * or beside each other as columns of one buffer; otherwise nothing that the
+ * call writes may overlap what it reads.  scale is a normal number in 32
+ * bits, also times log2(e). */
 int lmc_shared_prefix_attention(const lmc_tensor *query, const lmc_tensor *vllm_kv_caches, int32_t n_caches,
                                 const lmc_tensor *shared_blocks, int64_t shared_len,
                                 const lmc_tensor *block_table, const lmc_tensor *seq_lens,
