@@ -549,7 +549,8 @@ int lmc_build_slot_mapping(const lmc_tensor *query_lens, const lmc_tensor *conte
  * dtype) with any token and head strides; either may be null.  query_out and
  * key_out take the results (other dims are copied), null means in place.
  * positions: [T] int64 or int32, any values; inv_freq: device array of n_freq
- * doubles, radians per position.  Angles are formed in 64 bits. */
+ * doubles, radians per position.  Angles are formed in 64 bits.  T is at most
+ * 2^25 - 2. */
 int lmc_rotary_embedding(const lmc_tensor *positions, const lmc_tensor *query, const lmc_tensor *key,
                          int64_t head_size, const double *inv_freq, int64_t n_freq, double scale,
                          int32_t is_neox, int64_t rotary_offset, int32_t inverse,

@@ -418,12 +418,13 @@ void rotary(const lmc_tensor *positions, const lmc_tensor *query, const lmc_tens
   a.scale = static_cast<float>(scale);
   a.inverse = inverse;
   a.n_tokens = T;
-  expect(T <= INT32_MAX, "too many tokens");
   // Two tokens share a workgroup once there are workgroups enough (their
   // angles then fill its lanes): 16384 tokens of 32 + 8 + 8 heads to their
   // pages take 73 us with two, 74 with one, 79 with four and 93 with eight.
   const int tb = T >= 2048 ? kMaxTokens : 1;
   a.tokens_per_block = tb;
+  // A launch has less than 2^32 threads along a dimension.
+  expect((T + tb - 1) / tb <= UINT32_MAX / kThreads, "too many tokens");
   expect(static_cast<int64_t>(tb) * units <= INT32_MAX, "rows are too wide");
   DeviceGuard guard(dev);
   switch (lead.dtype) {

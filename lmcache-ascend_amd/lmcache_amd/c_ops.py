@@ -672,7 +672,8 @@ def rotary_embedding(
     get the other dims copied.  inverse turns back by the same angles (scale
     multiplies there too): the transpose, so the gradient, and for scale 1 the
     way from positioned keys to position-free ones.  positions ([T] int64 or
-    int32) may be negative: new - old positions re-rotate."""
+    int32) may be negative: new - old positions re-rotate.  T is at most
+    2^25 - 2."""
     if _ext is not None:
         _ext.rotary_embedding(positions, query, key, int(head_size), inv_freq, bool(is_neox), int(rotary_offset),
                               float(scale), bool(inverse), query_out, key_out)
