@@ -1,0 +1,70 @@
+"""The serving operators at the ends of their sizes, eager and captured."""
+
+import numpy as np
+import pytest
+import torch
+
+from oracle import serving as osv
+
+pytestmark = pytest.mark.gpu
+
+DEV = "cuda:0"
+
+
+@pytest.fixture(scope="module")
+def ops():
+    import lmcache_amd
+
+    return lmcache_amd.c_ops
+
+
+@pytest.mark.parametrize("T", [1, 2047, 2048, 2049])
+@pytest.mark.parametrize("n_freq", [4096, 2500])
+def test_rotary_heads_of_8192_dims(ops, T, n_freq):
+    """The longest angles' rows, one and two tokens' of them in a workgroup."""
+    dim = 8192
+    gen = torch.Generator().manual_seed(T)
+    x = torch.randn((T, dim), generator=gen).to(torch.bfloat16)
+    pos = torch.randint(0, 100000, (T,), generator=gen)
+    inv = 10000.0 ** (-torch.arange(n_freq, dtype=torch.float64) / n_freq)
+    got = x.to(DEV)
+    ops.rotary_embedding(pos.to(DEV), got, None, dim, inv.to(DEV))
+    torch.cuda.synchronize()
+    want, size = osv.rotate(x.double().numpy(), pos.numpy(), inv.numpy(), dim, True)
+    assert (np.abs(got.double().cpu().numpy() - want) <= osv.rotary_tolerance(want, size, x.dtype)).all()
+
+
+@pytest.mark.parametrize("R", [6200, 16384])
+def test_captured_slot_mapping_of_many_requests(ops, R):
+    """Two sums of more than 48 KiB in a workgroup, replayed on the lengths of
+    each replay's time."""
+    rng = np.random.default_rng(R)
+    block, width, n = 16, 6, 2 * R + 5
+    q, c = (torch.zeros(R, dtype=torch.int32, device=DEV) for _ in range(2))
+    table = torch.zeros((R, width), dtype=torch.int32, device=DEV)
+    free = torch.from_numpy(rng.permutation(3 * R).astype(np.int32)).to(DEV)
+    cursor, following = (torch.zeros(1, dtype=torch.int64, device=DEV) for _ in range(2))
+    slots, pos = (torch.empty(n, dtype=torch.int64, device=DEV) for _ in range(2))
+    starts, seq = torch.empty(R + 1, dtype=torch.int32, device=DEV), torch.empty(R, dtype=torch.int32, device=DEV)
+
+    def call():
+        ops.build_slot_mapping(q, c, table, block, slots, pos, starts, seq, free, cursor, following)
+
+    call()
+    torch.cuda.synchronize()
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        call()
+    for turn in range(3):
+        query, context = rng.integers(0, 4, R), rng.integers(0, 60, R)
+        pages = rng.permutation(R * width).reshape(R, width)
+        q.copy_(torch.from_numpy(query.astype(np.int32)))
+        c.copy_(torch.from_numpy(context.astype(np.int32)))
+        table.copy_(torch.from_numpy(pages.astype(np.int32)))
+        cursor.fill_(turn)
+        g.replay()
+        torch.cuda.synchronize()
+        want = osv.slot_mapping(query, context, pages, block, n, free.tolist(), turn)
+        for got, w in zip((slots, pos, starts, seq, table), want):
+            assert np.array_equal(got.cpu().numpy(), w)
+        assert following.item() == want[5]
