@@ -590,7 +590,9 @@ int lmc_rotary_embedding_to_paged(const lmc_tensor *positions, const lmc_tensor 
  * caches' rows less than 2^27 bytes apart.  output and lse may lie over query,
  * or beside each other as columns of one buffer; otherwise nothing that the
  * call writes may overlap what it reads.  scale is a normal number in 32
- * bits, also times log2(e). */
+ * bits, also times log2(e).  T * heads is less than 2^24 and R less than 2^19;
+ * a call that would take 2^26 waves (one to eight for each request, KV head
+ * and 32 rows, by the table's width) is refused. */
 int lmc_shared_prefix_attention(const lmc_tensor *query, const lmc_tensor *vllm_kv_caches, int32_t n_caches,
                                 const lmc_tensor *shared_blocks, int64_t shared_len,
                                 const lmc_tensor *block_table, const lmc_tensor *seq_lens,

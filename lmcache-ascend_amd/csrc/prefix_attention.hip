@@ -1117,6 +1117,10 @@ extern "C" int lmc_shared_prefix_attention(const lmc_tensor *query, const lmc_te
     const Plan p = make_plan(T, R, kv.heads, group, shared_len, keys);
     const int64_t parts = p.prefix_parts + p.own_parts, rows = T * Hq;
     const int64_t bytes = parts * rows * (kv.dim * 4 + 8);
+    // A launch has less than 2^32 threads along a dimension.
+    const int64_t own_items = R * kv.heads * p.own_tiles * p.own_parts, own_groups = (own_items + 31) / 32;
+    const int64_t prefix_groups = (kv.heads * p.prefix_parts + 7) / 8 * p.prefix_tiles;
+    expect((own_groups + prefix_groups) * 8 <= UINT32_MAX / 256, "too many rows");
     if (workspace_bytes) {
       *workspace_bytes = bytes;
       return;
@@ -1183,11 +1187,7 @@ extern "C" int lmc_shared_prefix_attention(const lmc_tensor *query, const lmc_te
     a.prefix_chunk = p.prefix_chunk;
     a.own_tiles = p.own_tiles;
     a.own_want = p.own_want;
-    const int64_t own_items = R * kv.heads * p.own_tiles * p.own_parts;
-    expect(own_items <= INT32_MAX / 2, "too many rows");
     a.own_items = static_cast<int>(own_items);
-    const int64_t own_groups = (own_items + 31) / 32;
-    const int64_t prefix_groups = (kv.heads * p.prefix_parts + 7) / 8 * p.prefix_tiles;
     a.prefix_groups = static_cast<int>(prefix_groups);
     DeviceGuard guard(dev);
     const hipStream_t s = static_cast<hipStream_t>(stream);

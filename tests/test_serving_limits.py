@@ -53,3 +53,28 @@ def _rotary(T, dim, n_freq):
 def test_rotary_refuses_more_tokens_than_a_launch_has_threads(T):
     """Two tokens a workgroup of 256 threads: 2^25 - 2 of them at most."""
     _refuses(_rotary(T, 64, 32), "too many tokens")
+
+
+def _attention(T, R, Hq, Hk, dim, block=16, width=64, P=0, **over):
+    """(status, workspace bytes): the call that only asks for the size."""
+    a = dict(q=_t(BF16, T, Hq, dim), o=_t(BF16, T, Hq, dim), lse=None,
+             caches=_array(*(_t(BF16, 6, block, Hk, dim) for _ in range(2))), fmt=2)
+    a.update(over)
+    table, seq, starts, shared = _t(I32, R, width), _t(I32, R), _t(I32, R + 1), _t(I32, -(-P // block))
+    size = ctypes.c_int64(-1)
+    status = L.lmc_shared_prefix_attention(_ref(a["q"]), a["caches"], len(a["caches"]), _ref(shared), P, _ref(table), _ref(seq),
+                                           _ref(starts), 1.0, _ref(a["o"]), _ref(a["lse"]), None, ctypes.byref(size), a["fmt"],
+                                           0, None)
+    return status, size.value
+
+
+@pytest.mark.parametrize("T,R,heads", [(1, 2**19 - 1, 256), (1, 2**17, 128), (2**14, 2**17, 128)])
+def test_attention_refuses_more_parts_than_a_launch_has_threads(T, R, heads):
+    """A wave for each request, KV head and part: 2^26 of them at most."""
+    status, _ = _attention(T, R, heads, heads, 64, width=1024)     # eight parts of a request's own keys
+    _refuses(status, "too many rows")
+
+
+def test_attention_takes_as_many_as_a_launch_has_threads():
+    status, size = _attention(1, 2**16, 64, 64, 64, width=1024)
+    assert status == _lib.OK and size > 0
