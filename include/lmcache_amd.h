@@ -561,7 +561,8 @@ int lmc_rotary_embedding(const lmc_tensor *positions, const lmc_tensor *query, c
  * to the paged caches (MERGED_KV or SEPARATE_KV, any strides) at
  * slot_mapping ([T] int64 or int32); key and value stay as they are.  Tokens
  * whose slot lies outside the caches are not written.  Two tokens with one
- * slot leave either's row. */
+ * slot leave either's row.  No row of the K cache may lie over one of the V
+ * cache. */
 int lmc_rotary_embedding_to_paged(const lmc_tensor *positions, const lmc_tensor *query, const lmc_tensor *key,
                                   const lmc_tensor *value, const lmc_tensor *vllm_kv_caches, int32_t n_caches,
                                   const lmc_tensor *slot_mapping, int64_t head_size, const double *inv_freq,

@@ -350,6 +350,7 @@ void rotary(const lmc_tensor *positions, const lmc_tensor *query, const lmc_tens
     expect(rows_apart({kv.pages, kv.block_size, kv.heads, kv.dim * es}, {kv.k_page, kv.k_token, kv.k_head, 1}) &&
                     rows_apart({kv.pages, kv.block_size, kv.heads, kv.dim * es}, {kv.v_page, kv.v_token, kv.v_head, 1}),
                 "the paged caches have overlapping rows");
+    expect(k_and_v_apart(kv), "the K and V caches overlap");
     expect(kv.dim == head_size, "the paged caches' heads are not of head_size");
     const HeadView k = add(a.k, key, nullptr, "key", "", head_size, true);
     const HeadView v = add(a.v, value, nullptr, "value", "", head_size, false);

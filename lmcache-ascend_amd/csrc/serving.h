@@ -86,6 +86,22 @@ struct PagedKv {
   int device;
 };
 
+// Whether no row of K is one of V's: the caches one behind the other, pages
+// that hold K's part and V's beside each other, or rows dealt in turn.
+inline bool k_and_v_apart(const PagedKv &g) {
+  const int64_t row = g.dim * dtype_size(g.dtype), d = g.v - g.k;
+  const int64_t wide_k = (g.block_size - 1) * g.k_token + (g.heads - 1) * g.k_head + row;  // of a page
+  const int64_t wide_v = (g.block_size - 1) * g.v_token + (g.heads - 1) * g.v_head + row;
+  if (g.pages == 0 || d >= (g.pages - 1) * g.k_page + wide_k || -d >= (g.pages - 1) * g.v_page + wide_v) return true;
+  if (g.pages > 1 && g.k_page != g.v_page) return false;
+  if (g.pages > 1) {
+    const int64_t at = ((d % g.k_page) + g.k_page) % g.k_page;
+    if (at >= wide_k && at + wide_v <= g.k_page) return true;
+  }
+  if ((g.block_size > 1 && g.k_token != g.v_token) || (g.heads > 1 && g.k_head != g.v_head)) return false;
+  return rows_apart({2, g.pages, g.block_size, g.heads, row}, {std::abs(d), g.k_page, g.k_token, g.k_head, 1});
+}
+
 inline PagedKv paged_kv(const lmc_tensor *caches, int n, int fmt, bool two_major, const char *op) {
   validate_vllm_caches(caches, n, fmt);
   if (fmt != LMC_FMT_MERGED_KV && fmt != LMC_FMT_SEPARATE_KV)

@@ -78,3 +78,54 @@ def test_attention_refuses_more_parts_than_a_launch_has_threads(T, R, heads):
 def test_attention_takes_as_many_as_a_launch_has_threads():
     status, size = _attention(1, 2**16, 64, 64, 64, width=1024)
     assert status == _lib.OK and size > 0
+
+
+def _to_paged(caches, fmt=2, two_major=0):
+    """A call of no tokens: the caches are looked at, nothing is launched."""
+    pos, k, v, slots = _t(I64, 0), _t(BF16, 0, 128), _t(BF16, 0, 128), _t(I64, 0)
+    return L.lmc_rotary_embedding_to_paged(_ref(pos), None, _ref(k), _ref(v), caches, len(caches), _ref(slots), 64, 1 << 35, 32,
+                                           1.0, 1, 0, None, fmt, two_major, None)
+
+
+# Two KV heads of 64 dims in blocks of 16: a row has 64 elements, a block 2048.
+def _pair(by, strides, pages=6, v_strides=None):
+    k = _t(BF16, pages, 16, 2, 64, strides=strides)
+    return _array(k, _t(BF16, pages, 16, 2, 64, strides=v_strides or strides, data=k.data + 2 * by))
+
+
+_PLAIN = [2048, 128, 64, 1]
+
+
+@pytest.mark.parametrize("caches,fmt", [
+    (_pair(0, _PLAIN), 2),                                          # one cache as K and as V
+    (_pair(2048, _PLAIN), 2),                                       # a block further
+    (_pair(-64, _PLAIN), 2),                                        # a head before
+    (_pair(6 * 2048 - 64, _PLAIN), 2),                              # K's last row is V's first
+    (_pair(2048 - 128, [4096, 128, 64, 1]), 2),                     # V begins inside K's part of a page
+    (_pair(4096 - 128, [4096, 128, 64, 1]), 2),                     # V ends in the next page's K
+    (_pair(64, [8192, 256, 128, 1], v_strides=[8192, 256, 64, 1]), 2),
+    (_array(_t(BF16, 6, 2, 16, 2, 64, strides=[2048, 0, 128, 64, 1])), 1),
+])
+def test_rotary_to_paged_refuses_k_and_v_in_one_place(caches, fmt):
+    """Both are written: a row of both would hold either."""
+    _refuses(_to_paged(caches, fmt), "K and V caches overlap")
+
+
+@pytest.mark.parametrize("caches,fmt,two_major", [
+    (_pair(6 * 2048, _PLAIN), 2, 0),                                # one behind the other
+    (_pair(-6 * 2048, _PLAIN), 2, 0),
+    (_pair(2048, [4096, 128, 64, 1]), 2, 0),                        # beside each other in a page
+    (_pair(-2048, [4096, 128, 64, 1]), 2, 0),
+    (_pair(5 * 2048, [4096, 128, 64, 1]), 2, 0),                    # V from the third page on
+    (_pair(2048, [4096, 128, 64, 1], v_strides=[4096, 64, 1024, 1]), 2, 0),  # V of a page head by head
+    (_pair(128, [4096, 256, 64, 1]), 2, 0),                         # in turn, token by token
+    (_pair(64, [4096, 256, 128, 1]), 2, 0),                         # in turn, row by row
+    (_pair(64, [4096, 128, 2048, 1]), 2, 0),                        # in turn within a head
+    (_pair(2048, [7, 128, 64, 1], pages=1, v_strides=[9, 128, 64, 1]), 2, 0),
+    (_array(_t(BF16, 6, 2, 16, 2, 64)), 1, 0),
+    (_array(_t(BF16, 2, 6, 16, 2, 64)), 1, 1),
+    (_array(_t(BF16, 6, 2, 16, 2, 64, strides=[4096, 64, 256, 128, 1])), 1, 0),
+])
+def test_rotary_to_paged_takes_k_and_v_beside_each_other(caches, fmt, two_major):
+    status = _to_paged(caches, fmt, two_major)
+    assert status == _lib.OK, L.lmc_last_error()
