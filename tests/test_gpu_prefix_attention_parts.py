@@ -213,3 +213,20 @@ def test_captured_calls_of_every_head_size(ops, dim, R):
         torch.cuda.synchronize()
         assert torch.equal(eager["out"], d["out"]) and torch.equal(eager["lse"], d["lse"])
         _hold(_want(now), d["out"], d["lse"])
+
+
+@pytest.mark.parametrize("dim", [64, 128])
+def test_one_token_of_a_projection_of_odd_width(ops, dim):
+    """The stride of a dim of one entry is not used: one token, one head."""
+    c = _case(9, [1], [37], 90, 16, 4, 1, dim)
+    d = _device(c)
+    wide = torch.zeros((1, 4 * dim + 3), dtype=BF16, device=DEV)
+    wide[:, : 4 * dim] = d["q"].view(1, -1)
+    d["q"] = wide[:, : 4 * dim].view(1, 4, dim)
+    d["out"] = torch.as_strided(d["out"], (1, 4, dim), (5, dim, 1))
+    assert d["q"].stride(0) == 4 * dim + 3
+    for x in "kv":
+        d[x] = torch.as_strided(d[x], d[x].shape, (16 * dim, dim, 7, 1))
+    _call(ops, d)
+    torch.cuda.synchronize()
+    _hold(_want(c), d["out"], d["lse"])

@@ -129,3 +129,26 @@ def test_rotary_to_paged_refuses_k_and_v_in_one_place(caches, fmt):
 def test_rotary_to_paged_takes_k_and_v_beside_each_other(caches, fmt, two_major):
     status = _to_paged(caches, fmt, two_major)
     assert status == _lib.OK, L.lmc_last_error()
+
+
+@pytest.mark.parametrize("over,sizes", [
+    ({"q": _t(BF16, 1, 8, 64, strides=[1203, 64, 1])}, (1, 8, 2)),              # a token of an odd projection
+    ({"o": _t(BF16, 1, 8, 64, strides=[7, 64, 1])}, (1, 8, 2)),
+    ({"q": _t(BF16, 5, 1, 64, strides=[64, 3, 1])}, (5, 1, 1)),                 # one head
+    ({"o": _t(BF16, 5, 1, 64, strides=[64, 1, 1])}, (5, 1, 1)),
+    ({"caches": _array(*(_t(BF16, 6, 16, 1, 64, strides=[1024, 64, 5, 1]) for _ in range(2)))}, (5, 4, 1)),
+    ({"caches": _array(*(_t(BF16, 1, 16, 2, 64, strides=[9, 128, 64, 1]) for _ in range(2)))}, (5, 8, 2)),
+])
+def test_attention_takes_any_stride_of_a_dim_of_one(over, sizes):
+    T, Hq, Hk = sizes
+    status, size = _attention(T, 1, Hq, Hk, 64, **over)
+    assert status == _lib.OK and size > 0, L.lmc_last_error()
+
+
+@pytest.mark.parametrize("over", [
+    {"q": _t(BF16, 2, 8, 64, strides=[1203, 64, 1])},
+    {"o": _t(BF16, 2, 8, 64, strides=[1024, 100, 1])},
+])
+def test_attention_refuses_rows_off_a_16_byte_boundary(over):
+    status, _ = _attention(2, 1, 8, 2, 64, **over)
+    _refuses(status, "rows of query and output must start")
