@@ -228,7 +228,8 @@ def decode_chunk(chunk: CacheGenChunk) -> torch.Tensor:
 # ---------------------------------------------------------------------------
 
 
-def rotary_inv_freq(rotary_dim: int, base: float = 10000.0, scaling=None, seq_len: int = 0):
+def rotary_inv_freq(rotary_dim: int, base: float = 10000.0, scaling=None, seq_len: int = 0,
+                    max_position_embeddings: int = 0, original_max_position_embeddings: int = 0):
     """(inv_freq, scale) for c_ops.rotary_embedding: float64 [rotary_dim / 2]
     radians per position on the CPU, and the factor on cos and sin.
 
@@ -249,6 +250,11 @@ def rotary_inv_freq(rotary_dim: int, base: float = 10000.0, scaling=None, seq_le
                 the original context, else by "short_factor"[i]; scale
                 sqrt(1 + ln(factor) / ln(original)) unless "attention_factor"
                 says otherwise
+
+    Configurations hold some of this beside the dict.  Where the dict has no
+    "original_max_position_embeddings" it is the argument of that name, or
+    else max_position_embeddings; a longrope dict without "factor" has
+    max_position_embeddings / original.
     """
     if rotary_dim <= 0 or rotary_dim % 2:
         raise ValueError("rotary_dim must be even and positive")
@@ -266,14 +272,23 @@ def rotary_inv_freq(rotary_dim: int, base: float = 10000.0, scaling=None, seq_le
             raise ValueError(f"{kind} scaling needs {name}")
         return scaling[name]
 
+    def original_context():
+        given = scaling.get("original_max_position_embeddings")
+        if given is None:
+            given = original_max_position_embeddings or max_position_embeddings or need("original_max_position_embeddings")
+        return float(given)
+
     if kind == "longrope":
-        original = float(need("original_max_position_embeddings"))
+        original = original_context()
         factors = torch.tensor(need("long_factor" if seq_len > original else "short_factor"), dtype=torch.float64)
         if factors.numel() != rotary_dim // 2:
             raise ValueError("longrope scaling needs one factor per frequency")
         scale = scaling.get("attention_factor")
         if scale is None:
-            factor = float(need("factor"))
+            if scaling.get("factor") is None and max_position_embeddings:
+                factor = max_position_embeddings / original
+            else:
+                factor = float(need("factor"))
             if not original > 1:
                 raise ValueError("original_max_position_embeddings must be above 1")
             scale = 1.0 if factor <= 1.0 else math.sqrt(1.0 + math.log(factor) / math.log(original))
@@ -284,7 +299,7 @@ def rotary_inv_freq(rotary_dim: int, base: float = 10000.0, scaling=None, seq_le
         raise ValueError("factor must be positive")
     if kind == "linear":
         return inv / factor, 1.0
-    original = float(need("original_max_position_embeddings"))
+    original = original_context()
     if not original > 0:
         raise ValueError("original_max_position_embeddings must be positive")
     if kind == "dynamic":
