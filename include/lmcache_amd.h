@@ -523,8 +523,8 @@ int lmc_layerwise_prefill_dma_copy_diagnose(const lmc_dma_segment *copies, int64
  * or -1 where the table has no page (a negative entry, or p past its row).
  * slot_mapping and positions ([N] int64) get -1 and 0 behind the last token;
  * tokens past N are left out.  query_start_loc ([R + 1] int32) and seq_lens
- * ([R] int32, context + query) stop at 2^31 - 1.  positions, query_start_loc
- * and seq_lens may be null.
+ * ([R] int32, context + query) stop at 2^31 - 1, positions at 2^63 - 1.
+ * positions, query_start_loc and seq_lens may be null.
  * With free_blocks ([F] int32) the table is completed in place: entries
  * ceil(context / block_size) .. ceil((context + query) / block_size) of each
  * row, at most W, take blocks from free_blocks[free_cursor] on, request by

@@ -61,6 +61,9 @@ __device__ __forceinline__ int64_t len_at(const void *p, int i64, int r) {
   return v < 0 ? 0 : v;
 }
 
+// The position of the i-th new token behind c tokens, 2^63 - 1 past that.
+__device__ __forceinline__ int64_t position(int64_t c, uint32_t i) { return c > INT64_MAX - i ? INT64_MAX : c + i; }
+
 // Pages that hold `tokens` tokens, at most the table's width.
 __device__ __forceinline__ uint32_t pages_for(int64_t tokens, const SlotMapArgs &a) {
   const int64_t cap = static_cast<int64_t>(a.width) * a.block_size;  // < 2^31
@@ -107,7 +110,7 @@ __global__ void __launch_bounds__(1024) slot_map(SlotMapArgs a) {
   const int64_t cursor = grow && a.cursor ? *a.cursor : 0;
   const int64_t cap = static_cast<int64_t>(a.width) * a.block_size;  // < 2^31
   auto free_at = [&](int64_t i) {
-    i += cursor;
+    i = static_cast<int64_t>(static_cast<uint64_t>(i) + static_cast<uint64_t>(cursor));  // (any cursor)
     return i >= 0 && i < a.n_free ? a.free_blocks[i] : -1;
   };
   auto write = [&](int64_t t, int64_t pos, uint32_t at, int32_t page) {
@@ -164,9 +167,9 @@ __global__ void __launch_bounds__(1024) slot_map(SlotMapArgs a) {
     }
     if (mine && q <= kShort) {
       for (uint32_t i = 0; i < q && start + i < a.n_tokens; ++i) {
-        const int64_t pos = c + i;
+        const int64_t pos = position(c, i);
         uint32_t at = 0;
-        if (pos >= 0 && pos < cap) {
+        if (pos < cap) {
           const uint32_t p = static_cast<uint32_t>(pos), j = p / a.block_size;
           at = p - j * a.block_size;
           if (j >= have) page = free_at(static_cast<int64_t>(before_b) + (j - have));
@@ -235,8 +238,8 @@ __global__ void __launch_bounds__(1024) slot_map(SlotMapArgs a) {
       at[u] = 0;
       if (!todo[u] || r[u] < 0) continue;
       const uint32_t have = grow ? pages_for(pos[u], a) : a.width;
-      pos[u] += static_cast<uint32_t>(t0 + 64 * u + lane) - sq[r[u]];
-      if (pos[u] >= 0 && pos[u] < cap) {
+      pos[u] = position(pos[u], static_cast<uint32_t>(t0 + 64 * u + lane) - sq[r[u]]);
+      if (pos[u] < cap) {
         const uint32_t p = static_cast<uint32_t>(pos[u]), j = p / a.block_size;
         at[u] = p - j * a.block_size;
         page[u] = j < have ? a.table[r[u] * a.table_stride + j] : free_at(static_cast<int64_t>(sb[r[u]]) + (j - have));

@@ -68,3 +68,28 @@ def test_captured_slot_mapping_of_many_requests(ops, R):
         for got, w in zip((slots, pos, starts, seq, table), want):
             assert np.array_equal(got.cpu().numpy(), w)
         assert following.item() == want[5]
+
+
+@pytest.mark.parametrize("q", [1, 5, 8, 9, 300])
+@pytest.mark.parametrize("grow", [False, True])
+def test_positions_past_64_bits(ops, q, grow):
+    """A request whose positions pass 2^63 - 1 stops there, without pages, and
+    its neighbours are as they would be; a cursor next to 2^63 - 1 finds no
+    block."""
+    top = 2**63 - 1
+    lens = torch.tensor([2, q, 3], dtype=torch.int64, device=DEV)
+    for back in (0, 1, 4):
+        context = torch.tensor([1, top - back, 4], dtype=torch.int64, device=DEV)
+        table = torch.tensor([[7, 3], [1, 2], [5, 6]], dtype=torch.int32, device=DEV)
+        slots, pos = (torch.full((q + 6,), -99, dtype=torch.int64, device=DEV) for _ in range(2))
+        more = {}
+        if grow:
+            more = {"free_blocks": torch.tensor([11, 12], dtype=torch.int32, device=DEV),
+                    "free_cursor": torch.tensor([top - 1], dtype=torch.int64, device=DEV)}
+        ops.build_slot_mapping(lens, context, table, 4, slots, pos, **more)
+        torch.cuda.synchronize()
+        far = [min(top, top - back + i) for i in range(q)]
+        assert pos.tolist() == [1, 2] + far + [4, 5, 6, 0]
+        own = [-1, -1, -1] if grow else [6 * 4, 6 * 4 + 1, 6 * 4 + 2]      # block 1 of request 2 is new
+        assert slots.tolist() == [7 * 4 + 1, 7 * 4 + 2] + [-1] * q + own + [-1]
+        assert table[2, 1].item() == (-1 if grow else 6)
