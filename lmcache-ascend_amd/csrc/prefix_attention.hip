@@ -148,7 +148,6 @@ template <int N> __device__ __forceinline__ void wait_loads() { asm volatile("s_
 // LDS reads have their data: what they read may be written again.
 __device__ __forceinline__ void wait_reads() { asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory"); }
 
-typedef __attribute__((address_space(3))) uint8_t LdsByte;
 typedef __attribute__((address_space(3))) s16x4 LdsS4;
 typedef __attribute__((address_space(3))) s16x8 LdsS8;
 
@@ -297,23 +296,21 @@ template <typename T, int D> __device__ __forceinline__ void refer_to(Rows32<T, 
 
 // Weights, rounded to the type once for the product with V (l sums them
 // before the rounding).
-template <typename T, int D, int NB>
-__device__ __forceinline__ void weigh(Rows32<T, D> &r, const f32x16 (&s)[NB], typename Mma<T>::V8 (&p)[2 * NB], float c) {
+template <typename T, int D>
+__device__ __forceinline__ void weigh(Rows32<T, D> &r, const f32x16 &s, typename Mma<T>::V8 (&p)[2], float c) {
   const float base = r.m == -INFINITY ? 0.f : r.m;
 #pragma unroll
-  for (int b = 0; b < NB; ++b)
-#pragma unroll
-    for (int i = 0; i < 16; ++i) {
-      const float w = __builtin_amdgcn_exp2f(s[b][i] * c - base);
-      r.l += w;
-      p[2 * b + i / 8][i % 8] = Mma<T>::from(w);
-    }
+  for (int i = 0; i < 16; ++i) {
+    const float w = __builtin_amdgcn_exp2f(s[i] * c - base);
+    r.l += w;
+    p[i / 8][i % 8] = Mma<T>::from(w);
+  }
 }
 
 // O^T += V^T P^T.  The sum over keys may take them in any order: the order in
 // which a lane holds its 8 of 16 weights, keys 4 hb + {0..3, 8..11}.
-template <typename T, int D, int NB>
-__device__ __forceinline__ void add_values(Rows32<T, D> &r, uint32_t v, const typename Mma<T>::V8 (&p)[2 * NB]) {
+template <typename T, int D>
+__device__ __forceinline__ void add_values(Rows32<T, D> &r, uint32_t v, const typename Mma<T>::V8 (&p)[2]) {
   using M = Mma<T>;
   constexpr int kPitch = Geometry<D>::kPitch;
   const int lane = threadIdx.x & 63, hb = lane >> 5, a = lane & 15;
@@ -322,7 +319,7 @@ __device__ __forceinline__ void add_values(Rows32<T, D> &r, uint32_t v, const ty
   const uint32_t vcol = 2 * ((lane >> 4) & 1) + ((a & 3) >> 1);
   const uint32_t vbase = v + vrow * kPitch + (a & 1) * 8;
 #pragma unroll
-  for (int c2 = 0; c2 < 2 * NB; ++c2)
+  for (int c2 = 0; c2 < 2; ++c2)
 #pragma unroll
     for (int t = 0; t < D / 32; ++t) {
       const uint32_t at = vbase + (((4 * t + vcol) ^ vx) << 4) + c2 * 16 * kPitch;
@@ -610,11 +607,11 @@ __device__ __forceinline__ void attend_narrow(const AttnArgs &a, Rows32<T, D> &r
       hide<1>(s, r.limit, j0, seen);
     }
     refer_to<T, D>(r, largest<1>(s, a.scale2));
-    weigh<T, D, 1>(r, s, p, a.scale2);
+    weigh<T, D>(r, s[0], p, a.scale2);
     if (more) wait_loads<2 * kPer>();
     else wait_loads<0>();
     if (cut && has_odd<T, D, 32>(v)) take_odd_out<T, D, 32, false>(r, v, j0, seen);
-    add_values<T, D, 1>(r, v, p);
+    add_values<T, D>(r, v, p);
     wait_reads();
     if (more) load_v(next);
   }

@@ -240,14 +240,13 @@ template <typename KD> void launch_style(const RotaryArgs &a, bool neox, int vp,
 // One tensor's token and head strides: [T, heads * D] or [T, heads, D].
 struct HeadView {
   const lmc_tensor *t = nullptr;
-  int64_t token = 0, head = 0, heads = 0, dim = 0;
+  int64_t token = 0, head = 0, heads = 0;
 };
 
 HeadView head_view(const lmc_tensor &t, const char *name, int64_t dim, int device, int32_t dtype) {
   check_on(t, name, device, dtype);
   HeadView v;
   v.t = &t;
-  v.dim = dim;
   expect(t.ndim == 2 || t.ndim == 3, name, " must be [tokens, heads * head_size] or [tokens, heads, head_size]");
   for (int i = 0; i < t.ndim; ++i) expect(t.strides[i] >= 0, name, ": negative strides unsupported");
   expect(size(t, -1) <= 1 || stride(t, -1) == 1, name, ": a head's dims must be adjacent");
