@@ -582,7 +582,8 @@ int lmc_rotary_embedding_to_paged(const lmc_tensor *positions, const lmc_tensor 
  * rows of the caches are never used, whatever they hold.  A token that sees
  * no key gets zeros and an lse of -infinity; rows of output and lse behind
  * query_start_loc[R] are left as they were.  lse ([T, heads] fp32, may be
- * null): log of the sum of exp(scale * q . k).
+ * null): log of the sum of exp(scale * q . k).  Sums and maxima have 32 bits;
+ * the softmax weights are rounded to the caches' type for the product with V.
  * The call works in `workspace`, a 1-D uint8 tensor of the GPU on a 16-byte
  * boundary: with workspace_bytes not null it only writes the size that this
  * call needs there (0 for a call without rows), from the tensors' sizes

@@ -27,11 +27,29 @@
 // registers; K and V go from memory to LDS without registers between, and V
 // is read from there transposed.
 //
+// The weights are rounded to the caches' type for the product with V: the
+// matrix instructions take both operands in 16 bits (in 32 they have a
+// sixteenth of the rate).  Scores, maximum, sum, lse and the sums of V stay in
+// 32 bits.  A weight is then off by at most half a step of the type, in
+// outputs of some thousand keys 0.0023 of their size against 64 bits, where
+// 32-bit weights and the output's own rounding give 0.0017 (bf16).
+//
 // 256 requests, 32 heads over 8 KV heads of 128 bf16 dims, 16384 shared and 1
-// to 1024 own keys: 153 us (71 GFLOP, 607 MB), of which 11 the join; the
-// prefix alone takes 95 us (750 TFLOP/s), the own keys alone 106 (5.1 TB/s).
-// 64 requests over 4096 shared and the same own keys: 42 us.  4 requests over
-// 1000 shared and 1 to 200 own keys: 12 us, the latency of two launches.
+// to 1024 own keys: 154 to 158 us (71 GFLOP, 607 MB), of which 11 the join;
+// calls of the prefix alone take 98 us (700 TFLOP/s), of the own keys alone
+// 115 (4.7 TB/s).  64 requests over 4096 shared and the same own keys: 42 to
+// 44 us.  4 requests over 1000 shared and 1 to 200 own keys: 12 us, the latency
+// of two launches.
+//
+// Prompts: 512 new tokens of one request over 16384 shared keys take 192 us
+// (730 TFLOP/s), 2048 take 764 (770).  Their own keys go at 32 rows a wave, to
+// the request's end also where a tile's rows end before: 8192 new tokens
+// without a prefix take 3.1 ms (180 TFLOP/s).
+//
+// Registers at 128 dims: 256 for wide tiles (2 of them spilled, 12 bytes of
+// scratch, two waves a SIMD), 195 for narrow ones; at 64 dims 193 and 131; 192
+// and 256 dims take accumulation registers too, a wave a SIMD.  48 to 60 scalar
+// registers are kept in vector registers.
 #include "rope_math.h"
 #include "serving.h"
 
@@ -128,9 +146,14 @@ __device__ __forceinline__ uint64_t uniform(const void *p) {
   const uint32_t hi = __builtin_amdgcn_readfirstlane(static_cast<uint32_t>(x >> 32));
   return (static_cast<uint64_t>(hi) << 32) | lo;
 }
-// ONCE: nothing else reads these keys (a request's own), so they need not
-// stay in the caches: own keys alone, 256 requests of 1 to 1024, take 106 us so
-// and 120 without; the shared keys, which all row tiles read, take 4% longer.
+// ONCE: a request's own keys, which its one tile of 32 rows reads once, so they
+// need not stay in the caches: own keys alone, 256 requests of 1 to 1024, take
+// 115 us so and 127 without, 64 requests with a prefix 43.5 and 50; the shared
+// keys, which all row tiles read, take 4% longer.  A prompt's tiles read its own
+// keys once each and would rather find them there: 2048 new tokens over 16384
+// shared keys take 764 us so and 743 without, 8192 over none 3.1 ms and 2.3.
+// The kernel is made for the former.  (m0 is reserved: nothing but these
+// statements writes it in this file's kernels, each right before its load.)
 template <bool ONCE> __device__ __forceinline__ void load_to_lds(const uint8_t *base, uint32_t off, uint32_t lds) {
   if constexpr (ONCE)
     asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2 nt" ::"s"(__builtin_amdgcn_readfirstlane(lds)),
@@ -294,8 +317,8 @@ template <typename T, int D> __device__ __forceinline__ void refer_to(Rows32<T, 
   }
 }
 
-// Weights, rounded to the type once for the product with V (l sums them
-// before the rounding).
+// Weights, rounded to the type once for the product with V, which takes 16
+// bits (l sums them before the rounding, so lse has none of it).
 template <typename T, int D>
 __device__ __forceinline__ void weigh(Rows32<T, D> &r, const f32x16 &s, typename Mma<T>::V8 (&p)[2], float c) {
   const float base = r.m == -INFINITY ? 0.f : r.m;
@@ -1000,7 +1023,11 @@ Plan make_plan(int64_t T, int64_t R, int64_t kv_heads, int64_t group, int64_t sh
   p.wide = rows > 64;
   const int64_t m = p.wide ? 128 : 32, tile = p.wide ? 64 : 128;
   p.prefix_tiles = static_cast<int>((rows + m - 1) / m);
-  const int64_t per = (T + R - 1) / R * group;  // rows of a request, about
+  // Rows of a request, about.  (The lengths are on the GPU.  A request far above
+  // the mean goes through its tiles in turn: 255 requests of one new token and
+  // one of 2048, over 4096 shared keys, take 4.3 ms together and 0.12 + 0.39 in
+  // two calls.)
+  const int64_t per = (T + R - 1) / R * group;
   p.own_tiles = static_cast<int>(std::max<int64_t>(1, (per + 31) / 32));
   const int64_t own = std::max<int64_t>(0, table_keys - shared_len);
   const int64_t items = p.prefix_tiles * kv_heads, own_items = R * kv_heads * p.own_tiles;

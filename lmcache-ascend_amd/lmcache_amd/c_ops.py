@@ -756,7 +756,13 @@ def shared_prefix_attention(
     used, whatever they hold.  Tokens that see no key (or whose every score is
     -infinity) get zeros and an lse of -infinity; rows behind the last request
     are left as they were.  lse ([T, heads] float32): log of the sum of
-    exp(scale * q . k), to join with attention over further keys."""
+    exp(scale * q . k), to join with attention over further keys.
+
+    Sums, maxima and lse are held in 32 bits; the softmax weights are rounded
+    to the caches' dtype for the product with V, as the output is at the end.
+    Blocks of a multiple of 16 keys are read a group at a time, others key by
+    key (three times the time).  Give requests with long prompts a call of
+    their own: tiles are dealt by the mean of the new tokens."""
     if _ext is not None:
         _ext.shared_prefix_attention(query, vllm_kv_caches, shared_blocks, int(shared_len), block_table, seq_lens,
                                      query_start_loc, float(scale), output, lse, int(kvcache_format_raw),
