@@ -5,6 +5,7 @@
 
 #include "kv_geom.h"
 
+#include <functional>
 #include <initializer_list>
 #include <sstream>
 
@@ -39,18 +40,57 @@ inline bool extents_meet(const lmc_tensor &a, const lmc_tensor &b) {
   return na > 0 && nb > 0 && pa < pb + nb && pb < pa + na;
 }
 
-// Whether two tensors may share an element.  Column slices of one buffer (the
-// same stride of the first dim, each row's elements inside it) are told apart.
+// A strided layout of bytes: (stride, size) of each dim of more than one
+// entry, strides descending, the element's bytes last.
+struct Layout {
+  std::pair<int64_t, int64_t> dims[LMC_MAX_DIMS + 1];
+  int n = 0;
+  bool empty = false;
+  void dim(int64_t size, int64_t stride) {
+    if (size == 0) empty = true;
+    if (size > 1) dims[n++] = {stride, size};
+  }
+  void sort() { std::sort(dims, dims + n, std::greater<>()); }
+};
+
+inline Layout layout_of(const lmc_tensor &t) {
+  Layout l;
+  const int64_t es = elem_size(t);
+  for (int i = 0; i < t.ndim; ++i) l.dim(t.sizes[i], t.strides[i] * es);
+  l.dim(es, 1);
+  l.sort();
+  return l;
+}
+
+// Whether no byte of a's dims from i on is one of b's from j on, b beginning d
+// bytes behind a.  Ranges that do not meet are apart; else, where both step
+// by the same outermost stride, each pair of steps whose inner ranges meet has
+// to be.  (A stride's two neighbours are the most that can; layouts that cross
+// themselves or step differently count as not apart.)
+inline bool apart(const Layout &a, const Layout &b, int64_t d, int i = 0, int j = 0) {
+  auto extent = [](const Layout &l, int k) {
+    int64_t n = 1;
+    for (; k < l.n; ++k) n += (l.dims[k].second - 1) * l.dims[k].first;
+    return n;
+  };
+  if (a.empty || b.empty || d >= extent(a, i) || -d >= extent(b, j)) return true;
+  if (i == a.n || j == b.n || a.dims[i].first != b.dims[j].first || a.dims[i].first <= 0) return false;
+  const int64_t s = a.dims[i].first, wide_a = extent(a, i + 1), wide_b = extent(b, j + 1);
+  auto floor_by_s = [s](int64_t x) { return (x >= 0 ? x : x - s + 1) / s; };
+  // b's entry n behind a's begins d + s n behind it: in (-wide_b, wide_a).
+  const int64_t first = std::max(1 - a.dims[i].second, floor_by_s(-wide_b - d) + 1);
+  const int64_t last = std::min(b.dims[j].second - 1, -floor_by_s(d - wide_a) - 1);
+  if (last - first > 1) return false;
+  for (int64_t n = first; n <= last; ++n)
+    if (!apart(a, b, d + s * n, i + 1, j + 1)) return false;
+  return true;
+}
+
+// Whether two tensors may share an element: column slices of one buffer, and
+// rows of theirs in turn, are told apart.
 inline bool may_share(const lmc_tensor &a, const lmc_tensor &b) {
-  if (!extents_meet(a, b)) return false;
-  if (a.ndim == 0 || b.ndim == 0) return true;
-  const int64_t s = a.strides[0] * elem_size(a);
-  const int64_t wa = extent_bytes(a) - (a.sizes[0] - 1) * s;
-  const int64_t wb = extent_bytes(b) - (b.sizes[0] - 1) * b.strides[0] * elem_size(b);
-  if (b.strides[0] * elem_size(b) != s || wa > s || wb > s) return true;
-  const int64_t d = reinterpret_cast<intptr_t>(b.data) - reinterpret_cast<intptr_t>(a.data);
-  const int64_t m = ((d % s) + s) % s;
-  return !(m >= wa && m + wb <= s);
+  return extents_meet(a, b) &&
+         !apart(layout_of(a), layout_of(b), reinterpret_cast<intptr_t>(b.data) - reinterpret_cast<intptr_t>(a.data));
 }
 
 // Whether no two elements of a strided layout are the same one: in order of
@@ -89,17 +129,18 @@ struct PagedKv {
 // Whether no row of K is one of V's: the caches one behind the other, pages
 // that hold K's part and V's beside each other, or rows dealt in turn.
 inline bool k_and_v_apart(const PagedKv &g) {
-  const int64_t row = g.dim * dtype_size(g.dtype), d = g.v - g.k;
-  const int64_t wide_k = (g.block_size - 1) * g.k_token + (g.heads - 1) * g.k_head + row;  // of a page
-  const int64_t wide_v = (g.block_size - 1) * g.v_token + (g.heads - 1) * g.v_head + row;
-  if (g.pages == 0 || d >= (g.pages - 1) * g.k_page + wide_k || -d >= (g.pages - 1) * g.v_page + wide_v) return true;
-  if (g.pages > 1 && g.k_page != g.v_page) return false;
-  if (g.pages > 1) {
-    const int64_t at = ((d % g.k_page) + g.k_page) % g.k_page;
-    if (at >= wide_k && at + wide_v <= g.k_page) return true;
-  }
-  if ((g.block_size > 1 && g.k_token != g.v_token) || (g.heads > 1 && g.k_head != g.v_head)) return false;
-  return rows_apart({2, g.pages, g.block_size, g.heads, row}, {std::abs(d), g.k_page, g.k_token, g.k_head, 1});
+  Layout k, v;
+  auto add = [&](int64_t size, int64_t k_stride, int64_t v_stride) {
+    k.dim(size, k_stride);
+    v.dim(size, v_stride);
+  };
+  add(g.pages, g.k_page, g.v_page);
+  add(g.block_size, g.k_token, g.v_token);
+  add(g.heads, g.k_head, g.v_head);
+  add(g.dim * dtype_size(g.dtype), 1, 1);
+  k.sort();
+  v.sort();
+  return apart(k, v, g.v - g.k);
 }
 
 inline PagedKv paged_kv(const lmc_tensor *caches, int n, int fmt, bool two_major, const char *op) {

@@ -93,3 +93,39 @@ def test_positions_past_64_bits(ops, q, grow):
         own = [-1, -1, -1] if grow else [6 * 4, 6 * 4 + 1, 6 * 4 + 2]      # block 1 of request 2 is new
         assert slots.tolist() == [7 * 4 + 1, 7 * 4 + 2] + [-1] * q + own + [-1]
         assert table[2, 1].item() == (-1 if grow else 6)
+
+
+@pytest.mark.parametrize("T,H", [(1, 3), (70, 4), (3000, 2)])
+def test_rotary_of_heads_dealt_in_turn(ops, T, H):
+    """q, k and v of a head beside each other: q and k in place, and k and v
+    to their pages with q in place."""
+    dim, block = 64, 16
+    gen = torch.Generator().manual_seed(T)
+    x = torch.randn((T, H, 3, dim), generator=gen).to(torch.bfloat16)
+    pos = torch.randint(0, 5000, (T,), generator=gen)
+    inv = 10000.0 ** (-torch.arange(dim // 2, dtype=torch.float64) / (dim // 2))
+
+    def holds(got, part):
+        src = x[:, :, part].reshape(T, H * dim)
+        want, size = osv.rotate(src.double().numpy(), pos.numpy(), inv.numpy(), dim, True)
+        err = np.abs(got.reshape(T, H * dim).double().cpu().numpy() - want)
+        assert (err <= osv.rotary_tolerance(want, size, x.dtype)).all()
+
+    d = x.to(DEV)
+    ops.rotary_embedding(pos.to(DEV), d[:, :, 0], d[:, :, 1], dim, inv.to(DEV))
+    torch.cuda.synchronize()
+    holds(d[:, :, 0], 0)
+    holds(d[:, :, 1], 1)
+    assert torch.equal(d[:, :, 2].cpu(), x[:, :, 2])
+    d = x.to(DEV)
+    caches = torch.zeros((-(-T // block) + 1, block, H, 2, dim), dtype=torch.bfloat16, device=DEV)
+    slots = torch.arange(T, device=DEV)
+    ops.rotary_embedding_to_paged(pos.to(DEV), d[:, :, 0], d[:, :, 1], d[:, :, 2], (caches[:, :, :, 0], caches[:, :, :, 1]),
+                                  slots, dim, inv.to(DEV))
+    torch.cuda.synchronize()
+    holds(d[:, :, 0], 0)
+    assert torch.equal(d[:, :, 1:].cpu(), x[:, :, 1:])
+    rows = caches.view(-1, H, 2, dim)
+    holds(rows[:T, :, 0], 1)
+    assert torch.equal(rows[:T, :, 1].cpu(), x[:, :, 2])
+    assert (rows[T:] == 0).all()

@@ -4,7 +4,9 @@ addresses that nothing reads)."""
 
 import ctypes
 
+import numpy as np
 import pytest
+import torch
 
 from lmcache_amd import _lib
 
@@ -152,3 +154,65 @@ def test_attention_takes_any_stride_of_a_dim_of_one(over, sizes):
 def test_attention_refuses_rows_off_a_16_byte_boundary(over):
     status, _ = _attention(2, 1, 8, 2, 64, **over)
     _refuses(status, "rows of query and output must start")
+
+
+def _heads(base, by, H, row=3 * 64, T=5):
+    """[T, H, 64] from element `by` on, rows `row` apart, tokens H rows."""
+    return _t(BF16, T, H, 64, strides=[H * row, row, 1], data=base + 2 * by)
+
+
+_BASE = 1 << 45
+
+
+@pytest.mark.skipif(torch.cuda.is_available(), reason="the calls are taken, on addresses that are nobody's")
+@pytest.mark.parametrize("q,k,qo", [
+    (_heads(_BASE, 0, 8), _heads(_BASE, 64, 8), None),                  # q, k and v of a head beside each other
+    (_heads(_BASE, 64, 8), _heads(_BASE, 0, 8), None),
+    (_heads(_BASE, 0, 8), None, _heads(_BASE, 128, 8)),                 # q turned to v's place
+    (_heads(_BASE, 0, 1), _heads(_BASE, 64, 1), None),
+    (_heads(_BASE, 0, 8, T=1), _heads(_BASE, 64, 8, T=1), None),
+    (_heads(_BASE, 0, 8, row=64), _heads(_BASE, 5 * 8 * 64, 8, row=64), None),
+])
+def test_rotary_takes_rows_in_turn_of_one_buffer(q, k, qo):
+    status = L.lmc_rotary_embedding(_ref(_t(I64, q.sizes[0])), _ref(q), _ref(k), 64, 1 << 35, 32, 1.0, 1, 0, 0, _ref(qo), None,
+                                    None)
+    assert status != _lib.ERR_VALUE, L.lmc_last_error()
+
+
+@pytest.mark.parametrize("q,k", [
+    (_heads(_BASE, 0, 8), _heads(_BASE, 63, 8)),
+    (_heads(_BASE, 0, 8), _heads(_BASE, 3 * 64, 8)),                     # a head further
+    (_heads(_BASE, 0, 8), _heads(_BASE, -3 * 64 * 8 + 130, 8)),
+    (_heads(_BASE, 0, 8), _t(BF16, 5, 512, strides=[3 * 512, 1], data=_BASE + 128)),
+])
+def test_rotary_refuses_rows_that_cross(q, k):
+    status = L.lmc_rotary_embedding(_ref(_t(I64, 5)), _ref(q), _ref(k), 64, 1 << 35, 32, 1.0, 1, 0, 0, None, None, None)
+    _refuses(status, "overlap")
+
+
+def test_caches_that_are_taken_do_not_cross():
+    """Layouts at random: none whose rows cross is taken, and of those whose
+    rows do not, most are."""
+    rng = np.random.default_rng(0)
+    taken = apart = 0
+    for _ in range(3000):
+        pages, block, heads = (int(rng.integers(1, 4)) for _ in range(3))
+        gaps = [int(rng.choice([1, 2, 3])) for _ in range(3)]
+        sizes, names, strides, span = {"p": pages, "b": block, "h": heads}, list(rng.permutation(["p", "b", "h"])), {}, 64
+        for name, gap in zip(names, gaps):
+            strides[name] = span * gap
+            span = strides[name] * sizes[name]
+        by = 64 * int(rng.integers(-12, 13)) + int(rng.choice([0, 0, 0, 32]))
+        st = [strides["p"], strides["b"], strides["h"], 1]
+        at = (np.arange(pages)[:, None, None, None] * st[0] + np.arange(block)[:, None, None] * st[1]
+              + np.arange(heads)[:, None] * st[2] + np.arange(64)).ravel()
+        crosses = np.intersect1d(at, at + by).size > 0
+        k = _t(BF16, pages, block, heads, 64, strides=st)
+        caches = _array(k, _t(BF16, pages, block, heads, 64, strides=st, data=k.data + 2 * by))
+        rows = _t(BF16, 0, heads * 64)
+        status = L.lmc_rotary_embedding_to_paged(_ref(_t(I64, 0)), None, _ref(rows), _ref(rows), caches, 2, _ref(_t(I64, 0)), 64,
+                                                 1 << 35, 32, 1.0, 1, 0, None, 2, 0, None)
+        assert not (crosses and status == _lib.OK), (sizes, st, by)
+        apart += not crosses
+        taken += status == _lib.OK
+    assert taken >= 0.95 * apart, (taken, apart)
