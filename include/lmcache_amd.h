@@ -602,6 +602,73 @@ int lmc_shared_prefix_attention(const lmc_tensor *query, const lmc_tensor *vllm_
                                 const lmc_tensor *lse, const lmc_tensor *workspace, int64_t *workspace_bytes,
                                 int32_t kvcache_format, int32_t vllm_two_major, void *stream);
 
+/* Masks and positions of trees of drafted tokens, in one launch.  Request r's
+ * tokens are query_start_loc[r] .. query_start_loc[r + 1] ([R + 1] int32, from 0
+ * and not decreasing), the last of its seq_lens[r] ([R] int32).  parents ([T]
+ * int32): the index, among its request's tokens, of the one that each follows;
+ * negative, or not before the token itself: the context.  tree_mask ([T, W]
+ * int64, W at most 16) gets bit j % 64 of word j / 64 for the token itself and
+ * each that it follows, directly or not; positions ([T] int64, may be null) the
+ * context's length plus the tokens followed.  Tokens from index 64 W on get an
+ * empty mask and the position behind the context; rows behind
+ * query_start_loc[R] get zeros.  Outputs overlap neither each other nor what
+ * the call reads. */
+int lmc_build_draft_tree(const lmc_tensor *parents, const lmc_tensor *query_start_loc, const lmc_tensor *seq_lens,
+                         const lmc_tensor *tree_mask, const lmc_tensor *positions, void *stream);
+
+/* Attention of drafted tokens over one layer's caches, which hold their rows
+ * already.  Arguments, limits, workspace and what may overlap as for
+ * lmc_shared_prefix_attention (without its shared prefix); tree_mask is [T, W]
+ * int64 (W up to 2^20).  A request's q tokens see its first seq_lens[r] - q keys,
+ * and of its last q key j behind those where bit j % 64 of word j / 64 of the
+ * token's row of tree_mask is set.  Key n lies in block
+ * block_table[r][n / block_size]. */
+int lmc_tree_attention(const lmc_tensor *query, const lmc_tensor *vllm_kv_caches, int32_t n_caches,
+                       const lmc_tensor *block_table, const lmc_tensor *seq_lens, const lmc_tensor *query_start_loc,
+                       const lmc_tensor *tree_mask, double scale, const lmc_tensor *output, const lmc_tensor *lse,
+                       const lmc_tensor *workspace, int64_t *workspace_bytes, int32_t kvcache_format,
+                       int32_t vllm_two_major, void *stream);
+
+/* Pages copied in every layer and plane.  layer_ptrs: device table [layers,
+ * n_caches] int64 of the addresses of each layer's caches; vllm_kv_caches are one
+ * layer's, whose shape, strides, dtype and alignment to 16 bytes all have
+ * (MERGED_KV and SEPARATE_KV with any strides; the caches of other formats
+ * [pages, block, (heads,) dim]).  pages: [n, 2] int64 or int32, (source,
+ * target); a pair with a page outside the caches is skipped.  No target may be
+ * another pair's source or target. */
+int lmc_copy_kv_pages(const lmc_tensor *layer_ptrs, const lmc_tensor *vllm_kv_caches, int32_t n_caches,
+                      const lmc_tensor *pages, int32_t kvcache_format, int32_t vllm_two_major, void *stream);
+
+/* Rows moved together, in place, in every layer and plane (layer_ptrs and
+ * vllm_kv_caches as for lmc_copy_kv_pages): of request r the row at position
+ * base_lens[r] + keep[r][i] to base_lens[r] + i for i < keep_lens[r] (at most M).
+ * base_lens and keep_lens are [R] int32, keep [R, M] int32, each list strictly
+ * increasing from 0 or more (another's rows end up in an order that is not
+ * said), block_table [R, W] int32.  A row that has no page, here or there, is
+ * not moved.  The rows that move, of all requests, lie in different places of
+ * the caches.  seq_lens ([R] int32, may be null) gets base_lens + keep_lens. */
+int lmc_compact_kv(const lmc_tensor *layer_ptrs, const lmc_tensor *vllm_kv_caches, int32_t n_caches,
+                   const lmc_tensor *block_table, const lmc_tensor *base_lens, const lmc_tensor *keep,
+                   const lmc_tensor *keep_lens, const lmc_tensor *seq_lens, int32_t kvcache_format,
+                   int32_t vllm_two_major, void *stream);
+
+/* Pages given back to the free list that lmc_build_slot_mapping takes from:
+ * entries ceil(keep_lens[r] / block_size) .. ceil(held_lens[r] / block_size)
+ * ([R] int32, negative lengths count as 0) of row r of block_table ([R, W]
+ * int32; entries outside [0, P) are skipped) lose a holder.  page_refs ([P]
+ * int32) counts the holders of each page beyond the first; a page whose count
+ * falls below 0 (one that was negative before too) is given back and its count
+ * set to 0.  With n of them, *next_cursor = *free_cursor - n ([1] int64 each,
+ * distinct), and free_blocks[*next_cursor + i] ([F] int32) gets the i-th in
+ * ascending order, where the list has that entry.  The call works in
+ * `workspace`, a 1-D uint8 tensor of the GPU on a 4-byte boundary; with
+ * workspace_bytes not null it only writes the size needed there.  Outputs
+ * overlap neither each other nor what the call reads. */
+int lmc_release_pages(const lmc_tensor *block_table, const lmc_tensor *held_lens, const lmc_tensor *keep_lens,
+                      int64_t block_size, const lmc_tensor *page_refs, const lmc_tensor *free_blocks,
+                      const lmc_tensor *free_cursor, const lmc_tensor *next_cursor, const lmc_tensor *workspace,
+                      int64_t *workspace_bytes, void *stream);
+
 /* Replaces get_gpu_pci_bus_id (pybind csrc/pybind.cpp:482): the PCI bus id
  * string of `device`, written NUL-terminated into buf[0..buf_len). */
 int lmc_get_gpu_pci_bus_id(int32_t device, char *buf, int32_t buf_len);

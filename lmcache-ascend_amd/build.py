@@ -22,7 +22,7 @@ BUILD = os.path.join(HERE, "_build")
 OUT = os.path.join(HERE, "lmcache_amd", "liblmcache_amd.so")
 SOURCES = ["kv_transfer.hip", "kv_noalloc.hip", "kv_direct.hip", "kv_sparse_graph.hip", "indexer_c8.hip", "cachegen.hip", "rope.hip",
            "host_mem.cpp", "host_shm.cpp", "dma_copy.hip", "blend.hip", "slot_map.hip", "rotary.hip",
-           "prefix_attention.hip"]
+           "prefix_attention.hip", "tree_attention.hip", "draft_tree.hip", "kv_pages.hip"]
 ARCH = "gfx950"
 
 # Packed-FP32 instructions are kept out of every code object.

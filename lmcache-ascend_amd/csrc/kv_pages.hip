@@ -1,0 +1,570 @@
+// Pages of the paged caches copied, rows moved together, and pages given back,
+// on MI355X (gfx950).
+//
+//   copy_kv_pages:  cache[l, p, dst] = cache[l, p, src]     for pairs (src, dst) of pages
+//   compact_kv:     row(base_r + i) = row(base_r + keep[r, i])   for i < keep_lens[r]
+//   release_pages:  pages ceil(keep / BS) <= j < ceil(held / BS) of each request lose a holder
+//
+// The first two in every layer l and plane p (K, V; the planes of an MLA
+// layer), through a table of the layers' addresses.
+#include "serving.h"
+
+#include <type_traits>
+
+namespace lmc {
+
+namespace {
+
+// A plane's bytes: row (page, token) has `heads` runs of `run` bytes.
+struct PagePlane {
+  int64_t offset;                 // from the layer's address
+  int64_t page, token, head;
+  int64_t heads, run;
+  int tensor;                     // which of the layer's addresses
+};
+
+struct PageGeom {
+  PagePlane plane[kMaxPlanes];
+  int n_planes, n_tensors, device;
+  int64_t pages, block_size;
+  uint64_t align;                 // all addresses and steps, as bits
+};
+
+PageGeom page_geom(const lmc_tensor *caches, int n, int fmt, bool two_major, const char *op) {
+  PageGeom g;
+  std::memset(&g, 0, sizeof(g));
+  if (fmt == LMC_FMT_MERGED_KV || fmt == LMC_FMT_SEPARATE_KV) {
+    const PagedKv kv = paged_kv(caches, n, fmt, two_major, op);
+    const int64_t run = kv.dim * dtype_size(kv.dtype);
+    const bool merged = fmt == LMC_FMT_MERGED_KV;
+    g.plane[0] = {0, kv.k_page, kv.k_token, kv.k_head, kv.heads, run, 0};
+    g.plane[1] = {merged ? kv.v - kv.k : 0, kv.v_page, kv.v_token, kv.v_head, kv.heads, run, merged ? 0 : 1};
+    g.n_planes = 2;
+    g.device = kv.device;
+    g.pages = kv.pages;
+    g.block_size = kv.block_size;
+  } else {
+    validate_vllm_caches(caches, n, fmt);
+    expect(n <= kMaxPlanes, "a layer has at most ", kMaxPlanes, " caches");
+    for (int i = 0; i < n; ++i) {
+      const lmc_tensor &t = deref(&caches[i], "vllm_kv_caches");
+      expect(t.ndim == 3 || t.ndim == 4, op, ": caches of this format are [pages, block, (heads,) dim]");
+      expect(t.device >= 0, op, ": the paged caches are not on a GPU");
+      expect(t.device == caches[0].device && t.sizes[0] == caches[0].sizes[0] && t.sizes[1] == caches[0].sizes[1],
+             "a layer's caches differ in pages, block or device");
+      for (int d = 0; d < t.ndim; ++d) expect(t.strides[d] >= 0, "negative strides unsupported");
+      const int64_t es = elem_size(t);
+      expect(t.sizes[t.ndim - 1] <= 1 || t.strides[t.ndim - 1] == 1, "a cache row's head dims must be adjacent");
+      expect(numel(t) > 0 || t.sizes[0] == 0, "the paged caches hold no rows");
+      g.plane[i] = {0, t.strides[0] * es, t.strides[1] * es, t.ndim == 4 ? t.strides[2] * es : 0,
+                    t.ndim == 4 ? t.sizes[2] : 1, t.sizes[t.ndim - 1] * es, i};
+    }
+    g.n_planes = n;
+    g.device = caches[0].device;
+    g.pages = caches[0].sizes[0];
+    g.block_size = caches[0].sizes[1];
+    expect(g.pages <= INT32_MAX && g.block_size <= INT32_MAX && g.pages * g.block_size <= static_cast<int64_t>(UINT32_MAX),
+           "paged caches of more than 2^32 slots are not supported");
+  }
+  g.n_tensors = n;
+  for (int i = 0; i < n; ++i) g.align |= reinterpret_cast<uintptr_t>(caches[i].data);
+  for (int i = 0; i < g.n_planes; ++i) {
+    PagePlane &p = g.plane[i];
+    // (the stride of a dim of one entry says nothing)
+    if (p.heads <= 1 || p.head == p.run) {
+      p.run *= p.heads;
+      p.heads = 1;
+      p.head = 0;
+    }
+    if (g.block_size <= 1) p.token = 0;
+    if (g.pages <= 1) p.page = 0;
+    g.align |= p.offset | p.page | p.token | p.head | p.run;
+    // Rows must be apart: what one row's copy writes is no other's.
+    expect(rows_apart({g.pages, g.block_size, p.heads, p.run}, {p.page, p.token, p.head, 1}), "the paged caches have overlapping rows");
+  }
+  return g;
+}
+
+// [layers, caches of a layer] addresses.
+int layers_of(const lmc_tensor &ptrs, const PageGeom &g) {
+  check_on(ptrs, "layer_ptrs", g.device, LMC_I64);
+  expect(ptrs.ndim == 2 && ptrs.sizes[1] == g.n_tensors, "layer_ptrs must be [layers, caches of a layer]");
+  expect((ptrs.sizes[1] <= 1 || ptrs.strides[1] == 1) && (ptrs.sizes[0] <= 1 || ptrs.strides[0] == ptrs.sizes[1]),
+         "layer_ptrs must be contiguous");
+  expect(ptrs.sizes[0] <= 65535, "more than 65535 layers");
+  return static_cast<int>(ptrs.sizes[0]);
+}
+
+// ---------------------------------------------------------------------------
+// Pages copied
+// ---------------------------------------------------------------------------
+
+// A page of a plane as n1 x n0 runs of bytes.
+struct CopyPlane {
+  int64_t offset, page, s1, s0;
+  uint32_t n0, pieces;            // runs in the inner dim; vectors of a run
+  uint32_t vectors;               // of the page
+  int tensor;
+};
+
+struct CopyArgs {
+  CopyPlane plane[kMaxPlanes];
+  const int64_t *ptrs;
+  int n_tensors, n_planes, n_layers;
+  const void *pairs;
+  int wide;                       // pairs are int64
+  int64_t pair_stride;
+  int64_t n_pages;
+  uint32_t groups;                // workgroups of a page
+};
+
+constexpr int kUnroll = 4;
+
+template <int VEC> __global__ void __launch_bounds__(256) copy_pages(CopyArgs a) {
+  using V = typename VecOf<VEC>::T;
+  const uint32_t piece = blockIdx.x % a.groups;
+  const uint32_t pair = blockIdx.x / a.groups;
+  const int p = blockIdx.y % a.n_planes, l = blockIdx.y / a.n_planes;
+  int64_t src, dst;
+  if (a.wide) {
+    const int64_t *x = static_cast<const int64_t *>(a.pairs) + pair * a.pair_stride;
+    src = x[0];
+    dst = x[1];
+  } else {
+    const int32_t *x = static_cast<const int32_t *>(a.pairs) + pair * a.pair_stride;
+    src = x[0];
+    dst = x[1];
+  }
+  const CopyPlane &c = a.plane[p];
+  uint8_t *base = reinterpret_cast<uint8_t *>(a.ptrs[l * a.n_tensors + c.tensor]) + c.offset;
+  if (src < 0 || src >= a.n_pages || dst < 0 || dst >= a.n_pages || src == dst) return;
+  const uint8_t *from = base + src * c.page;
+  uint8_t *to = base + dst * c.page;
+  V v[kUnroll];
+  int64_t at[kUnroll];
+#pragma unroll
+  for (int u = 0; u < kUnroll; ++u) {
+    const uint32_t x = (piece * kUnroll + u) * 256 + threadIdx.x;
+    at[u] = -1;
+    if (x >= c.vectors) continue;
+    const uint32_t run = x / c.pieces, i1 = run / c.n0;
+    at[u] = i1 * c.s1 + (run - i1 * c.n0) * c.s0 + (x - run * c.pieces) * static_cast<int64_t>(VEC);
+    v[u] = gload_nt(reinterpret_cast<const V *>(from + at[u]));
+  }
+#pragma unroll
+  for (int u = 0; u < kUnroll; ++u)
+    if (at[u] >= 0) gstore_nt(reinterpret_cast<V *>(to + at[u]), v[u]);
+}
+
+// ---------------------------------------------------------------------------
+// Rows moved together
+// ---------------------------------------------------------------------------
+
+struct MovePlane {
+  int64_t offset, page, token, head;
+  uint32_t pieces;                // vectors of a run
+  uint32_t vectors;               // of a row
+  int tensor;
+};
+
+struct MoveArgs {
+  MovePlane plane[kMaxPlanes];
+  const int64_t *ptrs;
+  int n_tensors, n_planes, n_layers;
+  const int32_t *table;
+  int64_t table_stride;
+  uint32_t width, block_size;
+  int64_t n_pages;
+  const int32_t *base_lens, *keep, *keep_lens;
+  int64_t keep_stride;
+  int most;                       // entries of a list
+  int32_t *seq_lens;              // may be null
+  int lanes;                      // threads of a row: a power of two, at most 256
+};
+
+// A workgroup moves a slice of one request's rows in one plane of one layer,
+// some rows at a time, in order: rows move down (keep[i] >= i), so what a step
+// writes has been read by it or by an earlier one.  The next step's rows are
+// loaded before this one's are written: they lie behind all that it writes.
+template <int VEC> __global__ void __launch_bounds__(256) move_rows(MoveArgs a) {
+  using V = typename VecOf<VEC>::T;
+  using Held = std::conditional_t<(VEC < 4), uint32_t, V>;  // in a register
+  const int p = blockIdx.y % a.n_planes, l = blockIdx.y / a.n_planes, r = blockIdx.z;
+  const MovePlane &c = a.plane[p];
+  const int64_t b = a.base_lens[r];
+  const int n = min(max(a.keep_lens[r], 0), a.most);
+  if (a.seq_lens && blockIdx.x == 0 && blockIdx.y == 0 && threadIdx.x == 0) a.seq_lens[r] = static_cast<int32_t>(min(b + n, static_cast<int64_t>(INT32_MAX)));
+  uint8_t *base = reinterpret_cast<uint8_t *>(a.ptrs[l * a.n_tensors + c.tensor]) + c.offset;
+  const int rows = 256 / a.lanes, own = threadIdx.x / a.lanes;
+  const uint32_t x = blockIdx.x * a.lanes + (threadIdx.x & (a.lanes - 1));
+  const bool in = x < c.vectors;
+  const int64_t column = (x / c.pieces) * c.head + (x % c.pieces) * static_cast<int64_t>(VEC);
+  const int32_t *keep = a.keep + r * a.keep_stride, *table = a.table + r * a.table_stride;
+  // The row of a position, or null where the caches have none.
+  auto row_of = [&](int64_t pos) -> uint8_t * {
+    if (pos < 0 || pos >= static_cast<int64_t>(a.width) * a.block_size) return nullptr;
+    const uint32_t j = static_cast<uint32_t>(pos) / a.block_size;
+    const int64_t page = table[j];
+    if (page < 0 || page >= a.n_pages) return nullptr;
+    return base + page * c.page + (static_cast<uint32_t>(pos) - j * a.block_size) * c.token + column;
+  };
+  const int step = rows * kUnroll;
+  Held now[kUnroll], next[kUnroll];
+  uint8_t *to[kUnroll], *to_next[kUnroll];
+  auto load = [&](int i0, Held (&v)[kUnroll], uint8_t *(&t)[kUnroll]) {
+#pragma unroll
+    for (int u = 0; u < kUnroll; ++u) {
+      const int i = i0 + u * rows + own;
+      t[u] = nullptr;
+      v[u] = Held{};
+      if (!in || i >= n) continue;
+      const int k = keep[i];
+      if (k == i) continue;
+      const uint8_t *from = row_of(b + k);
+      t[u] = row_of(b + i);
+      if (!from) t[u] = nullptr;
+      if (t[u]) v[u] = gload(reinterpret_cast<const V *>(from));
+    }
+  };
+  load(0, now, to);
+  for (int i0 = 0; i0 < n; i0 += step) {
+    load(i0 + step, next, to_next);
+    // This step's rows have arrived, in every wave.
+#pragma unroll
+    for (int u = 0; u < kUnroll; ++u) asm volatile("" : "+v"(now[u])::"memory");
+    __syncthreads();
+#pragma unroll
+    for (int u = 0; u < kUnroll; ++u)
+      if (to[u]) gstore(reinterpret_cast<V *>(to[u]), static_cast<V>(now[u]));
+#pragma unroll
+    for (int u = 0; u < kUnroll; ++u) {
+      now[u] = next[u];
+      to[u] = to_next[u];
+    }
+  }
+}
+
+// ---------------------------------------------------------------------------
+// Pages given back
+// ---------------------------------------------------------------------------
+
+struct ReleaseArgs {
+  const int32_t *table;
+  int64_t table_stride;
+  uint32_t width, block_size;
+  const int32_t *held, *keep;
+  int32_t *refs;
+  int n_pages;
+  int32_t *free_blocks;
+  int64_t n_free;
+  const int64_t *cursor;
+  int64_t *next_cursor;
+  int32_t *counts;                // pages given back of each run of kRun
+  int runs;
+};
+
+constexpr int kRun = 4096;
+
+// A holder less for each page that a request gives back.
+__global__ void __launch_bounds__(256) drop_holders(ReleaseArgs a) {
+  const int r = blockIdx.x;
+  auto pages_for = [&](int tokens) {
+    const uint32_t n = static_cast<uint32_t>(max(0, tokens));
+    return min(n / a.block_size + (n % a.block_size != 0), a.width);
+  };
+  const uint32_t first = pages_for(a.keep[r]), stop = pages_for(a.held[r]);
+  for (uint32_t j = first + threadIdx.x; j < stop; j += 256) {
+    const int page = a.table[r * a.table_stride + j];
+    if (page >= 0 && page < a.n_pages) atomicSub(a.refs + page, 1);
+  }
+}
+
+// Pages that have no holder left, of a thread's 16 of a run.
+__device__ __forceinline__ uint32_t without_holder(const ReleaseArgs &a, int run) {
+  uint32_t bits = 0;
+  const int p0 = run * kRun + threadIdx.x * 16;
+#pragma unroll
+  for (int i = 0; i < 16; ++i)
+    if (p0 + i < a.n_pages && a.refs[p0 + i] < 0) bits |= 1u << i;
+  return bits;
+}
+
+__global__ void __launch_bounds__(256) count_free(ReleaseArgs a) {
+  __shared__ int part[4];
+  int n = __popc(without_holder(a, blockIdx.x));
+#pragma unroll
+  for (int d = 32; d > 0; d >>= 1) n += __shfl_xor(n, d);
+  if ((threadIdx.x & 63) == 0) part[threadIdx.x >> 6] = n;
+  __syncthreads();
+  if (threadIdx.x == 0) a.counts[blockIdx.x] = part[0] + part[1] + part[2] + part[3];
+}
+
+__global__ void __launch_bounds__(256) place_free(ReleaseArgs a) {
+  __shared__ int part[3][4];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  int before = 0, total = 0;
+  for (int i = threadIdx.x; i < a.runs; i += 256) {
+    const int n = a.counts[i];
+    total += n;
+    if (i < static_cast<int>(blockIdx.x)) before += n;
+  }
+#pragma unroll
+  for (int d = 32; d > 0; d >>= 1) {
+    before += __shfl_xor(before, d);
+    total += __shfl_xor(total, d);
+  }
+  const uint32_t bits = without_holder(a, blockIdx.x);
+  const int own = __popc(bits);
+  int upto = own;
+#pragma unroll
+  for (int d = 1; d < 64; d <<= 1) {
+    const int below = __shfl_up(upto, d);
+    if (lane >= d) upto += below;
+  }
+  if (lane == 63) {
+    part[0][wave] = upto;
+    part[1][wave] = before;
+    part[2][wave] = total;
+  }
+  __syncthreads();
+  before = total = 0;
+#pragma unroll
+  for (int w = 0; w < 4; ++w) {
+    before += part[1][w] + (w < wave ? part[0][w] : 0);
+    total += part[2][w];
+  }
+  const int64_t cursor = *a.cursor;
+  int64_t at = cursor - total + before + upto - own;
+  if (blockIdx.x == 0 && threadIdx.x == 0) *a.next_cursor = cursor - total;
+  const int p0 = blockIdx.x * kRun + threadIdx.x * 16;
+#pragma unroll
+  for (int i = 0; i < 16; ++i) {
+    if (!(bits >> i & 1)) continue;
+    a.refs[p0 + i] = 0;
+    if (at >= 0 && at < a.n_free) a.free_blocks[at] = p0 + i;
+    ++at;
+  }
+}
+
+} // namespace
+
+} // namespace lmc
+
+using namespace lmc;
+
+extern "C" int lmc_copy_kv_pages(const lmc_tensor *layer_ptrs, const lmc_tensor *vllm_kv_caches, int32_t n_caches,
+                                 const lmc_tensor *pages, int32_t kvcache_format, int32_t vllm_two_major, void *stream) {
+  return guarded([&] {
+    const PageGeom g = page_geom(vllm_kv_caches, n_caches, kvcache_format, vllm_two_major != 0, "copy_kv_pages");
+    const lmc_tensor &lp = deref(layer_ptrs, "layer_ptrs");
+    const lmc_tensor &pr = deref(pages, "pages");
+    const int layers = layers_of(lp, g);
+    check_on(pr, "pages", g.device, LMC_I32, LMC_I64);
+    expect(pr.ndim == 2 && pr.sizes[1] == 2, "pages must be [pairs, 2]");
+    expect(pr.strides[1] == 1, "a pair's two pages must be adjacent");
+    expect(pr.strides[0] >= 0, "negative strides unsupported");
+    expect(pr.sizes[0] <= INT32_MAX, "too many pairs");
+    for (int i = 0; i < n_caches; ++i)
+      expect(!extents_meet(pr, vllm_kv_caches[i]) && !extents_meet(lp, vllm_kv_caches[i]), "pages or layer_ptrs overlap the paged caches");
+    if (pr.sizes[0] == 0 || layers == 0 || g.pages == 0) return;
+    CopyArgs a;
+    std::memset(&a, 0, sizeof(a));
+    const int vec = vec_for(static_cast<int64_t>(g.align));
+    int64_t most = 0;
+    for (int i = 0; i < g.n_planes; ++i) {
+      const PagePlane &p = g.plane[i];
+      int64_t run = p.run, n[2] = {p.heads, g.block_size}, s[2] = {p.head, p.token};
+      if (s[0] > s[1] && n[1] > 1) {
+        std::swap(n[0], n[1]);
+        std::swap(s[0], s[1]);
+      }
+      for (int d = 0; d < 2; ++d)
+        if (n[0] == 1 || s[0] == run) {
+          run *= n[0];
+          n[0] = n[1];
+          s[0] = s[1];
+          n[1] = 1;
+        }
+      a.plane[i] = {p.offset, p.page, s[1], s[0], static_cast<uint32_t>(n[0]), static_cast<uint32_t>(run / vec),
+                    static_cast<uint32_t>(run / vec * n[0] * n[1]), p.tensor};
+      expect(run / vec * n[0] * n[1] < (int64_t(1) << 31), "pages of 2^31 elements or more");
+      most = std::max(most, run / vec * n[0] * n[1]);
+    }
+    a.ptrs = static_cast<const int64_t *>(lp.data);
+    a.n_tensors = g.n_tensors;
+    a.n_planes = g.n_planes;
+    a.n_layers = layers;
+    a.pairs = pr.data;
+    a.wide = pr.dtype == LMC_I64;
+    a.pair_stride = pr.strides[0];
+    a.n_pages = g.pages;
+    a.groups = static_cast<uint32_t>((most + 256 * kUnroll - 1) / (256 * kUnroll));
+    expect(a.groups * pr.sizes[0] <= UINT32_MAX / 256 && layers * g.n_planes <= 65535, "too many pages");
+    DeviceGuard guard(g.device);
+    const dim3 grid(static_cast<uint32_t>(a.groups * pr.sizes[0]), static_cast<uint32_t>(layers * g.n_planes));
+    const hipStream_t s = static_cast<hipStream_t>(stream);
+    switch (vec) {
+    case 16: hipLaunchKernelGGL(copy_pages<16>, grid, dim3(256), 0, s, a); break;
+    case 8: hipLaunchKernelGGL(copy_pages<8>, grid, dim3(256), 0, s, a); break;
+    case 4: hipLaunchKernelGGL(copy_pages<4>, grid, dim3(256), 0, s, a); break;
+    case 2: hipLaunchKernelGGL(copy_pages<2>, grid, dim3(256), 0, s, a); break;
+    default: hipLaunchKernelGGL(copy_pages<1>, grid, dim3(256), 0, s, a); break;
+    }
+    hip_check(hipGetLastError(), "copy_pages launch");
+  });
+}
+
+extern "C" int lmc_compact_kv(const lmc_tensor *layer_ptrs, const lmc_tensor *vllm_kv_caches, int32_t n_caches,
+                              const lmc_tensor *block_table, const lmc_tensor *base_lens, const lmc_tensor *keep,
+                              const lmc_tensor *keep_lens, const lmc_tensor *seq_lens, int32_t kvcache_format,
+                              int32_t vllm_two_major, void *stream) {
+  return guarded([&] {
+    const PageGeom g = page_geom(vllm_kv_caches, n_caches, kvcache_format, vllm_two_major != 0, "compact_kv");
+    const lmc_tensor &lp = deref(layer_ptrs, "layer_ptrs");
+    const lmc_tensor &bt = deref(block_table, "block_table");
+    const lmc_tensor &bl = deref(base_lens, "base_lens");
+    const lmc_tensor &kp = deref(keep, "keep");
+    const lmc_tensor &kl = deref(keep_lens, "keep_lens");
+    const int layers = layers_of(lp, g), dev = g.device;
+    check_on(bt, "block_table", dev, LMC_I32);
+    check_vector(bl, "base_lens", dev, LMC_I32);
+    check_on(kp, "keep", dev, LMC_I32);
+    check_vector(kl, "keep_lens", dev, LMC_I32);
+    const int64_t R = bl.sizes[0];
+    expect(bt.ndim == 2 && bt.sizes[0] == R, "block_table must be [requests, pages]");
+    expect(bt.sizes[1] <= 1 || bt.strides[1] == 1, "block_table rows must be contiguous");
+    expect(kp.ndim == 2 && kp.sizes[0] == R, "keep must be [requests, rows]");
+    expect(kp.sizes[1] <= 1 || kp.strides[1] == 1, "keep's lists must be contiguous");
+    expect(kl.sizes[0] == R, "keep_lens must have one entry per request");
+    expect(bt.strides[0] >= 0 && kp.strides[0] >= 0, "negative strides unsupported");
+    expect(bt.sizes[1] == 0 || g.block_size <= INT32_MAX / bt.sizes[1], "a block_table row spans 2^31 positions or more");
+    expect(kp.sizes[1] <= INT32_MAX / 2 && R <= 65535, "more than 65535 requests, or lists of more than 2^30 rows");
+    if (seq_lens) {
+      const lmc_tensor &sl = deref(seq_lens, "seq_lens");
+      check_vector(sl, "seq_lens", dev, LMC_I32);
+      expect(sl.sizes[0] == R, "seq_lens must have one entry per request");
+      for (const lmc_tensor *in : {block_table, base_lens, keep, keep_lens, layer_ptrs})
+        expect(!extents_meet(sl, *in), "seq_lens overlaps what it is computed from");
+    }
+    for (const lmc_tensor *x : {block_table, base_lens, keep, keep_lens, seq_lens, layer_ptrs})
+      for (int i = 0; x && i < n_caches; ++i)
+        expect(!extents_meet(*x, vllm_kv_caches[i]), "the tables or lists overlap the paged caches");
+    if (R == 0 || layers == 0) return;
+    MoveArgs a;
+    std::memset(&a, 0, sizeof(a));
+    const int vec = vec_for(static_cast<int64_t>(g.align));
+    int64_t most = 0;
+    for (int i = 0; i < g.n_planes; ++i) {
+      const PagePlane &p = g.plane[i];
+      const int64_t vectors = p.run / vec * p.heads;
+      expect(vectors < (int64_t(1) << 30), "rows of 2^30 elements or more");
+      a.plane[i] = {p.offset, p.page, p.token, p.head, static_cast<uint32_t>(p.run / vec), static_cast<uint32_t>(vectors), p.tensor};
+      most = std::max(most, vectors);
+    }
+    a.ptrs = static_cast<const int64_t *>(lp.data);
+    a.n_tensors = g.n_tensors;
+    a.n_planes = g.n_planes;
+    a.n_layers = layers;
+    a.table = static_cast<const int32_t *>(bt.data);
+    a.table_stride = bt.strides[0];
+    a.width = static_cast<uint32_t>(bt.sizes[1]);
+    a.block_size = static_cast<uint32_t>(g.block_size);
+    a.n_pages = g.pages;
+    a.base_lens = static_cast<const int32_t *>(bl.data);
+    a.keep = static_cast<const int32_t *>(kp.data);
+    a.keep_lens = static_cast<const int32_t *>(kl.data);
+    a.keep_stride = kp.strides[0];
+    a.most = static_cast<int>(kp.sizes[1]);
+    a.seq_lens = seq_lens ? static_cast<int32_t *>(seq_lens->data) : nullptr;
+    a.lanes = 16;
+    while (a.lanes < 256 && a.lanes < most && R * layers * g.n_planes * ((most + 2 * a.lanes - 1) / (2 * a.lanes)) >= 1024) a.lanes *= 2;
+    const int64_t slices = (most + a.lanes - 1) / a.lanes;
+    expect(layers * g.n_planes <= 65535 && slices <= UINT32_MAX / 256, "too many layers");
+    DeviceGuard guard(dev);
+    const dim3 grid(static_cast<uint32_t>(slices), static_cast<uint32_t>(layers * g.n_planes), static_cast<uint32_t>(R));
+    const hipStream_t s = static_cast<hipStream_t>(stream);
+    switch (vec) {
+    case 16: hipLaunchKernelGGL(move_rows<16>, grid, dim3(256), 0, s, a); break;
+    case 8: hipLaunchKernelGGL(move_rows<8>, grid, dim3(256), 0, s, a); break;
+    case 4: hipLaunchKernelGGL(move_rows<4>, grid, dim3(256), 0, s, a); break;
+    case 2: hipLaunchKernelGGL(move_rows<2>, grid, dim3(256), 0, s, a); break;
+    default: hipLaunchKernelGGL(move_rows<1>, grid, dim3(256), 0, s, a); break;
+    }
+    hip_check(hipGetLastError(), "move_rows launch");
+  });
+}
+
+extern "C" int lmc_release_pages(const lmc_tensor *block_table, const lmc_tensor *held_lens, const lmc_tensor *keep_lens,
+                                 int64_t block_size, const lmc_tensor *page_refs, const lmc_tensor *free_blocks,
+                                 const lmc_tensor *free_cursor, const lmc_tensor *next_cursor,
+                                 const lmc_tensor *workspace, int64_t *workspace_bytes, void *stream) {
+  return guarded([&] {
+    const lmc_tensor &bt = deref(block_table, "block_table");
+    const lmc_tensor &hl = deref(held_lens, "held_lens");
+    const lmc_tensor &kl = deref(keep_lens, "keep_lens");
+    const lmc_tensor &pr = deref(page_refs, "page_refs");
+    const lmc_tensor &fb = deref(free_blocks, "free_blocks");
+    const lmc_tensor &fc = deref(free_cursor, "free_cursor");
+    const lmc_tensor &nc = deref(next_cursor, "next_cursor");
+    const int dev = pr.device;
+    expect(dev >= 0, "page_refs is not on a GPU");
+    check_vector(pr, "page_refs", dev, LMC_I32);
+    check_on(bt, "block_table", dev, LMC_I32);
+    check_vector(hl, "held_lens", dev, LMC_I32);
+    check_vector(kl, "keep_lens", dev, LMC_I32);
+    check_vector(fb, "free_blocks", dev, LMC_I32);
+    check_vector(fc, "free_cursor", dev, LMC_I64);
+    check_vector(nc, "next_cursor", dev, LMC_I64);
+    const int64_t R = hl.sizes[0], P = pr.sizes[0];
+    expect(kl.sizes[0] == R, "held_lens and keep_lens differ in length");
+    expect(bt.ndim == 2 && bt.sizes[0] == R, "block_table must be [requests, pages]");
+    expect(bt.sizes[1] <= 1 || bt.strides[1] == 1, "block_table rows must be contiguous");
+    expect(bt.strides[0] >= 0, "negative strides unsupported");
+    expect(bt.sizes[1] <= INT32_MAX / 2 && R <= INT32_MAX / 256, "block_table is too large");
+    expect(block_size > 0 && block_size < (int64_t(1) << 31), "block_size must be positive");
+    expect(P <= INT32_MAX - 2 * kRun, "page_refs has too many entries");
+    expect(fc.sizes[0] == 1, "free_cursor must have one entry");
+    expect(nc.sizes[0] == 1, "next_cursor must have one entry");
+    const int64_t runs = (P + kRun - 1) / kRun, bytes = std::max<int64_t>(1, runs) * 4;
+    if (workspace_bytes) {
+      *workspace_bytes = bytes;
+      return;
+    }
+    const lmc_tensor &ws = deref(workspace, "workspace");
+    check_on(ws, "workspace", dev, LMC_U8);
+    expect(ws.ndim == 1 && (ws.sizes[0] <= 1 || ws.strides[0] == 1) && ws.sizes[0] >= bytes &&
+               reinterpret_cast<uintptr_t>(ws.data) % 4 == 0,
+           "workspace must be 1-D, contiguous, on a 4-byte boundary and of at least ", bytes, " bytes");
+    const lmc_tensor *outs[] = {page_refs, free_blocks, next_cursor, workspace};
+    for (const lmc_tensor *out : outs) {
+      for (const lmc_tensor *in : {block_table, held_lens, keep_lens, free_cursor})
+        expect(!extents_meet(*out, *in), "an output overlaps what it is computed from");
+      for (const lmc_tensor *other : outs) expect(other == out || !extents_meet(*out, *other), "two outputs overlap");
+    }
+    ReleaseArgs a;
+    std::memset(&a, 0, sizeof(a));
+    a.table = static_cast<const int32_t *>(bt.data);
+    a.table_stride = bt.strides[0];
+    a.width = static_cast<uint32_t>(bt.sizes[1]);
+    a.block_size = static_cast<uint32_t>(block_size);
+    a.held = static_cast<const int32_t *>(hl.data);
+    a.keep = static_cast<const int32_t *>(kl.data);
+    a.refs = static_cast<int32_t *>(pr.data);
+    a.n_pages = static_cast<int>(P);
+    a.free_blocks = static_cast<int32_t *>(fb.data);
+    a.n_free = fb.sizes[0];
+    a.cursor = static_cast<const int64_t *>(fc.data);
+    a.next_cursor = static_cast<int64_t *>(nc.data);
+    a.counts = static_cast<int32_t *>(ws.data);
+    a.runs = static_cast<int>(runs);
+    DeviceGuard guard(dev);
+    const hipStream_t s = static_cast<hipStream_t>(stream);
+    if (R > 0) hipLaunchKernelGGL(drop_holders, dim3(static_cast<uint32_t>(R)), dim3(256), 0, s, a);
+    hip_check(hipGetLastError(), "drop_holders launch");
+    const uint32_t groups = static_cast<uint32_t>(std::max<int64_t>(1, runs));
+    hipLaunchKernelGGL(count_free, dim3(groups), dim3(256), 0, s, a);
+    hip_check(hipGetLastError(), "count_free launch");
+    hipLaunchKernelGGL(place_free, dim3(groups), dim3(256), 0, s, a);
+    hip_check(hipGetLastError(), "place_free launch");
+  });
+}

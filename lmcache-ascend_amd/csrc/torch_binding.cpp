@@ -52,6 +52,16 @@ using RotaryPagedFn = int (*)(const lmc_tensor *, const lmc_tensor *, const lmc_
 using PrefixAttnFn = int (*)(const lmc_tensor *, const lmc_tensor *, int32_t, const lmc_tensor *, int64_t,
                              const lmc_tensor *, const lmc_tensor *, const lmc_tensor *, double, const lmc_tensor *,
                              const lmc_tensor *, const lmc_tensor *, int64_t *, int32_t, int32_t, void *);
+using DraftTreeFn = int (*)(const lmc_tensor *, const lmc_tensor *, const lmc_tensor *, const lmc_tensor *,
+                            const lmc_tensor *, void *);
+using TreeAttnFn = int (*)(const lmc_tensor *, const lmc_tensor *, int32_t, const lmc_tensor *, const lmc_tensor *,
+                           const lmc_tensor *, const lmc_tensor *, double, const lmc_tensor *, const lmc_tensor *,
+                           const lmc_tensor *, int64_t *, int32_t, int32_t, void *);
+using CopyPagesFn = int (*)(const lmc_tensor *, const lmc_tensor *, int32_t, const lmc_tensor *, int32_t, int32_t, void *);
+using CompactFn = int (*)(const lmc_tensor *, const lmc_tensor *, int32_t, const lmc_tensor *, const lmc_tensor *,
+                          const lmc_tensor *, const lmc_tensor *, const lmc_tensor *, int32_t, int32_t, void *);
+using ReleaseFn = int (*)(const lmc_tensor *, const lmc_tensor *, const lmc_tensor *, int64_t, const lmc_tensor *,
+                          const lmc_tensor *, const lmc_tensor *, const lmc_tensor *, const lmc_tensor *, int64_t *, void *);
 using ErrFn = const char *(*)();
 
 struct Table {
@@ -71,6 +81,11 @@ struct Table {
   RotaryFn rotary = nullptr;
   RotaryPagedFn rotary_paged = nullptr;
   PrefixAttnFn prefix_attn = nullptr;
+  DraftTreeFn draft_tree = nullptr;
+  TreeAttnFn tree_attn = nullptr;
+  CopyPagesFn copy_pages = nullptr;
+  CompactFn compact = nullptr;
+  ReleaseFn release = nullptr;
   ErrFn last_error = nullptr;
 } g;
 
@@ -394,10 +409,86 @@ void shared_prefix_attention(const at::Tensor &query, const py::object &caches_o
   call(&w, nullptr);
 }
 
+void build_draft_tree(const at::Tensor &parents, const at::Tensor &query_start_loc, const at::Tensor &seq_lens,
+                      const at::Tensor &tree_mask, const c10::optional<at::Tensor> &positions) {
+  check_bound();
+  const int dev = gpu_of(tree_mask, "tree_mask");
+  const lmc_tensor p = desc(parents), l = desc(query_start_loc), n = desc(seq_lens), m = desc(tree_mask);
+  const Opt x(positions);
+  raise_for(g.draft_tree(&p, &l, &n, &m, x.ptr(), stream_of(dev)));
+}
+
+void tree_attention(const at::Tensor &query, const py::object &caches_obj, const at::Tensor &block_table,
+                    const at::Tensor &seq_lens, const at::Tensor &query_start_loc, const at::Tensor &tree_mask,
+                    double scale, const at::Tensor &output, const c10::optional<at::Tensor> &lse,
+                    int64_t kvcache_format_raw, bool vllm_two_major) {
+  check_bound();
+  const int dev = gpu_of(query, "query");
+  const std::vector<at::Tensor> caches = normalize_kv_caches(caches_obj);
+  std::vector<lmc_tensor> cd;
+  for (const auto &c : caches) cd.push_back(desc(c));
+  const lmc_tensor q = desc(query), t = desc(block_table), n = desc(seq_lens), l = desc(query_start_loc),
+                   m = desc(tree_mask), o = desc(output);
+  const Opt e(lse);
+  auto call = [&](const lmc_tensor *w, int64_t *bytes) {
+    raise_for(g.tree_attn(&q, cd.data(), static_cast<int32_t>(cd.size()), &t, &n, &l, &m, scale, &o, e.ptr(), w, bytes,
+                          static_cast<int32_t>(kvcache_format_raw), vllm_two_major, stream_of(dev)));
+  };
+  int64_t bytes = 0;
+  call(nullptr, &bytes);
+  if (bytes == 0) return;
+  // Scratch of this call: the allocator hands it out again in stream order.
+  const at::Tensor space = at::empty({bytes}, query.options().dtype(at::kByte));
+  const lmc_tensor w = desc(space);
+  call(&w, nullptr);
+}
+
+void copy_kv_pages(const at::Tensor &layer_ptrs, const std::vector<at::Tensor> &caches, const at::Tensor &pages,
+                   int64_t kvcache_format_raw, bool vllm_two_major) {
+  check_bound();
+  const int dev = gpu_of(layer_ptrs, "layer_ptrs");
+  std::vector<lmc_tensor> cd;
+  for (const auto &c : caches) cd.push_back(desc(c));
+  const lmc_tensor l = desc(layer_ptrs), p = desc(pages);
+  raise_for(g.copy_pages(&l, cd.data(), static_cast<int32_t>(cd.size()), &p, static_cast<int32_t>(kvcache_format_raw),
+                         vllm_two_major, stream_of(dev)));
+}
+
+void compact_kv(const at::Tensor &layer_ptrs, const std::vector<at::Tensor> &caches, const at::Tensor &block_table,
+                const at::Tensor &base_lens, const at::Tensor &keep, const at::Tensor &keep_lens,
+                const c10::optional<at::Tensor> &seq_lens, int64_t kvcache_format_raw, bool vllm_two_major) {
+  check_bound();
+  const int dev = gpu_of(layer_ptrs, "layer_ptrs");
+  std::vector<lmc_tensor> cd;
+  for (const auto &c : caches) cd.push_back(desc(c));
+  const lmc_tensor l = desc(layer_ptrs), t = desc(block_table), b = desc(base_lens), k = desc(keep), n = desc(keep_lens);
+  const Opt s(seq_lens);
+  raise_for(g.compact(&l, cd.data(), static_cast<int32_t>(cd.size()), &t, &b, &k, &n, s.ptr(),
+                      static_cast<int32_t>(kvcache_format_raw), vllm_two_major, stream_of(dev)));
+}
+
+void release_pages(const at::Tensor &block_table, const at::Tensor &held_lens, const at::Tensor &keep_lens,
+                   int64_t block_size, const at::Tensor &page_refs, const at::Tensor &free_blocks,
+                   const at::Tensor &free_cursor, const at::Tensor &next_cursor) {
+  check_bound();
+  const int dev = gpu_of(page_refs, "page_refs");
+  const lmc_tensor t = desc(block_table), h = desc(held_lens), k = desc(keep_lens), p = desc(page_refs),
+                   f = desc(free_blocks), c = desc(free_cursor), n = desc(next_cursor);
+  auto call = [&](const lmc_tensor *w, int64_t *bytes) {
+    raise_for(g.release(&t, &h, &k, block_size, &p, &f, &c, &n, w, bytes, stream_of(dev)));
+  };
+  int64_t bytes = 0;
+  call(nullptr, &bytes);
+  const at::Tensor space = at::empty({bytes}, page_refs.options().dtype(at::kByte));
+  const lmc_tensor w = desc(space);
+  call(&w, nullptr);
+}
+
 void bind(uintptr_t multi, uintptr_t single, uintptr_t load_flash, uintptr_t reshape_flash,
           uintptr_t rope, uintptr_t blend, uintptr_t cdf, uintptr_t encode, uintptr_t decode,
           uintptr_t encode_rows, uintptr_t pack_rows, uintptr_t decode_chunk,
           uintptr_t slot_map, uintptr_t rotary, uintptr_t rotary_paged, uintptr_t prefix_attn,
+          uintptr_t draft_tree, uintptr_t tree_attn, uintptr_t copy_pages, uintptr_t compact, uintptr_t release,
           uintptr_t last_error) {
   g.multi = reinterpret_cast<MultiFn>(multi);
   g.single = reinterpret_cast<SingleFn>(single);
@@ -415,6 +506,11 @@ void bind(uintptr_t multi, uintptr_t single, uintptr_t load_flash, uintptr_t res
   g.rotary = reinterpret_cast<RotaryFn>(rotary);
   g.rotary_paged = reinterpret_cast<RotaryPagedFn>(rotary_paged);
   g.prefix_attn = reinterpret_cast<PrefixAttnFn>(prefix_attn);
+  g.draft_tree = reinterpret_cast<DraftTreeFn>(draft_tree);
+  g.tree_attn = reinterpret_cast<TreeAttnFn>(tree_attn);
+  g.copy_pages = reinterpret_cast<CopyPagesFn>(copy_pages);
+  g.compact = reinterpret_cast<CompactFn>(compact);
+  g.release = reinterpret_cast<ReleaseFn>(release);
   g.last_error = reinterpret_cast<ErrFn>(last_error);
 }
 
@@ -442,6 +538,11 @@ PYBIND11_MODULE(_c_ops_ext, m) {
   m.def("rotary_embedding", &rotary_embedding);
   m.def("rotary_embedding_to_paged", &rotary_embedding_to_paged);
   m.def("shared_prefix_attention", &shared_prefix_attention);
+  m.def("build_draft_tree", &build_draft_tree);
+  m.def("tree_attention", &tree_attention);
+  m.def("copy_kv_pages", &copy_kv_pages);
+  m.def("compact_kv", &compact_kv);
+  m.def("release_pages", &release_pages);
   m.def("calculate_cdf", &calculate_cdf);
   m.def("cachegen_encode_chunk", &cachegen_encode_chunk);
   m.def("cachegen_decode_chunk", &cachegen_decode_chunk);

@@ -101,6 +101,13 @@ SIGNATURES = {
     "lmc_shared_prefix_attention": [
         _T, _T, _i32, _T, _i64, _T, _T, _T, ctypes.c_double, _T, _T, _T, ctypes.POINTER(_i64), _i32, _i32, _vp,
     ],
+    "lmc_build_draft_tree": [_T, _T, _T, _T, _T, _vp],
+    "lmc_tree_attention": [
+        _T, _T, _i32, _T, _T, _T, _T, ctypes.c_double, _T, _T, _T, ctypes.POINTER(_i64), _i32, _i32, _vp,
+    ],
+    "lmc_copy_kv_pages": [_T, _T, _i32, _T, _i32, _i32, _vp],
+    "lmc_compact_kv": [_T, _T, _i32, _T, _T, _T, _T, _T, _i32, _i32, _vp],
+    "lmc_release_pages": [_T, _T, _T, _i64, _T, _T, _T, _T, _T, ctypes.POINTER(_i64), _vp],
     "lmc_get_device_ptr": [_up, _sz, ctypes.POINTER(_up)],
     "lmc_register_mapping": [_up, _up, _sz, ctypes.POINTER(_up)],
     "lmc_unregister_ptr": [_up, ctypes.POINTER(_i32)],

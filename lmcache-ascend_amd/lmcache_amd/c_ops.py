@@ -54,6 +54,11 @@ try:
         _addr("lmc_rotary_embedding"),
         _addr("lmc_rotary_embedding_to_paged"),
         _addr("lmc_shared_prefix_attention"),
+        _addr("lmc_build_draft_tree"),
+        _addr("lmc_tree_attention"),
+        _addr("lmc_copy_kv_pages"),
+        _addr("lmc_compact_kv"),
+        _addr("lmc_release_pages"),
         _addr("lmc_last_error"),
     )
 except ImportError:
@@ -784,6 +789,226 @@ def shared_prefix_attention(
     call(None, ctypes.byref(size))
     if size.value:
         call(torch.empty(size.value, dtype=torch.uint8, device=query.device), None)
+
+
+# ---------------------------------------------------------------------------
+# Drafting and branching over the paged caches (no reference counterpart)
+# ---------------------------------------------------------------------------
+
+
+def build_draft_tree(
+    parents: torch.Tensor,
+    query_start_loc: torch.Tensor,
+    seq_lens: torch.Tensor,
+    tree_mask: torch.Tensor,
+    positions: Optional[torch.Tensor] = None,
+) -> None:
+    """Masks and positions of trees of drafted tokens, in one launch.
+
+    query_start_loc ([R + 1] int32) and seq_lens ([R] int32, the drafted tokens
+    included) are build_slot_mapping's.  parents ([T] int32): of each drafted
+    token the index, among its request's, of the token it follows; one that is
+    negative, or not before the token itself, says that it follows the context.
+    Writes tree_mask ([T, W] int64, W up to 16): bit j of a row (bit j % 64 of
+    word j // 64) for the token itself and each it follows, directly or not;
+    and, where given, positions ([T] int64): the context's length plus the
+    tokens followed, for rotary_embedding_to_paged.  (The row of a token in the
+    caches goes by its index: build_slot_mapping's slots.)  Tokens from index
+    64 * W on get an empty mask and the position behind the context; rows behind
+    the last request get zeros."""
+    if _ext is not None:
+        _ext.build_draft_tree(parents, query_start_loc, seq_lens, tree_mask, positions)
+        return
+    dev = _gpu_of(tree_mask, "tree_mask")
+    _run(
+        _L.lmc_build_draft_tree(
+            _opt(parents), _opt(query_start_loc), _opt(seq_lens), _opt(tree_mask), _opt(positions), _stream(dev),
+        )
+    )
+
+
+def tree_attention(
+    query: torch.Tensor,
+    vllm_kv_caches,
+    block_table: torch.Tensor,
+    seq_lens: torch.Tensor,
+    query_start_loc: torch.Tensor,
+    tree_mask: torch.Tensor,
+    scale: float,
+    output: torch.Tensor,
+    lse: Optional[torch.Tensor] = None,
+    kvcache_format_raw: int = 2,
+    vllm_two_major: bool = False,
+) -> None:
+    """Attention of drafted tokens, under their tree's mask, over one layer's
+    paged caches, which hold the drafted tokens' rows already.
+
+    Arguments as shared_prefix_attention's; tree_mask ([T, W] int64) is
+    build_draft_tree's, or any other: a request's q tokens see its first
+    seq_lens[r] - q keys, and of its last q key j behind those where bit j %
+    64 of word j // 64 of the token's row is set (j < 64 * W; bits from q on
+    are not looked at).  Key n is in block block_table[r, n // block_size].
+    Keys whose block is outside the caches are unseen, and unseen rows are not
+    used, whatever they hold.  Tokens that see no key (or whose every score is
+    -infinity) get zeros and an lse of -infinity; rows behind the last request
+    are left as they were.
+
+    Sums, maxima and lse are held in 32 bits; the softmax weights are rounded
+    to the caches' dtype for the product with V, as the output is at the end.
+    Blocks of a multiple of 16 keys are read a group at a time, others key by
+    key."""
+    if _ext is not None:
+        _ext.tree_attention(query, vllm_kv_caches, block_table, seq_lens, query_start_loc, tree_mask, float(scale), output,
+                            lse, int(kvcache_format_raw), bool(vllm_two_major))
+        return
+    dev = _gpu_of(query, "query")
+    caches = _normalize_kv_caches(vllm_kv_caches)
+
+    def call(workspace, size):
+        _run(
+            _L.lmc_tree_attention(
+                _opt(query), _cache_array(caches), len(caches), _opt(block_table), _opt(seq_lens),
+                _opt(query_start_loc), _opt(tree_mask), float(scale), _opt(output), _opt(lse), _opt(workspace), size,
+                int(kvcache_format_raw), int(bool(vllm_two_major)), _stream(dev),
+            )
+        )
+
+    size = ctypes.c_int64(0)
+    call(None, ctypes.byref(size))
+    if size.value:
+        call(torch.empty(size.value, dtype=torch.uint8, device=query.device), None)
+
+
+class KVPagesState:
+    """prepare_kv_pages' result: every layer's caches, checked once, and the
+    table of their addresses on the GPU.  It keeps the caches alive; build a
+    new one after reallocating them."""
+
+    __slots__ = ("layers", "layer_ptrs", "caches", "kvcache_format", "vllm_two_major")
+
+
+def prepare_kv_pages(layers, kvcache_format_raw: int = 2, vllm_two_major: bool = False) -> KVPagesState:
+    """The handle that copy_kv_pages and compact_kv take: `layers` holds each
+    layer's caches (a tensor or a tuple of them, of any KV format), all of one
+    shape, dtype, strides and GPU.  MERGED_KV and SEPARATE_KV caches may have any
+    strides; the others are [pages, block, (heads,) dim].  Caches of one-byte
+    dtypes are taken as they are."""
+    layers = [tuple(_normalize_kv_caches(x)) for x in layers]
+    if not layers:
+        raise ValueError("no layers are given")
+    first = layers[0]
+    for caches in layers:
+        if len(caches) != len(first):
+            raise ValueError("layers differ in the number of their caches")
+        for t, s in zip(caches, first):
+            if (t.shape, t.dtype, t.stride(), t.device) != (s.shape, s.dtype, s.stride(), s.device):
+                raise ValueError("layers differ in shape, dtype, strides or device")
+            # (a launch takes one width of access for all layers)
+            if t.data_ptr() % 16 != s.data_ptr() % 16:
+                raise ValueError("layers' caches differ in their alignment to 16 bytes")
+    _gpu_of(first[0], "the first cache")
+    st = KVPagesState()
+    st.layers = tuple(layers)
+    st.caches = [t.view(torch.uint8) if t.dtype not in _DTYPES and t.element_size() == 1 else t for t in first]
+    st.kvcache_format, st.vllm_two_major = int(kvcache_format_raw), bool(vllm_two_major)
+    st.layer_ptrs = torch.tensor([[t.data_ptr() for t in caches] for caches in layers], dtype=torch.int64,
+                                 device=first[0].device)
+    # A call without pairs checks the caches.
+    copy_kv_pages(st, torch.empty((0, 2), dtype=torch.int64, device=first[0].device))
+    return st
+
+
+def copy_kv_pages(state: KVPagesState, pages: torch.Tensor) -> None:
+    """Pages copied in every layer and plane, as forks need them: pages is
+    [n, 2] int64 or int32, (source, target) page numbers.  Pairs with a page
+    outside the caches are skipped.  No target may be another pair's source or
+    target; a source may serve several targets."""
+    if _ext is not None:
+        _ext.copy_kv_pages(state.layer_ptrs, state.caches, pages, state.kvcache_format, state.vllm_two_major)
+        return
+    dev = _gpu_of(state.layer_ptrs, "layer_ptrs")
+    _run(
+        _L.lmc_copy_kv_pages(
+            _opt(state.layer_ptrs), _cache_array(state.caches), len(state.caches), _opt(pages), state.kvcache_format,
+            int(state.vllm_two_major), _stream(dev),
+        )
+    )
+
+
+def compact_kv(
+    state: KVPagesState,
+    block_table: torch.Tensor,
+    base_lens: torch.Tensor,
+    keep: torch.Tensor,
+    keep_lens: torch.Tensor,
+    seq_lens: Optional[torch.Tensor] = None,
+) -> None:
+    """Rows that a request keeps moved together, in place, in every layer and
+    plane: the accepted path of its drafted tokens, or what is left of a context
+    after dropping tokens.
+
+    Of request r the first base_lens[r] rows ([R] int32) stay; the row at
+    position base_lens[r] + keep[r, i] moves to base_lens[r] + i for i <
+    keep_lens[r] ([R] int32, at most M).  keep is [R, M] int32; each list
+    strictly increases from 0 or more (else the rows from base_lens[r] on hold
+    some of the request's rows, which ones is not said).  block_table ([R, W]
+    int32) has the requests' pages; no two positions of the rows that move may
+    share a page row, within a request or between requests: shared pages are
+    copied first (copy_kv_pages).  A row that has no page, here or there, is not
+    moved.  seq_lens ([R] int32), where given, gets base_lens + keep_lens."""
+    if _ext is not None:
+        _ext.compact_kv(state.layer_ptrs, state.caches, block_table, base_lens, keep, keep_lens, seq_lens,
+                        state.kvcache_format, state.vllm_two_major)
+        return
+    dev = _gpu_of(state.layer_ptrs, "layer_ptrs")
+    _run(
+        _L.lmc_compact_kv(
+            _opt(state.layer_ptrs), _cache_array(state.caches), len(state.caches), _opt(block_table), _opt(base_lens),
+            _opt(keep), _opt(keep_lens), _opt(seq_lens), state.kvcache_format, int(state.vllm_two_major), _stream(dev),
+        )
+    )
+
+
+def release_pages(
+    block_table: torch.Tensor,
+    held_lens: torch.Tensor,
+    keep_lens: torch.Tensor,
+    block_size: int,
+    page_refs: torch.Tensor,
+    free_blocks: torch.Tensor,
+    free_cursor: torch.Tensor,
+    next_cursor: torch.Tensor,
+) -> None:
+    """Pages given back to the free list that build_slot_mapping takes from.
+
+    Request r holds pages for held_lens[r] tokens and keeps those for its first
+    keep_lens[r] ([R] int32): entries ceil(keep / block_size) to ceil(held /
+    block_size) of its row of block_table ([R, W] int32) lose a holder.
+    page_refs ([P] int32) counts each page's holders beyond the first: 0 for a
+    page of one table, one more for each fork that shares it.  A page that has
+    none left is given back, once, and its count is 0 again; the others' counts
+    go down.  Pages given back are put before free_blocks[free_cursor] in
+    ascending order, and next_cursor ([1] int64, another tensor) gets
+    free_cursor less their number, so that free_blocks[next_cursor:] is free;
+    those that the list has no place for are left out.  block_table stays as it
+    is; its entries outside [0, P) are skipped."""
+    if _ext is not None:
+        _ext.release_pages(block_table, held_lens, keep_lens, int(block_size), page_refs, free_blocks, free_cursor,
+                           next_cursor)
+        return
+    dev = _gpu_of(page_refs, "page_refs")
+
+    def call(workspace, size):
+        _run(
+            _L.lmc_release_pages(
+                _opt(block_table), _opt(held_lens), _opt(keep_lens), int(block_size), _opt(page_refs),
+                _opt(free_blocks), _opt(free_cursor), _opt(next_cursor), _opt(workspace), size, _stream(dev),
+            )
+        )
+
+    size = ctypes.c_int64(0)
+    call(None, ctypes.byref(size))
+    call(torch.empty(size.value, dtype=torch.uint8, device=page_refs.device), None)
 
 
 # ---------------------------------------------------------------------------
