@@ -33,6 +33,29 @@ struct TreeArgs : PagedArgs {
   struct Cut { int request, tile, more; } *cuts;  // of the place "ended behind": the pieces that follow, or request -1
 };
 
+// How a call's work is cut, from its sizes alone (the lengths are on the GPU).
+struct TreePlan {
+  int row_waves;                  // of 32 rows
+  int64_t pieces, groups;         // of a KV head's line; workgroups
+  int64_t cuts, join_groups;      // cut tiles at most; workgroups that share the rows of one
+};
+
+TreePlan make_plan(int64_t T, int64_t R, int64_t kv_heads, int64_t group, int64_t dim, int64_t keys) {
+  TreePlan p;
+  // Rows of a request and KV head, about.
+  const int64_t per = (T + R - 1) / R * group;
+  p.row_waves = per <= 64 ? 2 : per <= 128 || dim > 128 ? 4 : 8;
+  // Workgroups that the 256 CUs hold at once.
+  const int64_t places = dim <= 128 && p.row_waves < 8 ? 512 : 256, rows = 32 * p.row_waves;
+  const int64_t tiles = T * group / rows + R;
+  p.pieces = std::min(tiles * std::max<int64_t>(1, (keys + 63) / 64), std::max<int64_t>(1, places / kv_heads));
+  p.groups = p.pieces * kv_heads;
+  p.cuts = std::min(p.pieces - 1, tiles) * kv_heads;
+  const int64_t step = 64 / (dim / 4);  // rows of a workgroup's turn
+  p.join_groups = std::max<int64_t>(1, std::min((std::min(per, rows) + step - 1) / step, 8192 / std::max<int64_t>(1, p.cuts)));
+  return p;
+}
+
 // Rows that see the context and the drafted tokens of their mask.
 template <typename T, int D> struct TreeRows : RowSums<T, D> {
   int context;  // keys before the drafted tokens
@@ -158,23 +181,214 @@ template <typename T, int D> __device__ __forceinline__ void write_part(const Tr
     }
 }
 
-template <typename T, int D, int WAVES>
-__global__ void __launch_bounds__(64 * WAVES, D > 128 ? 1 : 2) attend_tree(TreeArgs a) {
-  constexpr int kRows = 32 * WAVES;
+// Row waves x key waves: 32 rows a wave, of each block of 64 keys all or half.
+// NK and NV: blocks of K and of V that LDS holds.
+template <int D, int RW, int KW> struct Shape {
+  static constexpr int kWaves = RW * KW, kRows = 32 * RW, kBlocks = 2 / KW;  // kBlocks: of 32 keys, a wave's
+  static constexpr int kDeep = RW == 8;
+  static constexpr int kNK = kDeep ? 5 : 2, kNV = kDeep ? 4 : 2;
+  static constexpr int kBytes = (kNK + kNV) * 64 * D * 2;
+  static constexpr int kPerSimd = D > 128 ? 1 : 2;  // waves of a SIMD
+};
+
+// The other waves are here too, all that was read from LDS has arrived.
+__device__ __forceinline__ void meet() { asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory"); }
+
+// The workgroup's rows over the keys of one piece, a block of 64 at a time, K
+// a block ahead of V: the scores of the next block are computed beside the
+// weights of this one, and their maximum beside the product with V.  K and V
+// have rings of blocks, which are loaded as soon as a place is free.
+template <typename T, int D, int RW, int KW, typename Rows>
+__device__ __forceinline__ void attend_ring(const PagedArgs &a, Rows &r, Keys &keys, int entry, int least, uint32_t lds) {
+  using M = Mma<T>;
+  using V8 = typename M::V8;
+  using S = Shape<D, RW, KW>;
+  constexpr int kPer = D / 32, NB = S::kBlocks, NK = S::kNK, NV = S::kNV, kPitch = Geometry<D>::kPitch;
+  constexpr int kScores = NB * D / 16, kValues = 2 * NB * kPer, kAhead = kScores < 8 ? kScores : 8;
+  constexpr uint32_t kBlock = 64 * kPitch, kGroup = 16 * kPitch;
+  // Of eight waves four load K and four V; else each loads 16 keys of both.
+  constexpr bool kSplit = S::kWaves == 8;
+  static_assert(S::kWaves == 4 || S::kWaves == 8, "");
+  static_assert(kSplit || NK == NV, "loads of K and V in turn");
+  const int all_waves = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), wave = all_waves & 3;
+  const bool of_k = !kSplit || all_waves < 4, of_v = !kSplit || !of_k;
+  const int half = KW == 2 ? 32 * (all_waves / RW) : 0;  // this wave's keys of a block
+  const float c = a.scale2;
+  const int k0 = keys.k0, k1 = keys.k1, n = (k1 - k0 + 63) / 64;
+  uint32_t k_off[kPer], v_off[kPer];
+#pragma unroll
+  for (int i = 0; i < kPer; ++i) {
+    k_off[i] = row_offset<D, false>(i, a.k_token);
+    v_off[i] = row_offset<D, true>(i, a.v_token);
+    if constexpr (kSplit) k_off[i] = v_off[i] = of_k ? k_off[i] : v_off[i];
+  }
+  const uint32_t own = lds + wave * kGroup;
+  auto load_k = [&](int j, uint32_t slot) {
+    load_group<D, false, true>(keys, keys.place(4 * j + wave), k0 + 64 * j + 16 * wave, k_off, own + slot * kBlock);
+  };
+  auto load_v = [&](int j, uint32_t slot) {
+    load_group<D, true, true>(keys, keys.place(4 * j + wave), k0 + 64 * j + 16 * wave, v_off, own + (NK + slot) * kBlock);
+  };
+  keys.look_up(0, entry);
+  for (int j = 0; j < NK && j < n; ++j) {
+    if (of_v && j > 0 && j < NV) load_v(j - 1, j - 1);
+    if (of_k) load_k(j, j);
+  }
+  // (what comes last in turn; with fewer blocks all that there are)
+  if (of_v && n < NV) load_v(n - 1, n - 1);
+  wait_rows<T, D>(r);
+  const int lane = threadIdx.x & 63, row = lane & 31, hb = lane >> 5, al = lane & 15;
+  const uint32_t vrow = 4 * hb + (al >> 2), vcol = 2 * ((lane >> 4) & 1) + ((al & 3) >> 1);
+  // A lane's first row and 16-byte piece of K and V.
+  uint32_t krow = (half + row) * kPitch, kpiece = hb ^ k_swizzle<D>(row);
+  uint32_t vlane = (half + vrow) * kPitch + (al & 1) * 8, vpiece = vcol ^ v_swizzle<D>(vrow);
+  auto read_k = [&](uint32_t k, int x) {
+    return *reinterpret_cast<const LdsS8 *>(k + krow + (((2 * (x / NB)) ^ kpiece) << 4) + x % NB * 32 * kPitch);
+  };
+  auto read_v = [&](uint32_t v, int c2, int t) {
+    const uint32_t at = v + vlane + (((4 * t) ^ vpiece) << 4) + c2 * 16 * kPitch;
+    const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16(reinterpret_cast<LdsS4 *>(at));
+    const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16(reinterpret_cast<LdsS4 *>(at + 8 * kPitch));
+    return static_cast<s16x8>(__builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
+  };
+  // The keys of block j that the row sees, from the wave's first one on.
+  auto seen_of = [&](int j0) { return keys.template seen<64>(j0) & r.visible(a, j0); };
+  auto cut_at = [&](int j0) { return least < min(j0 + 64, k1); };
+  if (kSplit && n >= NK) wait_loads<(NK - 1) * kPer>();
+  else wait_loads<0>();
+  meet();
+  f32x16 s[NB];
+#pragma unroll
+  for (int b = 0; b < NB; ++b)
+#pragma unroll
+    for (int i = 0; i < 16; ++i) s[b][i] = 0.f;
+#pragma unroll
+  for (int x = 0; x < kScores; ++x) s[x % NB] = M::mul(__builtin_bit_cast(V8, read_k(lds, x)), r.q[x / NB], s[x % NB]);
+  bool cut = cut_at(k0);
+  if (cut || !keys.template all<64>(k0)) hide<NB>(s, seen_of(k0) >> half);
+  float top = largest<NB>(s, c);
+  uint32_t ks = 0, vs = 0;  // places of K of block j and of V of block j
+#pragma unroll 1
+  for (int j = 0; j < n; ++j) {
+    // K of the next block and V of this one are there, and every wave has
+    // read K of this one and V of the last one.
+    if (!kSplit || j + NK > n) wait_loads<0>();
+    else if (of_k) wait_loads<(NK - 2) * kPer>();
+    else wait_loads<(NV - 2) * kPer>();
+    meet();
+    const int j0 = k0 + 64 * j;
+    if (of_v && j + NV - 1 < n) load_v(j + NV - 1, vs == 0 ? NV - 1 : vs - 1);
+    if (of_k && j + NK < n) load_k(j + NK, ks);
+    ks = ks + 1 == NK ? 0 : ks + 1;
+    const uint32_t k = lds + ks * kBlock, v = lds + (NK + vs) * kBlock;
+    vs = vs + 1 == NV ? 0 : vs + 1;
+    // (addresses are computed in each block and not kept in registers)
+    asm volatile("" : "+v"(krow), "+v"(kpiece), "+v"(vlane), "+v"(vpiece));
+    refer_to<T, D>(r, top);
+    const float base = r.m == -INFINITY ? 0.f : r.m;
+    V8 p[2 * NB];
+    auto weigh_one = [&](int i) {
+      const float w = __builtin_amdgcn_exp2f(s[i / 16][i % 16] * c - base);
+      r.l += w;
+      p[i / 8][i % 8] = M::from(w);
+    };
+    s16x8 kf[kAhead];
+#pragma unroll
+    for (int x = 0; x < kAhead; ++x) kf[x] = read_k(k, x);
+#pragma unroll
+    for (int i = 0; i < 8 * NB; ++i) weigh_one(i);
+    __builtin_amdgcn_sched_barrier(0);
+    f32x16 next[NB];
+#pragma unroll
+    for (int b = 0; b < NB; ++b)
+#pragma unroll
+      for (int i = 0; i < 16; ++i) next[b][i] = 0.f;
+#pragma unroll
+    for (int x = 0; x < kScores; ++x) {
+      next[x % NB] = M::mul(__builtin_bit_cast(V8, kf[x % kAhead]), r.q[x / NB], next[x % NB]);
+      if (x + kAhead < kScores) kf[x % kAhead] = read_k(k, x + kAhead);
+      // Between the products: the other half of the weights.
+#pragma unroll
+      for (int i = 8 * NB + x * 8 * NB / kScores; i < 8 * NB + (x + 1) * 8 * NB / kScores; ++i) weigh_one(i);
+      __builtin_amdgcn_sched_barrier(0);
+    }
+    // (the weights are computed here, not where they are used)
+#pragma unroll
+    for (int x = 0; x < 2 * NB; ++x) {
+      s16x8 y = __builtin_bit_cast(s16x8, p[x]);
+      asm volatile("" : "+v"(y));
+      p[x] = __builtin_bit_cast(V8, y);
+    }
+    if (cut && has_odd<T, D, 64>(v)) {
+      const uint64_t mine = KW == 2 ? uint64_t(0xffffffff) << half : ~uint64_t(0);
+      take_odd_out<T, D, 64, true>(r, v, seen_of(j0) & mine);
+    }
+    s16x8 vf[2][kPer];
+#pragma unroll
+    for (int t = 0; t < kPer; ++t) vf[0][t] = read_v(v, 0, t);
+#pragma unroll
+    for (int b = 0; b < NB; ++b) s[b] = next[b];
+    cut = cut_at(j0 + 64);
+    if (cut || !keys.template all<64>(j0 + 64)) hide<NB>(s, seen_of(j0 + 64) >> half);
+    top = s[0][0];
+#pragma unroll
+    for (int x = 0; x < kValues; ++x) {
+      const int t = x % kPer, c2 = x / kPer;
+      r.o[t] = M::mul(__builtin_bit_cast(V8, vf[c2 % 2][t]), p[c2], r.o[t]);
+      if (c2 + 1 < 2 * NB) vf[(c2 + 1) % 2][t] = read_v(v, c2 + 1, t);
+      // Between the products: the next block's maximum.
+#pragma unroll
+      for (int i = x * 16 * NB / kValues; i < (x + 1) * 16 * NB / kValues; ++i) top = fmaxf(top, s[i / 16][i % 16]);
+      __builtin_amdgcn_sched_barrier(0);
+    }
+    const float2 tops = both_halves(top);
+    top = fmaxf(tops.x, tops.y) * c;
+  }
+}
+
+// The sums of two waves of the same rows, over different keys, to the first's.
+template <typename T, int D, int RW> __device__ __forceinline__ void join_halves(RowSums<T, D> &r, uint8_t *lds) {
+  constexpr int kValues = D / 2 + 2;  // of a lane
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  float *at = reinterpret_cast<float *>(lds) + (wave % RW) * kValues * 64 + lane;
+  __syncthreads();  // (what LDS held has been read)
+  if (wave >= RW) {
+#pragma unroll
+    for (int t = 0; t < D / 32; ++t)
+#pragma unroll
+      for (int i = 0; i < 16; ++i) at[(t * 16 + i) * 64] = r.o[t][i];
+    at[(kValues - 2) * 64] = r.m;
+    at[(kValues - 1) * 64] = r.l;
+  }
+  __syncthreads();
+  if (wave >= RW) return;
+  const float m = at[(kValues - 2) * 64], top = fmaxf(r.m, m), base = top == -INFINITY ? 0.f : top;
+  const float f = __builtin_amdgcn_exp2f(r.m - base), g = __builtin_amdgcn_exp2f(m - base);
+  r.m = top;
+  r.l = r.l * f + at[(kValues - 1) * 64] * g;
+#pragma unroll
+  for (int t = 0; t < D / 32; ++t)
+#pragma unroll
+    for (int i = 0; i < 16; ++i) r.o[t][i] = r.o[t][i] * f + at[(t * 16 + i) * 64] * g;
+}
+
+template <typename T, int D, int RW, int KW>
+__global__ void __launch_bounds__(64 * RW * KW, (Shape<D, RW, KW>::kPerSimd)) attend_tree(TreeArgs a) {
+  using S = Shape<D, RW, KW>;
   extern __shared__ uint8_t lds[];
   const uint32_t at = static_cast<uint32_t>(reinterpret_cast<uintptr_t>((__attribute__((address_space(3))) uint8_t *)lds));
-  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), n = threadIdx.x & 31;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6) % RW, n = threadIdx.x & 31;
   const int h = blockIdx.x % a.kv_heads, piece = blockIdx.x / a.kv_heads;
-  const Begin begin = find_piece<kRows, 64 * WAVES>(a, piece);
+  const Begin begin = find_piece<S::kRows, 64 * S::kWaves>(a, piece);
   const int64_t each = (begin.total + a.pieces - 1) / a.pieces;
   int64_t left = min(each, begin.total - each * piece), unit = begin.unit;
   TreeArgs::Cut cut = {-1, 0, 0};
   for (int r = begin.r; left > 0; ++r, unit = 0) {
-    const Span s = span_of<kRows>(a, r);
+    const Span s = span_of<S::kRows>(a, r);
     while (left > 0 && unit < s.units) {
       const int tile = static_cast<int>(unit / s.blocks), b0 = static_cast<int>(unit - static_cast<int64_t>(tile) * s.blocks);
       const int blocks = static_cast<int>(min(left, static_cast<int64_t>(s.blocks - b0)));
-      const int x = tile * kRows + wave * 32 + n;
+      const int x = tile * S::kRows + wave * 32 + n;
       const int t = x < s.n_rows ? s.start + x / a.group : -1;
       TreeRows<T, D> rows;
       rows.context = s.context;
@@ -183,12 +397,14 @@ __global__ void __launch_bounds__(64 * WAVES, D > 128 ? 1 : 2) attend_tree(TreeA
       const int entry = keys.entry(0);
       load_rows<T, D>(a, rows, t, h * a.group + (t < 0 ? 0 : x % a.group));
       __syncthreads();  // the last tile's keys have been read
-      if (keys.k0 < keys.k1) attend_wide<T, D, WAVES>(a, rows, keys, entry, s.context, at);
+      if (keys.k0 < keys.k1) attend_ring<T, D, RW, KW>(a, rows, keys, entry, s.context, at);
+      if constexpr (KW == 2) join_halves<T, D, RW>(rows, lds);
+      const bool writes = KW == 1 || threadIdx.x < 64 * RW;
+      const bool ends = b0 + blocks < s.blocks && b0 == 0;
       if (blocks == s.blocks) {
-        write_rows<T, D>(a, rows);
+        if (writes) write_rows<T, D>(a, rows);
       } else {
-        const bool ends = b0 + blocks < s.blocks && b0 == 0;
-        write_part<T, D>(a, rows, (static_cast<int64_t>(blockIdx.x) * 2 + ends) * kRows + wave * 32);
+        if (writes) write_part<T, D>(a, rows, (static_cast<int64_t>(blockIdx.x) * 2 + ends) * S::kRows + wave * 32);
         if (ends) cut = {r, tile, static_cast<int>((s.blocks - blocks + each - 1) / each)};
       }
       left -= blocks;
@@ -198,36 +414,56 @@ __global__ void __launch_bounds__(64 * WAVES, D > 128 ? 1 : 2) attend_tree(TreeA
   if (threadIdx.x == 0) a.cuts[blockIdx.x] = cut;
 }
 
-// Joins the pieces of the tile that a workgroup began and a later one ended:
-// D / 4 lanes a row.
-constexpr int kJoinRows = 32;
-
-template <typename T, int D, int WAVES> __global__ void __launch_bounds__(256) join_tree(TreeArgs a) {
-  constexpr int kRows = 32 * WAVES, kQuads = D / 4, kStep = 256 / kQuads;
+// Joins the pieces of the tiles that are cut: the k-th of a KV head to the
+// workgroups (k, KV head, y), which find its first piece among the head's
+// cuts.  D / 4 lanes a row.  Tiles of few pieces take a wave a row (or two or
+// four), all pieces loaded together; those of many, four waves a row, with a
+// quarter of the pieces each.
+template <typename T, int D, int ROWS> __global__ void __launch_bounds__(256) join_tree(TreeArgs a) {
+  constexpr int kQuads = D / 4, kStep = 64 / kQuads, kFew = 8;
   using S = typename T::S;
-  const TreeArgs::Cut cut = a.cuts[blockIdx.x];
-  if (cut.request < 0) return;
-  const Span s = span_of<kRows>(a, cut.request);
+  __shared__ f32x4 sums[4][64];
+  __shared__ float2 weights[4][kStep];
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int h = blockIdx.x % a.kv_heads;
-  const int i0 = threadIdx.x / kQuads, d = threadIdx.x % kQuads * 4;
-  if (i0 >= kStep) return;
-  const int n = min(kRows, s.n_rows - cut.tile * kRows);
-  for (int i = blockIdx.y * kJoinRows + i0; i < min(n, static_cast<int>(blockIdx.y + 1) * kJoinRows); i += kStep) {
-    float m = -INFINITY, l = 0.f;
-    f32x4 o = {0.f, 0.f, 0.f, 0.f};
-    for (int k0 = 0; k0 <= cut.more; k0 += 4) {
-      float2 w[4];
-      f32x4 y[4];
+  int rank = blockIdx.x / a.kv_heads, piece = -1;
+  for (int p0 = 0; p0 < a.pieces; p0 += 64) {
+    const int p = p0 + lane;
+    uint64_t there = __ballot(p < a.pieces && a.cuts[p * a.kv_heads + h].request >= 0);
+    const int n = __popcll(there);
+    if (rank >= n) {
+      rank -= n;
+      continue;
+    }
+    for (; rank > 0; --rank) there &= there - 1;
+    piece = p0 + __ffsll(static_cast<unsigned long long>(there)) - 1;
+    break;
+  }
+  if (piece < 0) return;
+  const int first = piece * a.kv_heads + h;
+  const TreeArgs::Cut cut = a.cuts[first];
+  const Span s = span_of<ROWS>(a, cut.request);
+  const int i0 = lane / kQuads, d = lane % kQuads * 4, n = min(ROWS, s.n_rows - cut.tile * ROWS), parts = cut.more + 1;
+  float m, l;
+  f32x4 o;
+  // Row i of the parts k0, k0 + step, ...: kFew / 2 of them under way together.
+  auto gather = [&](int i, bool there, int k0, int step) {
+    m = -INFINITY;
+    l = 0.f;
+    o = {0.f, 0.f, 0.f, 0.f};
+    for (int k1 = k0; k1 < parts; k1 += step * (kFew / 2)) {
+      float2 w[kFew / 2];
+      f32x4 y[kFew / 2];
 #pragma unroll
-      for (int k = 0; k < 4; ++k) {
-        const int part = k0 + k;
-        const int64_t place = (static_cast<int64_t>(blockIdx.x) + static_cast<int64_t>(part) * a.kv_heads) * 2 + (part == 0);
-        const bool there = part <= cut.more;
-        w[k] = there ? a.part_ml[place * kRows + i] : make_float2(-INFINITY, 0.f);
-        if (there) y[k] = *reinterpret_cast<const f32x4 *>(a.part_o + (place * kRows + i) * D + d);
+      for (int k = 0; k < kFew / 2; ++k) {
+        const int part = k1 + step * k;
+        const int64_t at = (static_cast<int64_t>(first + part * a.kv_heads) * 2 + (part == 0)) * ROWS + i;
+        const bool in = there && part < parts;
+        w[k] = in ? a.part_ml[at] : make_float2(-INFINITY, 0.f);
+        if (in) y[k] = *reinterpret_cast<const f32x4 *>(a.part_o + at * D + d);
       }
 #pragma unroll
-      for (int k = 0; k < 4; ++k) {
+      for (int k = 0; k < kFew / 2; ++k) {
         if (w[k].y == 0.f) continue;
         const float top = fmaxf(m, w[k].x), base = top == -INFINITY ? 0.f : top;
         const float f = __builtin_amdgcn_exp2f(m - base), g = __builtin_amdgcn_exp2f(w[k].x - base);
@@ -237,34 +473,77 @@ template <typename T, int D, int WAVES> __global__ void __launch_bounds__(256) j
         m = top;
       }
     }
-    const float inv = l == 0.f ? 0.f : 1.f / l;
-    const int x = cut.tile * kRows + i, t = s.start + x / a.group, head = h * a.group + x % a.group;
+  };
+  auto write = [&](int i) {
+    const float inv = l == 0.f ? 0.f : 1.f / l, base = m == -INFINITY ? 0.f : m;
+    const int x = cut.tile * ROWS + i, t = s.start + x / a.group, head = h * a.group + x % a.group;
     Pack<S, 4> y;
 #pragma unroll
     for (int e = 0; e < 4; ++e) y.v[e] = from_f32<T>(o[e] * inv);
     *reinterpret_cast<Pack<S, 4> *>(static_cast<S *>(a.o) + t * a.o_token + head * a.o_head + d) = y;
-    if (a.lse && d == 0) a.lse[t * a.lse_token + head * a.lse_head] = l == 0.f ? -INFINITY : (m + log2f(l)) * 0.69314718056f;
+    if (a.lse && d == 0) a.lse[t * a.lse_token + head * a.lse_head] = l == 0.f ? -INFINITY : (base + log2f(l)) * 0.69314718056f;
+  };
+  if (parts <= kFew) {
+    for (int i = (blockIdx.y * 4 + wave) * kStep + i0; i - i0 < n; i += gridDim.y * 4 * kStep) {
+      const bool there = i0 < kStep && i < n;
+      gather(i, there, 0, 1);
+      if (there) write(i);
+    }
+    return;
+  }
+  for (int i1 = blockIdx.y * kStep; i1 < n; i1 += gridDim.y * kStep) {
+    const int i = i1 + i0;
+    const bool there = i0 < kStep && i < n;
+    gather(i, there, wave, 4);
+    __syncthreads();  // (of the last rows)
+    sums[wave][lane] = o;
+    if (there && d == 0) weights[wave][i0] = make_float2(m, l);
+    __syncthreads();
+    if (wave != 0 || !there) continue;
+    m = -INFINITY;
+#pragma unroll
+    for (int g = 0; g < 4; ++g) m = fmaxf(m, weights[g][i0].x);
+    const float base = m == -INFINITY ? 0.f : m;
+    l = 0.f;
+    o = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int g = 0; g < 4; ++g) {
+      const float2 w = weights[g][i0];
+      if (w.y == 0.f) continue;
+      const float f = __builtin_amdgcn_exp2f(w.x - base);
+      l += f * w.y;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) o[e] += f * sums[g][lane][e];
+    }
+    write(i);
   }
 }
 
-template <typename T, int D, int WAVES> void launch(const TreeArgs &a, hipStream_t s) {
-  constexpr int kBytes = 2 * 2 * 64 * D * 2;  // two blocks of K and of V
-  const void *fn = reinterpret_cast<const void *>(attend_tree<T, D, WAVES>);
-  hip_check(hipFuncSetAttribute(fn, hipFuncAttributeMaxDynamicSharedMemorySize, kBytes), "attend_tree shared memory");
-  const uint32_t groups = static_cast<uint32_t>(a.pieces) * a.kv_heads;
-  hipLaunchKernelGGL((attend_tree<T, D, WAVES>), dim3(groups), dim3(64 * WAVES), kBytes, s, a);
+template <typename T, int D, int RW, int KW> void launch(const TreeArgs &a, const TreePlan &p, hipStream_t s) {
+  using S = Shape<D, RW, KW>;
+  const void *fn = reinterpret_cast<const void *>(attend_tree<T, D, RW, KW>);
+  hip_check(hipFuncSetAttribute(fn, hipFuncAttributeMaxDynamicSharedMemorySize, S::kBytes), "attend_tree shared memory");
+  hipLaunchKernelGGL((attend_tree<T, D, RW, KW>), dim3(static_cast<uint32_t>(p.groups)), dim3(64 * S::kWaves), S::kBytes, s, a);
   hip_check(hipGetLastError(), "attend_tree launch");
-  hipLaunchKernelGGL((join_tree<T, D, WAVES>), dim3(groups, 32 * WAVES / kJoinRows), dim3(256), 0, s, a);
+  if (p.pieces == 1) return;  // nothing is cut
+  hipLaunchKernelGGL((join_tree<T, D, S::kRows>), dim3(static_cast<uint32_t>(p.cuts), static_cast<uint32_t>(p.join_groups)), dim3(256),
+                     0, s, a);
   hip_check(hipGetLastError(), "join_tree launch");
 }
 
-template <typename T> void launch_dim(const TreeArgs &a, int64_t dim, int waves, hipStream_t s) {
+template <typename T, int D> void launch_rows(const TreeArgs &a, const TreePlan &p, hipStream_t s) {
+  if (p.row_waves == 2) launch<T, D, 2, 2>(a, p, s);
+  else if (p.row_waves == 4) launch<T, D, 4, 1>(a, p, s);
+  else if constexpr (D <= 128) launch<T, D, 8, 1>(a, p, s);
+}
+
+template <typename T> void launch_dim(const TreeArgs &a, int64_t dim, const TreePlan &p, hipStream_t s) {
   switch (dim) {
-  case 64: waves == 8 ? launch<T, 64, 8>(a, s) : launch<T, 64, 4>(a, s); break;
-  case 96: waves == 8 ? launch<T, 96, 8>(a, s) : launch<T, 96, 4>(a, s); break;
-  case 128: waves == 8 ? launch<T, 128, 8>(a, s) : launch<T, 128, 4>(a, s); break;
-  case 192: launch<T, 192, 4>(a, s); break;
-  default: launch<T, 256, 4>(a, s); break;
+  case 64: launch_rows<T, 64>(a, p, s); break;
+  case 96: launch_rows<T, 96>(a, p, s); break;
+  case 128: launch_rows<T, 128>(a, p, s); break;
+  case 192: launch_rows<T, 192>(a, p, s); break;
+  default: launch_rows<T, 256>(a, p, s); break;
   }
 }
 
@@ -293,17 +572,11 @@ extern "C" int lmc_tree_attention(const lmc_tensor *query, const lmc_tensor *vll
     expect(tm.sizes[1] <= (1 << 20), "tree_mask has more than 2^20 words a row");
     if (workspace_bytes) *workspace_bytes = 0;
     if (n.tokens == 0 || n.heads == 0 || n.requests == 0) return;
-    // Rows of a request and KV head, about.
-    const int64_t per = (n.tokens + n.requests - 1) / n.requests * n.group;
-    const int waves = kv.dim <= 128 && per > 128 ? 8 : 4, rows = 32 * waves;
-    // Workgroups that the 256 CUs hold at once.
-    const int64_t places = kv.dim <= 128 && waves == 4 ? 512 : 256;
-    const int64_t most = (n.tokens * n.group / rows + n.requests) * std::max<int64_t>(1, (n.keys + 63) / 64);
-    a.pieces = static_cast<int>(std::min(most, std::max<int64_t>(1, places / kv.heads)));
-    const int64_t groups = a.pieces * kv.heads, parts = groups * 2 * rows;
-    const int64_t bytes = parts * (kv.dim * 4 + 8) + groups * static_cast<int64_t>(sizeof(TreeArgs::Cut));
+    const TreePlan p = make_plan(n.tokens, n.requests, kv.heads, n.group, kv.dim, n.keys);
+    const int64_t parts = p.groups * 2 * 32 * p.row_waves;
+    const int64_t bytes = parts * (kv.dim * 4 + 8) + p.groups * static_cast<int64_t>(sizeof(TreeArgs::Cut));
     // A launch has less than 2^32 threads along a dimension.
-    expect(groups <= UINT32_MAX / 512, "too many heads");
+    expect(p.groups <= UINT32_MAX / 512, "too many heads");
     if (workspace_bytes) {
       *workspace_bytes = bytes;
       return;
@@ -313,12 +586,13 @@ extern "C" int lmc_tree_attention(const lmc_tensor *query, const lmc_tensor *vll
     a.mask = static_cast<const int64_t *>(tm.data);
     a.mask_token = tm.strides[0];
     a.words = static_cast<int>(tm.sizes[1]);
+    a.pieces = static_cast<int>(p.pieces);
     a.part_o = static_cast<float *>(workspace->data);
     a.part_ml = reinterpret_cast<float2 *>(a.part_o + parts * kv.dim);
     a.cuts = reinterpret_cast<TreeArgs::Cut *>(a.part_ml + parts);
     DeviceGuard guard(kv.device);
     const hipStream_t s = static_cast<hipStream_t>(stream);
-    if (kv.dtype == LMC_BF16) launch_dim<BF16>(a, kv.dim, waves, s);
-    else launch_dim<F16>(a, kv.dim, waves, s);
+    if (kv.dtype == LMC_BF16) launch_dim<BF16>(a, kv.dim, p, s);
+    else launch_dim<F16>(a, kv.dim, p, s);
   });
 }
