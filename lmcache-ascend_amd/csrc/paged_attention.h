@@ -168,13 +168,12 @@ __device__ __forceinline__ bool has_odd(uint32_t v) {
   return __any(bad);
 }
 
-// Takes the infinities and NaN out of a tile of V that holds keys which some
-// rows see and others do not: a weight of zero would make NaN of them.  The
-// rows that see such a key (a bit of `seen`, of the lane's row) get its
-// infinities and NaN added here.  SHARED:
-// the four waves work on one tile, and all of them come here.
-template <typename T, int D, int KEYS, bool SHARED>
-__device__ __forceinline__ void take_odd_out(RowSums<T, D> &r, uint32_t v, uint64_t seen) {
+// Infinities and NaN in a tile of V that holds keys which some rows see and
+// others do not: a weight of zero would make NaN of them.  The rows that see
+// such a key (a bit of `seen`, of the lane's row) get its infinities and NaN
+// added here; then they are taken out of the tile.
+template <typename T, int D, int KEYS>
+__device__ __forceinline__ void add_odd(RowSums<T, D> &r, uint32_t v, uint64_t seen) {
   using M = Mma<T>;
   constexpr int kPitch = Geometry<D>::kPitch;
   const int lane = threadIdx.x & 63, hb = lane >> 5;
@@ -194,6 +193,12 @@ __device__ __forceinline__ void take_odd_out(RowSums<T, D> &r, uint32_t v, uint6
         asm volatile("" ::: "memory");  // (few registers here)
       }
   }
+}
+
+// SHARED: all waves work on one tile, and all of them come here.
+template <typename T, int D, int KEYS, bool SHARED> __device__ __forceinline__ void clear_odd(uint32_t v) {
+  using M = Mma<T>;
+  const int lane = threadIdx.x & 63;
   if constexpr (SHARED) __syncthreads();
 #pragma unroll 1
   for (int i = lane; i < KEYS * D / 8; i += 64) {
@@ -205,6 +210,12 @@ __device__ __forceinline__ void take_odd_out(RowSums<T, D> &r, uint32_t v, uint6
   }
   if constexpr (SHARED) __syncthreads();
   else wait_reads();
+}
+
+template <typename T, int D, int KEYS, bool SHARED>
+__device__ __forceinline__ void take_odd_out(RowSums<T, D> &r, uint32_t v, uint64_t seen) {
+  add_odd<T, D, KEYS>(r, v, seen);
+  clear_odd<T, D, KEYS, SHARED>(v);
 }
 
 // The steps of a tile of NB * 32 keys, in LDS at k and v.
@@ -445,148 +456,6 @@ template <typename T, int D> __device__ __forceinline__ void load_rows(const Pag
     for (int e = 0; e < 16; ++e) r.o[i][e] = 0.f;
   r.m = -INFINITY;
   r.l = 0.f;
-}
-
-// Waves of 32 rows each over blocks of 64 keys that they share: many
-// rows, bound by the matrix cores.  The scores of the next block are computed
-// beside the weights of this one, and their maximum beside the product with
-// V: a wave has a SIMD to itself, or shares it with one that waits for
-// memory, and has to keep matrix and vector units busy.  K and V have two
-// buffers each, K a block ahead.  Each wave loads a group of 16 keys.
-template <typename T, int D, int WAVES, typename Rows>
-__device__ __forceinline__ void attend_wide(const PagedArgs &a, Rows &r, Keys &keys, int entry, int least, uint32_t lds) {
-  using M = Mma<T>;
-  using V8 = typename M::V8;
-  constexpr int kPer = D / 32, kSteps = D / 8, kPitch = Geometry<D>::kPitch;
-  constexpr uint32_t kBlock = 64 * kPitch, kGroup = 16 * kPitch;
-  // With four waves each loads 16 keys of K and of V; of eight, four load K
-  // and four V.
-  static_assert(WAVES == 4 || WAVES == 8, "");
-  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6) & 3;
-  const bool of_k = WAVES == 4 || __builtin_amdgcn_readfirstlane(threadIdx.x >> 8) == 0, of_v = WAVES == 4 || !of_k;
-  const float c = a.scale2;
-  const int k0 = keys.k0, k1 = keys.k1, n = (k1 - k0 + 63) / 64;
-  uint32_t k_off[kPer], v_off[kPer];
-#pragma unroll
-  for (int i = 0; i < kPer; ++i) {
-    k_off[i] = row_offset<D, false>(i, a.k_token);
-    v_off[i] = row_offset<D, true>(i, a.v_token);
-    if constexpr (WAVES == 8) k_off[i] = v_off[i] = of_k ? k_off[i] : v_off[i];
-  }
-  const uint32_t own = lds + wave * kGroup;
-  keys.look_up(0, entry);
-  Place now = keys.place(wave), last;  // of the block whose K, and the one whose V is loaded
-  if (of_k) load_group<D, false, false>(keys, now, k0 + 16 * wave, k_off, own);
-  if (of_v) load_group<D, true, false>(keys, now, k0 + 16 * wave, v_off, own + 2 * kBlock);
-  if (n > 1) {
-    now = keys.place(4 + wave);
-    if (of_k) load_group<D, false, false>(keys, now, k0 + 64 + 16 * wave, k_off, own + kBlock);
-  }
-  wait_rows<T, D>(r);
-  wait_loads<0>();
-  __syncthreads();
-  f32x16 s[2];
-  scores<T, D, 2>(r, lds, s);
-  uint64_t seen = 0;
-  bool cut = least < min(k0 + 64, k1);
-  if (cut || !keys.template all<64>(k0)) {
-    seen = keys.template seen<64>(k0);
-    hide<2>(s, seen & r.visible(a, k0));
-  }
-  float top = largest<2>(s, c);
-  const int lane = threadIdx.x & 63, row = lane & 31, hb = lane >> 5, al = lane & 15;
-  const uint32_t vrow = 4 * hb + (al >> 2), vcol = 2 * ((lane >> 4) & 1) + ((al & 3) >> 1);
-  // A lane's first row and 16-byte piece of K and V.
-  uint32_t krow = row * kPitch, kpiece = hb ^ k_swizzle<D>(row);
-  uint32_t vlane = vrow * kPitch + (al & 1) * 8, vpiece = vcol ^ v_swizzle<D>(vrow);
-#pragma unroll 1
-  for (int j = 0; j < n; ++j) {
-    // K of the next block and V of this one are there, and every wave has
-    // read K of this one and V of the last one.
-    wait_loads<0>();
-    __syncthreads();
-    const int j0 = k0 + 64 * j;
-    const uint32_t odd = (j & 1) * kBlock;
-    if (j + 1 < n) {
-      last = now;
-      if (j + 2 < n) {
-        now = keys.place(4 * (j + 2) + wave);
-        if (of_k) load_group<D, false, false>(keys, now, j0 + 128 + 16 * wave, k_off, own + odd);
-      }
-      if (of_v) load_group<D, true, false>(keys, last, j0 + 64 + 16 * wave, v_off, own + 2 * kBlock + (kBlock - odd));
-    }
-    const uint32_t k = lds + (kBlock - odd), v = lds + 2 * kBlock + odd;
-    // (addresses are computed in each block and not kept in registers)
-    asm volatile("" : "+v"(krow), "+v"(kpiece), "+v"(vlane), "+v"(vpiece));
-    refer_to<T, D>(r, top);
-    const float base = r.m == -INFINITY ? 0.f : r.m;
-    auto read_k = [&](int x) {
-      return *reinterpret_cast<const LdsS8 *>(k + krow + (((2 * (x / 2)) ^ kpiece) << 4) + x % 2 * 32 * kPitch);
-    };
-    auto read_v = [&](int c2, int t) {
-      const uint32_t at = v + vlane + (((4 * t) ^ vpiece) << 4) + c2 * 16 * kPitch;
-      const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16(reinterpret_cast<LdsS4 *>(at));
-      const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16(reinterpret_cast<LdsS4 *>(at + 8 * kPitch));
-      return static_cast<s16x8>(__builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
-    };
-    V8 p[4];
-    auto weigh_one = [&](int i) {
-      const float w = __builtin_amdgcn_exp2f(s[i / 16][i % 16] * c - base);
-      r.l += w;
-      p[i / 8][i % 8] = M::from(w);
-    };
-    s16x8 kf[8];
-#pragma unroll
-    for (int x = 0; x < 8; ++x) kf[x] = read_k(x);
-#pragma unroll
-    for (int i = 0; i < 16; ++i) weigh_one(i);
-    __builtin_amdgcn_sched_barrier(0);
-    f32x16 next[2];
-#pragma unroll
-    for (int b = 0; b < 2; ++b)
-#pragma unroll
-      for (int i = 0; i < 16; ++i) next[b][i] = 0.f;
-#pragma unroll
-    for (int x = 0; x < kSteps; ++x) {
-      next[x % 2] = M::mul(__builtin_bit_cast(V8, kf[x % 8]), r.q[x / 2], next[x % 2]);
-      if (x + 8 < kSteps) kf[x % 8] = read_k(x + 8);
-      // Between the products: the other half of the weights.
-#pragma unroll
-      for (int i = 16 + x * 16 / kSteps; i < 16 + (x + 1) * 16 / kSteps; ++i) weigh_one(i);
-      __builtin_amdgcn_sched_barrier(0);
-    }
-    // (the weights are computed here, not where they are used)
-#pragma unroll
-    for (int x = 0; x < 4; ++x) {
-      s16x8 y = __builtin_bit_cast(s16x8, p[x]);
-      asm volatile("" : "+v"(y));
-      p[x] = __builtin_bit_cast(V8, y);
-    }
-    if (cut && has_odd<T, D, 64>(v)) take_odd_out<T, D, 64, true>(r, v, seen & r.visible(a, j0));
-    s16x8 vf[2][kPer];
-#pragma unroll
-    for (int t = 0; t < kPer; ++t) vf[0][t] = read_v(0, t);
-    s[0] = next[0];
-    s[1] = next[1];
-    cut = least < min(j0 + 128, k1);
-    if (cut || !keys.template all<64>(j0 + 64)) {
-      seen = keys.template seen<64>(j0 + 64);
-      hide<2>(s, seen & r.visible(a, j0 + 64));
-    }
-    top = s[0][0];
-#pragma unroll
-    for (int x = 0; x < kSteps; ++x) {
-      const int t = x % kPer, c2 = x / kPer;
-      r.o[t] = M::mul(__builtin_bit_cast(V8, vf[c2 % 2][t]), p[c2], r.o[t]);
-      if (c2 < 3) vf[(c2 + 1) % 2][t] = read_v(c2 + 1, t);
-      // Between the products: the next block's maximum.
-#pragma unroll
-      for (int i = x * 32 / kSteps; i < (x + 1) * 32 / kSteps; ++i) top = fmaxf(top, s[i / 16][i % 16]);
-      __builtin_amdgcn_sched_barrier(0);
-    }
-    const float2 tops = both_halves(top);
-    top = fmaxf(tops.x, tops.y) * c;
-  }
 }
 
 // Key numbers and what is added to them stay far from 2^31.

@@ -217,6 +217,143 @@ __device__ __forceinline__ void attend_narrow(const AttnArgs &a, Rows32<T, D> &r
   }
 }
 
+// Four waves of 32 rows each over blocks of 64 keys that they share: many
+// rows, bound by the matrix cores.  The scores of the next block are computed
+// beside the weights of this one, and their maximum beside the product with
+// V: a wave has a SIMD to itself, or shares it with one that waits for
+// memory, and has to keep matrix and vector units busy.  K and V have two
+// buffers each, K a block ahead.  Each wave loads a group of 16 keys.
+template <typename T, int D>
+__device__ __forceinline__ void attend_wide(const AttnArgs &a, Rows32<T, D> &r, Keys &keys, int entry, int least, uint32_t lds) {
+  using M = Mma<T>;
+  using V8 = typename M::V8;
+  constexpr int kPer = D / 32, kSteps = D / 8, kPitch = Geometry<D>::kPitch;
+  constexpr uint32_t kBlock = 64 * kPitch, kGroup = 16 * kPitch;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const float c = a.scale2;
+  const int k0 = keys.k0, k1 = keys.k1, n = (k1 - k0 + 63) / 64;
+  uint32_t k_off[kPer], v_off[kPer];
+#pragma unroll
+  for (int i = 0; i < kPer; ++i) {
+    k_off[i] = row_offset<D, false>(i, a.k_token);
+    v_off[i] = row_offset<D, true>(i, a.v_token);
+  }
+  const uint32_t own = lds + wave * kGroup;
+  keys.look_up(0, entry);
+  Place now = keys.place(wave), last;  // of the block whose K, and the one whose V is loaded
+  load_group<D, false, false>(keys, now, k0 + 16 * wave, k_off, own);
+  load_group<D, true, false>(keys, now, k0 + 16 * wave, v_off, own + 2 * kBlock);
+  if (n > 1) {
+    now = keys.place(4 + wave);
+    load_group<D, false, false>(keys, now, k0 + 64 + 16 * wave, k_off, own + kBlock);
+  }
+  wait_rows<T, D>(r);
+  wait_loads<0>();
+  __syncthreads();
+  f32x16 s[2];
+  scores<T, D, 2>(r, lds, s);
+  uint64_t seen = 0;
+  bool cut = least < min(k0 + 64, k1);
+  if (cut || !keys.template all<64>(k0)) {
+    seen = keys.template seen<64>(k0);
+    hide<2>(s, seen & r.visible(a, k0));
+  }
+  float top = largest<2>(s, c);
+  const int lane = threadIdx.x & 63, row = lane & 31, hb = lane >> 5, al = lane & 15;
+  const uint32_t vrow = 4 * hb + (al >> 2), vcol = 2 * ((lane >> 4) & 1) + ((al & 3) >> 1);
+  // A lane's first row and 16-byte piece of K and V.
+  uint32_t krow = row * kPitch, kpiece = hb ^ k_swizzle<D>(row);
+  uint32_t vlane = vrow * kPitch + (al & 1) * 8, vpiece = vcol ^ v_swizzle<D>(vrow);
+#pragma unroll 1
+  for (int j = 0; j < n; ++j) {
+    // K of the next block and V of this one are there, and every wave has
+    // read K of this one and V of the last one.
+    wait_loads<0>();
+    __syncthreads();
+    const int j0 = k0 + 64 * j;
+    const uint32_t odd = (j & 1) * kBlock;
+    if (j + 1 < n) {
+      last = now;
+      if (j + 2 < n) {
+        now = keys.place(4 * (j + 2) + wave);
+        load_group<D, false, false>(keys, now, j0 + 128 + 16 * wave, k_off, own + odd);
+      }
+      load_group<D, true, false>(keys, last, j0 + 64 + 16 * wave, v_off, own + 2 * kBlock + (kBlock - odd));
+    }
+    const uint32_t k = lds + (kBlock - odd), v = lds + 2 * kBlock + odd;
+    // (addresses are computed in each block and not kept in registers)
+    asm volatile("" : "+v"(krow), "+v"(kpiece), "+v"(vlane), "+v"(vpiece));
+    refer_to<T, D>(r, top);
+    const float base = r.m == -INFINITY ? 0.f : r.m;
+    auto read_k = [&](int x) {
+      return *reinterpret_cast<const LdsS8 *>(k + krow + (((2 * (x / 2)) ^ kpiece) << 4) + x % 2 * 32 * kPitch);
+    };
+    auto read_v = [&](int c2, int t) {
+      const uint32_t at = v + vlane + (((4 * t) ^ vpiece) << 4) + c2 * 16 * kPitch;
+      const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16(reinterpret_cast<LdsS4 *>(at));
+      const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16(reinterpret_cast<LdsS4 *>(at + 8 * kPitch));
+      return static_cast<s16x8>(__builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
+    };
+    V8 p[4];
+    auto weigh_one = [&](int i) {
+      const float w = __builtin_amdgcn_exp2f(s[i / 16][i % 16] * c - base);
+      r.l += w;
+      p[i / 8][i % 8] = M::from(w);
+    };
+    s16x8 kf[8];
+#pragma unroll
+    for (int x = 0; x < 8; ++x) kf[x] = read_k(x);
+#pragma unroll
+    for (int i = 0; i < 16; ++i) weigh_one(i);
+    __builtin_amdgcn_sched_barrier(0);
+    f32x16 next[2];
+#pragma unroll
+    for (int b = 0; b < 2; ++b)
+#pragma unroll
+      for (int i = 0; i < 16; ++i) next[b][i] = 0.f;
+#pragma unroll
+    for (int x = 0; x < kSteps; ++x) {
+      next[x % 2] = M::mul(__builtin_bit_cast(V8, kf[x % 8]), r.q[x / 2], next[x % 2]);
+      if (x + 8 < kSteps) kf[x % 8] = read_k(x + 8);
+      // Between the products: the other half of the weights.
+#pragma unroll
+      for (int i = 16 + x * 16 / kSteps; i < 16 + (x + 1) * 16 / kSteps; ++i) weigh_one(i);
+      __builtin_amdgcn_sched_barrier(0);
+    }
+    // (the weights are computed here, not where they are used)
+#pragma unroll
+    for (int x = 0; x < 4; ++x) {
+      s16x8 y = __builtin_bit_cast(s16x8, p[x]);
+      asm volatile("" : "+v"(y));
+      p[x] = __builtin_bit_cast(V8, y);
+    }
+    if (cut && has_odd<T, D, 64>(v)) take_odd_out<T, D, 64, true>(r, v, seen & r.visible(a, j0));
+    s16x8 vf[2][kPer];
+#pragma unroll
+    for (int t = 0; t < kPer; ++t) vf[0][t] = read_v(0, t);
+    s[0] = next[0];
+    s[1] = next[1];
+    cut = least < min(j0 + 128, k1);
+    if (cut || !keys.template all<64>(j0 + 64)) {
+      seen = keys.template seen<64>(j0 + 64);
+      hide<2>(s, seen & r.visible(a, j0 + 64));
+    }
+    top = s[0][0];
+#pragma unroll
+    for (int x = 0; x < kSteps; ++x) {
+      const int t = x % kPer, c2 = x / kPer;
+      r.o[t] = M::mul(__builtin_bit_cast(V8, vf[c2 % 2][t]), p[c2], r.o[t]);
+      if (c2 < 3) vf[(c2 + 1) % 2][t] = read_v(c2 + 1, t);
+      // Between the products: the next block's maximum.
+#pragma unroll
+      for (int i = x * 32 / kSteps; i < (x + 1) * 32 / kSteps; ++i) top = fmaxf(top, s[i / 16][i % 16]);
+      __builtin_amdgcn_sched_barrier(0);
+    }
+    const float2 tops = both_halves(top);
+    top = fmaxf(tops.x, tops.y) * c;
+  }
+}
+
 // Keys that token t sees of a request of `seq` keys whose tokens end at
 // `stop`; there are none behind the table's row.
 __device__ __forceinline__ int limit_of(const AttnArgs &a, int seq, int stop, int t) {
@@ -309,7 +446,7 @@ template <typename T, int D, bool WIDE> __global__ void __launch_bounds__(256, D
     load_rows<T, D>(a, r, t, h * a.group + (t < 0 ? 0 : x % a.group));
     r.limit = t >= 0 && limit > 0 ? limit : INT32_MAX;
     const int least = least_limit<WIDE>(r.limit, lds);
-    if constexpr (WIDE) attend_wide<T, D, 4>(a, r, keys, entry, least, at);
+    if constexpr (WIDE) attend_wide<T, D>(a, r, keys, entry, least, at);
     else attend_narrow<T, D, false>(a, r, keys, entry, least, at + wave * (2 * 32 * D * 2));
     store_part<T, D, !WIDE>(a, r, limit <= 0, part, lds);
     return;

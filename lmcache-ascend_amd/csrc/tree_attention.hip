@@ -35,7 +35,7 @@ struct TreeArgs : PagedArgs {
 
 // How a call's work is cut, from its sizes alone (the lengths are on the GPU).
 struct TreePlan {
-  int row_waves;                  // of 32 rows
+  int64_t rows;                   // of a tile: 64, 128 or 256
   int64_t pieces, groups;         // of a KV head's line; workgroups
   int64_t cuts, join_groups;      // cut tiles at most; workgroups that share the rows of one
 };
@@ -44,15 +44,15 @@ TreePlan make_plan(int64_t T, int64_t R, int64_t kv_heads, int64_t group, int64_
   TreePlan p;
   // Rows of a request and KV head, about.
   const int64_t per = (T + R - 1) / R * group;
-  p.row_waves = per <= 64 ? 2 : per <= 128 || dim > 128 ? 4 : 8;
+  p.rows = per <= 64 || dim == 256 ? 64 : per <= 128 || dim == 192 ? 128 : 256;
   // Workgroups that the 256 CUs hold at once.
-  const int64_t places = dim <= 128 && p.row_waves < 8 ? 512 : 256, rows = 32 * p.row_waves;
-  const int64_t tiles = T * group / rows + R;
+  const int64_t places = dim <= 128 && p.rows == 64 ? 512 : 256;
+  const int64_t tiles = T * group / p.rows + R;
   p.pieces = std::min(tiles * std::max<int64_t>(1, (keys + 63) / 64), std::max<int64_t>(1, places / kv_heads));
   p.groups = p.pieces * kv_heads;
   p.cuts = std::min(p.pieces - 1, tiles) * kv_heads;
   const int64_t step = 64 / (dim / 4);  // rows of a workgroup's turn
-  p.join_groups = std::max<int64_t>(1, std::min((std::min(per, rows) + step - 1) / step, 8192 / std::max<int64_t>(1, p.cuts)));
+  p.join_groups = std::max<int64_t>(1, std::min((std::min(per, p.rows) + step - 1) / step, 8192 / std::max<int64_t>(1, p.cuts)));
   return p;
 }
 
@@ -181,38 +181,42 @@ template <typename T, int D> __device__ __forceinline__ void write_part(const Tr
     }
 }
 
-// Row waves x key waves: 32 rows a wave, of each block of 64 keys all or half.
-// NK and NV: blocks of K and of V that LDS holds.
-template <int D, int RW, int KW> struct Shape {
-  static constexpr int kWaves = RW * KW, kRows = 32 * RW, kBlocks = 2 / KW;  // kBlocks: of 32 keys, a wave's
-  static constexpr int kDeep = RW == 8;
-  static constexpr int kNK = kDeep ? 5 : 2, kNV = kDeep ? 4 : 2;
+// Row waves x key waves: RB times 32 rows a wave, all or half of each block of 64
+// keys, in steps of 32.  kNK and kNV: blocks of K and of V that LDS holds.
+template <int D, int RW, int KW, int RB> struct Shape {
+  static constexpr int kWaves = RW * KW, kRows = 32 * RB * RW;
+  static constexpr int kSteps = 2 / KW;  // of a block
+  static constexpr int kNV = kRows > 128 || RB == 2 ? 4 : 2, kNK = kNV + kSteps - 1;
   static constexpr int kBytes = (kNK + kNV) * 64 * D * 2;
-  static constexpr int kPerSimd = D > 128 ? 1 : 2;  // waves of a SIMD
+  static constexpr int kPerSimd = D > 128 || RB == 2 ? 1 : 2;  // waves of a SIMD
 };
 
 // The other waves are here too, all that was read from LDS has arrived.
 __device__ __forceinline__ void meet() { asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory"); }
 
-// The workgroup's rows over the keys of one piece, a block of 64 at a time, K
-// a block ahead of V: the scores of the next block are computed beside the
-// weights of this one, and their maximum beside the product with V.  K and V
-// have rings of blocks, which are loaded as soon as a place is free.
-template <typename T, int D, int RW, int KW, typename Rows>
-__device__ __forceinline__ void attend_ring(const PagedArgs &a, Rows &r, Keys &keys, int entry, int least, uint32_t lds) {
+// The workgroup's rows over the keys of one piece, a block of 64 at a time, a
+// wave's 32 keys a step.  K runs a step ahead of V, and a step's softmax is
+// spread over two products: beside the product with V of step i stand the
+// maximum of step i + 1 and the first half of its weights, beside the scores of
+// step i + 2 the other half.  So matrix and vector units have work at any time,
+// also of one wave alone.  K and V have rings of blocks in LDS, loaded as soon
+// as a place is free.
+template <typename T, int D, int RW, int KW, int RB>
+__device__ __forceinline__ void attend_ring(const PagedArgs &a, TreeRows<T, D> (&r)[RB], Keys &keys, int entry, int least, uint32_t lds) {
   using M = Mma<T>;
   using V8 = typename M::V8;
-  using S = Shape<D, RW, KW>;
-  constexpr int kPer = D / 32, NB = S::kBlocks, NK = S::kNK, NV = S::kNV, kPitch = Geometry<D>::kPitch;
-  constexpr int kScores = NB * D / 16, kValues = 2 * NB * kPer, kAhead = kScores < 8 ? kScores : 8;
-  constexpr uint32_t kBlock = 64 * kPitch, kGroup = 16 * kPitch;
-  // Of eight waves four load K and four V; else each loads 16 keys of both.
+  using S = Shape<D, RW, KW, RB>;
+  constexpr int kPer = D / 32, NK = S::kNK, NV = S::kNV, kSteps = S::kSteps, kPitch = Geometry<D>::kPitch;
+  constexpr int kScores = D / 16, kAhead = 4;
+  constexpr uint32_t kBlock = 64 * kPitch, kGroup = 16 * kPitch, kStep = 32 * kPitch;
+  // K of the block before is still read where a block takes two steps.
+  constexpr int kAheadK = NV, kAheadV = NV - 1;
+  // Of eight waves four load K and four V; of four each loads 16 keys of both.
   constexpr bool kSplit = S::kWaves == 8;
-  static_assert(S::kWaves == 4 || S::kWaves == 8, "");
-  static_assert(kSplit || NK == NV, "loads of K and V in turn");
-  const int all_waves = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), wave = all_waves & 3;
-  const bool of_k = !kSplit || all_waves < 4, of_v = !kSplit || !of_k;
-  const int half = KW == 2 ? 32 * (all_waves / RW) : 0;  // this wave's keys of a block
+  static_assert(S::kWaves == 4 || (kSplit && KW == 1), "");
+  const int any_wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), wave = any_wave & 3;
+  const bool of_k = !kSplit || any_wave < 4, of_v = !kSplit || !of_k;
+  const int half = KW == 2 ? 32 * (wave / RW) : 0;  // this wave's keys of a block
   const float c = a.scale2;
   const int k0 = keys.k0, k1 = keys.k1, n = (k1 - k0 + 63) / 64;
   uint32_t k_off[kPer], v_off[kPer];
@@ -223,158 +227,250 @@ __device__ __forceinline__ void attend_ring(const PagedArgs &a, Rows &r, Keys &k
     if constexpr (kSplit) k_off[i] = v_off[i] = of_k ? k_off[i] : v_off[i];
   }
   const uint32_t own = lds + wave * kGroup;
+  // The wave's 16 keys of block j.
+  auto place = [&](int j) { return keys.place(4 * j + wave); };
   auto load_k = [&](int j, uint32_t slot) {
-    load_group<D, false, true>(keys, keys.place(4 * j + wave), k0 + 64 * j + 16 * wave, k_off, own + slot * kBlock);
+    load_group<D, false, true>(keys, place(j), k0 + 64 * j + 16 * wave, k_off, own + slot * kBlock);
   };
   auto load_v = [&](int j, uint32_t slot) {
-    load_group<D, true, true>(keys, keys.place(4 * j + wave), k0 + 64 * j + 16 * wave, v_off, own + (NK + slot) * kBlock);
+    load_group<D, true, true>(keys, place(j), k0 + 64 * j + 16 * wave, v_off, own + (NK + slot) * kBlock);
   };
   keys.look_up(0, entry);
-  for (int j = 0; j < NK && j < n; ++j) {
-    if (of_v && j > 0 && j < NV) load_v(j - 1, j - 1);
-    if (of_k) load_k(j, j);
+#pragma unroll
+  for (int j = 0; j < kAheadK; ++j) {
+    if (of_v && j > 0 && j - 1 < n) load_v(j - 1, j - 1);
+    if (of_k && j < n) load_k(j, j);
   }
-  // (what comes last in turn; with fewer blocks all that there are)
-  if (of_v && n < NV) load_v(n - 1, n - 1);
-  wait_rows<T, D>(r);
+#pragma unroll
+  for (int b = 0; b < RB; ++b) wait_rows<T, D>(r[b]);
   const int lane = threadIdx.x & 63, row = lane & 31, hb = lane >> 5, al = lane & 15;
   const uint32_t vrow = 4 * hb + (al >> 2), vcol = 2 * ((lane >> 4) & 1) + ((al & 3) >> 1);
   // A lane's first row and 16-byte piece of K and V.
   uint32_t krow = (half + row) * kPitch, kpiece = hb ^ k_swizzle<D>(row);
   uint32_t vlane = (half + vrow) * kPitch + (al & 1) * 8, vpiece = vcol ^ v_swizzle<D>(vrow);
-  auto read_k = [&](uint32_t k, int x) {
-    return *reinterpret_cast<const LdsS8 *>(k + krow + (((2 * (x / NB)) ^ kpiece) << 4) + x % NB * 32 * kPitch);
-  };
+  auto read_k = [&](uint32_t k, int x) { return *reinterpret_cast<const LdsS8 *>(k + krow + (((2 * x) ^ kpiece) << 4)); };
   auto read_v = [&](uint32_t v, int c2, int t) {
     const uint32_t at = v + vlane + (((4 * t) ^ vpiece) << 4) + c2 * 16 * kPitch;
     const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16(reinterpret_cast<LdsS4 *>(at));
     const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16(reinterpret_cast<LdsS4 *>(at + 8 * kPitch));
     return static_cast<s16x8>(__builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
   };
-  // The keys of block j that the row sees, from the wave's first one on.
-  auto seen_of = [&](int j0) { return keys.template seen<64>(j0) & r.visible(a, j0); };
+  f32x16 s[RB][1];
+  V8 p[RB][2];
+  float base[RB];
+  auto weigh_one = [&](V8 &to, int b, int i) {
+    const float w = __builtin_amdgcn_exp2f(s[b][0][i] * c - base[b]);
+    r[b].l += w;
+    to[i % 8] = M::from(w);
+  };
+  auto pin = [&](V8 &x) {  // (computed here, not where it is used)
+    s16x8 y = __builtin_bit_cast(s16x8, x);
+    asm volatile("" : "+v"(y));
+    x = __builtin_bit_cast(V8, y);
+  };
+  // Takes out the keys from block j0 on (this wave's 32 from `from` on) that a
+  // row does not see, or that the caches do not have.
   auto cut_at = [&](int j0) { return least < min(j0 + 64, k1); };
-  if (kSplit && n >= NK) wait_loads<(NK - 1) * kPer>();
+  auto hide_at = [&](int j0, int from) {
+    if (cut_at(j0) || !keys.template all<64>(j0)) {
+      const uint64_t there = keys.template seen<64>(j0);
+#pragma unroll
+      for (int b = 0; b < RB; ++b) hide<1>(s[b], (there & r[b].visible(a, j0)) >> from);
+    }
+  };
+  constexpr int kFirst = (kSplit ? 1 : 2) * (kAheadK - 1) * kPer;  // loads behind those of K's first block
+  static_assert(kFirst < 64, "");
+  if (n >= kAheadK) wait_loads<kFirst>();
   else wait_loads<0>();
   meet();
-  f32x16 s[NB];
 #pragma unroll
-  for (int b = 0; b < NB; ++b)
+  for (int b = 0; b < RB; ++b)
 #pragma unroll
-    for (int i = 0; i < 16; ++i) s[b][i] = 0.f;
+    for (int i = 0; i < 16; ++i) s[b][0][i] = 0.f;
 #pragma unroll
-  for (int x = 0; x < kScores; ++x) s[x % NB] = M::mul(__builtin_bit_cast(V8, read_k(lds, x)), r.q[x / NB], s[x % NB]);
-  bool cut = cut_at(k0);
-  if (cut || !keys.template all<64>(k0)) hide<NB>(s, seen_of(k0) >> half);
-  float top = largest<NB>(s, c);
+  for (int x = 0; x < kScores; ++x) {
+    const V8 k = __builtin_bit_cast(V8, read_k(lds, x));
+#pragma unroll
+    for (int b = 0; b < RB; ++b) s[b][0] = M::mul(k, r[b].q[x], s[b][0]);
+  }
+  hide_at(k0, half);
+#pragma unroll
+  for (int b = 0; b < RB; ++b) {
+    r[b].m = largest<1>(s[b], c);
+    base[b] = r[b].m == -INFINITY ? 0.f : r[b].m;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) weigh_one(p[b][0], b, i);
+  }
+  s16x8 kf[kAhead];
+  if constexpr (kSteps == 2) {
+#pragma unroll
+    for (int x = 0; x < kAhead; ++x) kf[x] = read_k(lds + kStep, x);
+  }
+  // Step i: the scores of the step behind it, whose K is at k; the product with
+  // V at v; and the first reads of the K behind that, at k_next (where a
+  // block takes two steps, it is there already).
+  auto step = [&](uint32_t k, uint32_t k_next, uint32_t v, int j0_next, int from) {
+    // (addresses are computed in each step and not kept in registers)
+    asm volatile("" : "+v"(krow), "+v"(kpiece), "+v"(vlane), "+v"(vpiece));
+    f32x16 next[RB];
+    s16x8 vf[2][kPer];
+#pragma unroll
+    for (int b = 0; b < RB; ++b)
+#pragma unroll
+      for (int i = 0; i < 16; ++i) next[b][i] = 0.f;
+    if constexpr (kSteps == 1) {
+#pragma unroll
+      for (int x = 0; x < kAhead; ++x) kf[x] = read_k(k, x);
+    }
+    constexpr int kFirstProducts = RB * kScores, kWeights = 8 * RB;
+#pragma unroll
+    for (int y = 0; y < kFirstProducts; ++y) {
+      const int x = y / RB, b = y % RB;
+      next[b] = M::mul(__builtin_bit_cast(V8, kf[x % kAhead]), r[b].q[x], next[b]);
+      if (b == RB - 1) {
+        if (x + kAhead < kScores) kf[x % kAhead] = read_k(k, x + kAhead);
+        else if (x + kAhead - kScores < kPer) vf[0][x + kAhead - kScores] = read_v(v, 0, x + kAhead - kScores);
+      }
+#pragma unroll
+      for (int i = y * kWeights / kFirstProducts; i < (y + 1) * kWeights / kFirstProducts; ++i) weigh_one(p[i % RB][1], i % RB, 8 + i / RB);
+      __builtin_amdgcn_sched_barrier(0);
+    }
+#pragma unroll
+    for (int t = kAhead; t < kPer; ++t) vf[0][t] = read_v(v, 0, t);
+#pragma unroll
+    for (int b = 0; b < RB; ++b) {
+      pin(p[b][1]);
+      s[b][0] = next[b];
+    }
+    hide_at(j0_next, from);
+    float top[RB], scale[RB];
+    bool moved = false;
+#pragma unroll
+    for (int b = 0; b < RB; ++b) top[b] = s[b][0][0], scale[b] = 1.f;
+    V8 first[RB];
+    constexpr int kProducts = 2 * RB * kPer, kTop = kProducts / 4, kRest = kProducts - kTop;
+#pragma unroll
+    for (int y = 0; y < kProducts; ++y) {
+      const int b = y % RB, t = y / RB % kPer, c2 = y / RB / kPer;
+      r[b].o[t] = M::mul(__builtin_bit_cast(V8, vf[c2][t]), p[b][c2], r[b].o[t]);
+      if (b == RB - 1) {
+        if (c2 == 0) vf[1][t] = read_v(v, 1, t);
+        else if (kSteps == 2 && t < kAhead) kf[t] = read_k(k_next, t);
+      }
+      if (y < kTop) {
+#pragma unroll
+        for (int i = y * 16 * RB / kTop; i < (y + 1) * 16 * RB / kTop; ++i) top[i % RB] = fmaxf(top[i % RB], s[i % RB][0][i / RB]);
+      }
+      if (y == kTop - 1) {
+        // The sums keep their reference point until a score passes it by 2^8:
+        // the weights stay below 256, where their relative rounding is the
+        // same.  What V's product adds meanwhile goes by the old point.
+#pragma unroll
+        for (int x = 0; x < RB; ++x) {
+          const float2 tops = both_halves(top[x]);
+          top[x] = fmaxf(tops.x, tops.y) * c;
+          if (__any(top[x] > r[x].m + 8.f)) {
+            const float m = fmaxf(r[x].m, top[x]);
+            scale[x] = m == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(r[x].m - m);
+            r[x].l *= scale[x];
+            r[x].m = m;
+            base[x] = m == -INFINITY ? 0.f : m;
+            moved = true;
+          }
+        }
+      }
+      if (y >= kTop) {
+#pragma unroll
+        for (int i = (y - kTop) * kWeights / kRest; i < (y - kTop + 1) * kWeights / kRest; ++i) weigh_one(first[i % RB], i % RB, i / RB);
+      }
+      __builtin_amdgcn_sched_barrier(0);
+    }
+    if constexpr (kSteps == 2) {
+#pragma unroll
+      for (int x = kPer; x < kAhead; ++x) kf[x] = read_k(k_next, x);
+    }
+#pragma unroll
+    for (int b = 0; b < RB; ++b) {
+      pin(first[b]);
+      p[b][0] = first[b];
+    }
+    if (moved) {
+#pragma unroll
+      for (int b = 0; b < RB; ++b)
+#pragma unroll
+        for (int t = 0; t < kPer; ++t)
+#pragma unroll
+          for (int i = 0; i < 16; ++i) r[b].o[t][i] *= scale[b];
+    }
+  };
   uint32_t ks = 0, vs = 0;  // places of K of block j and of V of block j
 #pragma unroll 1
   for (int j = 0; j < n; ++j) {
     // K of the next block and V of this one are there, and every wave has
-    // read K of this one and V of the last one.
-    if (!kSplit || j + NK > n) wait_loads<0>();
-    else if (of_k) wait_loads<(NK - 2) * kPer>();
-    else wait_loads<(NV - 2) * kPer>();
+    // read what the blocks loaded now take the place of.
+    constexpr int kBehind = (kSplit ? 1 : 2) * (kAheadV - 1) * kPer;
+    if (kBehind > 0 && j + kAheadK <= n) wait_loads<kBehind>();
+    else wait_loads<0>();
     meet();
     const int j0 = k0 + 64 * j;
-    if (of_v && j + NV - 1 < n) load_v(j + NV - 1, vs == 0 ? NV - 1 : vs - 1);
-    if (of_k && j + NK < n) load_k(j + NK, ks);
+    if (of_v && j + kAheadV < n) load_v(j + kAheadV, vs == 0 ? NV - 1 : vs - 1);
+    if (of_k && j + kAheadK < n) load_k(j + kAheadK, kSteps == 1 ? ks : ks == 0 ? NK - 1 : ks - 1);
+    const uint32_t k = lds + ks * kBlock;
     ks = ks + 1 == NK ? 0 : ks + 1;
-    const uint32_t k = lds + ks * kBlock, v = lds + (NK + vs) * kBlock;
+    const uint32_t k_next = lds + ks * kBlock, v = lds + (NK + vs) * kBlock;
     vs = vs + 1 == NV ? 0 : vs + 1;
-    // (addresses are computed in each block and not kept in registers)
-    asm volatile("" : "+v"(krow), "+v"(kpiece), "+v"(vlane), "+v"(vpiece));
-    refer_to<T, D>(r, top);
-    const float base = r.m == -INFINITY ? 0.f : r.m;
-    V8 p[2 * NB];
-    auto weigh_one = [&](int i) {
-      const float w = __builtin_amdgcn_exp2f(s[i / 16][i % 16] * c - base);
-      r.l += w;
-      p[i / 8][i % 8] = M::from(w);
-    };
-    s16x8 kf[kAhead];
+    if (cut_at(j0) && has_odd<T, D, 64>(v)) {
+      const uint64_t there = keys.template seen<64>(j0) & (KW == 2 ? uint64_t(0xffffffff) << half : ~uint64_t(0));
 #pragma unroll
-    for (int x = 0; x < kAhead; ++x) kf[x] = read_k(k, x);
-#pragma unroll
-    for (int i = 0; i < 8 * NB; ++i) weigh_one(i);
-    __builtin_amdgcn_sched_barrier(0);
-    f32x16 next[NB];
-#pragma unroll
-    for (int b = 0; b < NB; ++b)
-#pragma unroll
-      for (int i = 0; i < 16; ++i) next[b][i] = 0.f;
-#pragma unroll
-    for (int x = 0; x < kScores; ++x) {
-      next[x % NB] = M::mul(__builtin_bit_cast(V8, kf[x % kAhead]), r.q[x / NB], next[x % NB]);
-      if (x + kAhead < kScores) kf[x % kAhead] = read_k(k, x + kAhead);
-      // Between the products: the other half of the weights.
-#pragma unroll
-      for (int i = 8 * NB + x * 8 * NB / kScores; i < 8 * NB + (x + 1) * 8 * NB / kScores; ++i) weigh_one(i);
-      __builtin_amdgcn_sched_barrier(0);
+      for (int b = 0; b < RB; ++b) add_odd<T, D, 64>(r[b], v, there & r[b].visible(a, j0));
+      clear_odd<T, D, 64, true>(v);
     }
-    // (the weights are computed here, not where they are used)
-#pragma unroll
-    for (int x = 0; x < 2 * NB; ++x) {
-      s16x8 y = __builtin_bit_cast(s16x8, p[x]);
-      asm volatile("" : "+v"(y));
-      p[x] = __builtin_bit_cast(V8, y);
+    if constexpr (kSteps == 1) {
+      step(k_next, 0, v, j0 + 64, half);
+    } else {
+      step(k + kStep, k_next, v, j0, 32);
+      step(k_next, k_next + kStep, v + kStep, j0 + 64, 0);
     }
-    if (cut && has_odd<T, D, 64>(v)) {
-      const uint64_t mine = KW == 2 ? uint64_t(0xffffffff) << half : ~uint64_t(0);
-      take_odd_out<T, D, 64, true>(r, v, seen_of(j0) & mine);
-    }
-    s16x8 vf[2][kPer];
-#pragma unroll
-    for (int t = 0; t < kPer; ++t) vf[0][t] = read_v(v, 0, t);
-#pragma unroll
-    for (int b = 0; b < NB; ++b) s[b] = next[b];
-    cut = cut_at(j0 + 64);
-    if (cut || !keys.template all<64>(j0 + 64)) hide<NB>(s, seen_of(j0 + 64) >> half);
-    top = s[0][0];
-#pragma unroll
-    for (int x = 0; x < kValues; ++x) {
-      const int t = x % kPer, c2 = x / kPer;
-      r.o[t] = M::mul(__builtin_bit_cast(V8, vf[c2 % 2][t]), p[c2], r.o[t]);
-      if (c2 + 1 < 2 * NB) vf[(c2 + 1) % 2][t] = read_v(v, c2 + 1, t);
-      // Between the products: the next block's maximum.
-#pragma unroll
-      for (int i = x * 16 * NB / kValues; i < (x + 1) * 16 * NB / kValues; ++i) top = fmaxf(top, s[i / 16][i % 16]);
-      __builtin_amdgcn_sched_barrier(0);
-    }
-    const float2 tops = both_halves(top);
-    top = fmaxf(tops.x, tops.y) * c;
   }
 }
 
 // The sums of two waves of the same rows, over different keys, to the first's.
-template <typename T, int D, int RW> __device__ __forceinline__ void join_halves(RowSums<T, D> &r, uint8_t *lds) {
-  constexpr int kValues = D / 2 + 2;  // of a lane
+template <typename T, int D, int RW, int RB> __device__ __forceinline__ void join_halves(TreeRows<T, D> (&r)[RB], uint8_t *lds) {
+  constexpr int kValues = D / 2 + 2;  // of a lane and row
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  float *at = reinterpret_cast<float *>(lds) + (wave % RW) * kValues * 64 + lane;
+  float *at = reinterpret_cast<float *>(lds) + (wave % RW) * (RB * kValues * 64) + lane;
   __syncthreads();  // (what LDS held has been read)
   if (wave >= RW) {
 #pragma unroll
-    for (int t = 0; t < D / 32; ++t)
+    for (int b = 0; b < RB; ++b) {
+      float *x = at + b * (kValues * 64);
 #pragma unroll
-      for (int i = 0; i < 16; ++i) at[(t * 16 + i) * 64] = r.o[t][i];
-    at[(kValues - 2) * 64] = r.m;
-    at[(kValues - 1) * 64] = r.l;
+      for (int t = 0; t < D / 32; ++t)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) x[(t * 16 + i) * 64] = r[b].o[t][i];
+      x[(kValues - 2) * 64] = r[b].m;
+      x[(kValues - 1) * 64] = r[b].l;
+    }
   }
   __syncthreads();
   if (wave >= RW) return;
-  const float m = at[(kValues - 2) * 64], top = fmaxf(r.m, m), base = top == -INFINITY ? 0.f : top;
-  const float f = __builtin_amdgcn_exp2f(r.m - base), g = __builtin_amdgcn_exp2f(m - base);
-  r.m = top;
-  r.l = r.l * f + at[(kValues - 1) * 64] * g;
 #pragma unroll
-  for (int t = 0; t < D / 32; ++t)
+  for (int b = 0; b < RB; ++b) {
+    const float *x = at + b * (kValues * 64);
+    const float m = x[(kValues - 2) * 64], top = fmaxf(r[b].m, m), base = top == -INFINITY ? 0.f : top;
+    const float f = __builtin_amdgcn_exp2f(r[b].m - base), g = __builtin_amdgcn_exp2f(m - base);
+    r[b].m = top;
+    r[b].l = r[b].l * f + x[(kValues - 1) * 64] * g;
 #pragma unroll
-    for (int i = 0; i < 16; ++i) r.o[t][i] = r.o[t][i] * f + at[(t * 16 + i) * 64] * g;
+    for (int t = 0; t < D / 32; ++t)
+#pragma unroll
+      for (int i = 0; i < 16; ++i) r[b].o[t][i] = r[b].o[t][i] * f + x[(t * 16 + i) * 64] * g;
+  }
 }
 
-template <typename T, int D, int RW, int KW>
-__global__ void __launch_bounds__(64 * RW * KW, (Shape<D, RW, KW>::kPerSimd)) attend_tree(TreeArgs a) {
-  using S = Shape<D, RW, KW>;
+template <typename T, int D, int RW, int KW, int RB>
+__global__ void __launch_bounds__(64 * RW * KW, (Shape<D, RW, KW, RB>::kPerSimd)) attend_tree(TreeArgs a) {
+  using S = Shape<D, RW, KW, RB>;
   extern __shared__ uint8_t lds[];
   const uint32_t at = static_cast<uint32_t>(reinterpret_cast<uintptr_t>((__attribute__((address_space(3))) uint8_t *)lds));
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6) % RW, n = threadIdx.x & 31;
@@ -383,30 +479,34 @@ __global__ void __launch_bounds__(64 * RW * KW, (Shape<D, RW, KW>::kPerSimd)) at
   const int64_t each = (begin.total + a.pieces - 1) / a.pieces;
   int64_t left = min(each, begin.total - each * piece), unit = begin.unit;
   TreeArgs::Cut cut = {-1, 0, 0};
-  for (int r = begin.r; left > 0; ++r, unit = 0) {
-    const Span s = span_of<S::kRows>(a, r);
+  for (int q = begin.r; left > 0; ++q, unit = 0) {
+    const Span s = span_of<S::kRows>(a, q);
     while (left > 0 && unit < s.units) {
       const int tile = static_cast<int>(unit / s.blocks), b0 = static_cast<int>(unit - static_cast<int64_t>(tile) * s.blocks);
       const int blocks = static_cast<int>(min(left, static_cast<int64_t>(s.blocks - b0)));
-      const int x = tile * S::kRows + wave * 32 + n;
-      const int t = x < s.n_rows ? s.start + x / a.group : -1;
-      TreeRows<T, D> rows;
-      rows.context = s.context;
-      Keys keys{a, a.table + r * a.table_stride, a.width, b0 * 64, min(s.end, (b0 + blocks) * 64), b0 * 64, 32, h * a.k_head,
+      TreeRows<T, D> r[RB];
+      Keys keys{a, a.table + q * a.table_stride, a.width, b0 * 64, min(s.end, (b0 + blocks) * 64), b0 * 64, 32, h * a.k_head,
                 h * a.v_head, a.block_size % 16 != 0};
       const int entry = keys.entry(0);
-      load_rows<T, D>(a, rows, t, h * a.group + (t < 0 ? 0 : x % a.group));
-      __syncthreads();  // the last tile's keys have been read
-      if (keys.k0 < keys.k1) attend_ring<T, D, RW, KW>(a, rows, keys, entry, s.context, at);
-      if constexpr (KW == 2) join_halves<T, D, RW>(rows, lds);
-      const bool writes = KW == 1 || threadIdx.x < 64 * RW;
-      const bool ends = b0 + blocks < s.blocks && b0 == 0;
-      if (blocks == s.blocks) {
-        if (writes) write_rows<T, D>(a, rows);
-      } else {
-        if (writes) write_part<T, D>(a, rows, (static_cast<int64_t>(blockIdx.x) * 2 + ends) * S::kRows + wave * 32);
-        if (ends) cut = {r, tile, static_cast<int>((s.blocks - blocks + each - 1) / each)};
+#pragma unroll
+      for (int b = 0; b < RB; ++b) {
+        const int x = tile * S::kRows + (wave * RB + b) * 32 + n;
+        const int t = x < s.n_rows ? s.start + x / a.group : -1;
+        r[b].context = s.context;
+        load_rows<T, D>(a, r[b], t, h * a.group + (t < 0 ? 0 : x % a.group));
       }
+      __syncthreads();  // the last tile's keys have been read
+      if (keys.k0 < keys.k1) attend_ring<T, D, RW, KW, RB>(a, r, keys, entry, s.context, at);
+      if constexpr (KW == 2) join_halves<T, D, RW, RB>(r, lds);
+      const bool ends = b0 + blocks < s.blocks && b0 == 0;
+      if (KW == 1 || threadIdx.x < 64 * RW) {
+#pragma unroll
+        for (int b = 0; b < RB; ++b) {
+          if (blocks == s.blocks) write_rows<T, D>(a, r[b]);
+          else write_part<T, D>(a, r[b], (static_cast<int64_t>(blockIdx.x) * 2 + ends) * S::kRows + (wave * RB + b) * 32);
+        }
+      }
+      if (blocks < s.blocks && ends) cut = {q, tile, static_cast<int>((s.blocks - blocks + each - 1) / each)};
       left -= blocks;
       unit += blocks;
     }
@@ -519,11 +619,11 @@ template <typename T, int D, int ROWS> __global__ void __launch_bounds__(256) jo
   }
 }
 
-template <typename T, int D, int RW, int KW> void launch(const TreeArgs &a, const TreePlan &p, hipStream_t s) {
-  using S = Shape<D, RW, KW>;
-  const void *fn = reinterpret_cast<const void *>(attend_tree<T, D, RW, KW>);
+template <typename T, int D, int RW, int KW, int RB> void launch(const TreeArgs &a, const TreePlan &p, hipStream_t s) {
+  using S = Shape<D, RW, KW, RB>;
+  const void *fn = reinterpret_cast<const void *>(attend_tree<T, D, RW, KW, RB>);
   hip_check(hipFuncSetAttribute(fn, hipFuncAttributeMaxDynamicSharedMemorySize, S::kBytes), "attend_tree shared memory");
-  hipLaunchKernelGGL((attend_tree<T, D, RW, KW>), dim3(static_cast<uint32_t>(p.groups)), dim3(64 * S::kWaves), S::kBytes, s, a);
+  hipLaunchKernelGGL((attend_tree<T, D, RW, KW, RB>), dim3(static_cast<uint32_t>(p.groups)), dim3(64 * S::kWaves), S::kBytes, s, a);
   hip_check(hipGetLastError(), "attend_tree launch");
   if (p.pieces == 1) return;  // nothing is cut
   hipLaunchKernelGGL((join_tree<T, D, S::kRows>), dim3(static_cast<uint32_t>(p.cuts), static_cast<uint32_t>(p.join_groups)), dim3(256),
@@ -532,9 +632,11 @@ template <typename T, int D, int RW, int KW> void launch(const TreeArgs &a, cons
 }
 
 template <typename T, int D> void launch_rows(const TreeArgs &a, const TreePlan &p, hipStream_t s) {
-  if (p.row_waves == 2) launch<T, D, 2, 2>(a, p, s);
-  else if (p.row_waves == 4) launch<T, D, 4, 1>(a, p, s);
-  else if constexpr (D <= 128) launch<T, D, 8, 1>(a, p, s);
+  if (D == 256 || p.rows == 64) launch<T, D, 2, 2, 1>(a, p, s);
+  else if constexpr (D == 192) launch<T, D, 4, 1, 1>(a, p, s);
+  else if constexpr (D == 256) return;
+  else if (p.rows == 128) launch<T, D, 2, 2, 2>(a, p, s);
+  else launch<T, D, 8, 1, 1>(a, p, s);
 }
 
 template <typename T> void launch_dim(const TreeArgs &a, int64_t dim, const TreePlan &p, hipStream_t s) {
@@ -573,7 +675,7 @@ extern "C" int lmc_tree_attention(const lmc_tensor *query, const lmc_tensor *vll
     if (workspace_bytes) *workspace_bytes = 0;
     if (n.tokens == 0 || n.heads == 0 || n.requests == 0) return;
     const TreePlan p = make_plan(n.tokens, n.requests, kv.heads, n.group, kv.dim, n.keys);
-    const int64_t parts = p.groups * 2 * 32 * p.row_waves;
+    const int64_t parts = p.groups * 2 * p.rows;
     const int64_t bytes = parts * (kv.dim * 4 + 8) + p.groups * static_cast<int64_t>(sizeof(TreeArgs::Cut));
     // A launch has less than 2^32 threads along a dimension.
     expect(p.groups <= UINT32_MAX / 512, "too many heads");
