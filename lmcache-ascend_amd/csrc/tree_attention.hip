@@ -181,14 +181,13 @@ template <typename T, int D> __device__ __forceinline__ void write_part(const Tr
     }
 }
 
-// Row waves x key waves: RB times 32 rows a wave, all or half of each block of 64
-// keys, in steps of 32.  kNK and kNV: blocks of K and of V that LDS holds.
-template <int D, int RW, int KW, int RB> struct Shape {
-  static constexpr int kWaves = RW * KW, kRows = 32 * RB * RW;
+// Row waves x key waves: 32 rows a wave, all or half of each block of 64 keys,
+// in steps of 32.  kNK and kNV: blocks of K and of V that LDS holds.
+template <int D, int RW, int KW> struct Shape {
+  static constexpr int kWaves = RW * KW, kRows = 32 * RW;
   static constexpr int kSteps = 2 / KW;  // of a block
-  static constexpr int kNV = kRows > 128 || RB == 2 ? 4 : 2, kNK = kNV + kSteps - 1;
+  static constexpr int kNV = kWaves == 8 ? 4 : 2, kNK = kNV + kSteps - 1;
   static constexpr int kBytes = (kNK + kNV) * 64 * D * 2;
-  static constexpr int kPerSimd = D > 128 || RB == 2 ? 1 : 2;  // waves of a SIMD
 };
 
 // The other waves are here too, all that was read from LDS has arrived.
@@ -198,14 +197,13 @@ __device__ __forceinline__ void meet() { asm volatile("s_waitcnt lgkmcnt(0)\n\ts
 // wave's 32 keys a step.  K runs a step ahead of V, and a step's softmax is
 // spread over two products: beside the product with V of step i stand the
 // maximum of step i + 1 and the first half of its weights, beside the scores of
-// step i + 2 the other half.  So matrix and vector units have work at any time,
-// also of one wave alone.  K and V have rings of blocks in LDS, loaded as soon
-// as a place is free.
-template <typename T, int D, int RW, int KW, int RB>
-__device__ __forceinline__ void attend_ring(const PagedArgs &a, TreeRows<T, D> (&r)[RB], Keys &keys, int entry, int least, uint32_t lds) {
+// step i + 2 the other half.  So matrix and vector units have work at any time.
+// K and V have rings of blocks in LDS, loaded as soon as a place is free.
+template <typename T, int D, int RW, int KW>
+__device__ __forceinline__ void attend_ring(const PagedArgs &a, TreeRows<T, D> &r, Keys &keys, int entry, int least, uint32_t lds) {
   using M = Mma<T>;
   using V8 = typename M::V8;
-  using S = Shape<D, RW, KW, RB>;
+  using S = Shape<D, RW, KW>;
   constexpr int kPer = D / 32, NK = S::kNK, NV = S::kNV, kSteps = S::kSteps, kPitch = Geometry<D>::kPitch;
   constexpr int kScores = D / 16, kAhead = 4;
   constexpr uint32_t kBlock = 64 * kPitch, kGroup = 16 * kPitch, kStep = 32 * kPitch;
@@ -213,10 +211,10 @@ __device__ __forceinline__ void attend_ring(const PagedArgs &a, TreeRows<T, D> (
   constexpr int kAheadK = NV, kAheadV = NV - 1;
   // Of eight waves four load K and four V; of four each loads 16 keys of both.
   constexpr bool kSplit = S::kWaves == 8;
-  static_assert(S::kWaves == 4 || (kSplit && KW == 1), "");
+  static_assert(S::kWaves == 4 || kSplit, "");
   const int any_wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), wave = any_wave & 3;
   const bool of_k = !kSplit || any_wave < 4, of_v = !kSplit || !of_k;
-  const int half = KW == 2 ? 32 * (wave / RW) : 0;  // this wave's keys of a block
+  const int half = KW == 2 ? 32 * (any_wave / RW) : 0;  // this wave's keys of a block
   const float c = a.scale2;
   const int k0 = keys.k0, k1 = keys.k1, n = (k1 - k0 + 63) / 64;
   uint32_t k_off[kPer], v_off[kPer];
@@ -227,13 +225,11 @@ __device__ __forceinline__ void attend_ring(const PagedArgs &a, TreeRows<T, D> (
     if constexpr (kSplit) k_off[i] = v_off[i] = of_k ? k_off[i] : v_off[i];
   }
   const uint32_t own = lds + wave * kGroup;
-  // The wave's 16 keys of block j.
-  auto place = [&](int j) { return keys.place(4 * j + wave); };
   auto load_k = [&](int j, uint32_t slot) {
-    load_group<D, false, true>(keys, place(j), k0 + 64 * j + 16 * wave, k_off, own + slot * kBlock);
+    load_group<D, false, true>(keys, keys.place(4 * j + wave), k0 + 64 * j + 16 * wave, k_off, own + slot * kBlock);
   };
   auto load_v = [&](int j, uint32_t slot) {
-    load_group<D, true, true>(keys, place(j), k0 + 64 * j + 16 * wave, v_off, own + (NK + slot) * kBlock);
+    load_group<D, true, true>(keys, keys.place(4 * j + wave), k0 + 64 * j + 16 * wave, v_off, own + (NK + slot) * kBlock);
   };
   keys.look_up(0, entry);
 #pragma unroll
@@ -241,8 +237,7 @@ __device__ __forceinline__ void attend_ring(const PagedArgs &a, TreeRows<T, D> (
     if (of_v && j > 0 && j - 1 < n) load_v(j - 1, j - 1);
     if (of_k && j < n) load_k(j, j);
   }
-#pragma unroll
-  for (int b = 0; b < RB; ++b) wait_rows<T, D>(r[b]);
+  wait_rows<T, D>(r);
   const int lane = threadIdx.x & 63, row = lane & 31, hb = lane >> 5, al = lane & 15;
   const uint32_t vrow = 4 * hb + (al >> 2), vcol = 2 * ((lane >> 4) & 1) + ((al & 3) >> 1);
   // A lane's first row and 16-byte piece of K and V.
@@ -255,12 +250,12 @@ __device__ __forceinline__ void attend_ring(const PagedArgs &a, TreeRows<T, D> (
     const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16(reinterpret_cast<LdsS4 *>(at + 8 * kPitch));
     return static_cast<s16x8>(__builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
   };
-  f32x16 s[RB][1];
-  V8 p[RB][2];
-  float base[RB];
-  auto weigh_one = [&](V8 &to, int b, int i) {
-    const float w = __builtin_amdgcn_exp2f(s[b][0][i] * c - base[b]);
-    r[b].l += w;
+  f32x16 s[1];
+  V8 p[2];
+  float base;
+  auto weigh_one = [&](V8 &to, int i) {
+    const float w = __builtin_amdgcn_exp2f(s[0][i] * c - base);
+    r.l += w;
     to[i % 8] = M::from(w);
   };
   auto pin = [&](V8 &x) {  // (computed here, not where it is used)
@@ -272,11 +267,7 @@ __device__ __forceinline__ void attend_ring(const PagedArgs &a, TreeRows<T, D> (
   // row does not see, or that the caches do not have.
   auto cut_at = [&](int j0) { return least < min(j0 + 64, k1); };
   auto hide_at = [&](int j0, int from) {
-    if (cut_at(j0) || !keys.template all<64>(j0)) {
-      const uint64_t there = keys.template seen<64>(j0);
-#pragma unroll
-      for (int b = 0; b < RB; ++b) hide<1>(s[b], (there & r[b].visible(a, j0)) >> from);
-    }
+    if (cut_at(j0) || !keys.template all<64>(j0)) hide<1>(s, (keys.template seen<64>(j0) & r.visible(a, j0)) >> from);
   };
   constexpr int kFirst = (kSplit ? 1 : 2) * (kAheadK - 1) * kPer;  // loads behind those of K's first block
   static_assert(kFirst < 64, "");
@@ -284,23 +275,14 @@ __device__ __forceinline__ void attend_ring(const PagedArgs &a, TreeRows<T, D> (
   else wait_loads<0>();
   meet();
 #pragma unroll
-  for (int b = 0; b < RB; ++b)
+  for (int i = 0; i < 16; ++i) s[0][i] = 0.f;
 #pragma unroll
-    for (int i = 0; i < 16; ++i) s[b][0][i] = 0.f;
-#pragma unroll
-  for (int x = 0; x < kScores; ++x) {
-    const V8 k = __builtin_bit_cast(V8, read_k(lds, x));
-#pragma unroll
-    for (int b = 0; b < RB; ++b) s[b][0] = M::mul(k, r[b].q[x], s[b][0]);
-  }
+  for (int x = 0; x < kScores; ++x) s[0] = M::mul(__builtin_bit_cast(V8, read_k(lds, x)), r.q[x], s[0]);
   hide_at(k0, half);
+  r.m = largest<1>(s, c);
+  base = r.m == -INFINITY ? 0.f : r.m;
 #pragma unroll
-  for (int b = 0; b < RB; ++b) {
-    r[b].m = largest<1>(s[b], c);
-    base[b] = r[b].m == -INFINITY ? 0.f : r[b].m;
-#pragma unroll
-    for (int i = 0; i < 8; ++i) weigh_one(p[b][0], b, i);
-  }
+  for (int i = 0; i < 8; ++i) weigh_one(p[0], i);
   s16x8 kf[kAhead];
   if constexpr (kSteps == 2) {
 #pragma unroll
@@ -312,76 +294,60 @@ __device__ __forceinline__ void attend_ring(const PagedArgs &a, TreeRows<T, D> (
   auto step = [&](uint32_t k, uint32_t k_next, uint32_t v, int j0_next, int from) {
     // (addresses are computed in each step and not kept in registers)
     asm volatile("" : "+v"(krow), "+v"(kpiece), "+v"(vlane), "+v"(vpiece));
-    f32x16 next[RB];
+    f32x16 next;
     s16x8 vf[2][kPer];
 #pragma unroll
-    for (int b = 0; b < RB; ++b)
-#pragma unroll
-      for (int i = 0; i < 16; ++i) next[b][i] = 0.f;
+    for (int i = 0; i < 16; ++i) next[i] = 0.f;
     if constexpr (kSteps == 1) {
 #pragma unroll
       for (int x = 0; x < kAhead; ++x) kf[x] = read_k(k, x);
     }
-    constexpr int kFirstProducts = RB * kScores, kWeights = 8 * RB;
 #pragma unroll
-    for (int y = 0; y < kFirstProducts; ++y) {
-      const int x = y / RB, b = y % RB;
-      next[b] = M::mul(__builtin_bit_cast(V8, kf[x % kAhead]), r[b].q[x], next[b]);
-      if (b == RB - 1) {
-        if (x + kAhead < kScores) kf[x % kAhead] = read_k(k, x + kAhead);
-        else if (x + kAhead - kScores < kPer) vf[0][x + kAhead - kScores] = read_v(v, 0, x + kAhead - kScores);
-      }
+    for (int x = 0; x < kScores; ++x) {
+      next = M::mul(__builtin_bit_cast(V8, kf[x % kAhead]), r.q[x], next);
+      if (x + kAhead < kScores) kf[x % kAhead] = read_k(k, x + kAhead);
+      else if (x + kAhead - kScores < kPer) vf[0][x + kAhead - kScores] = read_v(v, 0, x + kAhead - kScores);
 #pragma unroll
-      for (int i = y * kWeights / kFirstProducts; i < (y + 1) * kWeights / kFirstProducts; ++i) weigh_one(p[i % RB][1], i % RB, 8 + i / RB);
+      for (int i = x * 8 / kScores; i < (x + 1) * 8 / kScores; ++i) weigh_one(p[1], 8 + i);
       __builtin_amdgcn_sched_barrier(0);
     }
 #pragma unroll
     for (int t = kAhead; t < kPer; ++t) vf[0][t] = read_v(v, 0, t);
-#pragma unroll
-    for (int b = 0; b < RB; ++b) {
-      pin(p[b][1]);
-      s[b][0] = next[b];
-    }
+    pin(p[1]);
+    s[0] = next;
     hide_at(j0_next, from);
-    float top[RB], scale[RB];
+    float top = s[0][0], scale = 1.f;
     bool moved = false;
-#pragma unroll
-    for (int b = 0; b < RB; ++b) top[b] = s[b][0][0], scale[b] = 1.f;
-    V8 first[RB];
-    constexpr int kProducts = 2 * RB * kPer, kTop = kProducts / 4, kRest = kProducts - kTop;
+    V8 first;
+    constexpr int kProducts = 2 * kPer, kTop = kProducts / 4, kRest = kProducts - kTop;
 #pragma unroll
     for (int y = 0; y < kProducts; ++y) {
-      const int b = y % RB, t = y / RB % kPer, c2 = y / RB / kPer;
-      r[b].o[t] = M::mul(__builtin_bit_cast(V8, vf[c2][t]), p[b][c2], r[b].o[t]);
-      if (b == RB - 1) {
-        if (c2 == 0) vf[1][t] = read_v(v, 1, t);
-        else if (kSteps == 2 && t < kAhead) kf[t] = read_k(k_next, t);
-      }
+      const int t = y % kPer, c2 = y / kPer;
+      r.o[t] = M::mul(__builtin_bit_cast(V8, vf[c2][t]), p[c2], r.o[t]);
+      if (c2 == 0) vf[1][t] = read_v(v, 1, t);
+      else if (kSteps == 2 && t < kAhead) kf[t] = read_k(k_next, t);
       if (y < kTop) {
 #pragma unroll
-        for (int i = y * 16 * RB / kTop; i < (y + 1) * 16 * RB / kTop; ++i) top[i % RB] = fmaxf(top[i % RB], s[i % RB][0][i / RB]);
+        for (int i = y * 16 / kTop; i < (y + 1) * 16 / kTop; ++i) top = fmaxf(top, s[0][i]);
       }
       if (y == kTop - 1) {
         // The sums keep their reference point until a score passes it by 2^8:
         // the weights stay below 256, where their relative rounding is the
         // same.  What V's product adds meanwhile goes by the old point.
-#pragma unroll
-        for (int x = 0; x < RB; ++x) {
-          const float2 tops = both_halves(top[x]);
-          top[x] = fmaxf(tops.x, tops.y) * c;
-          if (__any(top[x] > r[x].m + 8.f)) {
-            const float m = fmaxf(r[x].m, top[x]);
-            scale[x] = m == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(r[x].m - m);
-            r[x].l *= scale[x];
-            r[x].m = m;
-            base[x] = m == -INFINITY ? 0.f : m;
-            moved = true;
-          }
+        const float2 tops = both_halves(top);
+        top = fmaxf(tops.x, tops.y) * c;
+        if (__any(top > r.m + 8.f)) {
+          const float m = fmaxf(r.m, top);
+          scale = m == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(r.m - m);
+          r.l *= scale;
+          r.m = m;
+          base = m == -INFINITY ? 0.f : m;
+          moved = true;
         }
       }
       if (y >= kTop) {
 #pragma unroll
-        for (int i = (y - kTop) * kWeights / kRest; i < (y - kTop + 1) * kWeights / kRest; ++i) weigh_one(first[i % RB], i % RB, i / RB);
+        for (int i = (y - kTop) * 8 / kRest; i < (y - kTop + 1) * 8 / kRest; ++i) weigh_one(first, i);
       }
       __builtin_amdgcn_sched_barrier(0);
     }
@@ -389,18 +355,13 @@ __device__ __forceinline__ void attend_ring(const PagedArgs &a, TreeRows<T, D> (
 #pragma unroll
       for (int x = kPer; x < kAhead; ++x) kf[x] = read_k(k_next, x);
     }
-#pragma unroll
-    for (int b = 0; b < RB; ++b) {
-      pin(first[b]);
-      p[b][0] = first[b];
-    }
+    pin(first);
+    p[0] = first;
     if (moved) {
 #pragma unroll
-      for (int b = 0; b < RB; ++b)
+      for (int t = 0; t < kPer; ++t)
 #pragma unroll
-        for (int t = 0; t < kPer; ++t)
-#pragma unroll
-          for (int i = 0; i < 16; ++i) r[b].o[t][i] *= scale[b];
+        for (int i = 0; i < 16; ++i) r.o[t][i] *= scale;
     }
   };
   uint32_t ks = 0, vs = 0;  // places of K of block j and of V of block j
@@ -421,9 +382,7 @@ __device__ __forceinline__ void attend_ring(const PagedArgs &a, TreeRows<T, D> (
     vs = vs + 1 == NV ? 0 : vs + 1;
     if (cut_at(j0) && has_odd<T, D, 64>(v)) {
       const uint64_t there = keys.template seen<64>(j0) & (KW == 2 ? uint64_t(0xffffffff) << half : ~uint64_t(0));
-#pragma unroll
-      for (int b = 0; b < RB; ++b) add_odd<T, D, 64>(r[b], v, there & r[b].visible(a, j0));
-      clear_odd<T, D, 64, true>(v);
+      take_odd_out<T, D, 64, true>(r, v, there & r.visible(a, j0));
     }
     if constexpr (kSteps == 1) {
       step(k_next, 0, v, j0 + 64, half);
@@ -435,42 +394,34 @@ __device__ __forceinline__ void attend_ring(const PagedArgs &a, TreeRows<T, D> (
 }
 
 // The sums of two waves of the same rows, over different keys, to the first's.
-template <typename T, int D, int RW, int RB> __device__ __forceinline__ void join_halves(TreeRows<T, D> (&r)[RB], uint8_t *lds) {
-  constexpr int kValues = D / 2 + 2;  // of a lane and row
+template <typename T, int D, int RW> __device__ __forceinline__ void join_halves(RowSums<T, D> &r, uint8_t *lds) {
+  constexpr int kValues = D / 2 + 2;  // of a lane
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  float *at = reinterpret_cast<float *>(lds) + (wave % RW) * (RB * kValues * 64) + lane;
+  float *at = reinterpret_cast<float *>(lds) + (wave % RW) * (kValues * 64) + lane;
   __syncthreads();  // (what LDS held has been read)
   if (wave >= RW) {
 #pragma unroll
-    for (int b = 0; b < RB; ++b) {
-      float *x = at + b * (kValues * 64);
+    for (int t = 0; t < D / 32; ++t)
 #pragma unroll
-      for (int t = 0; t < D / 32; ++t)
-#pragma unroll
-        for (int i = 0; i < 16; ++i) x[(t * 16 + i) * 64] = r[b].o[t][i];
-      x[(kValues - 2) * 64] = r[b].m;
-      x[(kValues - 1) * 64] = r[b].l;
-    }
+      for (int i = 0; i < 16; ++i) at[(t * 16 + i) * 64] = r.o[t][i];
+    at[(kValues - 2) * 64] = r.m;
+    at[(kValues - 1) * 64] = r.l;
   }
   __syncthreads();
   if (wave >= RW) return;
+  const float m = at[(kValues - 2) * 64], top = fmaxf(r.m, m), base = top == -INFINITY ? 0.f : top;
+  const float f = __builtin_amdgcn_exp2f(r.m - base), g = __builtin_amdgcn_exp2f(m - base);
+  r.m = top;
+  r.l = r.l * f + at[(kValues - 1) * 64] * g;
 #pragma unroll
-  for (int b = 0; b < RB; ++b) {
-    const float *x = at + b * (kValues * 64);
-    const float m = x[(kValues - 2) * 64], top = fmaxf(r[b].m, m), base = top == -INFINITY ? 0.f : top;
-    const float f = __builtin_amdgcn_exp2f(r[b].m - base), g = __builtin_amdgcn_exp2f(m - base);
-    r[b].m = top;
-    r[b].l = r[b].l * f + x[(kValues - 1) * 64] * g;
+  for (int t = 0; t < D / 32; ++t)
 #pragma unroll
-    for (int t = 0; t < D / 32; ++t)
-#pragma unroll
-      for (int i = 0; i < 16; ++i) r[b].o[t][i] = r[b].o[t][i] * f + x[(t * 16 + i) * 64] * g;
-  }
+    for (int i = 0; i < 16; ++i) r.o[t][i] = r.o[t][i] * f + at[(t * 16 + i) * 64] * g;
 }
 
-template <typename T, int D, int RW, int KW, int RB>
-__global__ void __launch_bounds__(64 * RW * KW, (Shape<D, RW, KW, RB>::kPerSimd)) attend_tree(TreeArgs a) {
-  using S = Shape<D, RW, KW, RB>;
+template <typename T, int D, int RW, int KW>
+__global__ void __launch_bounds__(64 * RW * KW, D > 128 ? 1 : 2) attend_tree(TreeArgs a) {
+  using S = Shape<D, RW, KW>;
   extern __shared__ uint8_t lds[];
   const uint32_t at = static_cast<uint32_t>(reinterpret_cast<uintptr_t>((__attribute__((address_space(3))) uint8_t *)lds));
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6) % RW, n = threadIdx.x & 31;
@@ -484,27 +435,21 @@ __global__ void __launch_bounds__(64 * RW * KW, (Shape<D, RW, KW, RB>::kPerSimd)
     while (left > 0 && unit < s.units) {
       const int tile = static_cast<int>(unit / s.blocks), b0 = static_cast<int>(unit - static_cast<int64_t>(tile) * s.blocks);
       const int blocks = static_cast<int>(min(left, static_cast<int64_t>(s.blocks - b0)));
-      TreeRows<T, D> r[RB];
+      const int x = tile * S::kRows + wave * 32 + n;
+      const int t = x < s.n_rows ? s.start + x / a.group : -1;
+      TreeRows<T, D> r;
+      r.context = s.context;
       Keys keys{a, a.table + q * a.table_stride, a.width, b0 * 64, min(s.end, (b0 + blocks) * 64), b0 * 64, 32, h * a.k_head,
                 h * a.v_head, a.block_size % 16 != 0};
       const int entry = keys.entry(0);
-#pragma unroll
-      for (int b = 0; b < RB; ++b) {
-        const int x = tile * S::kRows + (wave * RB + b) * 32 + n;
-        const int t = x < s.n_rows ? s.start + x / a.group : -1;
-        r[b].context = s.context;
-        load_rows<T, D>(a, r[b], t, h * a.group + (t < 0 ? 0 : x % a.group));
-      }
+      load_rows<T, D>(a, r, t, h * a.group + (t < 0 ? 0 : x % a.group));
       __syncthreads();  // the last tile's keys have been read
-      if (keys.k0 < keys.k1) attend_ring<T, D, RW, KW, RB>(a, r, keys, entry, s.context, at);
-      if constexpr (KW == 2) join_halves<T, D, RW, RB>(r, lds);
+      if (keys.k0 < keys.k1) attend_ring<T, D, RW, KW>(a, r, keys, entry, s.context, at);
+      if constexpr (KW == 2) join_halves<T, D, RW>(r, lds);
       const bool ends = b0 + blocks < s.blocks && b0 == 0;
       if (KW == 1 || threadIdx.x < 64 * RW) {
-#pragma unroll
-        for (int b = 0; b < RB; ++b) {
-          if (blocks == s.blocks) write_rows<T, D>(a, r[b]);
-          else write_part<T, D>(a, r[b], (static_cast<int64_t>(blockIdx.x) * 2 + ends) * S::kRows + (wave * RB + b) * 32);
-        }
+        if (blocks == s.blocks) write_rows<T, D>(a, r);
+        else write_part<T, D>(a, r, (static_cast<int64_t>(blockIdx.x) * 2 + ends) * S::kRows + wave * 32);
       }
       if (blocks < s.blocks && ends) cut = {q, tile, static_cast<int>((s.blocks - blocks + each - 1) / each)};
       left -= blocks;
@@ -619,11 +564,11 @@ template <typename T, int D, int ROWS> __global__ void __launch_bounds__(256) jo
   }
 }
 
-template <typename T, int D, int RW, int KW, int RB> void launch(const TreeArgs &a, const TreePlan &p, hipStream_t s) {
-  using S = Shape<D, RW, KW, RB>;
-  const void *fn = reinterpret_cast<const void *>(attend_tree<T, D, RW, KW, RB>);
+template <typename T, int D, int RW, int KW> void launch(const TreeArgs &a, const TreePlan &p, hipStream_t s) {
+  using S = Shape<D, RW, KW>;
+  const void *fn = reinterpret_cast<const void *>(attend_tree<T, D, RW, KW>);
   hip_check(hipFuncSetAttribute(fn, hipFuncAttributeMaxDynamicSharedMemorySize, S::kBytes), "attend_tree shared memory");
-  hipLaunchKernelGGL((attend_tree<T, D, RW, KW, RB>), dim3(static_cast<uint32_t>(p.groups)), dim3(64 * S::kWaves), S::kBytes, s, a);
+  hipLaunchKernelGGL((attend_tree<T, D, RW, KW>), dim3(static_cast<uint32_t>(p.groups)), dim3(64 * S::kWaves), S::kBytes, s, a);
   hip_check(hipGetLastError(), "attend_tree launch");
   if (p.pieces == 1) return;  // nothing is cut
   hipLaunchKernelGGL((join_tree<T, D, S::kRows>), dim3(static_cast<uint32_t>(p.cuts), static_cast<uint32_t>(p.join_groups)), dim3(256),
@@ -632,11 +577,12 @@ template <typename T, int D, int RW, int KW, int RB> void launch(const TreeArgs 
 }
 
 template <typename T, int D> void launch_rows(const TreeArgs &a, const TreePlan &p, hipStream_t s) {
-  if (D == 256 || p.rows == 64) launch<T, D, 2, 2, 1>(a, p, s);
-  else if constexpr (D == 192) launch<T, D, 4, 1, 1>(a, p, s);
-  else if constexpr (D == 256) return;
-  else if (p.rows == 128) launch<T, D, 2, 2, 2>(a, p, s);
-  else launch<T, D, 8, 1, 1>(a, p, s);
+  if (p.rows == 64) launch<T, D, 2, 2>(a, p, s);
+  else if constexpr (D == 192) launch<T, D, 4, 1>(a, p, s);
+  else if constexpr (D <= 128) {
+    if (p.rows == 128) launch<T, D, 4, 2>(a, p, s);
+    else launch<T, D, 8, 1>(a, p, s);
+  }
 }
 
 template <typename T> void launch_dim(const TreeArgs &a, int64_t dim, const TreePlan &p, hipStream_t s) {
