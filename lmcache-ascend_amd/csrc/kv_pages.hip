@@ -118,42 +118,27 @@ struct CopyArgs {
   uint32_t groups;                // workgroups of a page
 };
 
-constexpr int kUnroll = 4;
-
+// A vector a thread: what is under way together is other waves'.
 template <int VEC> __global__ void __launch_bounds__(256) copy_pages(CopyArgs a) {
   using V = typename VecOf<VEC>::T;
-  const uint32_t piece = blockIdx.x % a.groups;
-  const uint32_t pair = blockIdx.x / a.groups;
+  const uint32_t pair = blockIdx.x / a.groups, x = (blockIdx.x - pair * a.groups) * 256 + threadIdx.x;
   const int p = blockIdx.y % a.n_planes, l = blockIdx.y / a.n_planes;
   int64_t src, dst;
   if (a.wide) {
-    const int64_t *x = static_cast<const int64_t *>(a.pairs) + pair * a.pair_stride;
-    src = x[0];
-    dst = x[1];
+    const int64_t *at = static_cast<const int64_t *>(a.pairs) + pair * a.pair_stride;
+    src = at[0];
+    dst = at[1];
   } else {
-    const int32_t *x = static_cast<const int32_t *>(a.pairs) + pair * a.pair_stride;
-    src = x[0];
-    dst = x[1];
+    const int32_t *at = static_cast<const int32_t *>(a.pairs) + pair * a.pair_stride;
+    src = at[0];
+    dst = at[1];
   }
   const CopyPlane &c = a.plane[p];
   uint8_t *base = reinterpret_cast<uint8_t *>(a.ptrs[l * a.n_tensors + c.tensor]) + c.offset;
-  if (src < 0 || src >= a.n_pages || dst < 0 || dst >= a.n_pages || src == dst) return;
-  const uint8_t *from = base + src * c.page;
-  uint8_t *to = base + dst * c.page;
-  V v[kUnroll];
-  int64_t at[kUnroll];
-#pragma unroll
-  for (int u = 0; u < kUnroll; ++u) {
-    const uint32_t x = (piece * kUnroll + u) * 256 + threadIdx.x;
-    at[u] = -1;
-    if (x >= c.vectors) continue;
-    const uint32_t run = x / c.pieces, i1 = run / c.n0;
-    at[u] = i1 * c.s1 + (run - i1 * c.n0) * c.s0 + (x - run * c.pieces) * static_cast<int64_t>(VEC);
-    v[u] = gload_nt(reinterpret_cast<const V *>(from + at[u]));
-  }
-#pragma unroll
-  for (int u = 0; u < kUnroll; ++u)
-    if (at[u] >= 0) gstore_nt(reinterpret_cast<V *>(to + at[u]), v[u]);
+  if (src < 0 || src >= a.n_pages || dst < 0 || dst >= a.n_pages || src == dst || x >= c.vectors) return;
+  const uint32_t run = x / c.pieces, i1 = run / c.n0;
+  const int64_t at = i1 * c.s1 + (run - i1 * c.n0) * c.s0 + (x - run * c.pieces) * static_cast<int64_t>(VEC);
+  st<V, true>(reinterpret_cast<V *>(base + dst * c.page + at), ld<V, true>(reinterpret_cast<const V *>(base + src * c.page + at)));
 }
 
 // ---------------------------------------------------------------------------
@@ -179,69 +164,122 @@ struct MoveArgs {
   int64_t keep_stride;
   int most;                       // entries of a list
   int32_t *seq_lens;              // may be null
-  int lanes;                      // threads of a row: a power of two, at most 256
+  int lanes;                      // threads of a row: a power of two, kLeastLanes to 256
 };
 
-// A workgroup moves a slice of one request's rows in one plane of one layer,
-// some rows at a time, in order: rows move down (keep[i] >= i), so what a step
-// writes has been read by it or by an earlier one.  The next step's rows are
-// loaded before this one's are written: they lie behind all that it writes.
-template <int VEC> __global__ void __launch_bounds__(256) move_rows(MoveArgs a) {
+constexpr int kRowsOnce = 4, kRowsMore = 8;  // rows of a thread in a step: with one step, with more
+constexpr int kBatch = 256;       // rows whose places are looked up together
+constexpr int kLeastLanes = 8;    // of a row
+// A step's rows are looked up: a batch holds whole steps.
+static_assert(kBatch % (256 / kLeastLanes * kRowsOnce) == 0 && kBatch % (256 / kLeastLanes * kRowsMore) == 0, "");
+
+// A workgroup moves a slice of one request's rows in one layer (in PL planes
+// of one geometry), some rows at a time, in order: rows move down (keep[i] >= i),
+// so what a step writes has been read by it or by an earlier one.  With MORE
+// than one step, the next one's rows are loaded before this one's are written:
+// they lie behind all that it writes.  A row's place takes a chain of two loads
+// (list, table), so a thread each looks up 256 rows at once, into LDS.
+template <int VEC, int PL, bool MORE> __global__ void __launch_bounds__(256) move_rows(MoveArgs a) {
   using V = typename VecOf<VEC>::T;
   using Held = std::conditional_t<(VEC < 4), uint32_t, V>;  // in a register
-  const int p = blockIdx.y % a.n_planes, l = blockIdx.y / a.n_planes, r = blockIdx.z;
+  constexpr int kUnroll = MORE ? kRowsMore : kRowsOnce;
+  __shared__ int64_t from[MORE ? 2 : 1][kBatch], to[MORE ? 2 : 1][kBatch];  // bytes from the plane's first row; -1: stays
+  const int groups = a.n_planes / PL, p = blockIdx.y % groups * PL, l = blockIdx.y / groups, r = blockIdx.z;
   const MovePlane &c = a.plane[p];
+  const int32_t *keep = a.keep + r * a.keep_stride, *table = a.table + r * a.table_stride;
+  const int first = a.most > 0 ? keep[min(static_cast<int>(threadIdx.x), a.most - 1)] : 0;  // (beside the lengths)
   const int64_t b = a.base_lens[r];
   const int n = min(max(a.keep_lens[r], 0), a.most);
-  if (a.seq_lens && blockIdx.x == 0 && blockIdx.y == 0 && threadIdx.x == 0) a.seq_lens[r] = static_cast<int32_t>(min(b + n, static_cast<int64_t>(INT32_MAX)));
-  uint8_t *base = reinterpret_cast<uint8_t *>(a.ptrs[l * a.n_tensors + c.tensor]) + c.offset;
-  const int rows = 256 / a.lanes, own = threadIdx.x / a.lanes;
+  if (a.seq_lens && blockIdx.x == 0 && blockIdx.y == 0 && threadIdx.x == 0)
+    a.seq_lens[r] = static_cast<int32_t>(min(b + n, static_cast<int64_t>(INT32_MAX)));
+  uint8_t *base[PL];
+#pragma unroll
+  for (int q = 0; q < PL; ++q) base[q] = reinterpret_cast<uint8_t *>(a.ptrs[l * a.n_tensors + a.plane[p + q].tensor]) + a.plane[p + q].offset;
+  // Where a position's row lies, or -1 where the caches have none.
+  auto place = [&](int64_t pos) -> int64_t {
+    if (pos < 0 || pos >= static_cast<int64_t>(a.width) * a.block_size) return -1;
+    const uint32_t j = static_cast<uint32_t>(pos) / a.block_size;
+    const int64_t page = table[j];
+    if (page < 0 || page >= a.n_pages) return -1;
+    return page * c.page + (static_cast<uint32_t>(pos) - j * a.block_size) * c.token;
+  };
+  auto look_up = [&](int batch, int k) {
+    const int x = threadIdx.x, i = batch * kBatch + x;
+    int64_t s = -1, d = -1;
+    if (i < n && k != i) {
+      s = place(b + k);
+      d = place(b + i);
+    }
+    from[MORE ? batch & 1 : 0][x] = s;
+    to[MORE ? batch & 1 : 0][x] = s < 0 ? -1 : d;
+  };
+  const int rows = 256 / a.lanes, own = threadIdx.x / a.lanes, step = rows * kUnroll;
   const uint32_t x = blockIdx.x * a.lanes + (threadIdx.x & (a.lanes - 1));
   const bool in = x < c.vectors;
   const int64_t column = (x / c.pieces) * c.head + (x % c.pieces) * static_cast<int64_t>(VEC);
-  const int32_t *keep = a.keep + r * a.keep_stride, *table = a.table + r * a.table_stride;
-  // The row of a position, or null where the caches have none.
-  auto row_of = [&](int64_t pos) -> uint8_t * {
-    if (pos < 0 || pos >= static_cast<int64_t>(a.width) * a.block_size) return nullptr;
-    const uint32_t j = static_cast<uint32_t>(pos) / a.block_size;
-    const int64_t page = table[j];
-    if (page < 0 || page >= a.n_pages) return nullptr;
-    return base + page * c.page + (static_cast<uint32_t>(pos) - j * a.block_size) * c.token + column;
-  };
-  const int step = rows * kUnroll;
-  Held now[kUnroll], next[kUnroll];
-  uint8_t *to[kUnroll], *to_next[kUnroll];
-  auto load = [&](int i0, Held (&v)[kUnroll], uint8_t *(&t)[kUnroll]) {
+  Held now[kUnroll][PL], next[kUnroll][PL];
+  auto load = [&](int i0, Held (&v)[kUnroll][PL]) {
 #pragma unroll
     for (int u = 0; u < kUnroll; ++u) {
       const int i = i0 + u * rows + own;
-      t[u] = nullptr;
-      v[u] = Held{};
-      if (!in || i >= n) continue;
-      const int k = keep[i];
-      if (k == i) continue;
-      const uint8_t *from = row_of(b + k);
-      t[u] = row_of(b + i);
-      if (!from) t[u] = nullptr;
-      if (t[u]) v[u] = gload(reinterpret_cast<const V *>(from));
+      const int64_t d = in && i < n ? to[MORE ? i / kBatch & 1 : 0][i % kBatch] : -1, s = from[MORE ? i / kBatch & 1 : 0][i % kBatch];
+#pragma unroll
+      for (int q = 0; q < PL; ++q) {
+        v[u][q] = Held{};
+        if (d >= 0) v[u][q] = gload(reinterpret_cast<const V *>(base[q] + s + column));
+      }
     }
   };
-  load(0, now, to);
-  for (int i0 = 0; i0 < n; i0 += step) {
-    load(i0 + step, next, to_next);
-    // This step's rows have arrived, in every wave.
-#pragma unroll
-    for (int u = 0; u < kUnroll; ++u) asm volatile("" : "+v"(now[u])::"memory");
-    __syncthreads();
-#pragma unroll
-    for (int u = 0; u < kUnroll; ++u)
-      if (to[u]) gstore(reinterpret_cast<V *>(to[u]), static_cast<V>(now[u]));
+  auto store = [&](int i0, const Held (&v)[kUnroll][PL]) {
 #pragma unroll
     for (int u = 0; u < kUnroll; ++u) {
-      now[u] = next[u];
-      to[u] = to_next[u];
+      const int i = i0 + u * rows + own;
+      const int64_t d = in && i < n ? to[MORE ? i / kBatch & 1 : 0][i % kBatch] : -1;
+#pragma unroll
+      for (int q = 0; q < PL; ++q)
+        if (d >= 0) gstore_nt(reinterpret_cast<V *>(base[q] + d + column), static_cast<V>(v[u][q]));
+    }
+  };
+  // A step's rows have arrived, in every wave.
+  auto arrive = [&](Held (&v)[kUnroll][PL]) {
+#pragma unroll
+    for (int u = 0; u < kUnroll; ++u)
+#pragma unroll
+      for (int q = 0; q < PL; ++q) asm volatile("" : "+v"(v[u][q])::"memory");
+    __syncthreads();
+  };
+  look_up(0, first);
+  __syncthreads();
+  load(0, now);
+  if constexpr (!MORE) {
+    arrive(now);
+    store(0, now);
+  } else {
+    for (int i0 = 0; i0 < n; i0 += step) {
+      // The batch behind this one, once every wave is done with the one before.
+      if (i0 % kBatch == 0) {
+        __syncthreads();
+        const int ahead = i0 / kBatch + 1, i = ahead * kBatch + threadIdx.x;
+        look_up(ahead, i < n ? keep[i] : 0);
+        __syncthreads();
+      }
+      load(i0 + step, next);
+      arrive(now);
+      store(i0, now);
+#pragma unroll
+      for (int u = 0; u < kUnroll; ++u)
+#pragma unroll
+        for (int q = 0; q < PL; ++q) now[u][q] = next[u][q];
     }
   }
+}
+
+template <int VEC> void launch_moves(const MoveArgs &a, int planes, bool more, dim3 grid, hipStream_t s) {
+  if (planes == 2 && more) hipLaunchKernelGGL((move_rows<VEC, 2, true>), grid, dim3(256), 0, s, a);
+  else if (planes == 2) hipLaunchKernelGGL((move_rows<VEC, 2, false>), grid, dim3(256), 0, s, a);
+  else if (more) hipLaunchKernelGGL((move_rows<VEC, 1, true>), grid, dim3(256), 0, s, a);
+  else hipLaunchKernelGGL((move_rows<VEC, 1, false>), grid, dim3(256), 0, s, a);
+  hip_check(hipGetLastError(), "move_rows launch");
 }
 
 // ---------------------------------------------------------------------------
@@ -254,6 +292,7 @@ struct ReleaseArgs {
   uint32_t width, block_size;
   const int32_t *held, *keep;
   int32_t *refs;
+  int whole;                      // refs is on a 16-byte boundary
   int n_pages;
   int32_t *free_blocks;
   int64_t n_free;
@@ -263,7 +302,7 @@ struct ReleaseArgs {
   int runs;
 };
 
-constexpr int kRun = 4096;
+constexpr int kRun = 1024;        // pages of a workgroup, four a thread
 
 // A holder less for each page that a request gives back.
 __global__ void __launch_bounds__(256) drop_holders(ReleaseArgs a) {
@@ -273,27 +312,55 @@ __global__ void __launch_bounds__(256) drop_holders(ReleaseArgs a) {
     return min(n / a.block_size + (n % a.block_size != 0), a.width);
   };
   const uint32_t first = pages_for(a.keep[r]), stop = pages_for(a.held[r]);
-  for (uint32_t j = first + threadIdx.x; j < stop; j += 256) {
+  for (uint32_t j = first + blockIdx.y * 256 + threadIdx.x; j < stop; j += gridDim.y * 256) {
     const int page = a.table[r * a.table_stride + j];
     if (page >= 0 && page < a.n_pages) atomicSub(a.refs + page, 1);
   }
 }
 
-// Pages that have no holder left, of a thread's 16 of a run.
-__device__ __forceinline__ uint32_t without_holder(const ReleaseArgs &a, int run) {
+// Which of the pages from p0 on (a multiple of 4) have no holder left.
+__device__ __forceinline__ uint32_t without_holder(const ReleaseArgs &a, int p0) {
   uint32_t bits = 0;
-  const int p0 = run * kRun + threadIdx.x * 16;
-#pragma unroll
-  for (int i = 0; i < 16; ++i)
-    if (p0 + i < a.n_pages && a.refs[p0 + i] < 0) bits |= 1u << i;
+  if (p0 + 4 <= a.n_pages && a.whole) {
+    const int4 x = *reinterpret_cast<const int4 *>(a.refs + p0);
+    bits = (x.x < 0) | (x.y < 0) << 1 | (x.z < 0) << 2 | (x.w < 0) << 3;
+  } else {
+    for (int i = 0; i < 4; ++i)
+      if (p0 + i < a.n_pages && a.refs[p0 + i] < 0) bits |= 1u << i;
+  }
   return bits;
+}
+
+// Those pages to the list from `at` on.
+__device__ __forceinline__ void give_back(const ReleaseArgs &a, int p0, uint32_t bits, int64_t at) {
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    if (!(bits >> i & 1)) continue;
+    a.refs[p0 + i] = 0;
+    if (at >= 0 && at < a.n_free) a.free_blocks[at] = p0 + i;
+    ++at;
+  }
+}
+
+__device__ __forceinline__ int sum_of_wave(int n) {
+#pragma unroll
+  for (int d = 32; d > 0; d >>= 1) n += __shfl_xor(n, d);
+  return n;
+}
+
+// The sum of the lanes up to this one.
+__device__ __forceinline__ int sum_to_lane(int n) {
+#pragma unroll
+  for (int d = 1; d < 64; d <<= 1) {
+    const int below = __shfl_up(n, d);
+    if ((threadIdx.x & 63) >= d) n += below;
+  }
+  return n;
 }
 
 __global__ void __launch_bounds__(256) count_free(ReleaseArgs a) {
   __shared__ int part[4];
-  int n = __popc(without_holder(a, blockIdx.x));
-#pragma unroll
-  for (int d = 32; d > 0; d >>= 1) n += __shfl_xor(n, d);
+  const int n = sum_of_wave(__popc(without_holder(a, blockIdx.x * kRun + threadIdx.x * 4)));
   if ((threadIdx.x & 63) == 0) part[threadIdx.x >> 6] = n;
   __syncthreads();
   if (threadIdx.x == 0) a.counts[blockIdx.x] = part[0] + part[1] + part[2] + part[3];
@@ -301,26 +368,18 @@ __global__ void __launch_bounds__(256) count_free(ReleaseArgs a) {
 
 __global__ void __launch_bounds__(256) place_free(ReleaseArgs a) {
   __shared__ int part[3][4];
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, p0 = blockIdx.x * kRun + threadIdx.x * 4;
+  const int64_t cursor = *a.cursor;
+  const uint32_t bits = without_holder(a, p0);
   int before = 0, total = 0;
   for (int i = threadIdx.x; i < a.runs; i += 256) {
     const int n = a.counts[i];
     total += n;
     if (i < static_cast<int>(blockIdx.x)) before += n;
   }
-#pragma unroll
-  for (int d = 32; d > 0; d >>= 1) {
-    before += __shfl_xor(before, d);
-    total += __shfl_xor(total, d);
-  }
-  const uint32_t bits = without_holder(a, blockIdx.x);
-  const int own = __popc(bits);
-  int upto = own;
-#pragma unroll
-  for (int d = 1; d < 64; d <<= 1) {
-    const int below = __shfl_up(upto, d);
-    if (lane >= d) upto += below;
-  }
+  before = sum_of_wave(before);
+  total = sum_of_wave(total);
+  const int own = __popc(bits), upto = sum_to_lane(own);
   if (lane == 63) {
     part[0][wave] = upto;
     part[1][wave] = before;
@@ -333,17 +392,8 @@ __global__ void __launch_bounds__(256) place_free(ReleaseArgs a) {
     before += part[1][w] + (w < wave ? part[0][w] : 0);
     total += part[2][w];
   }
-  const int64_t cursor = *a.cursor;
-  int64_t at = cursor - total + before + upto - own;
   if (blockIdx.x == 0 && threadIdx.x == 0) *a.next_cursor = cursor - total;
-  const int p0 = blockIdx.x * kRun + threadIdx.x * 16;
-#pragma unroll
-  for (int i = 0; i < 16; ++i) {
-    if (!(bits >> i & 1)) continue;
-    a.refs[p0 + i] = 0;
-    if (at >= 0 && at < a.n_free) a.free_blocks[at] = p0 + i;
-    ++at;
-  }
+  give_back(a, p0, bits, cursor - total + before + upto - own);
 }
 
 } // namespace
@@ -398,7 +448,7 @@ extern "C" int lmc_copy_kv_pages(const lmc_tensor *layer_ptrs, const lmc_tensor 
     a.wide = pr.dtype == LMC_I64;
     a.pair_stride = pr.strides[0];
     a.n_pages = g.pages;
-    a.groups = static_cast<uint32_t>((most + 256 * kUnroll - 1) / (256 * kUnroll));
+    a.groups = static_cast<uint32_t>((most + 255) / 256);
     expect(a.groups * pr.sizes[0] <= UINT32_MAX / 256 && layers * g.n_planes <= 65535, "too many pages");
     DeviceGuard guard(g.device);
     const dim3 grid(static_cast<uint32_t>(a.groups * pr.sizes[0]), static_cast<uint32_t>(layers * g.n_planes));
@@ -476,21 +526,26 @@ extern "C" int lmc_compact_kv(const lmc_tensor *layer_ptrs, const lmc_tensor *vl
     a.keep_stride = kp.strides[0];
     a.most = static_cast<int>(kp.sizes[1]);
     a.seq_lens = seq_lens ? static_cast<int32_t *>(seq_lens->data) : nullptr;
-    a.lanes = 16;
-    while (a.lanes < 256 && a.lanes < most && R * layers * g.n_planes * ((most + 2 * a.lanes - 1) / (2 * a.lanes)) >= 1024) a.lanes *= 2;
-    const int64_t slices = (most + a.lanes - 1) / a.lanes;
-    expect(layers * g.n_planes <= 65535 && slices <= UINT32_MAX / 256, "too many layers");
+    // K and V of one geometry go together.
+    const MovePlane &k = a.plane[0], &v = a.plane[1];
+    const int planes = g.n_planes == 2 && k.page == v.page && k.token == v.token && k.head == v.head && k.pieces == v.pieces &&
+                               k.vectors == v.vectors ? 2 : 1;
+    const int64_t items = R * layers * (g.n_planes / planes);
+    a.lanes = kLeastLanes;
+    while (a.lanes < 256 && a.lanes < most && items * ((most + 2 * a.lanes - 1) / (2 * a.lanes)) >= 1024) a.lanes *= 2;
+    const int64_t slices = (most + a.lanes - 1) / a.lanes, groups = layers * (g.n_planes / planes);
+    expect(groups <= 65535 && slices <= UINT32_MAX / 256, "too many layers");
     DeviceGuard guard(dev);
-    const dim3 grid(static_cast<uint32_t>(slices), static_cast<uint32_t>(layers * g.n_planes), static_cast<uint32_t>(R));
+    const dim3 grid(static_cast<uint32_t>(slices), static_cast<uint32_t>(groups), static_cast<uint32_t>(R));
     const hipStream_t s = static_cast<hipStream_t>(stream);
+    const bool more = a.most > 256 / a.lanes * kRowsOnce;
     switch (vec) {
-    case 16: hipLaunchKernelGGL(move_rows<16>, grid, dim3(256), 0, s, a); break;
-    case 8: hipLaunchKernelGGL(move_rows<8>, grid, dim3(256), 0, s, a); break;
-    case 4: hipLaunchKernelGGL(move_rows<4>, grid, dim3(256), 0, s, a); break;
-    case 2: hipLaunchKernelGGL(move_rows<2>, grid, dim3(256), 0, s, a); break;
-    default: hipLaunchKernelGGL(move_rows<1>, grid, dim3(256), 0, s, a); break;
+    case 16: launch_moves<16>(a, planes, more, grid, s); break;
+    case 8: launch_moves<8>(a, planes, more, grid, s); break;
+    case 4: launch_moves<4>(a, planes, more, grid, s); break;
+    case 2: launch_moves<2>(a, planes, more, grid, s); break;
+    default: launch_moves<1>(a, planes, more, grid, s); break;
     }
-    hip_check(hipGetLastError(), "move_rows launch");
   });
 }
 
@@ -525,7 +580,7 @@ extern "C" int lmc_release_pages(const lmc_tensor *block_table, const lmc_tensor
     expect(P <= INT32_MAX - 2 * kRun, "page_refs has too many entries");
     expect(fc.sizes[0] == 1, "free_cursor must have one entry");
     expect(nc.sizes[0] == 1, "next_cursor must have one entry");
-    const int64_t runs = (P + kRun - 1) / kRun, bytes = std::max<int64_t>(1, runs) * 4;
+    const int64_t runs = std::max<int64_t>(1, (P + kRun - 1) / kRun), bytes = runs * 4;
     if (workspace_bytes) {
       *workspace_bytes = bytes;
       return;
@@ -550,6 +605,7 @@ extern "C" int lmc_release_pages(const lmc_tensor *block_table, const lmc_tensor
     a.held = static_cast<const int32_t *>(hl.data);
     a.keep = static_cast<const int32_t *>(kl.data);
     a.refs = static_cast<int32_t *>(pr.data);
+    a.whole = reinterpret_cast<uintptr_t>(pr.data) % 16 == 0;
     a.n_pages = static_cast<int>(P);
     a.free_blocks = static_cast<int32_t *>(fb.data);
     a.n_free = fb.sizes[0];
@@ -559,12 +615,12 @@ extern "C" int lmc_release_pages(const lmc_tensor *block_table, const lmc_tensor
     a.runs = static_cast<int>(runs);
     DeviceGuard guard(dev);
     const hipStream_t s = static_cast<hipStream_t>(stream);
-    if (R > 0) hipLaunchKernelGGL(drop_holders, dim3(static_cast<uint32_t>(R)), dim3(256), 0, s, a);
+    const uint32_t turns = static_cast<uint32_t>(std::min<int64_t>(16, (bt.sizes[1] + 255) / 256));
+    if (R > 0 && turns > 0) hipLaunchKernelGGL(drop_holders, dim3(static_cast<uint32_t>(R), turns), dim3(256), 0, s, a);
     hip_check(hipGetLastError(), "drop_holders launch");
-    const uint32_t groups = static_cast<uint32_t>(std::max<int64_t>(1, runs));
-    hipLaunchKernelGGL(count_free, dim3(groups), dim3(256), 0, s, a);
+    hipLaunchKernelGGL(count_free, dim3(static_cast<uint32_t>(runs)), dim3(256), 0, s, a);
     hip_check(hipGetLastError(), "count_free launch");
-    hipLaunchKernelGGL(place_free, dim3(groups), dim3(256), 0, s, a);
+    hipLaunchKernelGGL(place_free, dim3(static_cast<uint32_t>(runs)), dim3(256), 0, s, a);
     hip_check(hipGetLastError(), "place_free launch");
   });
 }
