@@ -46,7 +46,7 @@ TreePlan make_plan(int64_t T, int64_t R, int64_t kv_heads, int64_t group, int64_
   const int64_t per = (T + R - 1) / R * group;
   p.rows = per <= 64 || dim == 256 ? 64 : per <= 128 || dim == 192 ? 128 : 256;
   // Workgroups that the 256 CUs hold at once.
-  const int64_t places = dim <= 128 && p.rows == 64 ? 512 : 256;
+  const int64_t places = dim == 64 && p.rows == 128 ? 768 : dim <= 128 && p.rows == 64 ? 512 : 256;
   const int64_t tiles = T * group / p.rows + R;
   p.pieces = std::min(tiles * std::max<int64_t>(1, (keys + 63) / 64), std::max<int64_t>(1, places / kv_heads));
   p.groups = p.pieces * kv_heads;
@@ -92,22 +92,31 @@ template <int ROWS> __device__ __forceinline__ Span span_of(const TreeArgs &a, i
   return s;
 }
 
-// The request and the unit of it where a workgroup's piece begins.
+// The request, and the unit of it, where a workgroup's piece begins.
 struct Begin {
-  int64_t total, unit;
+  int64_t each, left, unit;       // units of a piece, of this one; of the request before it
   int r;
+  Span span;
 };
+
+// Blocks of a piece at least: a piece more for the join costs about as much as
+// a block (2 requests of 8 tokens over 2000 keys: 17.2 us with 2, 17.7 with 1,
+// 18.7 with 4).
+constexpr int64_t kLeast = 2;
 
 // All requests' units, summed by the workgroup: each thread has a run of them.
 template <int ROWS, int THREADS> __device__ __forceinline__ Begin find_piece(const TreeArgs &a, int piece) {
   __shared__ int64_t sums[THREADS / 64];
-  __shared__ int64_t found_unit;
-  __shared__ int found_r;
+  __shared__ Begin found;
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   const int per = (a.n_requests + THREADS - 1) / THREADS;
   const int r0 = min(a.n_requests, static_cast<int>(threadIdx.x) * per), r1 = min(a.n_requests, r0 + per);
+  Span s;
   int64_t own = 0;
-  for (int r = r0; r < r1; ++r) own += span_of<ROWS>(a, r).units;
+  for (int r = r0; r < r1; ++r) {
+    s = span_of<ROWS>(a, r);
+    own += s.units;
+  }
   int64_t upto = own;
 #pragma unroll
   for (int d = 1; d < 64; d <<= 1) {
@@ -122,23 +131,28 @@ template <int ROWS, int THREADS> __device__ __forceinline__ Begin find_piece(con
     if (w < wave) upto += sums[w];
     total += sums[w];
   }
-  const int64_t first = (total + a.pieces - 1) / a.pieces * piece;
+  const int64_t each = max((total + a.pieces - 1) / a.pieces, kLeast), first = each * piece;
   if (first >= upto - own && first < upto) {
     int64_t at = upto - own;
     int r = r0;
-    for (; r < r1 - 1; ++r) {
-      const int64_t n = span_of<ROWS>(a, r).units;
-      if (first < at + n) break;
-      at += n;
+    if (per > 1) {
+      for (;; ++r) {
+        s = span_of<ROWS>(a, r);
+        if (r == r1 - 1 || first < at + s.units) break;
+        at += s.units;
+      }
     }
-    found_r = r;
-    found_unit = first - at;
+    found = {each, min(each, total - first), first - at, r, s};
   }
   __syncthreads();
-  Begin b;
-  b.total = total;
-  b.r = __builtin_amdgcn_readfirstlane(found_r);
-  b.unit = found_unit;
+  if (first >= total) return {each, 0, 0, 0, {}};
+  Begin b = found;
+  b.r = __builtin_amdgcn_readfirstlane(b.r);
+  b.span.start = __builtin_amdgcn_readfirstlane(b.span.start);
+  b.span.n_rows = __builtin_amdgcn_readfirstlane(b.span.n_rows);
+  b.span.context = __builtin_amdgcn_readfirstlane(b.span.context);
+  b.span.end = __builtin_amdgcn_readfirstlane(b.span.end);
+  b.span.blocks = __builtin_amdgcn_readfirstlane(b.span.blocks);
   return b;
 }
 
@@ -188,6 +202,7 @@ template <int D, int RW, int KW> struct Shape {
   static constexpr int kSteps = 2 / KW;  // of a block
   static constexpr int kNV = kWaves == 8 ? 4 : 2, kNK = kNV + kSteps - 1;
   static constexpr int kBytes = (kNK + kNV) * 64 * D * 2;
+  static constexpr int kPerSimd = D > 128 ? 1 : D == 64 && RW == 4 ? 3 : 2;  // waves of a SIMD
 };
 
 // The other waves are here too, all that was read from LDS has arrived.
@@ -395,43 +410,47 @@ __device__ __forceinline__ void attend_ring(const PagedArgs &a, TreeRows<T, D> &
 
 // The sums of two waves of the same rows, over different keys, to the first's.
 template <typename T, int D, int RW> __device__ __forceinline__ void join_halves(RowSums<T, D> &r, uint8_t *lds) {
-  constexpr int kValues = D / 2 + 2;  // of a lane
+  constexpr int kQuads = D / 8;  // of sums of a lane
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  float *at = reinterpret_cast<float *>(lds) + (wave % RW) * (kValues * 64) + lane;
+  f32x4 *at = reinterpret_cast<f32x4 *>(lds) + (wave % RW) * ((kQuads + 1) * 64) + lane;
   __syncthreads();  // (what LDS held has been read)
   if (wave >= RW) {
 #pragma unroll
     for (int t = 0; t < D / 32; ++t)
 #pragma unroll
-      for (int i = 0; i < 16; ++i) at[(t * 16 + i) * 64] = r.o[t][i];
-    at[(kValues - 2) * 64] = r.m;
-    at[(kValues - 1) * 64] = r.l;
+      for (int b = 0; b < 4; ++b) at[(t * 4 + b) * 64] = f32x4{r.o[t][4 * b], r.o[t][4 * b + 1], r.o[t][4 * b + 2], r.o[t][4 * b + 3]};
+    at[kQuads * 64] = f32x4{r.m, r.l, 0.f, 0.f};
   }
   __syncthreads();
   if (wave >= RW) return;
-  const float m = at[(kValues - 2) * 64], top = fmaxf(r.m, m), base = top == -INFINITY ? 0.f : top;
-  const float f = __builtin_amdgcn_exp2f(r.m - base), g = __builtin_amdgcn_exp2f(m - base);
+  const f32x4 ml = at[kQuads * 64];
+  const float top = fmaxf(r.m, ml[0]), base = top == -INFINITY ? 0.f : top;
+  const float f = __builtin_amdgcn_exp2f(r.m - base), g = __builtin_amdgcn_exp2f(ml[0] - base);
   r.m = top;
-  r.l = r.l * f + at[(kValues - 1) * 64] * g;
+  r.l = r.l * f + ml[1] * g;
 #pragma unroll
   for (int t = 0; t < D / 32; ++t)
 #pragma unroll
-    for (int i = 0; i < 16; ++i) r.o[t][i] = r.o[t][i] * f + at[(t * 16 + i) * 64] * g;
+    for (int b = 0; b < 4; ++b) {
+      const f32x4 x = at[(t * 4 + b) * 64];
+#pragma unroll
+      for (int e = 0; e < 4; ++e) r.o[t][4 * b + e] = r.o[t][4 * b + e] * f + x[e] * g;
+    }
 }
 
 template <typename T, int D, int RW, int KW>
-__global__ void __launch_bounds__(64 * RW * KW, D > 128 ? 1 : 2) attend_tree(TreeArgs a) {
+__global__ void __launch_bounds__(64 * RW * KW, (Shape<D, RW, KW>::kPerSimd)) attend_tree(TreeArgs a) {
   using S = Shape<D, RW, KW>;
   extern __shared__ uint8_t lds[];
   const uint32_t at = static_cast<uint32_t>(reinterpret_cast<uintptr_t>((__attribute__((address_space(3))) uint8_t *)lds));
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6) % RW, n = threadIdx.x & 31;
   const int h = blockIdx.x % a.kv_heads, piece = blockIdx.x / a.kv_heads;
   const Begin begin = find_piece<S::kRows, 64 * S::kWaves>(a, piece);
-  const int64_t each = (begin.total + a.pieces - 1) / a.pieces;
-  int64_t left = min(each, begin.total - each * piece), unit = begin.unit;
+  const int64_t each = begin.each;
+  int64_t left = begin.left, unit = begin.unit;
+  Span s = begin.span;
   TreeArgs::Cut cut = {-1, 0, 0};
-  for (int q = begin.r; left > 0; ++q, unit = 0) {
-    const Span s = span_of<S::kRows>(a, q);
+  for (int q = begin.r; left > 0;) {
     while (left > 0 && unit < s.units) {
       const int tile = static_cast<int>(unit / s.blocks), b0 = static_cast<int>(unit - static_cast<int64_t>(tile) * s.blocks);
       const int blocks = static_cast<int>(min(left, static_cast<int64_t>(s.blocks - b0)));
@@ -455,6 +474,9 @@ __global__ void __launch_bounds__(64 * RW * KW, D > 128 ? 1 : 2) attend_tree(Tre
       left -= blocks;
       unit += blocks;
     }
+    if (left <= 0) break;
+    s = span_of<S::kRows>(a, ++q);
+    unit = 0;
   }
   if (threadIdx.x == 0) a.cuts[blockIdx.x] = cut;
 }
@@ -580,8 +602,8 @@ template <typename T, int D> void launch_rows(const TreeArgs &a, const TreePlan 
   if (p.rows == 64) launch<T, D, 2, 2>(a, p, s);
   else if constexpr (D == 192) launch<T, D, 4, 1>(a, p, s);
   else if constexpr (D <= 128) {
-    if (p.rows == 128) launch<T, D, 4, 2>(a, p, s);
-    else launch<T, D, 8, 1>(a, p, s);
+    if (p.rows == 256) launch<T, D, 8, 1>(a, p, s);
+    else launch<T, D, 4, D == 64 ? 1 : 2>(a, p, s);
   }
 }
 
