@@ -56,6 +56,9 @@ struct PagedArgs {
   float scale2;             // scale * log2(e)
 };
 
+// Read by scalar loads: addresses that are the same for a wave.
+typedef const __attribute__((address_space(4))) int32_t *ScalarInts;
+
 // Rows of zeros, read in the place of keys that nobody sees.
 __device__ const uint4 zero_row[32] = {};
 
@@ -341,6 +344,14 @@ struct Keys {
   uint64_t groups = 0;   // which lanes' groups are whole
   uint64_t k = 0, v = 0;
 
+  // Other keys of the same caches and head.
+  __device__ __forceinline__ void turn_to(const int32_t *other, int from, int to, bool with_holes) {
+    list = other;
+    k0 = first = from;
+    k1 = to;
+    holes = with_holes;
+  }
+
   __device__ __forceinline__ uint32_t block_of(uint32_t j) const {
     return a.block_size == 1 ? j : __umulhi(j, a.block_mul) >> a.block_shift;
   }
@@ -354,9 +365,11 @@ struct Keys {
   __device__ __forceinline__ int key(int g) const { return first + g / 2 * stride + g % 2 * 16; }
   // The entry of the list for this lane's group of the 64 from g, and what
   // follows from it (apart, so that other loads can be under way between).
-  __device__ __forceinline__ int entry(int g) const {
-    const uint32_t b = block_of(min(max(key(g + (threadIdx.x & 63)), k0), k1));
-    return n_list ? list[min(b, n_list - 1)] : -1;
+  __device__ __forceinline__ int entry(int g) const { return entry_of(list, key(g + (threadIdx.x & 63)), k0, k1); }
+  // The entry of a list for a key of [from, to].
+  __device__ __forceinline__ int entry_of(const int32_t *of, int j, int from, int to) const {
+    const uint32_t b = block_of(min(max(j, from), to));
+    return n_list ? of[min(b, n_list - 1)] : -1;
   }
   __device__ __forceinline__ void look_up(int g, int entry) {
     base = g;
@@ -438,11 +451,10 @@ template <typename T, int D> __device__ __forceinline__ void wait_rows(RowSums<T
 }
 
 // A lane's query row to registers: head `head` of token t, -1 without one.
-template <typename T, int D> __device__ __forceinline__ void load_rows(const PagedArgs &a, RowSums<T, D> &r, int t, int head) {
+template <typename T, int D> __device__ __forceinline__ void load_query(const PagedArgs &a, RowSums<T, D> &r, int t, int head) {
   using S = typename T::S;
   const int hb = (threadIdx.x & 63) >> 5;
   const bool there = t >= 0;
-  r.row = there ? t * a.heads + head : -1;
   const S *q = static_cast<const S *>(a.q) + (there ? t * a.q_token + head * a.q_head : 0);
 #pragma unroll
   for (int kc = 0; kc < D / 16; ++kc) {
@@ -450,12 +462,22 @@ template <typename T, int D> __device__ __forceinline__ void load_rows(const Pag
     if (there) x = *reinterpret_cast<const s16x8 *>(q + kc * 16 + hb * 8);
     r.q[kc] = __builtin_bit_cast(typename Mma<T>::V8, x);
   }
+}
+
+// Nothing summed up.
+template <typename T, int D> __device__ __forceinline__ void clear_sums(RowSums<T, D> &r) {
 #pragma unroll
   for (int i = 0; i < D / 32; ++i)
 #pragma unroll
     for (int e = 0; e < 16; ++e) r.o[i][e] = 0.f;
   r.m = -INFINITY;
   r.l = 0.f;
+}
+
+template <typename T, int D> __device__ __forceinline__ void load_rows(const PagedArgs &a, RowSums<T, D> &r, int t, int head) {
+  r.row = t >= 0 ? t * a.heads + head : -1;
+  load_query(a, r, t, head);
+  clear_sums(r);
 }
 
 // Key numbers and what is added to them stay far from 2^31.

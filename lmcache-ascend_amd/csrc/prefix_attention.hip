@@ -391,8 +391,6 @@ struct Request {
   }
 };
 
-typedef const __attribute__((address_space(4))) int32_t *ScalarInts;
-
 // The least limit of a wave's rows, or (ALL) of the four waves'.
 template <bool ALL> __device__ __forceinline__ int least_limit(int limit, uint8_t *lds) {
 #pragma unroll

@@ -72,15 +72,21 @@ template <typename T, int D> struct TreeRows : RowSums<T, D> {
   }
 };
 
+// What a tile's start and end take, in blocks of keys: units of the line that
+// stand before the tile's first block, so that a piece with more tiles gets fewer
+// blocks.  (Measured in a piece, a tile more takes 5 to 10 us, a block 2.6.)
+// With 4: 32 requests of 16 tokens 125 us, trees of up to 77 45, of 64 over 16384
+// keys 412; with 0: 128, 52, 430; with 8: 124, 46, 421.
+constexpr int kStart = 4;
+
 // One request's part of the line.
 struct Span {
   int start, n_rows, context, end, blocks;  // rows of a KV head; keys; blocks of keys of a tile
   int64_t units;
 };
 
-template <int ROWS> __device__ __forceinline__ Span span_of(const TreeArgs &a, int r) {
+template <int ROWS> __device__ __forceinline__ Span span_of(const TreeArgs &a, int start, int stop, int seq) {
   Span s;
-  const int start = a.starts[r], stop = a.starts[r + 1], seq = a.seq_lens[r];
   s.start = max(0, start);
   s.n_rows = max(0, min(a.n_tokens, stop) - s.start) * a.group;
   s.end = max(0, min(seq, a.max_keys));
@@ -88,8 +94,16 @@ template <int ROWS> __device__ __forceinline__ Span span_of(const TreeArgs &a, i
   s.context = static_cast<int>(max(static_cast<int64_t>(seq) - stop + start, -(int64_t(1) << 29)));
   // (rows without keys are written too)
   s.blocks = max(1, (s.end + 63) / 64);
-  s.units = static_cast<int64_t>((s.n_rows + ROWS - 1) / ROWS) * s.blocks;
+  s.units = static_cast<int64_t>((s.n_rows + ROWS - 1) / ROWS) * (s.blocks + kStart);
   return s;
+}
+template <int ROWS> __device__ __forceinline__ Span span_of(const TreeArgs &a, int r) {
+  return span_of<ROWS>(a, a.starts[r], a.starts[r + 1], a.seq_lens[r]);
+}
+// The same for a request that the wave has in common.
+template <int ROWS> __device__ __forceinline__ Span span_of_all(const TreeArgs &a, int r) {
+  const ScalarInts starts = (ScalarInts)(a.starts + r), seq_lens = (ScalarInts)(a.seq_lens + r);
+  return span_of<ROWS>(a, starts[0], starts[1], seq_lens[0]);
 }
 
 // The request, and the unit of it, where a workgroup's piece begins.
@@ -145,34 +159,44 @@ template <int ROWS, int THREADS> __device__ __forceinline__ Begin find_piece(con
     found = {each, min(each, total - first), first - at, r, s};
   }
   __syncthreads();
-  if (first >= total) return {each, 0, 0, 0, {}};
-  Begin b = found;
-  b.r = __builtin_amdgcn_readfirstlane(b.r);
-  b.span.start = __builtin_amdgcn_readfirstlane(b.span.start);
-  b.span.n_rows = __builtin_amdgcn_readfirstlane(b.span.n_rows);
-  b.span.context = __builtin_amdgcn_readfirstlane(b.span.context);
-  b.span.end = __builtin_amdgcn_readfirstlane(b.span.end);
-  b.span.blocks = __builtin_amdgcn_readfirstlane(b.span.blocks);
+  // (the same in all lanes: to scalar registers)
+  auto all32 = [](int x) { return __builtin_amdgcn_readfirstlane(x); };
+  auto all64 = [&](int64_t x) {
+    const uint32_t lo = all32(static_cast<int>(x)), hi = all32(static_cast<int>(x >> 32));
+    return static_cast<int64_t>((static_cast<uint64_t>(hi) << 32) | lo);
+  };
+  Begin b;
+  b.each = all64(each);
+  b.left = b.unit = 0;
+  b.r = 0;
+  b.span = {0, 0, 0, 0, 1, 0};
+  if (all64(first) >= all64(total)) return b;
+  const Begin f = found;
+  b.left = all64(f.left);
+  b.unit = all64(f.unit);
+  b.r = all32(f.r);
+  b.span = {all32(f.span.start), all32(f.span.n_rows), all32(f.span.context), all32(f.span.end), all32(f.span.blocks), all64(f.span.units)};
   return b;
 }
 
 // The sums of a wave's rows, divided, to the output.
 template <typename T, int D> __device__ __forceinline__ void write_rows(const TreeArgs &a, const RowSums<T, D> &r) {
-  using S = typename T::S;
+  using M = Mma<T>;
+  using O4 = decltype(M::from(0.f)) __attribute__((ext_vector_type(4)));
   const int hb = (threadIdx.x & 63) >> 5;
   const float2 ls = both_halves(r.l);
   if (r.row < 0) return;
   const float l = ls.x + ls.y, inv = l == 0.f ? 0.f : 1.f / l;
   const uint32_t t = static_cast<uint32_t>(r.row) / static_cast<uint32_t>(a.heads), h = r.row - t * a.heads;
-  S *o = static_cast<S *>(a.o) + t * a.o_token + h * a.o_head;
+  typename T::S *o = static_cast<typename T::S *>(a.o) + t * a.o_token + h * a.o_head;
 #pragma unroll
   for (int x = 0; x < D / 32; ++x)
 #pragma unroll
     for (int b = 0; b < 4; ++b) {
-      Pack<S, 4> y;
-#pragma unroll
-      for (int e = 0; e < 4; ++e) y.v[e] = from_f32<T>(l == 0.f ? 0.f : r.o[x][4 * b + e] * inv);
-      *reinterpret_cast<Pack<S, 4> *>(o + 32 * x + 8 * b + 4 * hb) = y;
+      // (without a weight the sums are zeros)
+      const O4 y = {M::from(r.o[x][4 * b] * inv), M::from(r.o[x][4 * b + 1] * inv), M::from(r.o[x][4 * b + 2] * inv),
+                    M::from(r.o[x][4 * b + 3] * inv)};
+      *reinterpret_cast<O4 *>(o + 32 * x + 8 * b + 4 * hb) = y;
     }
   if (a.lse && hb == 0)
     a.lse[t * a.lse_token + h * a.lse_head] = l == 0.f ? -INFINITY : (r.m + log2f(l)) * 0.69314718056f;
@@ -201,57 +225,84 @@ template <int D, int RW, int KW> struct Shape {
   static constexpr int kWaves = RW * KW, kRows = 32 * RW;
   static constexpr int kSteps = 2 / KW;  // of a block
   static constexpr int kNV = kWaves == 8 ? 4 : 2, kNK = kNV + kSteps - 1;
-  static constexpr int kBytes = (kNK + kNV) * 64 * D * 2;
+  static constexpr int kRing = (kNK + kNV) * 64 * D * 2;
+  // Where waves of the same rows join: 32 dims of a row a lane pair, maximum and sum.
+  static constexpr int kJoin = KW == 2 ? RW * (16 * 64 * 4 + 64 * 8) : 0;
+  static constexpr int kBytes = kRing + kJoin;
   static constexpr int kPerSimd = D > 128 ? 1 : D == 64 && RW == 4 ? 3 : 2;  // waves of a SIMD
 };
 
 // The other waves are here too, all that was read from LDS has arrived.
 __device__ __forceinline__ void meet() { asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory"); }
 
-// The workgroup's rows over the keys of one piece, a block of 64 at a time, a
-// wave's 32 keys a step.  K runs a step ahead of V, and a step's softmax is
+// A workgroup's rows over keys, a block of 64 at a time, a wave's 32 keys a step.  K runs a step ahead of V, and a step's softmax is
 // spread over two products: beside the product with V of step i stand the
 // maximum of step i + 1 and the first half of its weights, beside the scores of
 // step i + 2 the other half.  So matrix and vector units have work at any time.
 // K and V have rings of blocks in LDS, loaded as soon as a place is free.
+template <typename T, int D, int RW, int KW> struct Ring {
+  using S = Shape<D, RW, KW>;
+  static constexpr int kPer = D / 32, NK = S::kNK, NV = S::kNV;
+  static constexpr uint32_t kBlock = 64 * Geometry<D>::kPitch, kGroup = 16 * Geometry<D>::kPitch;
+  // Blocks that are under way; K of the block before is still read where a
+  // block takes two steps.
+  static constexpr int kAheadK = NV, kAheadV = NV - 1;
+  // Of eight waves four load K and four V; of four each loads 16 keys of both.
+  static constexpr bool kSplit = S::kWaves == 8;
+  static_assert(S::kWaves == 4 || kSplit, "");
+
+  Keys keys;
+  uint32_t lds, own;              // the ring, this wave's first row of it
+  int wave;                       // of four
+  bool of_k, of_v;
+  uint32_t k_off[kPer], v_off[kPer];
+
+  __device__ __forceinline__ Ring(const PagedArgs &a, int h, uint32_t at)
+      : keys{a, nullptr, a.width, 0, 0, 0, 32, h * a.k_head, h * a.v_head, false}, lds(at) {
+    const int any = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    wave = any & 3;
+    of_k = !kSplit || any < 4;
+    of_v = !kSplit || !of_k;
+    own = lds + wave * kGroup;
+#pragma unroll
+    for (int i = 0; i < kPer; ++i) {
+      k_off[i] = row_offset<D, false>(i, a.k_token);
+      v_off[i] = row_offset<D, true>(i, a.v_token);
+      if constexpr (kSplit) k_off[i] = v_off[i] = of_k ? k_off[i] : v_off[i];
+    }
+  }
+  __device__ __forceinline__ int blocks() const { return (keys.k1 - keys.k0 + 63) / 64; }
+  __device__ __forceinline__ void load_k(int j, uint32_t slot) {
+    load_group<D, false, true>(keys, keys.place(4 * j + wave), keys.k0 + 64 * j + 16 * wave, k_off, own + slot * kBlock);
+  }
+  __device__ __forceinline__ void load_v(int j, uint32_t slot) {
+    load_group<D, true, true>(keys, keys.place(4 * j + wave), keys.k0 + 64 * j + 16 * wave, v_off, own + (NK + slot) * kBlock);
+  }
+  // The first blocks; every wave has read what was in the ring.
+  __device__ __forceinline__ void begin(int entry) {
+    const int n = blocks();
+    keys.look_up(0, entry);
+#pragma unroll
+    for (int j = 0; j < kAheadK; ++j) {
+      if (of_v && j > 0 && j - 1 < n) load_v(j - 1, j - 1);
+      if (of_k && j < n) load_k(j, j);
+    }
+  }
+  template <typename Last> __device__ __forceinline__ void run(const PagedArgs &a, TreeRows<T, D> &r, int least, const Last &last);
+};
+
+// The rows over all of the keys; last() is called in the last block, when the
+// ring loads nothing more.
 template <typename T, int D, int RW, int KW>
-__device__ __forceinline__ void attend_ring(const PagedArgs &a, TreeRows<T, D> &r, Keys &keys, int entry, int least, uint32_t lds) {
+template <typename Last>
+__device__ __forceinline__ void Ring<T, D, RW, KW>::run(const PagedArgs &a, TreeRows<T, D> &r, int least, const Last &last) {
   using M = Mma<T>;
   using V8 = typename M::V8;
-  using S = Shape<D, RW, KW>;
-  constexpr int kPer = D / 32, NK = S::kNK, NV = S::kNV, kSteps = S::kSteps, kPitch = Geometry<D>::kPitch;
-  constexpr int kScores = D / 16, kAhead = 4;
-  constexpr uint32_t kBlock = 64 * kPitch, kGroup = 16 * kPitch, kStep = 32 * kPitch;
-  // K of the block before is still read where a block takes two steps.
-  constexpr int kAheadK = NV, kAheadV = NV - 1;
-  // Of eight waves four load K and four V; of four each loads 16 keys of both.
-  constexpr bool kSplit = S::kWaves == 8;
-  static_assert(S::kWaves == 4 || kSplit, "");
-  const int any_wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), wave = any_wave & 3;
-  const bool of_k = !kSplit || any_wave < 4, of_v = !kSplit || !of_k;
-  const int half = KW == 2 ? 32 * (any_wave / RW) : 0;  // this wave's keys of a block
+  constexpr int kSteps = S::kSteps, kPitch = Geometry<D>::kPitch, kScores = D / 16, kAhead = 4;
+  constexpr uint32_t kStep = 32 * kPitch;
+  const int half = KW == 2 ? 32 * (__builtin_amdgcn_readfirstlane(threadIdx.x >> 6) / RW) : 0;  // this wave's keys of a block
   const float c = a.scale2;
-  const int k0 = keys.k0, k1 = keys.k1, n = (k1 - k0 + 63) / 64;
-  uint32_t k_off[kPer], v_off[kPer];
-#pragma unroll
-  for (int i = 0; i < kPer; ++i) {
-    k_off[i] = row_offset<D, false>(i, a.k_token);
-    v_off[i] = row_offset<D, true>(i, a.v_token);
-    if constexpr (kSplit) k_off[i] = v_off[i] = of_k ? k_off[i] : v_off[i];
-  }
-  const uint32_t own = lds + wave * kGroup;
-  auto load_k = [&](int j, uint32_t slot) {
-    load_group<D, false, true>(keys, keys.place(4 * j + wave), k0 + 64 * j + 16 * wave, k_off, own + slot * kBlock);
-  };
-  auto load_v = [&](int j, uint32_t slot) {
-    load_group<D, true, true>(keys, keys.place(4 * j + wave), k0 + 64 * j + 16 * wave, v_off, own + (NK + slot) * kBlock);
-  };
-  keys.look_up(0, entry);
-#pragma unroll
-  for (int j = 0; j < kAheadK; ++j) {
-    if (of_v && j > 0 && j - 1 < n) load_v(j - 1, j - 1);
-    if (of_k && j < n) load_k(j, j);
-  }
+  const int k0 = keys.k0, k1 = keys.k1, n = blocks();
   wait_rows<T, D>(r);
   const int lane = threadIdx.x & 63, row = lane & 31, hb = lane >> 5, al = lane & 15;
   const uint32_t vrow = 4 * hb + (al >> 2), vcol = 2 * ((lane >> 4) & 1) + ((al & 3) >> 1);
@@ -389,6 +440,7 @@ __device__ __forceinline__ void attend_ring(const PagedArgs &a, TreeRows<T, D> &
     else wait_loads<0>();
     meet();
     const int j0 = k0 + 64 * j;
+    if (j == n - 1) last();
     if (of_v && j + kAheadV < n) load_v(j + kAheadV, vs == 0 ? NV - 1 : vs - 1);
     if (of_k && j + kAheadK < n) load_k(j + kAheadK, kSteps == 1 ? ks : ks == 0 ? NK - 1 : ks - 1);
     const uint32_t k = lds + ks * kBlock;
@@ -408,77 +460,127 @@ __device__ __forceinline__ void attend_ring(const PagedArgs &a, TreeRows<T, D> &
   }
 }
 
-// The sums of two waves of the same rows, over different keys, to the first's.
+// The sums of two waves of the same rows, over different keys, to the first's,
+// 32 dims at a time.
 template <typename T, int D, int RW> __device__ __forceinline__ void join_halves(RowSums<T, D> &r, uint8_t *lds) {
-  constexpr int kQuads = D / 8;  // of sums of a lane
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  f32x4 *at = reinterpret_cast<f32x4 *>(lds) + (wave % RW) * ((kQuads + 1) * 64) + lane;
-  __syncthreads();  // (what LDS held has been read)
-  if (wave >= RW) {
+  f32x4 *at = reinterpret_cast<f32x4 *>(lds) + (wave % RW) * 256 + lane;
+  float2 *ml = reinterpret_cast<float2 *>(lds + RW * 4096) + (wave % RW) * 64 + lane;
+  float f = 0.f, g = 0.f;
 #pragma unroll
-    for (int t = 0; t < D / 32; ++t)
+  for (int t = 0; t < D / 32; ++t) {
+    if (wave >= RW) {
+      if (t == 0) *ml = make_float2(r.m, r.l);
 #pragma unroll
-      for (int b = 0; b < 4; ++b) at[(t * 4 + b) * 64] = f32x4{r.o[t][4 * b], r.o[t][4 * b + 1], r.o[t][4 * b + 2], r.o[t][4 * b + 3]};
-    at[kQuads * 64] = f32x4{r.m, r.l, 0.f, 0.f};
-  }
-  __syncthreads();
-  if (wave >= RW) return;
-  const f32x4 ml = at[kQuads * 64];
-  const float top = fmaxf(r.m, ml[0]), base = top == -INFINITY ? 0.f : top;
-  const float f = __builtin_amdgcn_exp2f(r.m - base), g = __builtin_amdgcn_exp2f(ml[0] - base);
-  r.m = top;
-  r.l = r.l * f + ml[1] * g;
-#pragma unroll
-  for (int t = 0; t < D / 32; ++t)
-#pragma unroll
-    for (int b = 0; b < 4; ++b) {
-      const f32x4 x = at[(t * 4 + b) * 64];
-#pragma unroll
-      for (int e = 0; e < 4; ++e) r.o[t][4 * b + e] = r.o[t][4 * b + e] * f + x[e] * g;
+      for (int b = 0; b < 4; ++b) at[b * 64] = f32x4{r.o[t][4 * b], r.o[t][4 * b + 1], r.o[t][4 * b + 2], r.o[t][4 * b + 3]};
     }
+    meet();
+    if (wave < RW) {
+      if (t == 0) {
+        const float2 x = *ml;
+        const float top = fmaxf(r.m, x.x), base = top == -INFINITY ? 0.f : top;
+        f = __builtin_amdgcn_exp2f(r.m - base);
+        g = __builtin_amdgcn_exp2f(x.x - base);
+        r.m = top;
+        r.l = r.l * f + x.y * g;
+      }
+#pragma unroll
+      for (int b = 0; b < 4; ++b) {
+        const f32x4 x = at[b * 64];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) r.o[t][4 * b + e] = r.o[t][4 * b + e] * f + x[e] * g;
+      }
+    }
+    meet();
+  }
 }
 
 template <typename T, int D, int RW, int KW>
 __global__ void __launch_bounds__(64 * RW * KW, (Shape<D, RW, KW>::kPerSimd)) attend_tree(TreeArgs a) {
   using S = Shape<D, RW, KW>;
-  extern __shared__ uint8_t lds[];
+  extern __shared__ __align__(128) uint8_t lds[];
   const uint32_t at = static_cast<uint32_t>(reinterpret_cast<uintptr_t>((__attribute__((address_space(3))) uint8_t *)lds));
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6) % RW, n = threadIdx.x & 31;
-  const int h = blockIdx.x % a.kv_heads, piece = blockIdx.x / a.kv_heads;
+  const int piece = blockIdx.x / a.kv_heads, h = blockIdx.x % a.kv_heads, me = piece * a.kv_heads + h;
   const Begin begin = find_piece<S::kRows, 64 * S::kWaves>(a, piece);
   const int64_t each = begin.each;
-  int64_t left = begin.left, unit = begin.unit;
-  Span s = begin.span;
   TreeArgs::Cut cut = {-1, 0, 0};
-  for (int q = begin.r; left > 0;) {
-    while (left > 0 && unit < s.units) {
-      const int tile = static_cast<int>(unit / s.blocks), b0 = static_cast<int>(unit - static_cast<int64_t>(tile) * s.blocks);
-      const int blocks = static_cast<int>(min(left, static_cast<int64_t>(s.blocks - b0)));
-      const int x = tile * S::kRows + wave * 32 + n;
-      const int t = x < s.n_rows ? s.start + x / a.group : -1;
-      TreeRows<T, D> r;
-      r.context = s.context;
-      Keys keys{a, a.table + q * a.table_stride, a.width, b0 * 64, min(s.end, (b0 + blocks) * 64), b0 * 64, 32, h * a.k_head,
-                h * a.v_head, a.block_size % 16 != 0};
-      const int entry = keys.entry(0);
-      load_rows<T, D>(a, r, t, h * a.group + (t < 0 ? 0 : x % a.group));
-      __syncthreads();  // the last tile's keys have been read
-      if (keys.k0 < keys.k1) attend_ring<T, D, RW, KW>(a, r, keys, entry, s.context, at);
-      if constexpr (KW == 2) join_halves<T, D, RW>(r, lds);
-      const bool ends = b0 + blocks < s.blocks && b0 == 0;
-      if (KW == 1 || threadIdx.x < 64 * RW) {
-        if (blocks == s.blocks) write_rows<T, D>(a, r);
-        else write_part<T, D>(a, r, (static_cast<int64_t>(blockIdx.x) * 2 + ends) * S::kRows + wave * 32);
-      }
-      if (blocks < s.blocks && ends) cut = {q, tile, static_cast<int>((s.blocks - blocks + each - 1) / each)};
-      left -= blocks;
-      unit += blocks;
+  // The part of a tile that is worked on: `blocks` of its blocks from b0 on.
+  Span s = begin.span;
+  int q = begin.r, tile = 0, b0 = 0, blocks = 0;
+  int64_t left = begin.left;
+  if (left > 0) {
+    tile = static_cast<int>(begin.unit / (s.blocks + kStart));
+    b0 = static_cast<int>(begin.unit - static_cast<int64_t>(tile) * (s.blocks + kStart)) - kStart;
+    if (b0 < 0) {
+      left += b0;
+      b0 = 0;
     }
-    if (left <= 0) break;
-    s = span_of<S::kRows>(a, ++q);
-    unit = 0;
+    blocks = static_cast<int>(max(static_cast<int64_t>(0), min(left, static_cast<int64_t>(s.blocks - b0))));
+    left -= blocks;
   }
-  if (threadIdx.x == 0) a.cuts[blockIdx.x] = cut;
+  const bool odd_blocks = a.block_size % 16 != 0;
+  Ring<T, D, RW, KW> ring(a, h, at);
+  TreeRows<T, D> r;
+  // The token of this lane's row of a tile, or -1, and its head.
+  auto token = [&](const Span &x, int i) { return i < x.n_rows ? x.start + i / a.group : -1; };
+  auto head = [&](const Span &x, int i) { return h * a.group + (i < x.n_rows ? i % a.group : 0); };
+  auto turn_to = [&](const Span &x, int request, int from, int count) {
+    ring.keys.turn_to(a.table + request * a.table_stride, from * 64, min(x.end, (from + count) * 64), odd_blocks);
+  };
+  if (blocks > 0) {
+    const int i = tile * S::kRows + wave * 32 + n;
+    turn_to(s, q, b0, blocks);
+    const int entry = ring.keys.entry(0);
+    load_rows<T, D>(a, r, token(s, i), head(s, i));
+    ring.begin(entry);
+  }
+  while (blocks > 0) {
+    r.context = s.context;
+    // The tile behind this one, of this request or the next with rows.
+    Span next = s;
+    int next_q = q, next_tile = tile + 1, next_blocks = 0, entry = 0;
+    left -= kStart;
+    if (left > 0) {
+      if (next_tile * S::kRows >= s.n_rows) {
+        next_tile = 0;
+        next.units = 0;
+        while (next.units == 0 && next_q + 1 < a.n_requests) next = span_of_all<S::kRows>(a, ++next_q);
+      }
+      if (next.units > 0) next_blocks = static_cast<int>(min(left, static_cast<int64_t>(next.blocks)));
+      left -= next_blocks;
+    }
+    const int32_t *list = a.table + next_q * a.table_stride;
+    const int next_end = min(next.end, next_blocks * 64);
+    if (ring.keys.k0 < ring.keys.k1)
+      ring.run(a, r, s.context, [&] {
+        if (next_blocks > 0) entry = ring.keys.entry_of(list, (threadIdx.x & 63) * 16, 0, next_end);
+      });
+    else if (next_blocks > 0) entry = ring.keys.entry_of(list, (threadIdx.x & 63) * 16, 0, next_end);
+    // What follows is under way while this one's sums are written.
+    meet();
+    const int i = next_tile * S::kRows + wave * 32 + n, next_t = token(next, i), next_h = head(next, i);
+    if (next_blocks > 0) {
+      turn_to(next, next_q, 0, next_blocks);
+      ring.begin(entry);
+      load_query<T, D>(a, r, next_t, next_h);
+    }
+    if constexpr (KW == 2) join_halves<T, D, RW>(r, lds + S::kRing);
+    const bool ends = b0 + blocks < s.blocks && b0 == 0;
+    if (KW == 1 || threadIdx.x < 64 * RW) {
+      if (blocks == s.blocks) write_rows<T, D>(a, r);
+      else write_part<T, D>(a, r, (static_cast<int64_t>(me) * 2 + ends) * S::kRows + wave * 32);
+    }
+    if (ends) cut = {q, tile, static_cast<int>((s.blocks - blocks + each - 1) / each)};
+    r.row = next_t >= 0 ? next_t * a.heads + next_h : -1;
+    clear_sums(r);
+    s = next;
+    q = next_q;
+    tile = next_tile;
+    b0 = 0;
+    blocks = next_blocks;
+  }
+  if (threadIdx.x == 0) a.cuts[me] = cut;
 }
 
 // Joins the pieces of the tiles that are cut: the k-th of a KV head to the
@@ -488,7 +590,8 @@ __global__ void __launch_bounds__(64 * RW * KW, (Shape<D, RW, KW>::kPerSimd)) at
 // quarter of the pieces each.
 template <typename T, int D, int ROWS> __global__ void __launch_bounds__(256) join_tree(TreeArgs a) {
   constexpr int kQuads = D / 4, kStep = 64 / kQuads, kFew = 8;
-  using S = typename T::S;
+  using M = Mma<T>;
+  using O4 = decltype(M::from(0.f)) __attribute__((ext_vector_type(4)));
   __shared__ f32x4 sums[4][64];
   __shared__ float2 weights[4][kStep];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -544,10 +647,8 @@ template <typename T, int D, int ROWS> __global__ void __launch_bounds__(256) jo
   auto write = [&](int i) {
     const float inv = l == 0.f ? 0.f : 1.f / l, base = m == -INFINITY ? 0.f : m;
     const int x = cut.tile * ROWS + i, t = s.start + x / a.group, head = h * a.group + x % a.group;
-    Pack<S, 4> y;
-#pragma unroll
-    for (int e = 0; e < 4; ++e) y.v[e] = from_f32<T>(o[e] * inv);
-    *reinterpret_cast<Pack<S, 4> *>(static_cast<S *>(a.o) + t * a.o_token + head * a.o_head + d) = y;
+    const O4 y = {M::from(o[0] * inv), M::from(o[1] * inv), M::from(o[2] * inv), M::from(o[3] * inv)};
+    *reinterpret_cast<O4 *>(static_cast<typename T::S *>(a.o) + t * a.o_token + head * a.o_head + d) = y;
     if (a.lse && d == 0) a.lse[t * a.lse_token + head * a.lse_head] = l == 0.f ? -INFINITY : (base + log2f(l)) * 0.69314718056f;
   };
   if (parts <= kFew) {
