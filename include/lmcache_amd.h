@@ -617,9 +617,10 @@ int lmc_build_draft_tree(const lmc_tensor *parents, const lmc_tensor *query_star
                          const lmc_tensor *tree_mask, const lmc_tensor *positions, void *stream);
 
 /* Attention of drafted tokens over one layer's caches, which hold their rows
- * already.  Arguments, limits, workspace and what may overlap as for
- * lmc_shared_prefix_attention (without its shared prefix); tree_mask is [T, W]
- * int64 (W up to 2^20).  A request's q tokens see its first seq_lens[r] - q keys,
+ * already.  Arguments, limits and workspace as for
+ * lmc_shared_prefix_attention (without its shared prefix); output may be query
+ * itself or lie beside it as columns of one buffer, lse lies apart from query.
+ * tree_mask is [T, W] int64 (W up to 2^20).  A request's q tokens see its first seq_lens[r] - q keys,
  * and of its last q key j behind those where bit j % 64 of word j / 64 of the
  * token's row of tree_mask is set.  Key n lies in block
  * block_table[r][n / block_size]. */

@@ -37,6 +37,7 @@ PageGeom page_geom(const lmc_tensor *caches, int n, int fmt, bool two_major, con
     const PagedKv kv = paged_kv(caches, n, fmt, two_major, op);
     const int64_t run = kv.dim * dtype_size(kv.dtype);
     const bool merged = fmt == LMC_FMT_MERGED_KV;
+    expect(k_and_v_apart(kv), "rows of the K and V caches overlap");
     g.plane[0] = {0, kv.k_page, kv.k_token, kv.k_head, kv.heads, run, 0};
     g.plane[1] = {merged ? kv.v - kv.k : 0, kv.v_page, kv.v_token, kv.v_head, kv.heads, run, merged ? 0 : 1};
     g.n_planes = 2;
@@ -53,6 +54,7 @@ PageGeom page_geom(const lmc_tensor *caches, int n, int fmt, bool two_major, con
       expect(t.device == caches[0].device && t.sizes[0] == caches[0].sizes[0] && t.sizes[1] == caches[0].sizes[1],
              "a layer's caches differ in pages, block or device");
       for (int d = 0; d < t.ndim; ++d) expect(t.strides[d] >= 0, "negative strides unsupported");
+      for (int k = 0; k < i; ++k) expect(!may_share(t, caches[k]), "a layer's caches overlap");
       const int64_t es = elem_size(t);
       expect(t.sizes[t.ndim - 1] <= 1 || t.strides[t.ndim - 1] == 1, "a cache row's head dims must be adjacent");
       expect(numel(t) > 0 || t.sizes[0] == 0, "the paged caches hold no rows");
@@ -594,8 +596,9 @@ extern "C" int lmc_release_pages(const lmc_tensor *block_table, const lmc_tensor
     for (const lmc_tensor *out : outs) {
       for (const lmc_tensor *in : {block_table, held_lens, keep_lens, free_cursor})
         expect(!extents_meet(*out, *in), "an output overlaps what it is computed from");
-      for (const lmc_tensor *other : outs) expect(other == out || !extents_meet(*out, *other), "two outputs overlap");
     }
+    for (int i = 0; i < 4; ++i)
+      for (int k = 0; k < i; ++k) expect(!extents_meet(*outs[i], *outs[k]), "two outputs overlap");
     ReleaseArgs a;
     std::memset(&a, 0, sizeof(a));
     a.table = static_cast<const int32_t *>(bt.data);

@@ -180,7 +180,7 @@ template <int ROWS, int THREADS> __device__ __forceinline__ Begin find_piece(con
 }
 
 // The sums of a wave's rows, divided, to the output.
-template <typename T, int D> __device__ __forceinline__ void write_rows(const TreeArgs &a, const RowSums<T, D> &r) {
+template <typename T, int D> __device__ __forceinline__ void write_rows(const TreeArgs &a, RowSums<T, D> &r) {
   using M = Mma<T>;
   using O4 = decltype(M::from(0.f)) __attribute__((ext_vector_type(4)));
   const int hb = (threadIdx.x & 63) >> 5;
@@ -188,12 +188,17 @@ template <typename T, int D> __device__ __forceinline__ void write_rows(const Tr
   if (r.row < 0) return;
   const float l = ls.x + ls.y, inv = l == 0.f ? 0.f : 1.f / l;
   const uint32_t t = static_cast<uint32_t>(r.row) / static_cast<uint32_t>(a.heads), h = r.row - t * a.heads;
+  if (l == 0.f) {  // (a key of weight zero may have left its infinities)
+#pragma unroll
+    for (int x = 0; x < D / 32; ++x)
+#pragma unroll
+      for (int i = 0; i < 16; ++i) r.o[x][i] = 0.f;
+  }
   typename T::S *o = static_cast<typename T::S *>(a.o) + t * a.o_token + h * a.o_head;
 #pragma unroll
   for (int x = 0; x < D / 32; ++x)
 #pragma unroll
     for (int b = 0; b < 4; ++b) {
-      // (without a weight the sums are zeros)
       const O4 y = {M::from(r.o[x][4 * b] * inv), M::from(r.o[x][4 * b + 1] * inv), M::from(r.o[x][4 * b + 2] * inv),
                     M::from(r.o[x][4 * b + 3] * inv)};
       *reinterpret_cast<O4 *>(o + 32 * x + 8 * b + 4 * hb) = y;
@@ -690,7 +695,8 @@ template <typename T, int D, int ROWS> __global__ void __launch_bounds__(256) jo
 template <typename T, int D, int RW, int KW> void launch(const TreeArgs &a, const TreePlan &p, hipStream_t s) {
   using S = Shape<D, RW, KW>;
   const void *fn = reinterpret_cast<const void *>(attend_tree<T, D, RW, KW>);
-  hip_check(hipFuncSetAttribute(fn, hipFuncAttributeMaxDynamicSharedMemorySize, S::kBytes), "attend_tree shared memory");
+  if (S::kBytes > 64 * 1024)
+    hip_check(hipFuncSetAttribute(fn, hipFuncAttributeMaxDynamicSharedMemorySize, S::kBytes), "attend_tree shared memory");
   hipLaunchKernelGGL((attend_tree<T, D, RW, KW>), dim3(static_cast<uint32_t>(p.groups)), dim3(64 * S::kWaves), S::kBytes, s, a);
   hip_check(hipGetLastError(), "attend_tree launch");
   if (p.pieces == 1) return;  // nothing is cut
@@ -752,6 +758,15 @@ extern "C" int lmc_tree_attention(const lmc_tensor *query, const lmc_tensor *vll
       *workspace_bytes = bytes;
       return;
     }
+    // A tile that is not cut is written while others' queries are read.
+    auto same = [](const lmc_tensor &x, const lmc_tensor &y) {
+      if (x.data != y.data) return false;
+      for (int i = 0; i < 3; ++i)
+        if (x.sizes[i] > 1 && x.strides[i] != y.strides[i]) return false;
+      return true;
+    };
+    expect(same(*output, *query) || !may_share(*output, *query), "output overlaps query and is not the same tensor");
+    expect(!lse || !extents_meet(*lse, *query), "lse overlaps query");
     check_outputs(query, output, lse, workspace, bytes, kv.device, vllm_kv_caches, n_caches,
                   {query_start_loc, seq_lens, block_table, tree_mask});
     a.mask = static_cast<const int64_t *>(tm.data);

@@ -843,7 +843,8 @@ def tree_attention(
     """Attention of drafted tokens, under their tree's mask, over one layer's
     paged caches, which hold the drafted tokens' rows already.
 
-    Arguments as shared_prefix_attention's; tree_mask ([T, W] int64) is
+    Arguments as shared_prefix_attention's (output may be query itself, or lie
+    beside it as columns of one buffer); tree_mask ([T, W] int64) is
     build_draft_tree's, or any other: a request's q tokens see its first
     seq_lens[r] - q keys, and of its last q key j behind those where bit j %
     64 of word j // 64 of the token's row is set (j < 64 * W; bits from q on
@@ -907,6 +908,8 @@ def prepare_kv_pages(layers, kvcache_format_raw: int = 2, vllm_two_major: bool =
             if t.data_ptr() % 16 != s.data_ptr() % 16:
                 raise ValueError("layers' caches differ in their alignment to 16 bytes")
     _gpu_of(first[0], "the first cache")
+    if len({t.data_ptr() for caches in layers for t in caches}) < len(layers) * len(first):
+        raise ValueError("a cache is given twice")
     st = KVPagesState()
     st.layers = tuple(layers)
     st.caches = [t.view(torch.uint8) if t.dtype not in _DTYPES and t.element_size() == 1 else t for t in first]

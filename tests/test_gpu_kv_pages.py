@@ -110,6 +110,29 @@ def test_pairs_with_a_stride_and_none(ops):
     ops.copy_kv_pages(c.state, wide[:0, 1:3])
 
 
+def test_states_that_are_refused(ops):
+    k, v = (torch.zeros((4, 16, 2, 64), dtype=torch.bfloat16, device=DEV) for _ in range(2))
+    with pytest.raises(ValueError, match="no layers"):
+        ops.prepare_kv_pages([])
+    with pytest.raises(ValueError, match="given twice"):
+        ops.prepare_kv_pages([(k, v), (k, v)])
+    with pytest.raises(ValueError, match="number of their caches"):
+        ops.prepare_kv_pages([(k, v), (k.clone(),)])
+    with pytest.raises(ValueError, match="shape, dtype"):
+        ops.prepare_kv_pages([(k, v), (k.half(), v.half())])
+    with pytest.raises(ValueError, match="shape, dtype"):
+        ops.prepare_kv_pages([(k, v), (k.transpose(1, 2).contiguous().transpose(1, 2), v.clone())])
+    with pytest.raises(ValueError, match="overlap"):
+        ops.prepare_kv_pages([(k[:3], k[1:])])
+    wide = torch.zeros((4, 16, 2, 64 + 4), dtype=torch.bfloat16, device=DEV)
+    with pytest.raises(ValueError, match="alignment"):
+        ops.prepare_kv_pages([(wide[..., :64], wide.clone()[..., :64]), (wide.clone()[..., 4:], wide.clone()[..., :64])])
+    with pytest.raises(ValueError, match="GPU"):
+        ops.prepare_kv_pages([(k.cpu(), v.cpu())])
+    with pytest.raises(RuntimeError, match="neither a Tensor"):
+        ops.prepare_kv_pages([[k, v]])
+
+
 def test_many_pairs(ops):
     c = Caches(ops, "two_major", 5, 900, 16, 2, 32)
     order = torch.randperm(900, generator=torch.Generator().manual_seed(1))

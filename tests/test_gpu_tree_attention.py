@@ -244,6 +244,38 @@ def test_scores_of_minus_infinity(ops):
     assert (out[2] == 0).all() and (lse[2] == -INF).all()
 
 
+def test_no_weight_beside_infinite_values(ops):
+    """Scores of -infinity leave zeros, whatever the values that go with them."""
+    c = _case(25, [1, 3], [20, 4], 16, 1, 1, 64)
+    c["q"].fill_(1.0)
+    c["k"].nan_to_num_(0.5)
+    c["v"].nan_to_num_(0.25)
+    for j in range(7):
+        c["k"][int(c["table"][1, 0]), j] = -INF
+    c["v"][int(c["table"][1, 0]), 5] = INF
+    c["mask"][1:] = [1, 3, 7]
+    caches, kw = _device_caches(c)
+    out, lse = c["out"].to(DEV), c["lse"].to(DEV)
+    _call(ops, c, caches, kw, c["q"].to(DEV), out, lse)
+    torch.cuda.synchronize()
+    assert (out[1:] == 0).all() and (lse[1:] == -INF).all()
+
+
+def test_two_calls_at_once(ops):
+    """Calls on two streams work in scratch of their own."""
+    cases = [_case(26 + i, [40, 9], [700, 1500], 16, 8, 2, 64) for i in range(2)]
+    args = [(_device_caches(c)[0], c["q"].to(DEV), c["out"].to(DEV), c["lse"].to(DEV)) for c in cases]
+    streams = [torch.cuda.Stream() for _ in cases]
+    torch.cuda.synchronize()
+    for _ in range(3):
+        for c, (caches, q, out, lse), s in zip(cases, args, streams):
+            with torch.cuda.stream(s):
+                _call(ops, c, caches, {}, q, out, lse)
+    torch.cuda.synchronize()
+    for c, (_, _, out, lse) in zip(cases, args):
+        _hold(out, lse, _want(c))
+
+
 def test_large_scores(ops):
     _check(ops, _case(18, [9, 70], [200, 64], 16, 8, 2, 128, spread=20.0))
 
