@@ -6,7 +6,15 @@
 //   release_pages:  pages ceil(keep / BS) <= j < ceil(held / BS) of each request lose a holder
 //
 // The first two in every layer l and plane p (K, V; the planes of an MLA
-// layer), through a table of the layers' addresses.
+// layer), through a table of the layers' addresses.  Both are copies, at the
+// rate of the memory system: 256 pages of 128 tokens in 8 layers (8 heads of 128
+// bf16 dims) 330 us, 5.7 TB/s of the bytes that differ; half of 8 contexts of 8000
+// tokens 264 us, 4.4 TB/s; the accepted rows of 64 requests in 32 layers 9.1 us.
+//
+// release_pages is latency, three launches: holders taken off with atomics, pages
+// without one counted for each 1024, and those written to the list in ascending
+// order, which does not depend on the order of the atomics.  64 requests' drafts
+// among 20000 pages 8.8 us, 256 requests that end among 300000 12 us.
 #include "serving.h"
 
 #include <type_traits>
@@ -120,7 +128,9 @@ struct CopyArgs {
   uint32_t groups;                // workgroups of a page
 };
 
-// A vector a thread: what is under way together is other waves'.
+// A vector a thread: what is under way together is other waves' (256 pages of 256
+// KiB in 16 planes: 330 us; two vectors 368, four 400, eight 590).  Stores are
+// written through: streaming ones take 344 us, 7.2 instead of 5.5 with 8 pages.
 template <int VEC> __global__ void __launch_bounds__(256) copy_pages(CopyArgs a) {
   using V = typename VecOf<VEC>::T;
   const uint32_t pair = blockIdx.x / a.groups, x = (blockIdx.x - pair * a.groups) * 256 + threadIdx.x;
@@ -169,7 +179,9 @@ struct MoveArgs {
   int lanes;                      // threads of a row: a power of two, kLeastLanes to 256
 };
 
-constexpr int kRowsOnce = 4, kRowsMore = 8;  // rows of a thread in a step: with one step, with more
+// Rows of a thread in a step, with one step and with more: half of 8 contexts
+// takes 267 us with 8, 304 with 4.
+constexpr int kRowsOnce = 4, kRowsMore = 8;
 constexpr int kBatch = 256;       // rows whose places are looked up together
 constexpr int kLeastLanes = 8;    // of a row
 // A step's rows are looked up: a batch holds whole steps.
@@ -533,6 +545,9 @@ extern "C" int lmc_compact_kv(const lmc_tensor *layer_ptrs, const lmc_tensor *vl
     const int planes = g.n_planes == 2 && k.page == v.page && k.token == v.token && k.head == v.head && k.pieces == v.pieces &&
                                k.vectors == v.vectors ? 2 : 1;
     const int64_t items = R * layers * (g.n_planes / planes);
+    // Slices of a row for 1024 workgroups or more, but no narrower than that takes
+    // (128 bytes at least: half of 8 contexts of 8000 tokens 276 us so; 64 requests
+    // of 6 rows 10.6 us with whole rows, 13.7 with slices for 4096 workgroups).
     a.lanes = kLeastLanes;
     while (a.lanes < 256 && a.lanes < most && items * ((most + 2 * a.lanes - 1) / (2 * a.lanes)) >= 1024) a.lanes *= 2;
     const int64_t slices = (most + a.lanes - 1) / a.lanes, groups = layers * (g.n_planes / planes);

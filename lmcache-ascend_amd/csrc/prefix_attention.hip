@@ -37,7 +37,7 @@
 //
 // Registers at 128 dims: 256 for wide tiles (2 of them spilled, 12 bytes of
 // scratch, two waves a SIMD), 195 for narrow ones; at 64 dims 193 and 131; 192
-// and 256 dims take accumulation registers too, a wave a SIMD.  48 to 60 scalar
+// and 256 dims take accumulation registers too, a wave a SIMD.  33 to 43 scalar
 // registers are kept in vector registers.
 #include "paged_attention.h"
 
