@@ -76,13 +76,17 @@ TreePlan make_plan(int64_t T, int64_t R, int64_t kv_heads, int64_t group, int64_
 // Rows that see the context and the drafted tokens of their mask.
 template <typename T, int D> struct TreeRows : RowSums<T, D> {
   int context;  // keys before the drafted tokens
+  uint64_t word0;  // of the mask (loaded beside the query, not when it is needed)
+  __device__ __forceinline__ void load_word(const TreeArgs &a, int t) {
+    word0 = t >= 0 && a.words > 0 ? static_cast<uint64_t>(a.mask[t * a.mask_token]) : 0;
+  }
   // Bit i: the row sees key j0 + i.
   __device__ __forceinline__ uint64_t visible(const PagedArgs &p, int j0) const {
     const TreeArgs &a = static_cast<const TreeArgs &>(p);
     const int d = j0 - context;
     if (d <= -64 || this->row < 0) return ~uint64_t(0);
     const int64_t *w = a.mask + static_cast<uint32_t>(this->row) / static_cast<uint32_t>(a.heads) * a.mask_token;
-    auto word = [&](int i) { return i < a.words ? static_cast<uint64_t>(w[i]) : 0; };
+    auto word = [&](int i) { return i == 0 ? word0 : i < a.words ? static_cast<uint64_t>(w[i]) : 0; };
     if (d < 0) return (~uint64_t(0) >> (64 + d)) | (word(0) << -d);
     const int i = d >> 6, s = d & 63;
     return s ? (word(i) >> s) | (word(i + 1) << (64 - s)) : word(i);
@@ -251,6 +255,7 @@ template <int D, int RW, int KW> struct Shape {
   // Where waves of the same rows join: 32 dims of a row a lane pair, maximum and sum.
   static constexpr int kJoin = KW == 2 ? RW * (16 * 64 * 4 + 64 * 8) : 0;
   static constexpr int kBytes = kRing + kJoin;
+  static_assert(KW == 1 || RW * 64 * 4 * D / 2 <= kRing, "all sums in the ring");
   static constexpr int kPerSimd = D > 128 ? 1 : D == 64 && RW == 4 ? 3 : 2;  // waves of a SIMD
 };
 
@@ -262,6 +267,28 @@ __device__ __forceinline__ void meet() { asm volatile("s_waitcnt lgkmcnt(0)\n\ts
 // maximum of step i + 1 and the first half of its weights, beside the scores of
 // step i + 2 the other half.  So matrix and vector units have work at any time.
 // K and V have rings of blocks in LDS, loaded as soon as a place is free.
+// Whether a block of V holds an infinity or a NaN: each wave looks at a part of
+// it and says so at `odd`, which no wave writes again before all have read it.
+template <typename T, int D, int WAVES> __device__ __forceinline__ bool any_odd(uint32_t v, uint32_t *odd) {
+  typedef unsigned short u16x8 __attribute__((ext_vector_type(8)));
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  u16x8 top = {0, 0, 0, 0, 0, 0, 0, 0};
+  // (1024 bytes a turn of the wave, of 128 D)
+  for (int i = wave; i < D / 8; i += WAVES) {
+    const s16x8 x = *reinterpret_cast<const LdsS8 *>(v + i * 1024 + (threadIdx.x & 63) * 16);
+    top = __builtin_elementwise_max(top, __builtin_bit_cast(u16x8, x) & static_cast<unsigned short>(0x7fff));
+  }
+  bool bad = false;
+#pragma unroll
+  for (int e = 0; e < 8; ++e) bad |= top[e] >= Mma<T>::kInf;
+  odd[wave] = __any(bad);
+  meet();
+  uint32_t all = 0;
+#pragma unroll
+  for (int w = 0; w < WAVES; ++w) all |= odd[w];
+  return __builtin_amdgcn_readfirstlane(all) != 0;
+}
+
 template <typename T, int D, int RW, int KW> struct Ring {
   using S = Shape<D, RW, KW>;
   static constexpr int kPer = D / 32, NK = S::kNK, NV = S::kNV;
@@ -278,9 +305,10 @@ template <typename T, int D, int RW, int KW> struct Ring {
   int wave;                       // of four
   bool of_k, of_v;
   uint32_t k_off[kPer], v_off[kPer];
+  uint32_t *odd;                  // two words for each wave
 
-  __device__ __forceinline__ Ring(const PagedArgs &a, int h, uint32_t at)
-      : keys{a, nullptr, a.width, 0, 0, 0, 32, h * a.k_head, h * a.v_head, false}, lds(at) {
+  __device__ __forceinline__ Ring(const PagedArgs &a, int h, uint32_t at, uint32_t *odd)
+      : keys{a, nullptr, a.width, 0, 0, 0, 32, h * a.k_head, h * a.v_head, false}, lds(at), odd(odd) {
     const int any = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     wave = any & 3;
     of_k = !kSplit || any < 4;
@@ -469,7 +497,7 @@ __device__ __forceinline__ void Ring<T, D, RW, KW>::run(const PagedArgs &a, Tree
     ks = ks + 1 == NK ? 0 : ks + 1;
     const uint32_t k_next = lds + ks * kBlock, v = lds + (NK + vs) * kBlock;
     vs = vs + 1 == NV ? 0 : vs + 1;
-    if (cut_at(j0) && has_odd<T, D, 64>(v)) {
+    if (cut_at(j0) && any_odd<T, D, S::kWaves>(v, odd + (j & 1) * S::kWaves)) {
       const uint64_t there = keys.template seen<64>(j0) & (KW == 2 ? uint64_t(0xffffffff) << half : ~uint64_t(0));
       take_odd_out<T, D, 64, true>(r, v, there & r.visible(a, j0));
     }
@@ -482,37 +510,53 @@ __device__ __forceinline__ void Ring<T, D, RW, KW>::run(const PagedArgs &a, Tree
   }
 }
 
-// The sums of two waves of the same rows, over different keys, to the first's,
-// 32 dims at a time.
-template <typename T, int D, int RW> __device__ __forceinline__ void join_halves(RowSums<T, D> &r, uint8_t *lds) {
+// The sums of two waves of the same rows, over different keys, to the first's:
+// 32 dims at a time beside the ring, or all of them in it where nothing is loaded
+// there any more (the last tile).
+template <typename T, int D, int RW> __device__ __forceinline__ void join_halves(RowSums<T, D> &r, uint8_t *ring, uint8_t *beside, bool last) {
+  // (192 and 256 dims have no registers for both ways: 1.3 times as long)
+  const bool once = D <= 128 && last;
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  f32x4 *at = reinterpret_cast<f32x4 *>(lds) + (wave % RW) * 256 + lane;
-  float2 *ml = reinterpret_cast<float2 *>(lds + RW * 4096) + (wave % RW) * 64 + lane;
+  f32x4 *at = reinterpret_cast<f32x4 *>(once ? ring : beside) + (wave % RW) * 256 + lane;
+  float2 *ml = reinterpret_cast<float2 *>(beside + RW * 4096) + (wave % RW) * 64 + lane;
+  const int step = once ? RW * 256 : 0;
   float f = 0.f, g = 0.f;
+  auto give = [&](int t) {
+    if (t == 0) *ml = make_float2(r.m, r.l);
+#pragma unroll
+    for (int b = 0; b < 4; ++b) at[t * step + b * 64] = f32x4{r.o[t][4 * b], r.o[t][4 * b + 1], r.o[t][4 * b + 2], r.o[t][4 * b + 3]};
+  };
+  auto take = [&](int t) {
+    if (t == 0) {
+      const float2 x = *ml;
+      const float top = fmaxf(r.m, x.x), base = top == -INFINITY ? 0.f : top;
+      f = __builtin_amdgcn_exp2f(r.m - base);
+      g = __builtin_amdgcn_exp2f(x.x - base);
+      r.m = top;
+      r.l = r.l * f + x.y * g;
+    }
+#pragma unroll
+    for (int b = 0; b < 4; ++b) {
+      const f32x4 x = at[t * step + b * 64];
+#pragma unroll
+      for (int e = 0; e < 4; ++e) r.o[t][4 * b + e] = r.o[t][4 * b + e] * f + x[e] * g;
+    }
+  };
+  if (once) {
+    if (wave >= RW)
+#pragma unroll
+      for (int t = 0; t < D / 32; ++t) give(t);
+    meet();
+    if (wave < RW)
+#pragma unroll
+      for (int t = 0; t < D / 32; ++t) take(t);
+    return;
+  }
 #pragma unroll
   for (int t = 0; t < D / 32; ++t) {
-    if (wave >= RW) {
-      if (t == 0) *ml = make_float2(r.m, r.l);
-#pragma unroll
-      for (int b = 0; b < 4; ++b) at[b * 64] = f32x4{r.o[t][4 * b], r.o[t][4 * b + 1], r.o[t][4 * b + 2], r.o[t][4 * b + 3]};
-    }
+    if (wave >= RW) give(t);
     meet();
-    if (wave < RW) {
-      if (t == 0) {
-        const float2 x = *ml;
-        const float top = fmaxf(r.m, x.x), base = top == -INFINITY ? 0.f : top;
-        f = __builtin_amdgcn_exp2f(r.m - base);
-        g = __builtin_amdgcn_exp2f(x.x - base);
-        r.m = top;
-        r.l = r.l * f + x.y * g;
-      }
-#pragma unroll
-      for (int b = 0; b < 4; ++b) {
-        const f32x4 x = at[b * 64];
-#pragma unroll
-        for (int e = 0; e < 4; ++e) r.o[t][4 * b + e] = r.o[t][4 * b + e] * f + x[e] * g;
-      }
-    }
+    if (wave < RW) take(t);
     meet();
   }
 }
@@ -542,7 +586,8 @@ __global__ void __launch_bounds__(64 * RW * KW, (Shape<D, RW, KW>::kPerSimd)) at
     left -= blocks;
   }
   const bool odd_blocks = a.block_size % 16 != 0;
-  Ring<T, D, RW, KW> ring(a, h, at);
+  __shared__ uint32_t odd[2 * S::kWaves];
+  Ring<T, D, RW, KW> ring(a, h, at, odd);
   TreeRows<T, D> r;
   // The token of this lane's row of a tile, or -1, and its head.
   auto token = [&](const Span &x, int i) { return i < x.n_rows ? x.start + i / a.group : -1; };
@@ -555,6 +600,7 @@ __global__ void __launch_bounds__(64 * RW * KW, (Shape<D, RW, KW>::kPerSimd)) at
     turn_to(s, q, b0, blocks);
     const int entry = ring.keys.entry(0);
     load_rows<T, D>(a, r, token(s, i), head(s, i));
+    r.load_word(a, token(s, i));
     ring.begin(entry);
   }
   while (blocks > 0) {
@@ -586,8 +632,9 @@ __global__ void __launch_bounds__(64 * RW * KW, (Shape<D, RW, KW>::kPerSimd)) at
       turn_to(next, next_q, 0, next_blocks);
       ring.begin(entry);
       load_query<T, D>(a, r, next_t, next_h);
+      r.load_word(a, next_t);
     }
-    if constexpr (KW == 2) join_halves<T, D, RW>(r, lds + S::kRing);
+    if constexpr (KW == 2) join_halves<T, D, RW>(r, lds, lds + S::kRing, next_blocks == 0);
     const bool ends = b0 + blocks < s.blocks && b0 == 0;
     if (KW == 1 || threadIdx.x < 64 * RW) {
       if (blocks == s.blocks) write_rows<T, D>(a, r);
