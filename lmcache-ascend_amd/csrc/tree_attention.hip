@@ -42,7 +42,9 @@ struct TreeArgs : PagedArgs {
   // Sums of cut tiles: [piece][KV head][begun before, ended behind][rows].
   float *part_o;
   float2 *part_ml;
-  struct Cut { int request, tile, more; } *cuts;  // of the place "ended behind": the pieces that follow, or request -1
+  // Of the place "ended behind": the pieces that follow (-1: nothing is there),
+  // the tile's rows and the request's first token.
+  struct Cut { int more, first_row, rows, start; } *cuts;
 };
 
 // How a call's work is cut, from its sizes alone (the lengths are on the GPU).
@@ -139,11 +141,48 @@ struct Begin {
 // 18.7 with 4).
 constexpr int64_t kLeast = 2;
 
-// All requests' units, summed by the workgroup: each thread has a run of them.
+// All requests' units, summed: of up to 64 by each wave for itself, a request a
+// lane (0.6 us less than through LDS), of more by the workgroup, a run of them a thread.
 template <int ROWS, int THREADS> __device__ __forceinline__ Begin find_piece(const TreeArgs &a, int piece) {
   __shared__ int64_t sums[THREADS / 64];
   __shared__ Begin found;
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  // (the same in all lanes: to scalar registers)
+  auto all32 = [](int x) { return __builtin_amdgcn_readfirstlane(x); };
+  auto all64 = [&](int64_t x) {
+    const uint32_t lo = all32(static_cast<int>(x)), hi = all32(static_cast<int>(x >> 32));
+    return static_cast<int64_t>((static_cast<uint64_t>(hi) << 32) | lo);
+  };
+  // The sum of the lanes up to this one.
+  auto sum_up = [&](int64_t x) {
+#pragma unroll
+    for (int d = 1; d < 64; d <<= 1) {
+      const int64_t below = __shfl_up(x, d);
+      if (lane >= d) x += below;
+    }
+    return x;
+  };
+  Begin b;
+  b.left = b.unit = 0;
+  b.r = 0;
+  b.span = {0, 0, 0, 0, 1, 0};
+  if (a.n_requests <= 64) {
+    Span s = span_of<ROWS>(a, min(lane, a.n_requests - 1));
+    if (lane >= a.n_requests) s.units = 0;
+    const int64_t upto = sum_up(s.units), total = all64(__shfl(upto, 63));
+    b.each = max((total + a.pieces - 1) / a.pieces, kLeast);
+    const int64_t first = b.each * piece;
+    const uint64_t here = __ballot(first >= upto - s.units && first < upto);
+    if (here == 0) return b;
+    const int from = __ffsll(static_cast<unsigned long long>(here)) - 1;
+    b.left = min(b.each, total - first);
+    b.unit = first - all64(__shfl(upto - s.units, from));
+    b.r = from;
+    b.span = {__builtin_amdgcn_readlane(s.start, from), __builtin_amdgcn_readlane(s.n_rows, from),
+              __builtin_amdgcn_readlane(s.context, from), __builtin_amdgcn_readlane(s.end, from),
+              __builtin_amdgcn_readlane(s.blocks, from), all64(__shfl(s.units, from))};
+    return b;
+  }
   const int per = (a.n_requests + THREADS - 1) / THREADS;
   const int r0 = min(a.n_requests, static_cast<int>(threadIdx.x) * per), r1 = min(a.n_requests, r0 + per);
   Span s;
@@ -152,12 +191,7 @@ template <int ROWS, int THREADS> __device__ __forceinline__ Begin find_piece(con
     s = span_of<ROWS>(a, r);
     own += s.units;
   }
-  int64_t upto = own;
-#pragma unroll
-  for (int d = 1; d < 64; d <<= 1) {
-    const int64_t below = __shfl_up(upto, d);
-    if (lane >= d) upto += below;
-  }
+  int64_t upto = sum_up(own);
   if (lane == 63) sums[wave] = upto;
   __syncthreads();
   int64_t total = 0;
@@ -180,17 +214,7 @@ template <int ROWS, int THREADS> __device__ __forceinline__ Begin find_piece(con
     found = {each, min(each, total - first), first - at, r, s};
   }
   __syncthreads();
-  // (the same in all lanes: to scalar registers)
-  auto all32 = [](int x) { return __builtin_amdgcn_readfirstlane(x); };
-  auto all64 = [&](int64_t x) {
-    const uint32_t lo = all32(static_cast<int>(x)), hi = all32(static_cast<int>(x >> 32));
-    return static_cast<int64_t>((static_cast<uint64_t>(hi) << 32) | lo);
-  };
-  Begin b;
   b.each = all64(each);
-  b.left = b.unit = 0;
-  b.r = 0;
-  b.span = {0, 0, 0, 0, 1, 0};
   if (all64(first) >= all64(total)) return b;
   const Begin f = found;
   b.left = all64(f.left);
@@ -570,7 +594,7 @@ __global__ void __launch_bounds__(64 * RW * KW, (Shape<D, RW, KW>::kPerSimd)) at
   const int piece = blockIdx.x / a.kv_heads, h = blockIdx.x % a.kv_heads, me = piece * a.kv_heads + h;
   const Begin begin = find_piece<S::kRows, 64 * S::kWaves>(a, piece);
   const int64_t each = begin.each;
-  TreeArgs::Cut cut = {-1, 0, 0};
+  TreeArgs::Cut cut = {-1, 0, 0, 0};
   // The part of a tile that is worked on: `blocks` of its blocks from b0 on.
   Span s = begin.span;
   int q = begin.r, tile = 0, b0 = 0, blocks = 0;
@@ -640,7 +664,8 @@ __global__ void __launch_bounds__(64 * RW * KW, (Shape<D, RW, KW>::kPerSimd)) at
       if (blocks == s.blocks) write_rows<T, D>(a, r);
       else write_part<T, D>(a, r, (static_cast<int64_t>(me) * 2 + ends) * S::kRows + wave * 32);
     }
-    if (ends) cut = {q, tile, static_cast<int>((s.blocks - blocks + each - 1) / each)};
+    if (ends)
+      cut = {static_cast<int>((s.blocks - blocks + each - 1) / each), tile * S::kRows, min(S::kRows, s.n_rows - tile * S::kRows), s.start};
     r.row = next_t >= 0 ? next_t * a.heads + next_h : -1;
     clear_sums(r);
     s = next;
@@ -666,23 +691,26 @@ template <typename T, int D, int ROWS> __global__ void __launch_bounds__(256) jo
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int h = blockIdx.x % a.kv_heads;
   int rank = blockIdx.x / a.kv_heads, piece = -1;
+  TreeArgs::Cut cut = {-1, 0, 0, 0};
   for (int p0 = 0; p0 < a.pieces; p0 += 64) {
     const int p = p0 + lane;
-    uint64_t there = __ballot(p < a.pieces && a.cuts[p * a.kv_heads + h].request >= 0);
+    if (p < a.pieces) cut = a.cuts[p * a.kv_heads + h];
+    uint64_t there = __ballot(p < a.pieces && cut.more >= 0);
     const int n = __popcll(there);
     if (rank >= n) {
       rank -= n;
       continue;
     }
     for (; rank > 0; --rank) there &= there - 1;
-    piece = p0 + __ffsll(static_cast<unsigned long long>(there)) - 1;
+    const int from = __ffsll(static_cast<unsigned long long>(there)) - 1;
+    piece = p0 + from;
+    cut = {__builtin_amdgcn_readlane(cut.more, from), __builtin_amdgcn_readlane(cut.first_row, from),
+           __builtin_amdgcn_readlane(cut.rows, from), __builtin_amdgcn_readlane(cut.start, from)};
     break;
   }
   if (piece < 0) return;
   const int first = piece * a.kv_heads + h;
-  const TreeArgs::Cut cut = a.cuts[first];
-  const Span s = span_of<ROWS>(a, cut.request);
-  const int i0 = lane / kQuads, d = lane % kQuads * 4, n = min(ROWS, s.n_rows - cut.tile * ROWS), parts = cut.more + 1;
+  const int i0 = lane / kQuads, d = lane % kQuads * 4, n = cut.rows, parts = cut.more + 1;
   float m, l;
   f32x4 o;
   // Row i of the parts k0, k0 + step, ...: kFew / 2 of them under way together.
@@ -715,7 +743,7 @@ template <typename T, int D, int ROWS> __global__ void __launch_bounds__(256) jo
   };
   auto write = [&](int i) {
     const float inv = l == 0.f ? 0.f : 1.f / l, base = m == -INFINITY ? 0.f : m;
-    const int x = cut.tile * ROWS + i, t = s.start + x / a.group, head = h * a.group + x % a.group;
+    const int x = cut.first_row + i, t = cut.start + x / a.group, head = h * a.group + x % a.group;
     const O4 y = {M::from(o[0] * inv), M::from(o[1] * inv), M::from(o[2] * inv), M::from(o[3] * inv)};
     *reinterpret_cast<O4 *>(static_cast<typename T::S *>(a.o) + t * a.o_token + head * a.o_head + d) = y;
     if (a.lse && d == 0) a.lse[t * a.lse_token + head * a.lse_head] = l == 0.f ? -INFINITY : (base + log2f(l)) * 0.69314718056f;
