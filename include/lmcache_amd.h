@@ -636,7 +636,7 @@ int lmc_tree_attention(const lmc_tensor *query, const lmc_tensor *vllm_kv_caches
  * (MERGED_KV and SEPARATE_KV with any strides; the caches of other formats
  * [pages, block, (heads,) dim]).  pages: [n, 2] int64 or int32, (source,
  * target); a pair with a page outside the caches is skipped.  No target may be
- * another pair's source or target. */
+ * another pair's source or target.  At most 65535 planes of all layers. */
 int lmc_copy_kv_pages(const lmc_tensor *layer_ptrs, const lmc_tensor *vllm_kv_caches, int32_t n_caches,
                       const lmc_tensor *pages, int32_t kvcache_format, int32_t vllm_two_major, void *stream);
 
@@ -647,7 +647,7 @@ int lmc_copy_kv_pages(const lmc_tensor *layer_ptrs, const lmc_tensor *vllm_kv_ca
  * increasing from 0 or more (another's rows end up in an order that is not
  * said), block_table [R, W] int32.  A row that has no page, here or there, is
  * not moved.  The rows that move, of all requests, lie in different places of
- * the caches.  seq_lens ([R] int32, may be null) gets base_lens + keep_lens. */
+ * the caches.  At most 65535 requests.  seq_lens ([R] int32, may be null) gets base_lens + keep_lens. */
 int lmc_compact_kv(const lmc_tensor *layer_ptrs, const lmc_tensor *vllm_kv_caches, int32_t n_caches,
                    const lmc_tensor *block_table, const lmc_tensor *base_lens, const lmc_tensor *keep,
                    const lmc_tensor *keep_lens, const lmc_tensor *seq_lens, int32_t kvcache_format,

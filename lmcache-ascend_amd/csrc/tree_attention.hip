@@ -21,13 +21,13 @@
 // softmax's vector work: 32 requests of up to 8192 keys, 32 heads over 8 KV heads
 // of 128 bf16 dims, take 99 us with one token each (5.6 TB/s), 118 with 16, 152
 // with 32 and 214 with 64 (663 TFLOP/s).  64 tokens over up to 16384 keys take
-// 364 to 415 us: the clock falls to 1.6 GHz there.  2 requests of 8 tokens over
-// 2000 keys: 17.6 us, the latency of two launches.  The join takes 10 us of 118
-// and 18 of 415.
+// 364 to 408 us: the clock falls to 1.6 GHz there.  2 requests of 8 tokens over
+// 2000 keys: 15.0 us, the latency of two launches.  The join takes 10 us of 118
+// and 18 of 400.
 //
-// Registers at 128 dims: 254 for 64 rows, 256 for more (20 spilled outside of the
-// loop over the keys), two waves a SIMD; at 64 dims 168 to 180; at 192 and 256 a
-// wave a SIMD, with accumulation registers.
+// Registers at 128 dims: 255 for 64 rows, 256 for more (12 to 18 spilled outside of
+// the loop over the keys), two waves a SIMD; at 64 dims 168 to 182; at 192 and 256
+// a wave a SIMD, with accumulation registers.
 #include "paged_attention.h"
 
 namespace lmc {
@@ -137,8 +137,8 @@ struct Begin {
 };
 
 // Blocks of a piece at least: a piece more for the join costs about as much as
-// a block (2 requests of 8 tokens over 2000 keys: 17.2 us with 2, 17.7 with 1,
-// 18.7 with 4).
+// a block (2 requests of 8 tokens over 2000 keys: 17.5 us with 2, 18.3 with 1,
+// 18.4 with 3, all before lengths were summed in registers).
 constexpr int64_t kLeast = 2;
 
 // All requests' units, summed: of up to 64 by each wave for itself, a request a

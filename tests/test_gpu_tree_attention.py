@@ -215,6 +215,44 @@ def test_what_a_row_does_not_see_is_not_used(ops, odd):
     assert (err[~sees.numpy()] <= rest[2][~sees.numpy()]).all()
 
 
+@pytest.mark.parametrize("dim", [64, 96, 128, 192, 256])
+@pytest.mark.parametrize("q,Hq", [(40, 1), (60, 2), (60, 4)])
+@pytest.mark.parametrize("odd", [INF, NAN])
+def test_odd_values_anywhere_in_a_block(ops, dim, q, Hq, odd):
+    """Tiles of every shape: each of several drafted keys, odd in one dim, is
+    seen by one token alone."""
+    c = _case(30 + dim, [q], [45], 16, Hq, 1, dim, density=0.0)
+    c["k"].nan_to_num_(0.5)
+    c["v"].nan_to_num_(0.25)
+    c["mask"] = [1 << i for i in range(q)]
+    put = {0: 0, 7: dim - 1, 18: dim // 2, 19: dim // 2 - 1, q - 1: 31, q - 9: dim - 33}
+    for i, d in put.items():
+        c["v"][int(c["table"][0, (45 + i) // 16]), (45 + i) % 16, 0, d] = odd
+    caches, kw = _device_caches(c)
+    out = c["out"].to(DEV)
+    _call(ops, c, caches, kw, c["q"].to(DEV), out, None)
+    torch.cuda.synchronize()
+    got = out.double().cpu().numpy()
+    for i, d in put.items():
+        c["v"][int(c["table"][0, (45 + i) // 16]), (45 + i) % 16, 0, d] = 0.0
+    want, _, tol, _ = _want(c)
+    hit = np.zeros_like(got, dtype=bool)
+    for i, d in put.items():
+        hit[i, :, d] = True
+    assert (np.isnan(got[hit]) if odd != odd else got[hit] == INF).all()
+    assert (np.abs(got - want)[~hit] <= tol[~hit]).all()
+
+
+@pytest.mark.parametrize("R", [63, 64, 65, 256, 257])
+def test_numbers_of_requests(ops, R):
+    """Up to 64 requests are summed up in another way than more."""
+    gen = torch.Generator().manual_seed(R)
+    q_lens = torch.randint(0, 4, (R,), generator=gen).tolist()
+    contexts = torch.randint(0, 90, (R,), generator=gen).tolist()
+    contexts[R // 2] = 1200
+    _check(ops, _case(R, q_lens, contexts, 16, 2, 2, 64, pad=1))
+
+
 def test_a_key_of_infinities_hidden_from_some(ops):
     c = _case(16, [4], [20], 16, 2, 1, 64, density=0.0)
     c["mask"] = [1, 2, 4, 8]
