@@ -286,11 +286,6 @@ template <int D, int RW, int KW> struct Shape {
 // The other waves are here too, all that was read from LDS has arrived.
 __device__ __forceinline__ void meet() { asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory"); }
 
-// A workgroup's rows over keys, a block of 64 at a time, a wave's 32 keys a step.  K runs a step ahead of V, and a step's softmax is
-// spread over two products: beside the product with V of step i stand the
-// maximum of step i + 1 and the first half of its weights, beside the scores of
-// step i + 2 the other half.  So matrix and vector units have work at any time.
-// K and V have rings of blocks in LDS, loaded as soon as a place is free.
 // Whether a block of V holds an infinity or a NaN: each wave looks at a part of
 // it and says so at `odd`, which no wave writes again before all have read it.
 template <typename T, int D, int WAVES> __device__ __forceinline__ bool any_odd(uint32_t v, uint32_t *odd) {
@@ -313,6 +308,12 @@ template <typename T, int D, int WAVES> __device__ __forceinline__ bool any_odd(
   return __builtin_amdgcn_readfirstlane(all) != 0;
 }
 
+// A workgroup's rows over keys, a block of 64 at a time, a wave's 32 keys a step.
+// K runs a step ahead of V, and a step's softmax is spread over two products:
+// beside the product with V of step i stand the maximum of step i + 1 and the
+// first half of its weights, beside the scores of step i + 2 the other half.  So
+// matrix and vector units have work at any time.  K and V have rings of blocks
+// in LDS, loaded as soon as a place is free.
 template <typename T, int D, int RW, int KW> struct Ring {
   using S = Shape<D, RW, KW>;
   static constexpr int kPer = D / 32, NK = S::kNK, NV = S::kNV;
