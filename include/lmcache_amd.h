@@ -659,9 +659,11 @@ int lmc_compact_kv(const lmc_tensor *layer_ptrs, const lmc_tensor *vllm_kv_cache
  * int32; entries outside [0, P) are skipped) lose a holder.  page_refs ([P]
  * int32) counts the holders of each page beyond the first; a page whose count
  * falls below 0 (one that was negative before too) is given back and its count
- * set to 0.  With n of them, *next_cursor = *free_cursor - n ([1] int64 each,
- * distinct), and free_blocks[*next_cursor + i] ([F] int32) gets the i-th in
- * ascending order, where the list has that entry.  The call works in
+ * set to 0.  With n of them, *next_cursor = min(*free_cursor, F) - n ([1] int64
+ * each, distinct: a cursor behind the list's end says that pages were missing,
+ * and the entries there were never handed out), and free_blocks[*next_cursor +
+ * i] ([F] int32) gets the i-th in ascending order, where the list has that
+ * entry.  The call works in
  * `workspace`, a 1-D uint8 tensor of the GPU on a 4-byte boundary; with
  * workspace_bytes not null it only writes the size needed there.  Outputs
  * overlap neither each other nor what the call reads. */

@@ -383,7 +383,8 @@ __global__ void __launch_bounds__(256) count_free(ReleaseArgs a) {
 __global__ void __launch_bounds__(256) place_free(ReleaseArgs a) {
   __shared__ int part[3][4];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, p0 = blockIdx.x * kRun + threadIdx.x * 4;
-  const int64_t cursor = *a.cursor;
+  // (places past the list's end were never handed out)
+  const int64_t cursor = min(*a.cursor, a.n_free);
   const uint32_t bits = without_holder(a, p0);
   int before = 0, total = 0;
   for (int i = threadIdx.x; i < a.runs; i += 256) {

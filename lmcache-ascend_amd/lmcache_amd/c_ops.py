@@ -991,10 +991,12 @@ def release_pages(
     page of one table, one more for each fork that shares it.  A page that has
     none left is given back, once, and its count is 0 again; the others' counts
     go down.  Pages given back are put before free_blocks[free_cursor] in
-    ascending order, and next_cursor ([1] int64, another tensor) gets
-    free_cursor less their number, so that free_blocks[next_cursor:] is free;
-    those that the list has no place for are left out.  block_table stays as it
-    is; its entries outside [0, P) are skipped."""
+    ascending order (before the list's end, where the cursor is behind it:
+    build_slot_mapping counts pages there that it could not hand out), and
+    next_cursor ([1] int64, another tensor) gets that place less their number, so
+    that free_blocks[next_cursor:] is free; those that the list has no place for
+    are left out.  block_table stays as it is; its entries outside [0, P) are
+    skipped."""
     if _ext is not None:
         _ext.release_pages(block_table, held_lens, keep_lens, int(block_size), page_refs, free_blocks, free_cursor,
                            next_cursor)

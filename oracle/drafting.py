@@ -121,6 +121,7 @@ def release(table, held, keep, block, refs, free, cursor):
             if 0 <= row[j] < len(refs):
                 refs[row[j]] -= 1
     given = [p for p, n in enumerate(refs) if n < 0]
+    cursor = min(cursor, len(free))
     for i, p in enumerate(given):
         refs[p] = 0
         if 0 <= cursor - len(given) + i < len(free):

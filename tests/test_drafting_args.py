@@ -354,3 +354,9 @@ def test_oracle_catches_a_planted_mistake():
     assert [m & ~(1 << i) for i, m in enumerate(mask)] != mask
     right = od.release([[1, 2]], [8], [0], 4, [0] * 3, [9] * 3, 3)
     assert od.release([[1, 2]], [7], [0], 8, [0] * 3, [9] * 3, 3) != right
+
+
+def test_oracle_release_past_the_list():
+    """Places behind the list's end were never handed out: pages go below it."""
+    assert od.release([[0, 1, 2, -1], [3, -1, -1, -1]], [64, 32], [0, 0], 16, [0] * 4, [9] * 4, 6) == ([0] * 4, [0, 1, 2, 3], 0)
+    assert od.release([[0, 1]], [32], [16], 16, [0] * 4, [9] * 4, 6) == ([0] * 4, [9, 9, 9, 1], 3)

@@ -397,3 +397,44 @@ def test_given_back_pages_are_taken_again(ops):
         used = sum(-(-k // 16) for k in keep)
         assert cur.item() == used
         assert sorted(free[used:].tolist() + [int(x) for r in range(2) for x in table[r, : -(-keep[r] // 16)]]) == list(range(64))
+
+
+@pytest.mark.parametrize("cursor", [9, 10, 13, 2**31, 2**63 - 1])
+@pytest.mark.parametrize("pages", [9, 5000])
+def test_places_past_the_list_were_never_handed_out(ops, cursor, pages):
+    """A cursor past the list's end, as build_slot_mapping leaves it when pages
+    run short: the pages go below the list's end, none is lost."""
+    table = [[1, 2, 3, 4], [8, -1, -1, -1]]
+    _release(ops, table, [64, 64], [16, 0], 16, [0] * pages, [99] * 9, cursor)
+    i32, i64 = dict(dtype=torch.int32, device=DEV), dict(dtype=torch.int64, device=DEV)
+    free, nxt = torch.full((9,), 99, **i32), torch.zeros(1, **i64)
+    ops.release_pages(torch.tensor(table, **i32), torch.tensor([64, 64], **i32), torch.tensor([16, 0], **i32), 16,
+                      torch.zeros(pages, **i32), free, torch.tensor([cursor], **i64), nxt)
+    torch.cuda.synchronize()
+    assert nxt.item() == 5 and free.tolist() == [99] * 5 + [2, 3, 4, 8]
+
+
+@pytest.mark.parametrize("pages,lens", [(4, [96, 0]), (4, [40, 70]), (7, [160, 160]), (1, [16, 17])])
+def test_no_page_is_lost_when_the_list_runs_short(ops, pages, lens):
+    """More pages asked for than there are, time and again: what is given back
+    is the whole list each time, every page in it once."""
+    i32, i64 = dict(dtype=torch.int32, device=DEV), dict(dtype=torch.int64, device=DEV)
+    free = torch.arange(pages, **i32).flip(0).contiguous()
+    cur, nxt, refs = torch.zeros(1, **i64), torch.zeros(1, **i64), torch.zeros(pages, **i32)
+    none, seq = torch.zeros(2, **i32), torch.zeros(2, **i32)
+    asked = sum(-(-n // 16) for n in lens)
+    assert asked > pages
+    for _ in range(3):
+        table, slots = torch.full((2, 12), -1, **i32), torch.empty(sum(lens), **i64)
+        ops.build_slot_mapping(torch.tensor(lens, **i32), none, table, 16, slots, seq_lens=seq, free_blocks=free,
+                               free_cursor=cur, next_cursor=nxt)
+        assert nxt.item() == asked and (table >= 0).sum() == pages
+        cur.copy_(nxt)
+        # Half of the first request's tokens first, then the rest.
+        half = torch.tensor([lens[0] // 2, lens[1]], **i32)
+        ops.release_pages(table, seq, half, 16, refs, free, cur, nxt)
+        cur.copy_(nxt)
+        ops.release_pages(table, half, none, 16, refs, free, cur, nxt)
+        cur.copy_(nxt)
+        torch.cuda.synchronize()
+        assert cur.item() == 0 and sorted(free.tolist()) == list(range(pages)) and refs.sum() == 0
