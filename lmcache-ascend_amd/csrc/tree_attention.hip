@@ -479,7 +479,10 @@ __device__ __forceinline__ void Ring<T, D, RW, KW>::run(const PagedArgs &a, Tree
         top = fmaxf(tops.x, tops.y) * c;
         if (__any(top > r.m + 8.f)) {
           const float m = fmaxf(r.m, top);
-          scale = m == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(r.m - m);
+          // (A row without a reference point has no sums yet, but may have
+          // infinities from the other half of the block: zero times those
+          // would be NaN.)
+          scale = r.m == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(r.m - m);
           r.l *= scale;
           r.m = m;
           base = m == -INFINITY ? 0.f : m;

@@ -431,3 +431,33 @@ def test_nothing_to_do(ops):
                        torch.tensor([0, 3], **i32), torch.full((3, 1), -1, dtype=torch.int64, device=DEV), 1.0, out)
     torch.cuda.synchronize()
     assert (out == 0).all()
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("dim,Hq", [(64, 1), (64, 2), (96, 2), (128, 1), (128, 2), (192, 1), (256, 1)])
+@pytest.mark.parametrize("context", [0, 64])
+@pytest.mark.parametrize("odd", [INF, -INF, NAN])
+def test_odd_values_of_a_rows_first_keys(ops, dtype, dim, Hq, context, odd):
+    """Tokens that see themselves alone (and the context), the values of some
+    odd: nothing is summed up in their row, or the piece of it, before."""
+    q = 100
+    c = _case(40 + dim, [q], [context], 16, Hq, 1, dim, dtype, density=0.0)
+    c["k"].nan_to_num_(0.5)
+    c["v"].nan_to_num_(0.25)
+    c["mask"] = [1 << i for i in range(q)]
+    put = {0: 1, 5: dim - 1, 31: 3, 32: 0, 47: dim // 2, 63: 7, 64: 2, 95: dim - 2, 96: 33, 99: 4}
+    for i, d in put.items():
+        c["v"][int(c["table"][0, (context + i) // 16]), (context + i) % 16, 0, d] = odd
+    caches, kw = _device_caches(c)
+    out = c["out"].to(DEV)
+    _call(ops, c, caches, kw, c["q"].to(DEV), out, None)
+    torch.cuda.synchronize()
+    got = out.double().cpu().numpy()
+    for i, d in put.items():
+        c["v"][int(c["table"][0, (context + i) // 16]), (context + i) % 16, 0, d] = 0.0
+    want, _, tol, _ = _want(c)
+    hit = np.zeros_like(got, dtype=bool)
+    for i, d in put.items():
+        hit[i, :, d] = True
+    assert (np.isnan(got[hit]) if odd != odd else got[hit] == odd).all(), np.argwhere(hit & np.isnan(got))
+    assert (np.abs(got - want)[~hit] <= tol[~hit]).all()
