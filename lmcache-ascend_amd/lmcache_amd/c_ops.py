@@ -908,7 +908,8 @@ def prepare_kv_pages(layers, kvcache_format_raw: int = 2, vllm_two_major: bool =
             if t.data_ptr() % 16 != s.data_ptr() % 16:
                 raise ValueError("layers' caches differ in their alignment to 16 bytes")
     _gpu_of(first[0], "the first cache")
-    if len({t.data_ptr() for caches in layers for t in caches}) < len(layers) * len(first):
+    whole = [t for caches in layers for t in caches if t.numel()]
+    if len({t.data_ptr() for t in whole}) < len(whole):
         raise ValueError("a cache is given twice")
     st = KVPagesState()
     st.layers = tuple(layers)

@@ -438,3 +438,16 @@ def test_no_page_is_lost_when_the_list_runs_short(ops, pages, lens):
         cur.copy_(nxt)
         torch.cuda.synchronize()
         assert cur.item() == 0 and sorted(free.tolist()) == list(range(pages)) and refs.sum() == 0
+
+
+def test_caches_without_pages(ops):
+    """Caches that hold nothing have no address: they are not one cache."""
+    none = torch.zeros((0, 16, 2, 64), dtype=torch.bfloat16, device=DEV)
+    state = ops.prepare_kv_pages([(none, none.clone()), (none.clone(), none.clone())])
+    ops.copy_kv_pages(state, torch.tensor([[0, 1]], device=DEV))
+    i32 = dict(dtype=torch.int32, device=DEV)
+    seq = torch.zeros(2, **i32)
+    ops.compact_kv(state, torch.zeros((2, 3), **i32), torch.tensor([3, 4], **i32), torch.tensor([[1, 2], [0, 5]], **i32),
+                   torch.tensor([2, 1], **i32), seq)
+    torch.cuda.synchronize()
+    assert seq.tolist() == [5, 5]
