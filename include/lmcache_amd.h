@@ -630,13 +630,20 @@ int lmc_tree_attention(const lmc_tensor *query, const lmc_tensor *vllm_kv_caches
                        const lmc_tensor *workspace, int64_t *workspace_bytes, int32_t kvcache_format,
                        int32_t vllm_two_major, void *stream);
 
+/* LMC_ERR_VALUE where two of n caches share an element (those of all layers, in
+ * any order; rows dealt in turn in one buffer are told apart).  For the callers
+ * of lmc_copy_kv_pages and lmc_compact_kv, which see the layers' addresses on the
+ * GPU alone.  Touches the host only. */
+int lmc_check_layers_apart(const lmc_tensor *caches, int64_t n);
+
 /* Pages copied in every layer and plane.  layer_ptrs: device table [layers,
  * n_caches] int64 of the addresses of each layer's caches; vllm_kv_caches are one
  * layer's, whose shape, strides, dtype and alignment to 16 bytes all have
  * (MERGED_KV and SEPARATE_KV with any strides; the caches of other formats
- * [pages, block, (heads,) dim]).  pages: [n, 2] int64 or int32, (source,
- * target); a pair with a page outside the caches is skipped.  No target may be
- * another pair's source or target.  At most 65535 planes of all layers. */
+ * [pages, block, (heads,) dim]); no two caches share an element.  pages:
+ * [n, 2] int64 or int32, (source, target); a pair with a page outside the
+ * caches is skipped.  No target may be another pair's source or target.  At
+ * most 65535 planes of all layers. */
 int lmc_copy_kv_pages(const lmc_tensor *layer_ptrs, const lmc_tensor *vllm_kv_caches, int32_t n_caches,
                       const lmc_tensor *pages, int32_t kvcache_format, int32_t vllm_two_major, void *stream);
 

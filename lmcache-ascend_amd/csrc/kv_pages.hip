@@ -18,6 +18,7 @@
 #include "serving.h"
 
 #include <type_traits>
+#include <vector>
 
 namespace lmc {
 
@@ -416,6 +417,22 @@ __global__ void __launch_bounds__(256) place_free(ReleaseArgs a) {
 } // namespace lmc
 
 using namespace lmc;
+
+extern "C" int lmc_check_layers_apart(const lmc_tensor *caches, int64_t n) {
+  return guarded([&] {
+    std::vector<const lmc_tensor *> by_address;
+    for (int64_t i = 0; i < n; ++i)
+      if (extent_bytes(deref(&caches[i], "caches")) > 0) by_address.push_back(&caches[i]);
+    auto begin = [](const lmc_tensor *t) { return reinterpret_cast<uintptr_t>(t->data); };
+    std::sort(by_address.begin(), by_address.end(), [&](const lmc_tensor *a, const lmc_tensor *b) { return begin(a) < begin(b); });
+    for (size_t i = 0; i < by_address.size(); ++i) {
+      const lmc_tensor &a = *by_address[i];
+      const uintptr_t end = begin(&a) + extent_bytes(a);
+      for (size_t k = i + 1; k < by_address.size() && begin(by_address[k]) < end; ++k)
+        expect(a.device != by_address[k]->device || !may_share(a, *by_address[k]), "two of the layers' caches overlap");
+    }
+  });
+}
 
 extern "C" int lmc_copy_kv_pages(const lmc_tensor *layer_ptrs, const lmc_tensor *vllm_kv_caches, int32_t n_caches,
                                  const lmc_tensor *pages, int32_t kvcache_format, int32_t vllm_two_major, void *stream) {

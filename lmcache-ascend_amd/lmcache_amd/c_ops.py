@@ -891,9 +891,13 @@ class KVPagesState:
 def prepare_kv_pages(layers, kvcache_format_raw: int = 2, vllm_two_major: bool = False) -> KVPagesState:
     """The handle that copy_kv_pages and compact_kv take: `layers` holds each
     layer's caches (a tensor or a tuple of them, of any KV format), all of one
-    shape, dtype, strides and GPU.  MERGED_KV and SEPARATE_KV caches may have any
-    strides; the others are [pages, block, (heads,) dim].  Caches of one-byte
-    dtypes are taken as they are."""
+    shape, dtype, strides and GPU, none over another.  MERGED_KV and SEPARATE_KV
+    caches may have any strides; the others are [pages, block, (heads,) dim].
+    Caches of one-byte dtypes are taken as they are."""
+
+    def plain(t):
+        return t.view(torch.uint8) if t.dtype not in _DTYPES and t.element_size() == 1 else t
+
     layers = [tuple(_normalize_kv_caches(x)) for x in layers]
     if not layers:
         raise ValueError("no layers are given")
@@ -911,9 +915,10 @@ def prepare_kv_pages(layers, kvcache_format_raw: int = 2, vllm_two_major: bool =
     whole = [t for caches in layers for t in caches if t.numel()]
     if len({t.data_ptr() for t in whole}) < len(whole):
         raise ValueError("a cache is given twice")
+    _run(_L.lmc_check_layers_apart(_cache_array([plain(t) for t in whole]), len(whole)))
     st = KVPagesState()
     st.layers = tuple(layers)
-    st.caches = [t.view(torch.uint8) if t.dtype not in _DTYPES and t.element_size() == 1 else t for t in first]
+    st.caches = [plain(t) for t in first]
     st.kvcache_format, st.vllm_two_major = int(kvcache_format_raw), bool(vllm_two_major)
     st.layer_ptrs = torch.tensor([[t.data_ptr() for t in caches] for caches in layers], dtype=torch.int64,
                                  device=first[0].device)

@@ -360,3 +360,57 @@ def test_oracle_release_past_the_list():
     """Places behind the list's end were never handed out: pages go below it."""
     assert od.release([[0, 1, 2, -1], [3, -1, -1, -1]], [64, 32], [0, 0], 16, [0] * 4, [9] * 4, 6) == ([0] * 4, [0, 1, 2, 3], 0)
     assert od.release([[0, 1]], [32], [16], 16, [0] * 4, [9] * 4, 6) == ([0] * 4, [9, 9, 9, 1], 3)
+
+
+def _layers_check(caches):
+    return L.lmc_check_layers_apart(_array(caches), len(caches))
+
+
+def _at(data, *shape, strides=None, dtype=BF16, device=0):
+    return _t(dtype, *shape, data=data, strides=strides, device=device)
+
+
+_BASE_AT = 1 << 50
+_ROW = 16 * 2 * 64                       # elements of a page of 16 tokens, 2 heads of 64 dims
+
+
+@pytest.mark.parametrize("caches", [
+    # Layers of one buffer that begin two pages after each other.
+    [_at(_BASE_AT, 4, 16, 2, 64), _at(_BASE_AT + 2 * 2 * _ROW, 4, 16, 2, 64)],
+    # A last row that is the next layer's first, with others between them.
+    [_at(_BASE_AT, 4, 16, 2, 64), _at(1 << 52, 4, 16, 2, 64), _at(_BASE_AT + 4 * 2 * _ROW - 2, 4, 16, 2, 64)],
+    # One inside another.
+    [_at(_BASE_AT + 2 * _ROW, 1, 16, 2, 64), _at(_BASE_AT, 9, 16, 2, 64)],
+    # Rows in turn, one token too far.
+    [_at(_BASE_AT, 4, 16, 2, 64, strides=[3 * _ROW, 128, 64, 1]),
+     _at(_BASE_AT + 2 * (_ROW - 128), 4, 16, 2, 64, strides=[3 * _ROW, 128, 64, 1])],
+])
+def test_layers_that_overlap_are_refused(caches):
+    for order in (caches, caches[::-1]):
+        _refuses(_layers_check(order), "two of the layers' caches overlap")
+
+
+@pytest.mark.parametrize("caches", [
+    [],
+    [_at(_BASE_AT, 4, 16, 2, 64)],
+    # One behind the other.
+    [_at(_BASE_AT + 2 * 4 * _ROW * i, 4, 16, 2, 64) for i in (3, 0, 1, 2)],
+    # The layers' pages, K's and V's, in turn in one buffer; rows in turn; heads in turn.
+    [_at(_BASE_AT + 2 * _ROW * i, 4, 16, 2, 64, strides=[10 * _ROW, 128, 64, 1]) for i in range(10)],
+    [_at(_BASE_AT + 2 * 128 * i, 4, 16, 2, 64, strides=[6 * _ROW, 6 * 128, 64, 1]) for i in range(6)],
+    [_at(_BASE_AT + 2 * 64 * i, 4, 16, 2, 64, strides=[6 * _ROW, 6 * 128, 6 * 64, 1]) for i in range(6)],
+    # Heads before tokens.
+    [_at(_BASE_AT + 2 * _ROW * i, 4, 16, 2, 64, strides=[10 * _ROW, 64, 1024, 1]) for i in range(10)],
+    # Caches of no pages, and the same address on two GPUs.
+    [_at(_BASE_AT, 0, 16, 2, 64), _at(_BASE_AT, 4, 16, 2, 64), _at(_BASE_AT, 4, 16, 2, 64, device=1)],
+])
+def test_layers_side_by_side_are_taken(caches):
+    assert _layers_check(caches) == _lib.OK, L.lmc_last_error()
+
+
+def test_many_layers_in_one_buffer_are_told_apart_at_once():
+    n = 600
+    caches = [_at(_BASE_AT + 2 * _ROW * i, 50, 16, 2, 64, strides=[n * _ROW, 128, 64, 1]) for i in range(n)]
+    assert _layers_check(caches) == _lib.OK
+    caches[400].data += 2 * 64
+    _refuses(_layers_check(caches), "two of the layers' caches overlap")

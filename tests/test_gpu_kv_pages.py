@@ -451,3 +451,31 @@ def test_caches_without_pages(ops):
                    torch.tensor([2, 1], **i32), seq)
     torch.cuda.synchronize()
     assert seq.tolist() == [5, 5]
+
+
+def test_layers_over_each_other_are_refused(ops):
+    both = torch.zeros((2, 9, 16, 2, 64), dtype=torch.bfloat16, device=DEV)
+    k, v = both[0], both[1]
+    with pytest.raises(ValueError, match="two of the layers' caches overlap"):
+        ops.prepare_kv_pages([(k[:4], v[:4]), (k[2:6], v[4:8])])
+    with pytest.raises(ValueError, match="two of the layers' caches overlap"):
+        ops.prepare_kv_pages([both[:, :5], both[:, 4:]], 1, True)
+    with pytest.raises(ValueError, match="two of the layers' caches overlap"):
+        ops.prepare_kv_pages([(k[:4].view(torch.float8_e4m3fn), v[:4].view(torch.float8_e4m3fn)),
+                              (k[3:7].view(torch.float8_e4m3fn), v[4:8].view(torch.float8_e4m3fn))])
+
+
+def test_layers_in_turn_in_one_buffer(ops):
+    """Pages that hold every layer's K and V beside each other."""
+    gen = torch.Generator().manual_seed(8)
+    x = torch.randn((12, 3, 2, 16, 2, 64), generator=gen).to(torch.bfloat16)
+    gpu = x.to(DEV)
+    state = ops.prepare_kv_pages([(gpu[:, i, 0], gpu[:, i, 1]) for i in range(3)])
+    pairs = [(3, 7), (0, 11)]
+    ops.copy_kv_pages(state, torch.tensor(pairs, device=DEV))
+    i32 = [torch.tensor(a, dtype=torch.int32, device=DEV) for a in ([[4, 5, 6]], [3], [[0, 2, 20]], [3])]
+    ops.compact_kv(state, *i32)
+    torch.cuda.synchronize()
+    planes = [x[:, :, p].transpose(0, 1) for p in range(2)]
+    want = od.compact(od.copy_pages(planes, pairs), [[4, 5, 6]], [3], [[0, 2, 20]], [3])
+    assert torch.equal(gpu.cpu(), torch.stack([w.transpose(0, 1) for w in want], dim=2))
