@@ -636,6 +636,12 @@ int lmc_tree_attention(const lmc_tensor *query, const lmc_tensor *vllm_kv_caches
  * GPU alone.  Touches the host only. */
 int lmc_check_layers_apart(const lmc_tensor *caches, int64_t n);
 
+/* LMC_ERR_VALUE where one of the tensors (null ones are passed over) reaches
+ * into one of n ranges of addresses, [ranges[2 i], ranges[2 i + 1]), ascending
+ * and apart: those of all layers' caches, beside which the tables and lists of
+ * lmc_copy_kv_pages and lmc_compact_kv have to lie.  Touches the host only. */
+int lmc_check_outside(const int64_t *ranges, int64_t n, const lmc_tensor *const *tensors, int32_t n_tensors);
+
 /* Pages copied in every layer and plane.  layer_ptrs: device table [layers,
  * n_caches] int64 of the addresses of each layer's caches; vllm_kv_caches are one
  * layer's, whose shape, strides, dtype and alignment to 16 bytes all have
@@ -643,7 +649,8 @@ int lmc_check_layers_apart(const lmc_tensor *caches, int64_t n);
  * [pages, block, (heads,) dim]); no two caches share an element.  pages:
  * [n, 2] int64 or int32, (source, target); a pair with a page outside the
  * caches is skipped.  No target may be another pair's source or target.  At
- * most 65535 planes of all layers. */
+ * most 65535 planes of all layers.  pages and layer_ptrs lie apart from every
+ * layer's caches; the call itself sees vllm_kv_caches alone. */
 int lmc_copy_kv_pages(const lmc_tensor *layer_ptrs, const lmc_tensor *vllm_kv_caches, int32_t n_caches,
                       const lmc_tensor *pages, int32_t kvcache_format, int32_t vllm_two_major, void *stream);
 
@@ -654,7 +661,8 @@ int lmc_copy_kv_pages(const lmc_tensor *layer_ptrs, const lmc_tensor *vllm_kv_ca
  * increasing from 0 or more (another's rows end up in an order that is not
  * said), block_table [R, W] int32.  A row that has no page, here or there, is
  * not moved.  The rows that move, of all requests, lie in different places of
- * the caches.  At most 65535 requests.  seq_lens ([R] int32, may be null) gets base_lens + keep_lens. */
+ * the caches.  At most 65535 requests.  seq_lens ([R] int32, may be null) gets
+ * base_lens + keep_lens.  All of these lie apart from every layer's caches. */
 int lmc_compact_kv(const lmc_tensor *layer_ptrs, const lmc_tensor *vllm_kv_caches, int32_t n_caches,
                    const lmc_tensor *block_table, const lmc_tensor *base_lens, const lmc_tensor *keep,
                    const lmc_tensor *keep_lens, const lmc_tensor *seq_lens, int32_t kvcache_format,

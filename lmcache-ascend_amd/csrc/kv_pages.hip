@@ -434,6 +434,23 @@ extern "C" int lmc_check_layers_apart(const lmc_tensor *caches, int64_t n) {
   });
 }
 
+extern "C" int lmc_check_outside(const int64_t *ranges, int64_t n, const lmc_tensor *const *tensors, int32_t n_tensors) {
+  return guarded([&] {
+    for (int i = 0; i < n_tensors; ++i) {
+      const int64_t bytes = tensors[i] ? extent_bytes(*tensors[i]) : 0;
+      if (bytes == 0) continue;
+      const int64_t from = reinterpret_cast<int64_t>(tensors[i]->data);
+      int64_t lo = 0, hi = n;  // the first range that ends behind `from`
+      while (lo < hi) {
+        const int64_t mid = (lo + hi) / 2;
+        if (ranges[2 * mid + 1] > from) hi = mid;
+        else lo = mid + 1;
+      }
+      expect(lo == n || ranges[2 * lo] >= from + bytes, "the call's tables or lists overlap the paged caches of a layer");
+    }
+  });
+}
+
 extern "C" int lmc_copy_kv_pages(const lmc_tensor *layer_ptrs, const lmc_tensor *vllm_kv_caches, int32_t n_caches,
                                  const lmc_tensor *pages, int32_t kvcache_format, int32_t vllm_two_major, void *stream) {
   return guarded([&] {

@@ -57,6 +57,7 @@ using DraftTreeFn = int (*)(const lmc_tensor *, const lmc_tensor *, const lmc_te
 using TreeAttnFn = int (*)(const lmc_tensor *, const lmc_tensor *, int32_t, const lmc_tensor *, const lmc_tensor *,
                            const lmc_tensor *, const lmc_tensor *, double, const lmc_tensor *, const lmc_tensor *,
                            const lmc_tensor *, int64_t *, int32_t, int32_t, void *);
+using OutsideFn = int (*)(const int64_t *, int64_t, const lmc_tensor *const *, int32_t);
 using CopyPagesFn = int (*)(const lmc_tensor *, const lmc_tensor *, int32_t, const lmc_tensor *, int32_t, int32_t, void *);
 using CompactFn = int (*)(const lmc_tensor *, const lmc_tensor *, int32_t, const lmc_tensor *, const lmc_tensor *,
                           const lmc_tensor *, const lmc_tensor *, const lmc_tensor *, int32_t, int32_t, void *);
@@ -83,6 +84,7 @@ struct Table {
   PrefixAttnFn prefix_attn = nullptr;
   DraftTreeFn draft_tree = nullptr;
   TreeAttnFn tree_attn = nullptr;
+  OutsideFn outside = nullptr;
   CopyPagesFn copy_pages = nullptr;
   CompactFn compact = nullptr;
   ReleaseFn release = nullptr;
@@ -443,26 +445,35 @@ void tree_attention(const at::Tensor &query, const py::object &caches_obj, const
   call(&w, nullptr);
 }
 
-void copy_kv_pages(const at::Tensor &layer_ptrs, const std::vector<at::Tensor> &caches, const at::Tensor &pages,
-                   int64_t kvcache_format_raw, bool vllm_two_major) {
+// `ranges`: the addresses of all layers' caches (of the host).
+void check_outside(const at::Tensor &ranges, std::initializer_list<const lmc_tensor *> tensors) {
+  raise_for(g.outside(static_cast<const int64_t *>(ranges.data_ptr()), ranges.numel() / 2, tensors.begin(),
+                      static_cast<int32_t>(tensors.size())));
+}
+
+void copy_kv_pages(const at::Tensor &layer_ptrs, const std::vector<at::Tensor> &caches, const at::Tensor &ranges,
+                   const at::Tensor &pages, int64_t kvcache_format_raw, bool vllm_two_major) {
   check_bound();
   const int dev = gpu_of(layer_ptrs, "layer_ptrs");
   std::vector<lmc_tensor> cd;
   for (const auto &c : caches) cd.push_back(desc(c));
   const lmc_tensor l = desc(layer_ptrs), p = desc(pages);
+  check_outside(ranges, {&p});
   raise_for(g.copy_pages(&l, cd.data(), static_cast<int32_t>(cd.size()), &p, static_cast<int32_t>(kvcache_format_raw),
                          vllm_two_major, stream_of(dev)));
 }
 
-void compact_kv(const at::Tensor &layer_ptrs, const std::vector<at::Tensor> &caches, const at::Tensor &block_table,
-                const at::Tensor &base_lens, const at::Tensor &keep, const at::Tensor &keep_lens,
-                const c10::optional<at::Tensor> &seq_lens, int64_t kvcache_format_raw, bool vllm_two_major) {
+void compact_kv(const at::Tensor &layer_ptrs, const std::vector<at::Tensor> &caches, const at::Tensor &ranges,
+                const at::Tensor &block_table, const at::Tensor &base_lens, const at::Tensor &keep,
+                const at::Tensor &keep_lens, const c10::optional<at::Tensor> &seq_lens, int64_t kvcache_format_raw,
+                bool vllm_two_major) {
   check_bound();
   const int dev = gpu_of(layer_ptrs, "layer_ptrs");
   std::vector<lmc_tensor> cd;
   for (const auto &c : caches) cd.push_back(desc(c));
   const lmc_tensor l = desc(layer_ptrs), t = desc(block_table), b = desc(base_lens), k = desc(keep), n = desc(keep_lens);
   const Opt s(seq_lens);
+  check_outside(ranges, {&t, &b, &k, &n, s.ptr()});
   raise_for(g.compact(&l, cd.data(), static_cast<int32_t>(cd.size()), &t, &b, &k, &n, s.ptr(),
                       static_cast<int32_t>(kvcache_format_raw), vllm_two_major, stream_of(dev)));
 }
@@ -488,8 +499,8 @@ void bind(uintptr_t multi, uintptr_t single, uintptr_t load_flash, uintptr_t res
           uintptr_t rope, uintptr_t blend, uintptr_t cdf, uintptr_t encode, uintptr_t decode,
           uintptr_t encode_rows, uintptr_t pack_rows, uintptr_t decode_chunk,
           uintptr_t slot_map, uintptr_t rotary, uintptr_t rotary_paged, uintptr_t prefix_attn,
-          uintptr_t draft_tree, uintptr_t tree_attn, uintptr_t copy_pages, uintptr_t compact, uintptr_t release,
-          uintptr_t last_error) {
+          uintptr_t draft_tree, uintptr_t tree_attn, uintptr_t outside, uintptr_t copy_pages, uintptr_t compact,
+          uintptr_t release, uintptr_t last_error) {
   g.multi = reinterpret_cast<MultiFn>(multi);
   g.single = reinterpret_cast<SingleFn>(single);
   g.load_flash = reinterpret_cast<FlashFn>(load_flash);
@@ -508,6 +519,7 @@ void bind(uintptr_t multi, uintptr_t single, uintptr_t load_flash, uintptr_t res
   g.prefix_attn = reinterpret_cast<PrefixAttnFn>(prefix_attn);
   g.draft_tree = reinterpret_cast<DraftTreeFn>(draft_tree);
   g.tree_attn = reinterpret_cast<TreeAttnFn>(tree_attn);
+  g.outside = reinterpret_cast<OutsideFn>(outside);
   g.copy_pages = reinterpret_cast<CopyPagesFn>(copy_pages);
   g.compact = reinterpret_cast<CompactFn>(compact);
   g.release = reinterpret_cast<ReleaseFn>(release);

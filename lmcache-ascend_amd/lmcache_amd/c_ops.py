@@ -56,6 +56,7 @@ try:
         _addr("lmc_shared_prefix_attention"),
         _addr("lmc_build_draft_tree"),
         _addr("lmc_tree_attention"),
+        _addr("lmc_check_outside"),
         _addr("lmc_copy_kv_pages"),
         _addr("lmc_compact_kv"),
         _addr("lmc_release_pages"),
@@ -885,7 +886,26 @@ class KVPagesState:
     table of their addresses on the GPU.  It keeps the caches alive; build a
     new one after reallocating them."""
 
-    __slots__ = ("layers", "layer_ptrs", "caches", "kvcache_format", "vllm_two_major")
+    __slots__ = ("layers", "layer_ptrs", "caches", "ranges", "kvcache_format", "vllm_two_major")
+
+
+def _address_ranges(tensors) -> torch.Tensor:
+    """[n, 2] on the host: where the tensors lie, ascending and apart."""
+    ranges = []
+    for t in sorted(tensors, key=torch.Tensor.data_ptr):
+        begin = t.data_ptr()
+        end = begin + (sum((n - 1) * s for n, s in zip(t.shape, t.stride())) + 1) * t.element_size()
+        if ranges and begin <= ranges[-1][1]:
+            ranges[-1][1] = max(ranges[-1][1], end)
+        else:
+            ranges.append([begin, end])
+    return torch.tensor(ranges, dtype=torch.int64).view(-1, 2)
+
+
+def _check_outside(state: KVPagesState, *tensors) -> None:
+    descs = [None if t is None else ctypes.pointer(_desc(t)) for t in tensors]
+    _run(_L.lmc_check_outside(state.ranges.data_ptr(), state.ranges.shape[0], (ctypes.POINTER(_lib.LmcTensor) * len(descs))(*descs),
+                              len(descs)))
 
 
 def prepare_kv_pages(layers, kvcache_format_raw: int = 2, vllm_two_major: bool = False) -> KVPagesState:
@@ -919,6 +939,7 @@ def prepare_kv_pages(layers, kvcache_format_raw: int = 2, vllm_two_major: bool =
     st = KVPagesState()
     st.layers = tuple(layers)
     st.caches = [plain(t) for t in first]
+    st.ranges = _address_ranges(whole)
     st.kvcache_format, st.vllm_two_major = int(kvcache_format_raw), bool(vllm_two_major)
     st.layer_ptrs = torch.tensor([[t.data_ptr() for t in caches] for caches in layers], dtype=torch.int64,
                                  device=first[0].device)
@@ -931,11 +952,13 @@ def copy_kv_pages(state: KVPagesState, pages: torch.Tensor) -> None:
     """Pages copied in every layer and plane, as forks need them: pages is
     [n, 2] int64 or int32, (source, target) page numbers.  Pairs with a page
     outside the caches are skipped.  No target may be another pair's source or
-    target; a source may serve several targets."""
+    target; a source may serve several targets.  pages lies apart from the caches
+    of all layers."""
     if _ext is not None:
-        _ext.copy_kv_pages(state.layer_ptrs, state.caches, pages, state.kvcache_format, state.vllm_two_major)
+        _ext.copy_kv_pages(state.layer_ptrs, state.caches, state.ranges, pages, state.kvcache_format, state.vllm_two_major)
         return
     dev = _gpu_of(state.layer_ptrs, "layer_ptrs")
+    _check_outside(state, pages)
     _run(
         _L.lmc_copy_kv_pages(
             _opt(state.layer_ptrs), _cache_array(state.caches), len(state.caches), _opt(pages), state.kvcache_format,
@@ -964,12 +987,14 @@ def compact_kv(
     int32) has the requests' pages; no two positions of the rows that move may
     share a page row, within a request or between requests: shared pages are
     copied first (copy_kv_pages).  A row that has no page, here or there, is not
-    moved.  seq_lens ([R] int32), where given, gets base_lens + keep_lens."""
+    moved.  seq_lens ([R] int32), where given, gets base_lens + keep_lens.  None of
+    them may lie over the caches of any layer."""
     if _ext is not None:
-        _ext.compact_kv(state.layer_ptrs, state.caches, block_table, base_lens, keep, keep_lens, seq_lens,
+        _ext.compact_kv(state.layer_ptrs, state.caches, state.ranges, block_table, base_lens, keep, keep_lens, seq_lens,
                         state.kvcache_format, state.vllm_two_major)
         return
     dev = _gpu_of(state.layer_ptrs, "layer_ptrs")
+    _check_outside(state, block_table, base_lens, keep, keep_lens, seq_lens)
     _run(
         _L.lmc_compact_kv(
             _opt(state.layer_ptrs), _cache_array(state.caches), len(state.caches), _opt(block_table), _opt(base_lens),

@@ -414,3 +414,39 @@ def test_many_layers_in_one_buffer_are_told_apart_at_once():
     assert _layers_check(caches) == _lib.OK
     caches[400].data += 2 * 64
     _refuses(_layers_check(caches), "two of the layers' caches overlap")
+
+
+def _outside(ranges, *tensors):
+    flat = [x for r in ranges for x in r]
+    ptrs = [None if t is None else ctypes.pointer(t) for t in tensors]
+    return L.lmc_check_outside((ctypes.c_int64 * max(1, len(flat)))(*flat), len(ranges),
+                               (ctypes.POINTER(_lib.LmcTensor) * max(1, len(ptrs)))(*ptrs), len(ptrs))
+
+
+_RANGES = [(1 << 40, (1 << 40) + 4096), ((1 << 40) + 8192, (1 << 40) + 8208), (1 << 44, 1 << 45)]
+
+
+@pytest.mark.parametrize("offset,shape,strides", [
+    (0, (1,), None), (4092, (1,), None), (-4, (2,), None), (-64, (4000,), None), (4096, (1025,), None), (8204, (1,), None),
+    (4096 - 8, (3, 2), [64, 1]), (4096, (2, 2), [1023, 1]), ((1 << 45) - (1 << 40) - 4, (7,), None), (-4, (1 << 43,), None),
+])
+def test_lists_over_the_caches_of_a_layer_are_refused(offset, shape, strides):
+    t = _t(I32, *shape, data=(1 << 40) + offset, strides=strides)
+    _refuses(_outside(_RANGES, None, _t(I32, 9, data=1 << 39), t), "overlap the paged caches of a layer")
+
+
+@pytest.mark.parametrize("offset,shape,strides", [
+    (-4, (1,), None), (4096, (1024,), None), (4096, (2, 2), [1022, 1]), (8208, (99,), None), ((1 << 45) - (1 << 40), (7,), None),
+    (100, (0,), None), (100, (3, 0), None),
+])
+def test_lists_beside_the_caches_are_taken(offset, shape, strides):
+    t = _t(I32, *shape, data=(1 << 40) + offset, strides=strides)
+    assert _outside(_RANGES, t, None) == _lib.OK and _outside([], t) == _lib.OK and _outside(_RANGES) == _lib.OK
+
+
+def test_address_ranges_are_put_in_order():
+    x = torch.zeros((6, 4, 8), dtype=torch.bfloat16)
+    at = x.data_ptr()
+    parts = [x[4:], x[0], x[1, :, :4], x[1, :, 4:], x[3, 0]]
+    assert c_ops._address_ranges(parts).tolist() == [[at, at + 128], [at + 192, at + 208], [at + 256, at + 384]]
+    assert c_ops._address_ranges([]).shape == (0, 2)

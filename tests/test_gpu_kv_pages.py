@@ -479,3 +479,30 @@ def test_layers_in_turn_in_one_buffer(ops):
     planes = [x[:, :, p].transpose(0, 1) for p in range(2)]
     want = od.compact(od.copy_pages(planes, pairs), [[4, 5, 6]], [3], [[0, 2, 20]], [3])
     assert torch.equal(gpu.cpu(), torch.stack([w.transpose(0, 1) for w in want], dim=2))
+
+
+@pytest.mark.parametrize("direct", [False, True])
+def test_lists_in_the_caches_of_any_layer_are_refused(ops, monkeypatch, direct):
+    if direct:
+        monkeypatch.setattr(ops, "_ext", None)
+    space = torch.zeros(4 * 4096 * 2 + 64, dtype=torch.int32, device=DEV)
+    whole = space[: 4 * 4096].view(torch.bfloat16).view(4, 4, 16, 2, 64)
+    k, v = whole[:2], whole[2:]
+    state = ops.prepare_kv_pages([(k[i], v[i]) for i in range(2)])
+    assert state.ranges.shape == (1, 2)
+    i32 = dict(dtype=torch.int32, device=DEV)
+    fine = [torch.zeros(s, **i32) for s in ((2, 3), (2,), (2, 3), (2,), (2,))]
+    behind = space[4 * 4096:]
+    # Beside the caches in their buffer.
+    ops.copy_kv_pages(state, behind[:6].view(3, 2))
+    ops.compact_kv(state, *fine[:4], behind[6:8])
+    torch.cuda.synchronize()
+    for layer in (k[0], k[1], v[0], v[1]):
+        inside = layer.view(-1)[-16:].view(torch.int32)
+        with pytest.raises(ValueError, match="overlap the paged caches"):
+            ops.copy_kv_pages(state, inside[:6].view(3, 2))
+        for i, t in enumerate(fine):
+            args = list(fine)
+            args[i] = inside[: t.numel()].view(t.shape)
+            with pytest.raises(ValueError, match="overlap the paged caches"):
+                ops.compact_kv(state, *args)
