@@ -121,7 +121,7 @@ struct CopyPlane {
 struct CopyArgs {
   CopyPlane plane[kMaxPlanes];
   const int64_t *ptrs;
-  int n_tensors, n_planes, n_layers;
+  int n_tensors, n_planes;
   const void *pairs;
   int wide;                       // pairs are int64
   int64_t pair_stride;
@@ -207,6 +207,7 @@ template <int VEC, int PL, bool MORE> __global__ void __launch_bounds__(256) mov
   const int n = min(max(a.keep_lens[r], 0), a.most);
   if (a.seq_lens && blockIdx.x == 0 && blockIdx.y == 0 && threadIdx.x == 0)
     a.seq_lens[r] = static_cast<int32_t>(min(b + n, static_cast<int64_t>(INT32_MAX)));
+  if (l >= a.n_layers) return;  // (a call without layers)
   uint8_t *base[PL];
 #pragma unroll
   for (int q = 0; q < PL; ++q) base[q] = reinterpret_cast<uint8_t *>(a.ptrs[l * a.n_tensors + a.plane[p + q].tensor]) + a.plane[p + q].offset;
@@ -492,7 +493,6 @@ extern "C" int lmc_copy_kv_pages(const lmc_tensor *layer_ptrs, const lmc_tensor 
     a.ptrs = static_cast<const int64_t *>(lp.data);
     a.n_tensors = g.n_tensors;
     a.n_planes = g.n_planes;
-    a.n_layers = layers;
     a.pairs = pr.data;
     a.wide = pr.dtype == LMC_I64;
     a.pair_stride = pr.strides[0];
@@ -548,7 +548,7 @@ extern "C" int lmc_compact_kv(const lmc_tensor *layer_ptrs, const lmc_tensor *vl
     for (const lmc_tensor *x : {block_table, base_lens, keep, keep_lens, seq_lens, layer_ptrs})
       for (int i = 0; x && i < n_caches; ++i)
         expect(!extents_meet(*x, vllm_kv_caches[i]), "the tables or lists overlap the paged caches");
-    if (R == 0 || layers == 0) return;
+    if (R == 0 || (layers == 0 && !seq_lens)) return;
     MoveArgs a;
     std::memset(&a, 0, sizeof(a));
     const int vec = vec_for(static_cast<int64_t>(g.align));
@@ -579,13 +579,13 @@ extern "C" int lmc_compact_kv(const lmc_tensor *layer_ptrs, const lmc_tensor *vl
     const MovePlane &k = a.plane[0], &v = a.plane[1];
     const int planes = g.n_planes == 2 && k.page == v.page && k.token == v.token && k.head == v.head && k.pieces == v.pieces &&
                                k.vectors == v.vectors ? 2 : 1;
-    const int64_t items = R * layers * (g.n_planes / planes);
+    const int64_t groups = std::max(1, layers) * (g.n_planes / planes), items = R * groups;
     // Slices of a row for 1024 workgroups or more, but no narrower than that takes
     // (128 bytes at least: half of 8 contexts of 8000 tokens 276 us so; 64 requests
     // of 6 rows 10.6 us with whole rows, 13.7 with slices for 4096 workgroups).
     a.lanes = kLeastLanes;
     while (a.lanes < 256 && a.lanes < most && items * ((most + 2 * a.lanes - 1) / (2 * a.lanes)) >= 1024) a.lanes *= 2;
-    const int64_t slices = (most + a.lanes - 1) / a.lanes, groups = layers * (g.n_planes / planes);
+    const int64_t slices = (most + a.lanes - 1) / a.lanes;
     expect(groups <= 65535 && slices <= UINT32_MAX / 256, "too many layers");
     DeviceGuard guard(dev);
     const dim3 grid(static_cast<uint32_t>(slices), static_cast<uint32_t>(groups), static_cast<uint32_t>(R));

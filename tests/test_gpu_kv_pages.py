@@ -506,3 +506,16 @@ def test_lists_in_the_caches_of_any_layer_are_refused(ops, monkeypatch, direct):
             args[i] = inside[: t.numel()].view(t.shape)
             with pytest.raises(ValueError, match="overlap the paged caches"):
                 ops.compact_kv(state, *args)
+
+
+def test_lengths_without_layers(ops):
+    """No layer moves a row, seq_lens is written all the same."""
+    c = Caches(ops, "separate", 2, 6, 16, 2, 64)
+    c.state.layer_ptrs = c.state.layer_ptrs[:0]
+    i32 = dict(dtype=torch.int32, device=DEV)
+    seq = torch.full((3,), -7, **i32)
+    ops.compact_kv(c.state, torch.tensor([[0, 1]] * 3, **i32), torch.tensor([3, 4, 2**31 - 1], **i32),
+                   torch.tensor([[1, 2]] * 3, **i32), torch.tensor([2, 9, 1], **i32), seq)
+    ops.copy_kv_pages(c.state, torch.tensor([[0, 1]], device=DEV))
+    c.hold(c.planes)
+    assert seq.tolist() == [5, 6, 2**31 - 1]
