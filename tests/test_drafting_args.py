@@ -450,3 +450,32 @@ def test_address_ranges_are_put_in_order():
     parts = [x[4:], x[0], x[1, :, :4], x[1, :, 4:], x[3, 0]]
     assert c_ops._address_ranges(parts).tolist() == [[at, at + 128], [at + 192, at + 208], [at + 256, at + 384]]
     assert c_ops._address_ranges([]).shape == (0, 2)
+
+
+@pytest.mark.parametrize("T,R,Hq,Hk,dim,width,rows,pieces", [
+    # Few rows (64 of a tile; the pieces that the keys allow), and a whole chip of them.
+    (9, 3, 8, 2, 64, 5, 64, 6),
+    (512, 32, 32, 8, 128, 512, 64, 64),
+    (32, 32, 32, 8, 192, 512, 64, 32),
+    (32, 32, 32, 8, 256, 512, 64, 32),
+    # 65 to 128 rows; more; 192 dims have 128 rows at most, 256 dims 64.
+    (1024, 32, 32, 8, 64, 512, 128, 96),
+    (1024, 32, 32, 8, 128, 512, 128, 32),
+    (2048, 32, 32, 8, 64, 512, 256, 32),
+    (2048, 32, 32, 8, 96, 512, 256, 32),
+    (2048, 32, 32, 8, 192, 512, 128, 32),
+    (2048, 32, 32, 8, 256, 512, 64, 32),
+    # More KV heads than places: one piece each.
+    (1, 1, 600, 600, 128, 4096, 64, 1),
+    # Seven heads a KV head; a table without pages.
+    (13, 13, 28, 4, 64, 300, 64, 128),
+    (4, 2, 4, 4, 128, 0, 64, 2),
+])
+def test_tree_attention_workspace_is_what_the_plan_needs(T, R, Hq, Hk, dim, width, rows, pieces):
+    """Two places of `rows` rows (sums of `dim` and two more numbers) for each
+    workgroup, and 16 bytes; a byte less is refused."""
+    sizes = dict(q=_t(BF16, T, Hq, dim), out=_t(BF16, T, Hq, dim), lse=None, mask=_t(I64, T, 1),
+                 caches=_caches(heads=Hk, dim=dim), table=_t(I32, R, width), seq=_t(I32, R), starts=_t(I32, R + 1))
+    need = pieces * Hk * (2 * rows * (4 * dim + 8) + 16)
+    assert _attend(True, **sizes) == (_lib.OK, need)
+    _refuses(_attend(ws=_t(U8, need - 1), **sizes), f"at least {need} bytes")

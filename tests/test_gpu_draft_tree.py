@@ -86,3 +86,28 @@ def test_a_chain_is_causal(ops):
     mask = torch.empty((100, 2), dtype=torch.int64, device=DEV)
     ops.build_draft_tree(parents.to(DEV), starts.to(DEV), seq.to(DEV), mask)
     assert od.mask_of(mask.cpu()) == [(1 << (i + 1)) - 1 for i in range(100)]
+
+
+@pytest.mark.parametrize("words", [1, 12, 16])
+def test_captured_and_replayed_on_other_trees(ops, words):
+    """Rows in more LDS than a launch has by itself, captured too."""
+    lens = [[64 * words, 3, 0], [1, 64 * words - 40, 30], [0, 0, 5], [200, 1, 64 * words - 300 if words > 9 else 9]]
+    T = 64 * words + 300
+    i32 = dict(dtype=torch.int32, device=DEV)
+    parents, starts, seq = torch.zeros(T, **i32), torch.zeros(4, **i32), torch.zeros(3, **i32)
+    mask, pos = (torch.empty(s, dtype=torch.int64, device=DEV) for s in ((T, words), (T,)))
+    ops.build_draft_tree(parents, starts, seq, mask, pos)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        ops.build_draft_tree(parents, starts, seq, mask, pos)
+    for n, some in enumerate(lens):
+        x = _random(50 + n, some, pad=T - sum(some), deep=n % 2 == 0)
+        for a, b in zip((parents, starts, seq), x):
+            a.copy_(b)
+        mask.fill_(77)
+        pos.fill_(77)
+        graph.replay()
+        torch.cuda.synchronize()
+        want, places = od.draft_tree(x[0].tolist(), x[1].tolist(), x[2].tolist(), T, words)
+        assert torch.equal(mask.cpu(), od.words_of(want, words)) and pos.tolist() == places

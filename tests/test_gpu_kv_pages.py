@@ -519,3 +519,22 @@ def test_lengths_without_layers(ops):
     ops.copy_kv_pages(c.state, torch.tensor([[0, 1]], device=DEV))
     c.hold(c.planes)
     assert seq.tolist() == [5, 6, 2**31 - 1]
+
+
+@pytest.mark.parametrize("offset", [1, 2, 3])
+@pytest.mark.parametrize("pages", [5, 1023, 1025, 5000])
+def test_counts_off_a_16_byte_boundary(ops, offset, pages):
+    gen = torch.Generator().manual_seed(pages + offset)
+    i32 = dict(dtype=torch.int32, device=DEV)
+    n = min(pages, 400)
+    table = torch.randperm(pages, generator=gen)[:n].view(1, n)
+    refs = torch.randint(0, 2, (pages,), generator=gen).tolist()
+    space = torch.full((pages + 8,), -50, **i32)
+    refs_d = space[offset: offset + pages]
+    refs_d.copy_(torch.tensor(refs, dtype=torch.int32))
+    free, cur, nxt = torch.full((n,), 99, **i32), torch.tensor([n], device=DEV), torch.tensor([0], device=DEV)
+    ops.release_pages(table.to(**i32), torch.tensor([16 * n], **i32), torch.tensor([0], **i32), 16, refs_d, free, cur, nxt)
+    torch.cuda.synchronize()
+    want = od.release(table.tolist(), [16 * n], [0], 16, refs, [99] * n, n)
+    assert (refs_d.tolist(), free.tolist(), nxt.item()) == want
+    assert (space[:offset] == -50).all() and (space[offset + pages:] == -50).all()

@@ -461,3 +461,58 @@ def test_odd_values_of_a_rows_first_keys(ops, dtype, dim, Hq, context, odd):
         hit[i, :, d] = True
     assert (np.isnan(got[hit]) if odd != odd else got[hit] == odd).all(), np.argwhere(hit & np.isnan(got))
     assert (np.abs(got - want)[~hit] <= tol[~hit]).all()
+
+
+def _spread_pages(c, pages, at):
+    """The case's pages at page `at(p)` of caches of `pages` pages of NaN."""
+    caches = []
+    for x in (c["k"], c["v"]):
+        big = torch.full((pages, *x.shape[1:]), NAN, dtype=x.dtype, device=DEV)
+        big[torch.tensor([at(p) for p in range(x.shape[0])], device=DEV)] = x.to(DEV)
+        caches.append(big)
+    return tuple(caches)
+
+
+@pytest.mark.parametrize("Hq,dim,block", [(4, 128, 16), (4, 64, 24)])
+def test_caches_past_4_gib(ops, Hq, dim, block):
+    """Pages on both sides of 2^31 and 2^32 bytes."""
+    c = _case(31, [20, 7], [150, 40], block, Hq, 2, dim)
+    page = block * 2 * dim * 2
+    pages = (2**32 + 2**31) // page + 100
+    caches = _spread_pages(c, pages, lambda p: pages - 1 - p * ((pages - 1) // c["k"].shape[0]))
+    table = c["table"].clone()
+    for r, n in enumerate(c["seq"].tolist()):
+        for j in range(-(-n // block)):
+            table[r, j] = pages - 1 - int(table[r, j]) * ((pages - 1) // c["k"].shape[0])
+    out, lse = c["out"].to(DEV), c["lse"].to(DEV)
+    ops.tree_attention(c["q"].to(DEV), caches, table.to(DEV), c["seq"].to(DEV), c["starts"].to(DEV),
+                       od.words_of(c["mask"], c["words"]).to(DEV), c["scale"], out, lse)
+    torch.cuda.synchronize()
+    _hold(out, lse, _want(c))
+
+
+@pytest.mark.parametrize("dim,q_lens", [(64, [20, 7]), (128, [70, 80])])
+def test_rows_far_apart(ops, dim, q_lens):
+    """Cache rows 2^27 - 16 bytes apart, the most that is taken (a group of 16
+    spans 2 GiB); query, output, lse and masks of rows hundreds of MB apart."""
+    c = _case(32, q_lens, [60, 35], 16, 2, 1, dim)
+    pages, step = c["k"].shape[0], (2**27 - 16) // 2
+    caches = []
+    for x in (c["k"], c["v"]):
+        space = torch.empty(15 * step + pages * dim, dtype=x.dtype, device=DEV)
+        far = space.as_strided((pages, 16, 1, dim), (dim, step, dim, 1))
+        far.copy_(x.to(DEV))
+        caches.append(far)
+    T = c["q"].shape[0]
+
+    def apart(x, row):
+        space = torch.empty((T - 1) * row + x[0].numel(), dtype=x.dtype, device=DEV)
+        far = space.as_strided(x.shape, (row, *x.stride()[1:]))
+        far.copy_(x.to(DEV))
+        return far
+
+    q, out, lse = apart(c["q"], 2**33 // T // 16 * 8), apart(c["out"], 2**33 // T // 16 * 8), apart(c["lse"], 2**32 // T)
+    mask = apart(od.words_of(c["mask"], c["words"]), 2**32 // T // 2)
+    ops.tree_attention(q, tuple(caches), c["table"].to(DEV), c["seq"].to(DEV), c["starts"].to(DEV), mask, c["scale"], out, lse)
+    torch.cuda.synchronize()
+    _hold(out, lse, _want(c))
