@@ -633,13 +633,15 @@ int lmc_tree_attention(const lmc_tensor *query, const lmc_tensor *vllm_kv_caches
 /* LMC_ERR_VALUE where two of n caches share an element (those of all layers, in
  * any order; rows dealt in turn in one buffer are told apart).  For the callers
  * of lmc_copy_kv_pages and lmc_compact_kv, which see the layers' addresses on the
- * GPU alone.  Touches the host only. */
-int lmc_check_layers_apart(const lmc_tensor *caches, int64_t n);
+ * GPU alone.  Where ranges is not null, it gets the addresses that the caches
+ * span, *n_ranges (at most n) pairs [begin, end), ascending and apart.  Touches
+ * the host only. */
+int lmc_check_layers_apart(const lmc_tensor *caches, int64_t n, int64_t *ranges, int64_t *n_ranges);
 
 /* LMC_ERR_VALUE where one of the tensors (null ones are passed over) reaches
- * into one of n ranges of addresses, [ranges[2 i], ranges[2 i + 1]), ascending
- * and apart: those of all layers' caches, beside which the tables and lists of
- * lmc_copy_kv_pages and lmc_compact_kv have to lie.  Touches the host only. */
+ * into one of the n ranges that lmc_check_layers_apart gave: the tables and lists
+ * of lmc_copy_kv_pages and lmc_compact_kv lie apart from every layer's caches.
+ * Touches the host only. */
 int lmc_check_outside(const int64_t *ranges, int64_t n, const lmc_tensor *const *tensors, int32_t n_tensors);
 
 /* Pages copied in every layer and plane.  layer_ptrs: device table [layers,

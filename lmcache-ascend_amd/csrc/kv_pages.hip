@@ -419,19 +419,36 @@ __global__ void __launch_bounds__(256) place_free(ReleaseArgs a) {
 
 using namespace lmc;
 
-extern "C" int lmc_check_layers_apart(const lmc_tensor *caches, int64_t n) {
+extern "C" int lmc_check_layers_apart(const lmc_tensor *caches, int64_t n, int64_t *ranges, int64_t *n_ranges) {
   return guarded([&] {
-    std::vector<const lmc_tensor *> by_address;
-    for (int64_t i = 0; i < n; ++i)
-      if (extent_bytes(deref(&caches[i], "caches")) > 0) by_address.push_back(&caches[i]);
-    auto begin = [](const lmc_tensor *t) { return reinterpret_cast<uintptr_t>(t->data); };
-    std::sort(by_address.begin(), by_address.end(), [&](const lmc_tensor *a, const lmc_tensor *b) { return begin(a) < begin(b); });
-    for (size_t i = 0; i < by_address.size(); ++i) {
-      const lmc_tensor &a = *by_address[i];
-      const uintptr_t end = begin(&a) + extent_bytes(a);
-      for (size_t k = i + 1; k < by_address.size() && begin(by_address[k]) < end; ++k)
-        expect(a.device != by_address[k]->device || !may_share(a, *by_address[k]), "two of the layers' caches overlap");
+    struct Cache {
+      int64_t begin, end;
+      int device;
+      Layout layout;
+    };
+    std::vector<Cache> all;
+    for (int64_t i = 0; i < n; ++i) {
+      const lmc_tensor &t = deref(&caches[i], "caches");
+      const int64_t begin = reinterpret_cast<int64_t>(t.data), bytes = extent_bytes(t);
+      if (bytes > 0) all.push_back({begin, begin + bytes, t.device, layout_of(t)});
     }
+    std::sort(all.begin(), all.end(), [](const Cache &a, const Cache &b) { return a.begin < b.begin; });
+    for (size_t i = 0; i < all.size(); ++i)
+      for (size_t k = i + 1; k < all.size() && all[k].begin < all[i].end; ++k)
+        expect(all[i].device != all[k].device || apart(all[i].layout, all[k].layout, all[k].begin - all[i].begin),
+               "two of the layers' caches overlap");
+    if (!ranges) return;
+    int64_t count = 0;
+    for (const Cache &c : all) {
+      if (count > 0 && c.begin <= ranges[2 * count - 1]) {
+        ranges[2 * count - 1] = std::max(ranges[2 * count - 1], c.end);
+        continue;
+      }
+      ranges[2 * count] = c.begin;
+      ranges[2 * count + 1] = c.end;
+      ++count;
+    }
+    *n_ranges = count;
   });
 }
 

@@ -57,6 +57,7 @@ using DraftTreeFn = int (*)(const lmc_tensor *, const lmc_tensor *, const lmc_te
 using TreeAttnFn = int (*)(const lmc_tensor *, const lmc_tensor *, int32_t, const lmc_tensor *, const lmc_tensor *,
                            const lmc_tensor *, const lmc_tensor *, double, const lmc_tensor *, const lmc_tensor *,
                            const lmc_tensor *, int64_t *, int32_t, int32_t, void *);
+using LayersFn = int (*)(const lmc_tensor *, int64_t, int64_t *, int64_t *);
 using OutsideFn = int (*)(const int64_t *, int64_t, const lmc_tensor *const *, int32_t);
 using CopyPagesFn = int (*)(const lmc_tensor *, const lmc_tensor *, int32_t, const lmc_tensor *, int32_t, int32_t, void *);
 using CompactFn = int (*)(const lmc_tensor *, const lmc_tensor *, int32_t, const lmc_tensor *, const lmc_tensor *,
@@ -84,6 +85,7 @@ struct Table {
   PrefixAttnFn prefix_attn = nullptr;
   DraftTreeFn draft_tree = nullptr;
   TreeAttnFn tree_attn = nullptr;
+  LayersFn layers = nullptr;
   OutsideFn outside = nullptr;
   CopyPagesFn copy_pages = nullptr;
   CompactFn compact = nullptr;
@@ -445,7 +447,18 @@ void tree_attention(const at::Tensor &query, const py::object &caches_obj, const
   call(&w, nullptr);
 }
 
-// `ranges`: the addresses of all layers' caches (of the host).
+// The addresses that all layers' caches span, [n, 2] on the host.
+at::Tensor address_ranges(const std::vector<at::Tensor> &caches) {
+  check_bound();
+  std::vector<lmc_tensor> cd;
+  cd.reserve(caches.size());
+  for (const auto &c : caches) cd.push_back(desc(c));
+  int64_t n = 0;
+  at::Tensor ranges = at::empty({static_cast<int64_t>(cd.size()), 2}, at::kLong);
+  raise_for(g.layers(cd.data(), static_cast<int64_t>(cd.size()), static_cast<int64_t *>(ranges.data_ptr()), &n));
+  return ranges.narrow(0, 0, n);
+}
+
 void check_outside(const at::Tensor &ranges, std::initializer_list<const lmc_tensor *> tensors) {
   raise_for(g.outside(static_cast<const int64_t *>(ranges.data_ptr()), ranges.numel() / 2, tensors.begin(),
                       static_cast<int32_t>(tensors.size())));
@@ -499,8 +512,8 @@ void bind(uintptr_t multi, uintptr_t single, uintptr_t load_flash, uintptr_t res
           uintptr_t rope, uintptr_t blend, uintptr_t cdf, uintptr_t encode, uintptr_t decode,
           uintptr_t encode_rows, uintptr_t pack_rows, uintptr_t decode_chunk,
           uintptr_t slot_map, uintptr_t rotary, uintptr_t rotary_paged, uintptr_t prefix_attn,
-          uintptr_t draft_tree, uintptr_t tree_attn, uintptr_t outside, uintptr_t copy_pages, uintptr_t compact,
-          uintptr_t release, uintptr_t last_error) {
+          uintptr_t draft_tree, uintptr_t tree_attn, uintptr_t layers, uintptr_t outside, uintptr_t copy_pages,
+          uintptr_t compact, uintptr_t release, uintptr_t last_error) {
   g.multi = reinterpret_cast<MultiFn>(multi);
   g.single = reinterpret_cast<SingleFn>(single);
   g.load_flash = reinterpret_cast<FlashFn>(load_flash);
@@ -519,6 +532,7 @@ void bind(uintptr_t multi, uintptr_t single, uintptr_t load_flash, uintptr_t res
   g.prefix_attn = reinterpret_cast<PrefixAttnFn>(prefix_attn);
   g.draft_tree = reinterpret_cast<DraftTreeFn>(draft_tree);
   g.tree_attn = reinterpret_cast<TreeAttnFn>(tree_attn);
+  g.layers = reinterpret_cast<LayersFn>(layers);
   g.outside = reinterpret_cast<OutsideFn>(outside);
   g.copy_pages = reinterpret_cast<CopyPagesFn>(copy_pages);
   g.compact = reinterpret_cast<CompactFn>(compact);
@@ -552,6 +566,7 @@ PYBIND11_MODULE(_c_ops_ext, m) {
   m.def("shared_prefix_attention", &shared_prefix_attention);
   m.def("build_draft_tree", &build_draft_tree);
   m.def("tree_attention", &tree_attention);
+  m.def("address_ranges", &address_ranges);
   m.def("copy_kv_pages", &copy_kv_pages);
   m.def("compact_kv", &compact_kv);
   m.def("release_pages", &release_pages);

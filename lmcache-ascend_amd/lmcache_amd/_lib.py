@@ -105,7 +105,7 @@ SIGNATURES = {
     "lmc_tree_attention": [
         _T, _T, _i32, _T, _T, _T, _T, ctypes.c_double, _T, _T, _T, ctypes.POINTER(_i64), _i32, _i32, _vp,
     ],
-    "lmc_check_layers_apart": [_T, _i64],
+    "lmc_check_layers_apart": [_T, _i64, ctypes.POINTER(_i64), ctypes.POINTER(_i64)],
     "lmc_check_outside": [_vp, _i64, ctypes.POINTER(_T), _i32],
     "lmc_copy_kv_pages": [_T, _T, _i32, _T, _i32, _i32, _vp],
     "lmc_compact_kv": [_T, _T, _i32, _T, _T, _T, _T, _T, _i32, _i32, _vp],

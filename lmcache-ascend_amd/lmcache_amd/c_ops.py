@@ -56,6 +56,7 @@ try:
         _addr("lmc_shared_prefix_attention"),
         _addr("lmc_build_draft_tree"),
         _addr("lmc_tree_attention"),
+        _addr("lmc_check_layers_apart"),
         _addr("lmc_check_outside"),
         _addr("lmc_copy_kv_pages"),
         _addr("lmc_compact_kv"),
@@ -890,16 +891,13 @@ class KVPagesState:
 
 
 def _address_ranges(tensors) -> torch.Tensor:
-    """[n, 2] on the host: where the tensors lie, ascending and apart."""
-    ranges = []
-    for t in sorted(tensors, key=torch.Tensor.data_ptr):
-        begin = t.data_ptr()
-        end = begin + (sum((n - 1) * s for n, s in zip(t.shape, t.stride())) + 1) * t.element_size()
-        if ranges and begin <= ranges[-1][1]:
-            ranges[-1][1] = max(ranges[-1][1], end)
-        else:
-            ranges.append([begin, end])
-    return torch.tensor(ranges, dtype=torch.int64).view(-1, 2)
+    """[n, 2] on the host: the addresses that caches of any layers span,
+    ascending and apart.  Caches that overlap are refused."""
+    if _ext is not None:
+        return _ext.address_ranges(tensors)
+    ranges, n = (ctypes.c_int64 * (2 * len(tensors)))(), ctypes.c_int64(0)
+    _run(_L.lmc_check_layers_apart(_cache_array(tensors), len(tensors), ranges, ctypes.byref(n)))
+    return torch.tensor(list(ranges[: 2 * n.value]), dtype=torch.int64).view(-1, 2)
 
 
 def _check_outside(state: KVPagesState, *tensors) -> None:
@@ -935,11 +933,10 @@ def prepare_kv_pages(layers, kvcache_format_raw: int = 2, vllm_two_major: bool =
     whole = [t for caches in layers for t in caches if t.numel()]
     if len({t.data_ptr() for t in whole}) < len(whole):
         raise ValueError("a cache is given twice")
-    _run(_L.lmc_check_layers_apart(_cache_array([plain(t) for t in whole]), len(whole)))
     st = KVPagesState()
     st.layers = tuple(layers)
     st.caches = [plain(t) for t in first]
-    st.ranges = _address_ranges(whole)
+    st.ranges = _address_ranges([plain(t) for t in whole])
     st.kvcache_format, st.vllm_two_major = int(kvcache_format_raw), bool(vllm_two_major)
     st.layer_ptrs = torch.tensor([[t.data_ptr() for t in caches] for caches in layers], dtype=torch.int64,
                                  device=first[0].device)

@@ -363,7 +363,7 @@ def test_oracle_release_past_the_list():
 
 
 def _layers_check(caches):
-    return L.lmc_check_layers_apart(_array(caches), len(caches))
+    return L.lmc_check_layers_apart(_array(caches), len(caches), None, None)
 
 
 def _at(data, *shape, strides=None, dtype=BF16, device=0):
@@ -444,7 +444,10 @@ def test_lists_beside_the_caches_are_taken(offset, shape, strides):
     assert _outside(_RANGES, t, None) == _lib.OK and _outside([], t) == _lib.OK and _outside(_RANGES) == _lib.OK
 
 
-def test_address_ranges_are_put_in_order():
+@pytest.mark.parametrize("direct", [False, True])
+def test_address_ranges_are_put_in_order(monkeypatch, direct):
+    if direct:
+        monkeypatch.setattr(c_ops, "_ext", None)
     x = torch.zeros((6, 4, 8), dtype=torch.bfloat16)
     at = x.data_ptr()
     parts = [x[4:], x[0], x[1, :, :4], x[1, :, 4:], x[3, 0]]
