@@ -620,9 +620,9 @@ int lmc_build_draft_tree(const lmc_tensor *parents, const lmc_tensor *query_star
  * already.  Arguments, limits and workspace as for
  * lmc_shared_prefix_attention (without its shared prefix); output may be query
  * itself or lie beside it as columns of one buffer, lse lies apart from query.
- * tree_mask is [T, W] int64 (W up to 2^20).  A request's q tokens see its first seq_lens[r] - q keys,
- * and of its last q key j behind those where bit j % 64 of word j / 64 of the
- * token's row of tree_mask is set.  Key n lies in block
+ * tree_mask is [T, W] int64 (W up to 2^20).  A request's q tokens see its first
+ * seq_lens[r] - q keys, and of its last q key j behind those where bit j % 64 of
+ * word j / 64 of the token's row of tree_mask is set.  Key n lies in block
  * block_table[r][n / block_size]. */
 int lmc_tree_attention(const lmc_tensor *query, const lmc_tensor *vllm_kv_caches, int32_t n_caches,
                        const lmc_tensor *block_table, const lmc_tensor *seq_lens, const lmc_tensor *query_start_loc,

@@ -6,15 +6,17 @@
 //   release_pages:  pages ceil(keep / BS) <= j < ceil(held / BS) of each request lose a holder
 //
 // The first two in every layer l and plane p (K, V; the planes of an MLA
-// layer), through a table of the layers' addresses.  Both are copies, at the
-// rate of the memory system: 256 pages of 128 tokens in 8 layers (8 heads of 128
-// bf16 dims) 330 us, 5.7 TB/s of the bytes that differ; half of 8 contexts of 8000
-// tokens 264 us, 4.4 TB/s; the accepted rows of 64 requests in 32 layers 9.1 us.
+// layer), through a table of the layers' addresses.  Both are copies.  Pages go
+// at the rate of the memory system: 256 of 128 tokens in 8 layers (8 heads of 128
+// bf16 dims) 317 us in order (6.8 TB/s), 331 at random, 327 with a quarter of them
+// read twice.  Rows at random do not: half of 8 contexts of 8000 tokens 264 to 286
+// us, 4.1 to 4.5 TB/s (lists of one length 258, 4.6 TB/s; runs of adjacent rows
+// 5.4 TB/s).  The accepted rows of 64 requests in 32 layers take 9.1 to 9.9 us.
 //
 // release_pages is latency, three launches: holders taken off with atomics, pages
 // without one counted for each 1024, and those written to the list in ascending
 // order, which does not depend on the order of the atomics.  64 requests' drafts
-// among 20000 pages 8.8 us, 256 requests that end among 300000 12 us.
+// among 20000 pages 8.8 to 10.5 us, 256 requests that end among 300000 12 us.
 #include "serving.h"
 
 #include <type_traits>

@@ -1,7 +1,10 @@
 // Attention over paged K and V caches on the matrix cores of MI355X (gfx950):
 // what the kernels of prefix_attention.hip and tree_attention.hip share.  The
 // arguments of a call and their checks, tiles of keys from the caches to LDS,
-// and the steps of a tile.
+// their infinities, masks and largest scores; and the steps of a tile that
+// prefix_attention.hip takes (Rows32, has_odd, scores, refer_to, weigh,
+// add_values: tree_attention.hip spreads a step over two products and has its
+// own).
 //
 // S^T = K Q^T and O^T = V^T P^T on 32 x 32 x 16 matrix instructions: a lane
 // holds one row's weights for half of a block's keys, in the order in which
@@ -103,7 +106,8 @@ __device__ __forceinline__ uint64_t uniform(const void *p) {
 // keys, which all row tiles read, take 4% longer.  A prompt's tiles read its own
 // keys once each and would rather find them there: 2048 new tokens over 16384
 // shared keys take 764 us so and 743 without, 8192 over none 3.1 ms and 2.3.
-// The kernel is made for the former.  (m0 is reserved: nothing but these
+// That kernel, prefix_attention.hip's, is made for the former;
+// tree_attention.hip's loads all keys so.  (m0 is reserved: nothing but these
 // statements writes it in this file's kernels, each right before its load.)
 template <bool ONCE> __device__ __forceinline__ void load_to_lds(const uint8_t *base, uint32_t off, uint32_t lds) {
   if constexpr (ONCE)
@@ -591,8 +595,9 @@ inline PagedSizes paged_call(PagedArgs &a, const char *op, const lmc_tensor *que
 }
 
 // The caller's scratch: large enough, and apart from all that the call reads
-// and writes.  Parts are joined in a launch of their own, so output and lse may
-// lie over query; `inputs` are the call's tables and lengths.
+// and writes; output and lse apart from the caches and from `inputs`, the call's
+// tables and lengths.  Whether output or lse may lie over query is the call's to
+// check: it depends on when the kernel writes them.
 inline void check_outputs(const lmc_tensor *query, const lmc_tensor *output, const lmc_tensor *lse,
                           const lmc_tensor *workspace, int64_t bytes, int device, const lmc_tensor *vllm_kv_caches,
                           int32_t n_caches, std::initializer_list<const lmc_tensor *> inputs) {

@@ -671,6 +671,7 @@ extern "C" int lmc_shared_prefix_attention(const lmc_tensor *query, const lmc_te
       *workspace_bytes = bytes;
       return;
     }
+    // (output and lse may lie over query: parts are joined in a launch of their own)
     check_outputs(query, output, lse, workspace, bytes, kv.device, vllm_kv_caches, n_caches,
                   {query_start_loc, seq_lens, block_table, shared_blocks});
     a.shared = static_cast<const int32_t *>(sb.data);

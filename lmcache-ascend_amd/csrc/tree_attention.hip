@@ -17,17 +17,22 @@
 // launch joins.  Each workgroup has two places for sums: one for a tile that an
 // earlier workgroup began, one for a tile that a later one ends.
 //
-// Few rows are bound by the bytes of K and V, many by the products and the
-// softmax's vector work: 32 requests of up to 8192 keys, 32 heads over 8 KV heads
-// of 128 bf16 dims, take 99 us with one token each (5.6 TB/s), 118 with 16, 152
-// with 32 and 214 with 64 (663 TFLOP/s).  64 tokens over up to 16384 keys take
-// 364 to 408 us: the clock falls to 1.6 GHz there.  2 requests of 8 tokens over
-// 2000 keys: 15.0 us, the latency of two launches.  The join takes 10 us of 118
-// and 18 of 400.
+// Few rows are bound by the bytes of K and V, many by vector work beside the
+// products (a wave's step of 32 keys at 128 dims: 16 products, about 96 vector
+// instructions, of which 25 are addresses in LDS and 16 exponentials of four
+// times the length) and by loads that are waited for once a block (below): 32
+// requests of up to 8192 keys, 32 heads over 8 KV heads of 128 bf16 dims, take 95
+// to 99 us with one token each (5.6 to 5.9 TB/s), 116 with 16, 147 to 152 with 32
+// and 198 to 214 with 64 (663 to 725 TFLOP/s).  64 tokens over up to 16384 keys
+// take 356 to 408 us: the clock falls to 1.6 GHz there.  2 requests of 8 tokens
+// over 2000 keys: 15.0 us, the latency of two launches.  The join takes 10 us of
+// 116 and 18 of 400.
 //
-// Registers at 128 dims: 255 for 64 rows, 256 for more (12 to 18 spilled outside of
-// the loop over the keys), two waves a SIMD; at 64 dims 168 to 182; at 192 and 256
-// a wave a SIMD, with accumulation registers.
+// Registers at 128 dims: 255 for 64 rows, 256 for more (10 to 18 spilled outside of
+// the loop over the keys), two waves a SIMD; at 96 dims 204 to 206; at 64 dims 176
+// to 183, and 168 for 128 rows (three waves a SIMD, 6 or 7 spilled); at 192 and 256
+// a wave a SIMD, with 128 to 204 accumulation registers.  111 to 155 scalar
+// registers are kept in vector registers.
 #include "paged_attention.h"
 
 namespace lmc {
@@ -61,7 +66,9 @@ TreePlan make_plan(int64_t T, int64_t R, int64_t kv_heads, int64_t group, int64_
   // take 157 us with four row waves and halves, 220 as a tile of 256; 64 rows
   // take 128 us on 64 and 157 on 128.  At 64 dims 128 rows have workgroups of four
   // waves, three a CU (88 us; 100 with eight waves and halves).  192 dims do not
-  // fit 256 rows' registers, 256 dims not 128.
+  // fit 256 rows' registers (two waves a SIMD), 256 dims not 128 rows' blocks in
+  // LDS (five of 32 KB).  (The mean counts all rows, padding too: one wide tree
+  // among many short ones reads its keys once for each 64 rows.)
   const int64_t per = (T + R - 1) / R * group;
   p.rows = per <= 64 || dim == 256 ? 64 : per <= 128 || dim == 192 ? 128 : 256;
   // Workgroups that the 256 CUs hold at once.
@@ -313,7 +320,11 @@ template <typename T, int D, int WAVES> __device__ __forceinline__ bool any_odd(
 // beside the product with V of step i stand the maximum of step i + 1 and the
 // first half of its weights, beside the scores of step i + 2 the other half.  So
 // matrix and vector units have work at any time.  K and V have rings of blocks
-// in LDS, loaded as soon as a place is free.
+// in LDS, loaded as soon as a place is free.  The waits for them are counted, but
+// the compiler adds one for all loads to every block but the last: last() loads a
+// register there, which has to be settled on the other path too.  So the blocks
+// that are under way arrive together, and deep rings give less than they could;
+// kNV and kStart were measured like that.
 template <typename T, int D, int RW, int KW> struct Ring {
   using S = Shape<D, RW, KW>;
   static constexpr int kPer = D / 32, NK = S::kNK, NV = S::kNV;
@@ -347,6 +358,8 @@ template <typename T, int D, int RW, int KW> struct Ring {
     }
   }
   __device__ __forceinline__ int blocks() const { return (keys.k1 - keys.k0 + 63) / 64; }
+  // (Streaming loads: a request of one tile for each KV head reads its keys once.
+  // Those of several tiles, more than 256 rows, are read so too.)
   __device__ __forceinline__ void load_k(int j, uint32_t slot) {
     load_group<D, false, true>(keys, keys.place(4 * j + wave), keys.k0 + 64 * j + 16 * wave, k_off, own + slot * kBlock);
   }
@@ -653,7 +666,8 @@ __global__ void __launch_bounds__(64 * RW * KW, (Shape<D, RW, KW>::kPerSimd)) at
         if (next_blocks > 0) entry = ring.keys.entry_of(list, (threadIdx.x & 63) * 16, 0, next_end);
       });
     else if (next_blocks > 0) entry = ring.keys.entry_of(list, (threadIdx.x & 63) * 16, 0, next_end);
-    // What follows is under way while this one's sums are written.
+    // What follows is loaded while this one's sums are written (run() then waits
+    // for all of it: the query, which it needs first, is loaded last).
     meet();
     const int i = next_tile * S::kRows + wave * 32 + n, next_t = token(next, i), next_h = head(next, i);
     if (next_blocks > 0) {
