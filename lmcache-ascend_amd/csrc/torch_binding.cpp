@@ -454,7 +454,7 @@ at::Tensor address_ranges(const std::vector<at::Tensor> &caches) {
   cd.reserve(caches.size());
   for (const auto &c : caches) cd.push_back(desc(c));
   int64_t n = 0;
-  at::Tensor ranges = at::empty({static_cast<int64_t>(cd.size()), 2}, at::kLong);
+  at::Tensor ranges = at::empty({static_cast<int64_t>(cd.size()), 2}, at::TensorOptions(at::kCPU).dtype(at::kLong));
   raise_for(g.layers(cd.data(), static_cast<int64_t>(cd.size()), static_cast<int64_t *>(ranges.data_ptr()), &n));
   return ranges.narrow(0, 0, n);
 }

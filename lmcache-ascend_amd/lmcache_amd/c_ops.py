@@ -897,7 +897,7 @@ def _address_ranges(tensors) -> torch.Tensor:
         return _ext.address_ranges(tensors)
     ranges, n = (ctypes.c_int64 * (2 * len(tensors)))(), ctypes.c_int64(0)
     _run(_L.lmc_check_layers_apart(_cache_array(tensors), len(tensors), ranges, ctypes.byref(n)))
-    return torch.tensor(list(ranges[: 2 * n.value]), dtype=torch.int64).view(-1, 2)
+    return torch.tensor(list(ranges[: 2 * n.value]), dtype=torch.int64, device="cpu").view(-1, 2)
 
 
 def _check_outside(state: KVPagesState, *tensors) -> None:

@@ -538,3 +538,19 @@ def test_counts_off_a_16_byte_boundary(ops, offset, pages):
     want = od.release(table.tolist(), [16 * n], [0], 16, refs, [99] * n, n)
     assert (refs_d.tolist(), free.tolist(), nxt.item()) == want
     assert (space[:offset] == -50).all() and (space[offset + pages:] == -50).all()
+
+
+@pytest.mark.parametrize("direct", [False, True])
+def test_prepared_under_a_default_device(ops, monkeypatch, direct):
+    """The ranges that the calls look up on the host stay there."""
+    if direct:
+        monkeypatch.setattr(ops, "_ext", None)
+    k = torch.zeros((3, 4, 16, 2, 64), dtype=torch.bfloat16, device=DEV)
+    torch.set_default_device(DEV)
+    try:
+        state = ops.prepare_kv_pages([(k[i], k[i].clone()) for i in range(3)])
+    finally:
+        torch.set_default_device(None)
+    assert state.ranges.device.type == "cpu" and state.layer_ptrs.is_cuda
+    ops.copy_kv_pages(state, torch.tensor([[0, 1]], device=DEV))
+    torch.cuda.synchronize()
